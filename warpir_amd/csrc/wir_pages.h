@@ -50,4 +50,58 @@ WIR_HD unsigned scale_bits(unsigned amax) {
   return (unsigned)(imax(e, -126) + 127) << 23;
 }
 
+// ---------------------------------------------------------------------------
+// Attention: rows and tiles.  The query rows of one sequence and key/value
+// head are r = t * group + j, token t of query head j of the group; a block
+// has `rows_per_block` of them.  A tile is TILE positions.
+// ---------------------------------------------------------------------------
+constexpr int TILE = 64;
+
+// Positions that some row of block rb sees: 0 .. keys - 1.
+WIR_HD int block_keys(const Span& s, int rb, int rows_per_block, int rows, int group) {
+  const int first = rb * rows_per_block / group;
+  const int last = imin((imin(rows, (rb + 1) * rows_per_block) - 1) / group, s.count - 1);
+  if (first >= s.count || s.start + last < 0) return 0;
+  return imin(s.start + last + 1, s.held);
+}
+
+// Its units of work: tiles, and one where there are none (its rows are written all the same).
+WIR_HD int block_units(int keys) { return imax((int)(((i64)keys + TILE - 1) / TILE), 1); }
+
+// Division of the units of all (sequence, block) pairs, heads of a pair in
+// turn, tiles of a head in turn, into shares of `share` consecutive units for
+// the programs.  A program that takes part of a head's units leaves a partial
+// result in one of its two slots: the first segment of its share in slot
+// 2 * program, another one, which is then its last, in 2 * program + 1.
+WIR_HD i64 share_of(i64 total, int programs, int least) {
+  const i64 even = (total + programs - 1) / programs;
+  return even > least ? even : least;
+}
+
+struct Segment {
+  int head, first, last;   // tiles first .. last - 1 of the head's
+  i64 begin;               // the unit it starts at
+  bool whole;              // all of the head's
+};
+
+// The segment at unit u of a pair whose units start at `base`, `units` a head; the program's share ends at `end`.
+WIR_HD Segment segment_at(i64 u, i64 base, int units, i64 end) {
+  Segment g;
+  g.head = (int)((u - base) / units);
+  g.first = (int)((u - base) % units);
+  g.last = (int)(units - g.first < end - u ? units : g.first + (end - u));
+  g.begin = u;
+  g.whole = g.first == 0 && g.last == units;
+  return g;
+}
+
+// Slot of the partial result of a segment that starts at unit u, in the program of that share.
+WIR_HD int slot_of(i64 u, i64 share) { return (int)(2 * (u / share) + (u % share ? 1 : 0)); }
+
+// Partial results of a head whose units are begin .. begin + units - 1, and the slot of each.
+WIR_HD int parts_of(i64 begin, int units, i64 share) {
+  return (int)((begin + units - 1) / share - begin / share) + 1;
+}
+WIR_HD int slot_of_part(int first_slot, int part) { return part == 0 ? first_slot : 2 * (first_slot / 2 + part); }
+
 }  // namespace wir

@@ -10,6 +10,7 @@ from warpir_amd.handwritten import DevicePlans, check_tensor, check_written, lau
 PAGE_SIZES = (16, 32, 64, 128)
 _write_plans = DevicePlans("kv_cache_write")
 _read_plans = DevicePlans("kv_cache_read")
+_attention_plans = DevicePlans("attention_cached")
 
 
 class KVCache(NamedTuple):
@@ -159,4 +160,111 @@ def kv_cache_read(cache: KVCache, page_table, lengths, tokens: int, k=None, v=No
     return outs[0], outs[1]
 
 
-__all__ = ["KVCache", "kv_cache_write", "kv_cache_read"]
+class _AttnArgs(ctypes.Structure):
+    _fields_ = [*((n, ctypes.c_void_p) for n in ("q", "k", "v", "k_scale", "v_scale", "table", "lengths", "counts",
+                                                 "out", "lse", "partial", "info")),
+                *((n, ctypes.c_longlong) for n in ("qb", "qh", "qt", "ob", "oh", "ot", "lb", "lh", "lt", "tb")),
+                *((n, ctypes.c_int) for n in ("batch", "heads", "group", "tokens", "page_shift", "pages", "columns",
+                                              "blocks", "programs", "least"))]
+
+
+TILE = 64        # positions of a tile (csrc/wir_pages.h)
+
+
+def _attention_form(rows: int, columns: int, page: int):
+    """(rows of a block, programs, fewest tiles of one) of the kernel for
+    ``rows`` query rows a key/value head over a table of ``columns`` pages;
+    programs 0: one for each sequence, block and head."""
+    block = 16 if rows <= 16 else 32 if rows <= 32 else 128
+    if columns * page <= 8 * TILE:
+        return block, 0, 0
+    return block, 512, 4
+
+
+def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=None, lse=None,
+                     workspace=None) -> Tuple[object, object]:
+    """Attention of new queries ``[B, H, T, D]`` (bf16, H a multiple of the
+    cache's heads) over a paged cache; returns ``(O, LSE)``, bf16 ``[B, H, T, D]`` and
+    fp32 ``[B, H, T]`` (natural log), as ``api.attention_forward``.
+
+    The sequences are as in ``kv_cache_write``, which has put the new tokens'
+    keys and values there: query ``t < counts[b]`` (default T) has position
+    ``lengths[b] - counts[b] + t`` and sees the positions up to its own.  Keys in
+    pages that the cache does not have (-1) are seen by no row.  A row that
+    sees no key (also ``t >= counts[b]``, or a position below 0) gives O = 0 and
+    LSE = -inf.
+
+    The keys of a sequence are divided over the chip by its lengths as they
+    are on the GPU; partial results go through ``workspace`` (fp32, as many
+    elements as ``attention_cached_workspace`` says, allocated if omitted)."""
+    import torch
+
+    fn, done = "attention_cached", None
+    if isinstance(cache, KVCache) and workspace is None:
+        done = _attention_plans.run(0, q, *cache, page_table, lengths, counts, out, lse)
+        if done is not None and done is not False:
+            return done
+    batch, heads, page, d, device = _validate(fn, cache, page_table, lengths, counts)
+    check_tensor(fn, "q", q, torch.bfloat16, (batch, None, None, d), device)
+    h, tokens = q.shape[1:3]
+    need(fn, h > 0 and h % heads == 0, f"{h} query heads are not a multiple of {heads} key/value heads")
+    group = h // heads
+    need(fn, tokens * group <= 1 << 30, "more than 2^30 query rows a key/value head")
+    rec = _attention_plans.recording(done, q, *cache, page_table, lengths, counts, out, lse)
+    if out is None:
+        out = rec.alloc(torch.empty(q.shape, dtype=q.dtype, device=device))
+    if lse is None:
+        lse = rec.alloc(torch.empty(q.shape[:3], dtype=torch.float32, device=device))
+    check_tensor(fn, "out", out, torch.bfloat16, q.shape, device)
+    check_tensor(fn, "lse", lse, torch.float32, q.shape[:3], device, rows=False)
+    for name, x in (("out", out), ("lse", lse)):
+        check_written(fn, name, x)
+    if batch * tokens == 0:
+        return out, lse
+    if page_table.shape[1] == 0:
+        return out.zero_(), lse.fill_(float("-inf"))
+    rows = tokens * group
+    block, programs, least = _attention_form(rows, page_table.shape[1], page)
+    blocks = -(-rows // block)
+    items = batch * blocks * heads
+    need(fn, items * min(rows, block) < 1 << 24, "2^24 query rows or more in one call")
+    args = _AttnArgs(*[None] * 12, *q.stride()[:3], *out.stride()[:3], *lse.stride(), page_table.stride(0), batch, heads,
+                     group, tokens, page.bit_length() - 1, cache.k.shape[0], page_table.shape[1], blocks, programs,
+                     least)
+    floats = _workspace_floats(programs, block, d, items)
+    if floats:
+        if workspace is None:
+            workspace = rec.alloc(torch.empty(floats, dtype=torch.float32, device=device))
+        check_tensor(fn, "workspace", workspace, torch.float32, (None,), device)
+        need(fn, workspace.numel() >= floats, f"workspace needs {floats} elements")
+    else:
+        workspace = None
+    tensors = {"q": q, "k": cache.k, "v": cache.v, "k_scale": cache.k_scale, "v_scale": cache.v_scale,
+               "table": page_table, "lengths": lengths, "counts": counts, "out": out, "lse": lse,
+               "partial": workspace, "info": workspace}
+    past = {"info": 4 * (floats - 2 * items)}
+    launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}", (programs or items, 1, 1), (256, 1, 1),
+           args, tensors, past)
+    if programs:
+        launch(rec, device, "attn_cached.hsaco", f"wir_attn_join_d{d}_r{block}", (items * min(rows, block), 1, 1),
+               (256, 1, 1), args, tensors, past)
+    if rec:
+        _attention_plans.add(0, rec, out, lse)
+    return out, lse
+
+
+def _workspace_floats(programs: int, block: int, d: int, items: int) -> int:
+    """Two slots of a program, each a block's unnormalised rows, maxima and
+    sums, and two words of every (sequence, block, head)."""
+    return 2 * programs * block * (d + 2) + 2 * items if programs else 0
+
+
+def attention_cached_workspace(q, cache: KVCache, page_table) -> int:
+    """Elements that ``attention_cached`` needs of a ``workspace`` for these tensors."""
+    pages, heads, page, d = cache.k.shape
+    rows = q.shape[2] * (q.shape[1] // heads)
+    block, programs, _ = _attention_form(rows, page_table.shape[1], page)
+    return _workspace_floats(programs, block, d, q.shape[0] * -(-rows // block) * heads)
+
+
+__all__ = ["KVCache", "kv_cache_write", "kv_cache_read", "attention_cached", "attention_cached_workspace"]
