@@ -97,16 +97,17 @@ static void division() {
       i64 base = 0;
       while (u >= base + (i64)heads * units[pair]) base += (i64)heads * units[pair++];
       while (u < end) {
-        const Segment g = segment_at(u, base, units[pair], end);
+        const Segment g = segment_at(u, base, units[pair], end, share);
         CHECK(g.head >= 0 && g.head < heads && g.first >= 0 && g.first < g.last && g.last <= units[pair]);
         const std::pair<int, int> item(pair, g.head);
         for (int t = g.first; t < g.last; ++t) covered[item].push_back(t);
-        const int slot = slot_of(u, share);
+        const int slot = g.slot;
         if (!g.whole) {
           CHECK(slot >= 0 && slot < 2 * programs && slot / 2 == w && used.insert(slot).second);
           slots[item].push_back(slot);
         }
-        if (g.first == 0) info[item] = {slot, g.whole ? 1 : parts_of(u, units[pair], share)};
+        CHECK(g.whole == (g.parts == 1));
+        if (g.first == 0) info[item] = {slot, g.parts};
         u += g.last - g.first;
         if (u == base + (i64)heads * units[pair]) base = u, ++pair;
       }
@@ -121,8 +122,36 @@ static void division() {
         const int parts = info[item].second;
         if (slots[item].empty()) { CHECK(parts == 1); continue; }
         CHECK(parts == (int)slots[item].size());
-        for (int i = 0; i < parts; ++i) CHECK(slot_of_part(info[item].first, i) == slots[item][i]);
+        for (int i = 0; i < parts; ++i) CHECK(slot_of_part(info[item].first, i, false) == slots[item][i]);
       }
+  }
+}
+
+// The same in equal parts of single heads.
+static void even_division() {
+  for (int it = 0; it < 20000; ++it) {
+    const int pairs = draw(1, 12), heads = draw(1, 5), least = draw(1, 9), programs = pairs * heads + draw(1, 90);
+    std::vector<int> units(pairs);
+    for (int& n : units) n = draw(0, 9) ? draw(1, 30) : draw(1, 4000);
+    i64 total = 0;
+    for (int n : units) total += (i64)heads * n;
+    const i64 share = share_even(total, programs, pairs * heads, least);
+    int base = 0;
+    for (int p = 0; p < pairs; ++p) {
+      const int parts = parts_even(units[p], share);
+      for (int h = 0; h < heads; ++h)
+        for (int n = 0, next = 0; n < parts; ++n) {
+          const int w = base + h * parts + n;
+          const Segment g = segment_even(w, base, units[p], share);
+          CHECK(g.head == h && g.first == next && g.last > g.first && g.last - g.first <= share);
+          CHECK(g.parts == parts && g.whole == (parts == 1) && g.slot == w);
+          CHECK(slot_of_part(base + h * parts, n, true) == w);
+          next = g.last;
+          CHECK(n + 1 < parts || next == units[p]);
+        }
+      base += heads * parts;
+    }
+    CHECK(base <= programs);
   }
 }
 
@@ -131,6 +160,7 @@ int main() {
   keys();
   scales();
   division();
+  even_division();
   std::puts("ok");
 }
 """

@@ -4,9 +4,17 @@
 // A token's key is k = code * ks and its value v = code * vs, ks and vs one
 // scale for each page and head.  For query row r at position p:
 //   s_j = q . code_j * ks / sqrt(D) for j <= p,  O = sum_j softmax(s)_j vs code_j.
-// The scales stay out of the products: ks multiplies a score, vs a
-// probability (before its rounding to bf16), and e4m3 codes are exact in bf16,
-// so the products run on v_mfma_f32_16x16x32_bf16 with codes as they are.
+//
+// First product: the codes go to v_mfma_f32_16x16x128_f8f6f4 as they are.  A
+// query row is written as 2^e (hi + lo) with two e4m3 terms, which hold bf16's
+// 8 bits of fraction (hi rounds to 4 of them, the rest has 4 more); what is
+// lost lies below 2^-19 of the row's largest value.  Two terms at twice the
+// bf16 rate cost what bf16 would, without converting K.  The scales and 2^e
+// multiply the fp32 score.
+//
+// Second product: codes times the power of two vs are exact in bf16, one
+// instruction for two values (what a scale has beside its power of two goes
+// to the probability), and probabilities are rounded to bf16 once.
 //
 // Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, with 16
 // query rows (the heads that share a key/value head, and the new tokens) as
@@ -14,28 +22,30 @@
 // 64-token tile are turned into the second product's operand without leaving
 // the lane: the rows of K go to the matrix core in an order that gives lane
 // group g (16 lanes) the tokens 16 g .. 16 g + 15.  V pages are [D, token], so
-// that operand's other side is 16 contiguous bytes of one column.  K and V
-// come from memory straight into registers, every byte once, with no LDS and
-// no barrier in the loop: K of the next tile is in flight during the softmax
-// and the second product, V during the next tile's first product.
+// that operand's other side is 16 contiguous bytes of one column.
 //
-// What bounds it: the cache's bytes for few rows (a decode step).
-#include <hip/hip_runtime.h>
-
+// Few rows (16 or 32 of a key/value head): K and V come from memory straight
+// into registers, every byte once, with no LDS and no barrier in the loop; a
+// workgroup's waves take every WK-th tile and are joined at the end.  Bound by
+// the cache's bytes.
+// Many rows: a workgroup's waves take 32 rows each and share the tiles, which
+// LDS-DMA brings in the lanes' operand order (a fragment is 64 consecutive
+// 16-byte chunks), one tile ahead.
+#include "wir_cdna4.h"
 #include "wir_pages.h"
 
 namespace {
 
 using wir::i64;
+using wir::bf16;
+using wir::bf16x8;
+using wir::f32x4;
 
-typedef __bf16 bf16;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-constexpr int WAVES = 4;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct attn_args {
@@ -54,15 +64,20 @@ struct attn_args {
   i64 qb, qh, qt, ob, oh, ot, lb, lh, lt, tb;
   int batch, heads, group, tokens, page_shift, pages, columns;
   int blocks;                  // row blocks of a sequence and head
-  int programs, least;         // 0: one program for each (sequence, block, head)
+  int programs;                // 0: one for each (sequence, block, head)
+  int least;                   // > 0: equal parts of single heads, of that many tiles at least
+  int slots;                   // of partial results
 };
 
-// The eight codes of two words in bf16 (exact).
-__device__ __forceinline__ bf16x8 unpack8(unsigned a, unsigned b) {
-  const bf16x2 w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
-  const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
-  const bf16x2 y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
-  const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+// (by value: a bit cast of a vector's element in place gives element 0)
+__device__ __forceinline__ unsigned bits_of(bf16 x) { return (unsigned)__builtin_bit_cast(unsigned short, x); }
+
+// The eight codes of two words, times a power of two, in bf16 (exact).
+__device__ __forceinline__ bf16x8 unpack8(unsigned a, unsigned b, float scale) {
+  const bf16x2 w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false);
+  const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true);
+  const bf16x2 y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false);
+  const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true);
   return bf16x8{w[0], w[1], x[0], x[1], y[0], y[1], z[0], z[1]};
 }
 
@@ -75,34 +90,50 @@ __device__ __forceinline__ float over_groups(float x, F op) {
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// One of a sequence's row blocks of one head, over some of its tiles.
-template <int D, int NQ, int WR>
+// Inclusive sums over the lanes of a wave.
+__device__ __forceinline__ i64 wave_scan(i64 x) {
+  const int lane = wir::lane_id();
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const i64 y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// One of a sequence's row blocks of one head, over some of its tiles: W waves, of 16 * NQ rows each, WR side by side
+// and the others dividing the tiles.
+template <int D, int NQ, int WR, int W>
 struct Program {
-  static constexpr int WK = WAVES / WR;          // waves that divide the tiles
+  static constexpr int WK = W / WR;              // waves that divide the tiles
+  static constexpr bool SHARED = WR > 1;         // tiles go through LDS
   static constexpr int ROWS = 16 * NQ;           // query rows of a wave
   static constexpr int BLOCK = ROWS * WR;        // and of the workgroup
   static constexpr int KC = D / 64, DT = D / 16, PITCH = D + 4;
+  static constexpr int CHUNKS = 4 * KC + DT;     // 1 KiB fragments of a tile
+  static_assert(!SHARED || (WK == 1 && CHUNKS % (2 * W) == 0), "");
 
-  struct Shared {
-    float o[WAVES * ROWS * PITCH];
-    float ml[WAVES * ROWS * 2];
-    i64 scan[256];
-    i64 found_base;
-    int found;
+  struct Results {
+    float o[W * ROWS * PITCH];
+    float ml[W * ROWS * 2];
+  };
+  union Shared {
+    Results r;
+    char ring[SHARED ? 2 * CHUNKS * 1024 : 16];
   };
 
   const attn_args& a;
   Shared& sh;
-  int lane, col, grp, wr, wk;
+  int lane, col, grp, wave, wr, wk;
   // the pair's
   int b, rb;
   wir::Span span;
 
   __device__ __forceinline__ Program(const attn_args& args, Shared& shared) : a(args), sh(shared) {
-    lane = threadIdx.x % 64;
+    lane = wir::lane_id();
     col = lane % 16;
     grp = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    wave = wir::wave_id();
     wr = wave % WR;
     wk = wave / WR;
   }
@@ -122,59 +153,221 @@ struct Program {
     return r < rows() && t < span.count ? max(span.start + t, -1) : -1;
   }
 
-  struct Page {      // of a lane's 16 tokens of a tile
-    int k, v;        // ids for the K operand's rows and for the scores and V, -1: none
+  // A wave's running softmax and output, and its queries as operands.
+  struct State {
+    i32x8 q[NQ][KC];      // D = 128: hi, lo of the 32 values of a lane; D = 64: both, 16 values each
+    float qs[NQ];         // 2^e log2(e) / sqrt(D)
+    int pos[NQ];
+    int low;              // no row that sees anything sees less
+    f32x4 o[DT][NQ];
+    float m[NQ], l[NQ];
   };
 
-  __device__ __forceinline__ Page pages_of(int tile) const {
-    const int* row = a.table + b * a.tb;
-    const int tk = tile * wir::TILE + 16 * (col / 4), tv = tile * wir::TILE + 16 * grp;
-    Page p;
-    p.k = tk < span.held ? row[tk >> a.page_shift] : -1;
-    p.v = tv < span.held ? row[tv >> a.page_shift] : -1;
-    return p;
-  }
+  // The lane's 16 tokens of a tile.
+  struct Tokens {
+    float ks, vs;
+    int have;             // how many the sequence holds
+  };
 
-  // Tiles first .. last - 1 of `head`; -> sh.o, sh.ml.
-  __device__ __forceinline__ void walk(int head, int first, int last) {
-    const int mask = (1 << a.page_shift) - 1;
-    const float c = (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));   // log2(e) / sqrt(D)
+  __device__ __forceinline__ void begin(State& s, int head) const {
+    const float c = (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));
     const int row0 = rb * BLOCK + wr * ROWS;
-    // q: the operand's k order is that of K's 16-byte loads
-    bf16x8 q[NQ][2 * KC];
-    int pos[NQ];
+    s.low = max(span.start + min(row0 / a.group, span.count), 0);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int r = row0 + n * 16 + col;
-      pos[n] = position(r);
+      s.pos[n] = position(r);
       const int rr = r < rows() ? r : 0, t = rr / a.group;
       const bf16* p = a.q + b * a.qb + (i64)(head * a.group + rr - t * a.group) * a.qh + t * a.qt + 16 * grp;
+      bf16x8 x[2 * KC];
+      unsigned top = 0;
 #pragma unroll
-      for (int u = 0; u < 2 * KC; ++u) q[n][u] = *(const bf16x8*)(p + u / 2 * 64 + u % 2 * 8);
+      for (int u = 0; u < 2 * KC; ++u) x[u] = *(const bf16x8*)(p + u / 2 * 64 + u % 2 * 8);
+#pragma unroll
+      for (int u = 0; u < 2 * KC; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned y = bits_of(x[u][e]) & 0x7fffu;
+          top = max(top, y < 0x7f80u ? y : 0u);
+        }
+      const float amax = over_groups(__uint_as_float(top << 16), [](float y, float z) { return fmaxf(y, z); });
+      const float scale = __uint_as_float(wir::scale_bits(__float_as_uint(amax))), inv = 1.0f / scale;
+      s.qs[n] = scale * c;
+#pragma unroll
+      for (int w = 0; w < 4 * KC; ++w) {   // words of 4 values
+        float y[4], z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = (float)x[w / 2][w % 2 * 4 + e] * inv;
+          if (!(__builtin_fabsf(y[e]) < __builtin_inff())) y[e] = __builtin_nanf("");
+        }
+        unsigned hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0u, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], hi, true);
+        const f32x2 h0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), h1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+        z[0] = y[0] - h0[0], z[1] = y[1] - h0[1], z[2] = y[2] - h1[0], z[3] = y[3] - h1[1];
+        unsigned lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0u, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
+        s.q[n][0][w] = hi;
+        if (KC == 2)
+          s.q[n][1 % KC][w] = lo;
+        else
+          s.q[n][0][4 + w % 4] = lo;
+      }
+      s.m[n] = -__builtin_inff(), s.l[n] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) s.o[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int low = max(span.start + min(row0 / a.group, span.count), 0);   // no row that sees anything sees less
-    f32x4 o[DT][NQ];
-    float m[NQ], l[NQ];
+  }
+
+  // One tile: key(j) the K operand of tokens 16 g + 4 j .. + 3, value(d) the V words of column 16 d + col, read() once
+  // the keys are used.
+  template <class Key, class Value, class Read>
+  __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Value value, Read read) const {
+    f32x4 x[4][NQ];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const i32x8 kf = key(j);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        x[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < KC; ++u)
+          x[j][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, s.q[n][u], x[j][n], 0, 0, 0, 127, 0, 127);
+      }
+    }
+    const int at = t * wir::TILE + 16 * grp;   // the lane's tokens: at .. at + have - 1
+    const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
+    read();
+    // vs = 2^e g; a scale that is no positive normal number is all g
+    const unsigned bits = __float_as_uint(k.vs), exponent = bits & 0x7f800000u;
+    const bool normal = bits < 0x7f800000u && exponent != 0;
+    const float power = normal ? __uint_as_float(exponent) : 1.f;
+    const float g = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : k.vs;
+    const bool plain = __builtin_amdgcn_ballot_w64(g != 1.f) == 0;
+    bf16x8 p[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      m[n] = -__builtin_inff(), l[n] = 0.f;
+      float f = k.ks * s.qs[n];
+      if (edge) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[j][n][i] = 4 * j + i < k.have && at + 4 * j + i <= s.pos[n] ? x[j][n][i] * f : -__builtin_inff();
+        f = 1.f;
+      }
+      float top = x[0][n][0];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[j][n][i]);
+      top = fmaxf(over_groups(top * f, [](float y, float z) { return fmaxf(y, z); }), s.m[n]);
+      const float base = top == -__builtin_inff() ? 0.f : top;
+      const float corr = __builtin_amdgcn_exp2f(s.m[n] - base);
+      s.m[n] = top;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][n][i], f, -base));
+          sum[i % 2] += y;
+          // (a key that the row does not see adds nothing, whatever its scale is)
+          p[n][j / 2][j % 2 * 4 + i] = (bf16)(plain ? y : edge && x[j][n][i] == -__builtin_inff() ? 0.f : y * g);
+        }
+      s.l[n] = s.l[n] * corr + (sum[0] + sum[1]);
+      if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) s.o[d][n] *= corr;
+      }
     }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      u32x4 v = value(d);
+      if (edge) edge_value(s, d, v, k.have, at);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8 w = unpack8(v[2 * u], v[2 * u + 1], power);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s.o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, p[n][u], s.o[d][n], 0, 0, 0);
+      }
+    }
+  }
 
+  // Values of a tile that not all rows see: bytes past the sequence's end
+  // become 0 (0 * NaN is NaN in the product), and so do NaN codes, which
+  // instead make NaN of exactly the rows that see them, by a product of
+  // where they are with who sees them.
+  __device__ __forceinline__ void edge_value(State& s, int d, u32x4& v, int have, int at) const {
+    unsigned some = 0;
+    u32x4 is;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int n = min(max(have - 4 * w, 0), 4);
+      const unsigned x = v[w] & (n == 4 ? ~0u : (1u << 8 * n) - 1);
+      const unsigned high = ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // of bytes 0x7f and 0xff
+      some |= high;
+      const unsigned bytes = (high >> 7) * 0xffu;
+      v[w] = x & ~bytes;
+      is[w] = bytes & 0x38383838u;   // 1.0 in e4m3
+    }
+    if (__builtin_amdgcn_ballot_w64(some != 0) == 0) return;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      f32x4 count = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        bf16x8 sees;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sees[e] = (bf16)(8 * u + e < have && at + 8 * u + e <= s.pos[n] ? 1.f : 0.f);
+        count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(unpack8(is[2 * u], is[2 * u + 1], 1.f), sees, count, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (count[i] > 0.f) s.o[d][n][i] = __builtin_nanf("");
+    }
+  }
+
+  // Page id of the tile's 16-token segment `seg`; -1 past the sequence.
+  __device__ __forceinline__ int page_of(int t, int seg) const {
+    const int at = t * wir::TILE + 16 * seg;
+    return at < span.held ? a.table[b * a.tb + (at >> a.page_shift)] : -1;
+  }
+  // The lane's own segment of it (its V operand and scores).
+  __device__ __forceinline__ void scales_of(Tokens& k, int t, int page, int head) const {
+    const int id = wir::checked_page(page, a.pages);
+    const i64 at = (i64)max(id, 0) * a.heads + head;
+    k.have = id < 0 ? 0 : min(max(span.held - (t * wir::TILE + 16 * grp), 0), 16);
+    k.ks = a.k_scale[at];
+    k.vs = a.v_scale[at];
+    if (id < 0) k.ks = k.vs = 1.f;
+  }
+  // A page that is none is read as page 0, and its tokens masked.
+  __device__ __forceinline__ const unsigned char* key_at(int t, int page, int head) const {
+    const i64 at = (i64)max(wir::checked_page(page, a.pages), 0) * a.heads + head;
+    const int in_page = (t * wir::TILE + 16 * (col / 4)) & ((1 << a.page_shift) - 1);
+    return a.k + ((at << a.page_shift) + in_page + col % 4) * D + 16 * grp;
+  }
+  __device__ __forceinline__ const unsigned char* value_at(int t, int page, int head) const {
+    const i64 at = (i64)max(wir::checked_page(page, a.pages), 0) * a.heads + head;
+    const int in_page = (t * wir::TILE + 16 * grp) & ((1 << a.page_shift) - 1);
+    return a.v + ((at * D + col) << a.page_shift) + in_page;
+  }
+
+  static __device__ __forceinline__ i32x8 key_operand(const u32x4& x, const u32x4& y) {
+    return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+  }
+
+  // Tiles first .. last - 1 of `head`, every WK-th from the wave's, through registers: K of the next tile is in
+  // flight during the softmax and the second product, V during the next tile's first product.
+  __device__ __forceinline__ void walk_registers(State& s, int head, int first, int last) const {
     u32x4 kf[4][KC], vf[DT];
-    float ks, vs;
-    int there;               // of the lane group's 16 tokens, how many the sequence holds
+    Tokens tok;
     const unsigned char* vp;
-    auto load_k = [&](int tile, const Page& p) {
-      const int tk = tile * wir::TILE + 16 * (col / 4), tv = tile * wir::TILE + 16 * grp;
-      const int ik = max(wir::checked_page(p.k, a.pages), 0), iv = wir::checked_page(p.v, a.pages);
-      there = iv < 0 ? 0 : min(max(span.held - tv, 0), 16);
-      const i64 index_k = (i64)ik * a.heads + head, index_v = (i64)max(iv, 0) * a.heads + head;
-      ks = iv < 0 ? 0.f : a.k_scale[index_v] * c;
-      vs = iv < 0 ? 0.f : a.v_scale[index_v];
-      const unsigned char* kp = a.k + ((index_k << a.page_shift) + (tk & mask) + col % 4) * D + 16 * grp;
-      vp = a.v + (((index_v * D) + col) << a.page_shift) + (tv & mask);
+    auto load_k = [&](int t, int page_k, int page_v) {
+      scales_of(tok, t, page_v, head);
+      const unsigned char* kp = key_at(t, page_k, head);
+      vp = value_at(t, page_v, head);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -184,153 +377,104 @@ struct Program {
 #pragma unroll
       for (int d = 0; d < DT; ++d) vf[d] = *(const u32x4*)(vp + ((i64)(16 * d) << a.page_shift));
     };
-
-    int t = first + wk;
-    Page next;
+    int t = first + wk, next_k = -1, next_v = -1;
     if (t < last) {
-      load_k(t, pages_of(t));
-      if (t + WK < last) next = pages_of(t + WK);
+      load_k(t, page_of(t, col / 4), page_of(t, grp));
+      if (t + WK < last) next_k = page_of(t + WK, col / 4), next_v = page_of(t + WK, grp);
       load_v();
     }
+    begin(s, head);
     for (; t < last; t += WK) {
-      f32x4 s[4][NQ];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) s[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < 2 * KC; ++u) {
-          const bf16x8 k = unpack8(kf[j][u / 2][u % 2 * 2], kf[j][u / 2][u % 2 * 2 + 1]);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) s[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[n][u], s[j][n], 0, 0, 0);
-        }
-      }
-      const float f = ks, g = vs;
-      const int have = there, at = t * wir::TILE + 16 * grp;   // the lane group's tokens at .. at + have - 1
-      const bool edge = __builtin_amdgcn_ballot_w64(have < 16 || at + 15 > low) != 0;
-      if (t + WK < last) {   // kf is read: the next tile's keys
-        const Page p = next;
-        if (t + 2 * WK < last) next = pages_of(t + 2 * WK);
-        load_k(t + WK, p);
-      }
-      bf16x8 pb[NQ][2];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float top = m[n];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = s[j][n][i] * f;
-            if (edge) x = 4 * j + i < have && at + 4 * j + i <= pos[n] ? x : -__builtin_inff();
-            s[j][n][i] = x;
-            top = fmaxf(top, x);
-          }
-        top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
-        const float base = top == -__builtin_inff() ? 0.f : top;
-        const float corr = __builtin_amdgcn_exp2f(m[n] - base);
-        m[n] = top;
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = __builtin_amdgcn_exp2f(s[j][n][i] - base);
-            sum += p;
-            // a key that the row does not see adds nothing, whatever its scale is
-            pb[n][j / 2][j % 2 * 4 + i] = (bf16)(edge && s[j][n][i] == -__builtin_inff() ? 0.f : p * g);
-          }
-        l[n] = l[n] * corr + sum;
-        if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[d][n] *= corr;
-        }
-      }
-      if (edge) edge_values(vf, o, have, at, pos);
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bf16x8 v = unpack8(vf[d][2 * u], vf[d][2 * u + 1]);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[n][u], o[d][n], 0, 0, 0);
-        }
+      const Tokens now = tok;
+      tile(s, t, now, [&](int j) { return key_operand(kf[j][0], kf[j][KC - 1]); }, [&](int d) { return vf[d]; },
+           [&]() {
+             if (t + WK >= last) return;
+             const int page_k = next_k, page_v = next_v;
+             if (t + 2 * WK < last) next_k = page_of(t + 2 * WK, col / 4), next_v = page_of(t + 2 * WK, grp);
+             load_k(t + WK, page_k, page_v);
+           });
       if (t + WK < last) load_v();
-    }
-
-    const int wave = wk * WR + wr;
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const float sum = over_groups(l[n], [](float x, float y) { return x + y; });
-      const int row = wave * ROWS + n * 16 + col;
-      if (grp == 0) sh.ml[2 * row] = m[n], sh.ml[2 * row + 1] = sum;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) *(f32x4*)(sh.o + row * PITCH + 16 * d + 4 * grp) = o[d][n];
     }
   }
 
-  // Values of a tile that not all rows see: bytes past the sequence's end
-  // become 0 (0 * NaN is NaN in the product), and so do NaN codes, which
-  // instead make NaN of exactly the rows that see them, by a product of
-  // where they are with who sees them.
-  __device__ __forceinline__ void edge_values(u32x4 (&vf)[DT], f32x4 (&o)[DT][NQ], int have, int at, const int (&pos)[NQ]) {
-    unsigned keep[4], some = 0;
+  // The same through LDS, every tile for all waves: a wave brings CHUNKS / W of a tile's fragments, the first half of
+  // the waves K's, the others V's.  Everything asked for in one iteration is there in the next.
+  __device__ __forceinline__ void walk_shared(State& s, int head, int first, int last) const {
+    constexpr int MINE = CHUNKS / W;
+    const bool mine_k = wave < W / 2;
+    const int mine = wave * MINE, seg = mine_k ? col / 4 : grp;
+    auto bring = [&](int t, int slot, int page) {
+      const unsigned char* from = mine_k ? key_at(t, page, head) : value_at(t, page, head);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int n = min(max(have - 4 * w, 0), 4);
-      keep[w] = n == 4 ? ~0u : (1u << 8 * n) - 1;
+      for (int i = 0; i < MINE; ++i) {
+        const int c = mine + i;
+        const i64 off = mine_k ? (i64)(4 * (c / KC) * D + 64 * (c % KC)) : (i64)(16 * (c - 4 * KC)) << a.page_shift;
+        wir::dma16_v(from + off, wir::lds_addr(sh.ring + (slot * CHUNKS + c) * 1024));
+      }
+    };
+    Tokens tok;
+    int next = -1, next_own = -1, slot = 0;
+    if (first < last) {
+      const int page = page_of(first, seg), own = page_of(first, grp);
+      bring(first, 0, page);
+      scales_of(tok, first, own, head);
+      if (first + 1 < last) next = page_of(first + 1, seg), next_own = page_of(first + 1, grp);
     }
-    u32x4 is[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const unsigned x = vf[d][w] & keep[w];
-        const unsigned high = ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // of bytes 0x7f and 0xff
-        some |= high;
-        const unsigned bytes = (high >> 7) * 0xffu;
-        vf[d][w] = x & ~bytes;
-        is[d][w] = bytes & 0x38383838u;   // 1.0 in e4m3
+    begin(s, head);
+    for (int t = first; t < last; ++t, slot ^= 1) {
+      wir::wait_vm_barrier<0>();
+      // loaded before the wait: no later wait for them, which would count the transfers that follow
+      asm volatile("" : "+v"(tok.ks), "+v"(tok.vs), "+v"(next), "+v"(next_own));
+      const Tokens now = tok;
+      if (t + 1 < last) {
+        bring(t + 1, slot ^ 1, next);
+        scales_of(tok, t + 1, next_own, head);
+        if (t + 2 < last) next = page_of(t + 2, seg), next_own = page_of(t + 2, grp);
       }
-    if (__builtin_amdgcn_ballot_w64(some != 0) == 0) return;
-    bf16x8 sees[NQ][2];
+      typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+      const lds_u32x4* from = (const lds_u32x4*)wir::lds(sh.ring + slot * CHUNKS * 1024) + lane;
+      tile(s, t, now, [&](int j) { return key_operand(from[j * KC * 64], from[(j * KC + KC - 1) * 64]); },
+           [&](int d) { return (u32x4)from[(4 * KC + d) * 64]; }, []() {});
+    }
+    __syncthreads();   // the ring is read: results go there
+  }
+
+  // Tiles first .. last - 1 of `head` -> sh.r
+  __device__ __forceinline__ void walk(int head, int first, int last) {
+    State s;
+    if constexpr (SHARED)
+      walk_shared(s, head, first, last);
+    else
+      walk_registers(s, head, first, last);
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int n = 0; n < NQ; ++n) {
+      const float sum = over_groups(s.l[n], [](float x, float y) { return x + y; });
+      const int row = wave * ROWS + n * 16 + col;
+      if (grp == 0) sh.r.ml[2 * row] = s.m[n], sh.r.ml[2 * row + 1] = sum;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sees[n][e / 8][e % 8] = (bf16)(e < have && at + e <= pos[n] ? 1.f : 0.f);
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        f32x4 count = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(unpack8(is[d][2 * u], is[d][2 * u + 1]), sees[n][u], count, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (count[i] > 0.f) o[d][n][i] = __builtin_nanf("");
-      }
+      for (int d = 0; d < DT; ++d) *(f32x4*)(sh.r.o + row * PITCH + 16 * d + 4 * grp) = s.o[d][n];
+    }
   }
 
   // The waves' results of a block, joined: the outputs, or the partial result of `slot`.
   __device__ __forceinline__ void store(int head, int slot) {
     constexpr int CH = D / 8;
     const int left = min(rows() - rb * BLOCK, BLOCK);
-    for (int idx = threadIdx.x; idx < left * CH; idx += 256) {
+    for (int idx = threadIdx.x; idx < left * CH; idx += 64 * W) {
       const int row = idx / CH, ch = idx % CH;
       float top = -__builtin_inff();
 #pragma unroll
-      for (int w = 0; w < WK; ++w) top = fmaxf(top, sh.ml[2 * (w * BLOCK + row)]);
+      for (int w = 0; w < WK; ++w) top = fmaxf(top, sh.r.ml[2 * (w * BLOCK + row)]);
       const float base = top == -__builtin_inff() ? 0.f : top;
       float sum = 0.f;
       f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
 #pragma unroll
       for (int w = 0; w < WK; ++w) {
         const int at = w * BLOCK + row;
-        const float f = __builtin_amdgcn_exp2f(sh.ml[2 * at] - base);
-        sum += f * sh.ml[2 * at + 1];
-        x += f * *(const f32x4*)(sh.o + at * PITCH + 8 * ch);
-        y += f * *(const f32x4*)(sh.o + at * PITCH + 8 * ch + 4);
+        const float f = __builtin_amdgcn_exp2f(sh.r.ml[2 * at] - base);
+        sum += f * sh.r.ml[2 * at + 1];
+        x += f * *(const f32x4*)(sh.r.o + at * PITCH + 8 * ch);
+        y += f * *(const f32x4*)(sh.r.o + at * PITCH + 8 * ch + 4);
       }
       if (position(rb * BLOCK + row) < 0) {   // it took part in tiles that every row with a position sees
         top = -__builtin_inff(), sum = 0.f;
@@ -341,7 +485,7 @@ struct Program {
         *(f32x4*)to = x;
         *(f32x4*)(to + 4) = y;
         if (ch == 0)
-          *(f32x2*)(a.partial + (i64)2 * a.programs * BLOCK * D + ((i64)slot * BLOCK + row) * 2) = f32x2{top, sum};
+          *(f32x2*)(a.partial + (i64)a.slots * BLOCK * D + ((i64)slot * BLOCK + row) * 2) = f32x2{top, sum};
       } else {
         put(a, b, head, rb * BLOCK + row, ch, x, y, top, sum);
       }
@@ -363,65 +507,78 @@ struct Program {
           sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 
-  __device__ __forceinline__ void segment(int pair, int keys, const wir::Segment& g, i64 share) {
+  __device__ __forceinline__ void segment(int pair, int keys, const wir::Segment& g) {
     b = pair / a.blocks;
     rb = pair % a.blocks;
     span = span_at(b);
     walk(g.head, g.first, min(g.last, (int)(((i64)keys + wir::TILE - 1) / wir::TILE)));
     __syncthreads();
-    const int slot = g.whole ? -1 : wir::slot_of(g.begin, share);
     if (threadIdx.x == 0 && a.programs && g.first == 0) {
       int* info = a.info + 2 * ((i64)pair * a.heads + g.head);
-      info[0] = slot;
-      info[1] = g.whole ? 1 : wir::parts_of(g.begin, wir::block_units(keys), share);
+      info[0] = g.slot;
+      info[1] = g.parts;
     }
-    store(g.head, slot);
+    store(g.head, g.whole ? -1 : g.slot);
     __syncthreads();
   }
 
+  // The pair in which item u lies, of `own` items of this lane's pairs from .. and as many as `weight` says of each,
+  // and the items before the pair.  All lanes get them; false: there are no u items.
+  template <class Weight>
+  __device__ __forceinline__ bool find(i64 u, i64 own, int from, int each, Weight weight, int& pair, i64& base) const {
+    const i64 upto = wave_scan(own);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(u < upto);
+    if (past == 0) return false;
+    const int src = __builtin_ctzll(past);
+    i64 before = upto - own;
+    int p = from;
+    if (lane == src && each > 1) {
+      for (;; ++p) {
+        const i64 n = weight(p);
+        if (u < before + n) break;
+        before += n;
+      }
+    }
+    pair = __builtin_amdgcn_readfirstlane(__shfl(p, src));
+    base = __shfl(before, src);
+    return true;
+  }
+
   __device__ __forceinline__ void run() {
-    const int pairs = a.batch * a.blocks;
-    if (!a.programs) {
-      const int pair = blockIdx.x / a.heads, keys = keys_at(pair);
-      segment(pair, keys, wir::Segment{(int)(blockIdx.x % a.heads), 0, wir::block_units(keys), 0, true}, 1);
+    if (!a.programs) {   // a head's blocks, the longest first, next to one another on one XCD
+      const int id = wir::remap_xcd(blockIdx.x, gridDim.x), item = id / a.blocks;
+      const int pair = item / a.heads * a.blocks + a.blocks - 1 - id % a.blocks, keys = keys_at(pair);
+      segment(pair, keys, wir::Segment{item % a.heads, 0, wir::block_units(keys), true, -1, 1});
       return;
     }
-    // units before every thread's pairs
-    const int each = (pairs + 255) / 256, from = threadIdx.x * each;
+    // every wave for itself: a lane takes `each` pairs
+    const int pairs = a.batch * a.blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
+    auto units = [&](int p) { return (i64)a.heads * wir::block_units(keys_at(p)); };
     i64 own = 0;
-    for (int p = from; p < min(from + each, pairs); ++p) own += (i64)a.heads * wir::block_units(keys_at(p));
-    sh.scan[threadIdx.x] = own;
-    __syncthreads();
-    for (int d = 1; d < 256; d *= 2) {
-      const i64 x = threadIdx.x >= d ? sh.scan[threadIdx.x - d] : 0;
-      __syncthreads();
-      sh.scan[threadIdx.x] += x;
-      __syncthreads();
+    for (int p = from; p < to; ++p) own += units(p);
+    const i64 total = __shfl(wave_scan(own), 63);
+    int pair;
+    i64 base;
+    if (a.least) {
+      const i64 share = wir::share_even(total, a.programs, pairs * a.heads, a.least);
+      auto parts = [&](int p) { return (i64)a.heads * wir::parts_even(wir::block_units(keys_at(p)), share); };
+      own = 0;
+      for (int p = from; p < to; ++p) own += parts(p);
+      if (!find(blockIdx.x, own, from, each, parts, pair, base)) return;
+      const int keys = keys_at(pair);
+      segment(pair, keys, wir::segment_even(blockIdx.x, (int)base, wir::block_units(keys), share));
+      return;
     }
-    const i64 total = sh.scan[255], share = wir::share_of(total, a.programs, a.least);
+    const i64 share = wir::share_of(total, a.programs, 1);
     i64 u = (i64)blockIdx.x * share;
-    if (u >= total) return;
+    if (!find(u, own, from, each, units, pair, base)) return;
     const i64 end = u + share < total ? u + share : total;
-    i64 base = sh.scan[threadIdx.x] - own;
-    if (base <= u && u < base + own) {
-      int p = from;
-      for (;; ++p) {
-        const i64 n = (i64)a.heads * wir::block_units(keys_at(p));
-        if (u < base + n) break;
-        base += n;
-      }
-      sh.found = p;
-      sh.found_base = base;
-    }
-    __syncthreads();
-    int pair = sh.found;
-    base = sh.found_base;
     while (u < end) {
-      const int keys = keys_at(pair), units = wir::block_units(keys);
-      const wir::Segment g = wir::segment_at(u, base, units, end);
-      segment(pair, keys, g, share);
+      const int keys = keys_at(pair), n = wir::block_units(keys);
+      const wir::Segment g = wir::segment_at(u, base, n, end, share);
+      segment(pair, keys, g);
       u += g.last - g.first;
-      if (u == base + (i64)a.heads * units) base = u, ++pair;
+      if (u == base + (i64)a.heads * n) base = u, ++pair;
     }
   }
 };
@@ -440,9 +597,9 @@ __device__ __forceinline__ void join(const attn_args& a) {
   if (r >= a.tokens * a.group) return;
   const int slot = a.info[2 * (i64)item], parts = a.info[2 * (i64)item + 1];
   if (parts <= 1) return;
-  const f32x2* ml = (const f32x2*)(a.partial + (i64)2 * a.programs * BLOCK * D);
+  const f32x2* ml = (const f32x2*)(a.partial + (i64)a.slots * BLOCK * D);
   float top = -__builtin_inff();
-  for (int p = threadIdx.x; p < parts; p += 256) top = fmaxf(top, ml[(i64)wir::slot_of_part(slot, p) * BLOCK + row][0]);
+  for (int p = threadIdx.x; p < parts; p += 256) top = fmaxf(top, ml[(i64)wir::slot_of_part(slot, p, a.least > 0) * BLOCK + row][0]);
   tops[threadIdx.x] = top;
   __syncthreads();
   for (int d = 128; d; d /= 2) {
@@ -456,7 +613,7 @@ __device__ __forceinline__ void join(const attn_args& a) {
   float l = 0.f;
 #pragma unroll 4
   for (int p = w; p < parts; p += PER) {
-    const i64 at = (i64)wir::slot_of_part(slot, p) * BLOCK + row;
+    const i64 at = (i64)wir::slot_of_part(slot, p, a.least > 0) * BLOCK + row;
     const f32x2 y = ml[at];
     const float f = __builtin_amdgcn_exp2f(y[0] - base);
     l += f * y[1];
@@ -473,26 +630,26 @@ __device__ __forceinline__ void join(const attn_args& a) {
     hi += sums[i * CH + 2 * threadIdx.x + 1];
     l += ls[i];
   }
-  Program<D, BLOCK / 16, 1>::put(a, b, head, r, threadIdx.x, lo, hi, top, l);
+  Program<D, 1, 1, 1>::put(a, b, head, r, threadIdx.x, lo, hi, top, l);
 }
 
 }  // namespace
 
-#define ATTN_KERNEL(NAME, D, NQ, WR, OCC)                                                                        \
-  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(OCC, OCC))) \
-  NAME(const attn_args args) {                                                                                   \
-    __shared__ __attribute__((aligned(16))) Program<D, NQ, WR>::Shared shared;                                   \
-    Program<D, NQ, WR>(args, shared).run();                                                                      \
+#define ATTN_KERNEL(NAME, D, NQ, WR, W, OCC)                                                                            \
+  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W), amdgpu_waves_per_eu(OCC, OCC))) \
+  NAME(const attn_args args) {                                                                                          \
+    __shared__ __attribute__((aligned(1024))) Program<D, NQ, WR, W>::Shared shared;                                     \
+    Program<D, NQ, WR, W>(args, shared).run();                                                                          \
   }
 #define JOIN_KERNEL(NAME, D, BLOCK) \
   extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args args) { join<D, BLOCK>(args); }
 
-ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 2)
-ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 2)
-ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 2)
-ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 1)
-ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 1)
+ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2)
 JOIN_KERNEL(wir_attn_join_d64_r16, 64, 16)
 JOIN_KERNEL(wir_attn_join_d64_r32, 64, 32)
 JOIN_KERNEL(wir_attn_join_d64_r128, 64, 128)

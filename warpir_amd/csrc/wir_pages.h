@@ -69,10 +69,16 @@ WIR_HD int block_keys(const Span& s, int rb, int rows_per_block, int rows, int g
 WIR_HD int block_units(int keys) { return imax((int)(((i64)keys + TILE - 1) / TILE), 1); }
 
 // Division of the units of all (sequence, block) pairs, heads of a pair in
-// turn, tiles of a head in turn, into shares of `share` consecutive units for
-// the programs.  A program that takes part of a head's units leaves a partial
-// result in one of its two slots: the first segment of its share in slot
-// 2 * program, another one, which is then its last, in 2 * program + 1.
+// turn, tiles of a head in turn, over the programs.
+//
+// With more heads than programs can have one each, a program takes `share`
+// consecutive units, parts of one or more heads.  One that takes part of a
+// head's units leaves a partial result in one of its two slots: the first
+// segment of its share in slot 2 * program, another one, which is then its
+// last, in 2 * program + 1.
+//
+// With fewer heads, a head's units go to parts_even(units) programs of its
+// own in equal parts, and program w's slot is w.
 WIR_HD i64 share_of(i64 total, int programs, int least) {
   const i64 even = (total + programs - 1) / programs;
   return even > least ? even : least;
@@ -80,28 +86,44 @@ WIR_HD i64 share_of(i64 total, int programs, int least) {
 
 struct Segment {
   int head, first, last;   // tiles first .. last - 1 of the head's
-  i64 begin;               // the unit it starts at
   bool whole;              // all of the head's
+  int slot, parts;         // of its partial result; partial results of the head
 };
 
+// Slot of the partial result of a segment that starts at unit u.
+WIR_HD int slot_of(i64 u, i64 share) { return (int)(2 * (u / share) + (u % share ? 1 : 0)); }
+
 // The segment at unit u of a pair whose units start at `base`, `units` a head; the program's share ends at `end`.
-WIR_HD Segment segment_at(i64 u, i64 base, int units, i64 end) {
+WIR_HD Segment segment_at(i64 u, i64 base, int units, i64 end, i64 share) {
   Segment g;
   g.head = (int)((u - base) / units);
   g.first = (int)((u - base) % units);
   g.last = (int)(units - g.first < end - u ? units : g.first + (end - u));
-  g.begin = u;
   g.whole = g.first == 0 && g.last == units;
+  const i64 begin = u - g.first;
+  g.slot = slot_of(u, share);
+  g.parts = (int)((begin + units - 1) / share - begin / share) + 1;
   return g;
 }
 
-// Slot of the partial result of a segment that starts at unit u, in the program of that share.
-WIR_HD int slot_of(i64 u, i64 share) { return (int)(2 * (u / share) + (u % share ? 1 : 0)); }
+// Slot of a head's n-th partial result, from that of its first.
+WIR_HD int slot_of_part(int first, int n, bool even) { return even ? first + n : n == 0 ? first : 2 * (first / 2 + n); }
 
-// Partial results of a head whose units are begin .. begin + units - 1, and the slot of each.
-WIR_HD int parts_of(i64 begin, int units, i64 share) {
-  return (int)((begin + units - 1) / share - begin / share) + 1;
+// Equal parts: the share that gives all heads together at most `programs` of them (heads < programs).
+WIR_HD i64 share_even(i64 total, int programs, int heads, int least) { return share_of(total, programs - heads, least); }
+WIR_HD int parts_even(int units, i64 share) { return (int)((units + share - 1) / share); }
+
+// Part n of the pair's parts, which start with program `base`.
+WIR_HD Segment segment_even(int program, int base, int units, i64 share) {
+  Segment g;
+  g.parts = parts_even(units, share);
+  g.head = (program - base) / g.parts;
+  const int n = (program - base) % g.parts;
+  g.first = (int)((i64)units * n / g.parts);
+  g.last = (int)((i64)units * (n + 1) / g.parts);
+  g.whole = g.parts == 1;
+  g.slot = program;
+  return g;
 }
-WIR_HD int slot_of_part(int first_slot, int part) { return part == 0 ? first_slot : 2 * (first_slot / 2 + part); }
 
 }  // namespace wir

@@ -43,7 +43,7 @@ launch_fn g_launch = nullptr;          // wir_launch of libwarpir_rt.so
 PyObject* g_current_stream = nullptr;  // torch._C._cuda_getCurrentRawStream
 
 constexpr size_t MAX_PLANS = 256;
-constexpr int MAX_SLOTS = 16;
+constexpr int MAX_SLOTS = 24;
 constexpr size_t MAX_ARGS = 1024;      // bytes of one launch's arguments
 
 struct Pointer {

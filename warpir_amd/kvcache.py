@@ -165,20 +165,25 @@ class _AttnArgs(ctypes.Structure):
                                                  "out", "lse", "partial", "info")),
                 *((n, ctypes.c_longlong) for n in ("qb", "qh", "qt", "ob", "oh", "ot", "lb", "lh", "lt", "tb")),
                 *((n, ctypes.c_int) for n in ("batch", "heads", "group", "tokens", "page_shift", "pages", "columns",
-                                              "blocks", "programs", "least"))]
+                                              "blocks", "programs", "least", "slots"))]
 
 
 TILE = 64        # positions of a tile (csrc/wir_pages.h)
 
 
-def _attention_form(rows: int, columns: int, page: int):
-    """(rows of a block, programs, fewest tiles of one) of the kernel for
-    ``rows`` query rows a key/value head over a table of ``columns`` pages;
-    programs 0: one for each sequence, block and head."""
+def _attention_form(rows: int, items_of, columns: int, page: int):
+    """(rows of a block, programs, least, slots) of the kernel for ``rows`` query
+    rows a key/value head over a table of ``columns`` pages; ``items_of`` gives the
+    number of (sequence, block, head) for a block's rows.  Programs 0: one for
+    each of those; least 0: shares of all heads' tiles in turn, else equal
+    parts of single heads with at least that many tiles."""
     block = 16 if rows <= 16 else 32 if rows <= 32 else 128
-    if columns * page <= 8 * TILE:
-        return block, 0, 0
-    return block, 512, 4
+    items, programs = items_of(block), 512
+    if columns * page <= 8 * TILE or (block == 128 and items >= programs):
+        return block, 0, 0, 0
+    if items <= programs // 2:
+        return block, programs, 4, programs
+    return block, programs, 0, 2 * programs
 
 
 def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=None, lse=None,
@@ -224,14 +229,15 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     if page_table.shape[1] == 0:
         return out.zero_(), lse.fill_(float("-inf"))
     rows = tokens * group
-    block, programs, least = _attention_form(rows, page_table.shape[1], page)
+    block, programs, least, slots = _attention_form(rows, lambda n: batch * -(-rows // n) * heads,
+                                                    page_table.shape[1], page)
     blocks = -(-rows // block)
     items = batch * blocks * heads
     need(fn, items * min(rows, block) < 1 << 24, "2^24 query rows or more in one call")
     args = _AttnArgs(*[None] * 12, *q.stride()[:3], *out.stride()[:3], *lse.stride(), page_table.stride(0), batch, heads,
                      group, tokens, page.bit_length() - 1, cache.k.shape[0], page_table.shape[1], blocks, programs,
-                     least)
-    floats = _workspace_floats(programs, block, d, items)
+                     least, slots)
+    floats = _workspace_floats(slots, block, d, items)
     if floats:
         if workspace is None:
             workspace = rec.alloc(torch.empty(floats, dtype=torch.float32, device=device))
@@ -253,18 +259,22 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     return out, lse
 
 
-def _workspace_floats(programs: int, block: int, d: int, items: int) -> int:
-    """Two slots of a program, each a block's unnormalised rows, maxima and
-    sums, and two words of every (sequence, block, head)."""
-    return 2 * programs * block * (d + 2) + 2 * items if programs else 0
+def _workspace_floats(slots: int, block: int, d: int, items: int) -> int:
+    """A slot is a block's unnormalised rows, maxima and sums; two words of
+    every (sequence, block, head) say where its partial results are."""
+    return slots * block * (d + 2) + 2 * items if slots else 0
 
 
 def attention_cached_workspace(q, cache: KVCache, page_table) -> int:
     """Elements that ``attention_cached`` needs of a ``workspace`` for these tensors."""
-    pages, heads, page, d = cache.k.shape
+    _, heads, page, d = cache.k.shape
     rows = q.shape[2] * (q.shape[1] // heads)
-    block, programs, _ = _attention_form(rows, page_table.shape[1], page)
-    return _workspace_floats(programs, block, d, q.shape[0] * -(-rows // block) * heads)
+
+    def items(block):
+        return q.shape[0] * -(-rows // block) * heads
+
+    block, _, _, slots = _attention_form(rows, items, page_table.shape[1], page)
+    return _workspace_floats(slots, block, d, items(block))
 
 
 __all__ = ["KVCache", "kv_cache_write", "kv_cache_read", "attention_cached", "attention_cached_workspace"]
