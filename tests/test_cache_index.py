@@ -82,20 +82,20 @@ static void division() {
     const int pairs = draw(1, 12), heads = draw(1, 5), programs = draw(1, 70), least = draw(1, 9);
     std::vector<int> units(pairs);
     for (int& n : units) n = draw(0, 9) ? draw(1, 30) : draw(1, 400);
-    i64 total = 0;
-    for (int n : units) total += (i64)heads * n;
-    const i64 share = share_of(total, programs, least);
-    CHECK(share >= least && share * programs >= total);
+    int total = 0;
+    for (int n : units) total += heads * n;
+    const int share = share_of(total, programs, least);
+    CHECK(share >= least && (i64)share * programs >= total);
     std::map<std::pair<int, int>, std::vector<int>> covered, slots;   // (pair, head) -> tiles, slots in order of tiles
     std::map<std::pair<int, int>, std::pair<int, int>> info;          // -> (first slot, parts)
     std::set<int> used;
     for (int w = 0; w < programs; ++w) {
-      i64 u = w * share;
+      int u = w * share;
       if (u >= total) break;
-      const i64 end = u + share < total ? u + share : total;
+      const int end = u + share < total ? u + share : total;
       int pair = 0;
-      i64 base = 0;
-      while (u >= base + (i64)heads * units[pair]) base += (i64)heads * units[pair++];
+      int base = 0;
+      while (u >= base + heads * units[pair]) base += heads * units[pair++];
       while (u < end) {
         const Segment g = segment_at(u, base, units[pair], end, share);
         CHECK(g.head >= 0 && g.head < heads && g.first >= 0 && g.first < g.last && g.last <= units[pair]);
@@ -109,7 +109,7 @@ static void division() {
         CHECK(g.whole == (g.parts == 1));
         if (g.first == 0) info[item] = {slot, g.parts};
         u += g.last - g.first;
-        if (u == base + (i64)heads * units[pair]) base = u, ++pair;
+        if (u == base + heads * units[pair]) base = u, ++pair;
       }
       CHECK(u == end);
     }
@@ -133,9 +133,9 @@ static void even_division() {
     const int pairs = draw(1, 12), heads = draw(1, 5), least = draw(1, 9), programs = pairs * heads + draw(1, 90);
     std::vector<int> units(pairs);
     for (int& n : units) n = draw(0, 9) ? draw(1, 30) : draw(1, 4000);
-    i64 total = 0;
-    for (int n : units) total += (i64)heads * n;
-    const i64 share = share_even(total, programs, pairs * heads, least);
+    int total = 0;
+    for (int n : units) total += heads * n;
+    const int share = share_even(total, programs, pairs * heads, least);
     int base = 0;
     for (int p = 0; p < pairs; ++p) {
       const int parts = parts_even(units[p], share);

@@ -91,11 +91,11 @@ __device__ __forceinline__ float over_groups(float x, F op) {
 }
 
 // Inclusive sums over the lanes of a wave.
-__device__ __forceinline__ i64 wave_scan(i64 x) {
+__device__ __forceinline__ int wave_scan(int x) {
   const int lane = wir::lane_id();
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const i64 y = __shfl_up(x, d);
+    const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
   return x;
@@ -234,6 +234,7 @@ struct Program {
         for (int u = 0; u < KC; ++u)
           x[j][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, s.q[n][u], x[j][n], 0, 0, 0, 127, 0, 127);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     const int at = t * wir::TILE + 16 * grp;   // the lane's tokens: at .. at + have - 1
     const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
@@ -249,11 +250,11 @@ struct Program {
     for (int n = 0; n < NQ; ++n) {
       float f = k.ks * s.qs[n];
       if (edge) {
+        const int seen = min(k.have, s.pos[n] - at + 1);   // of the lane's tokens
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[j][n][i] = 4 * j + i < k.have && at + 4 * j + i <= s.pos[n] ? x[j][n][i] * f : -__builtin_inff();
+          for (int i = 0; i < 4; ++i) x[j][n][i] = 4 * j + i < seen ? x[j][n][i] * f : -__builtin_inff();
         f = 1.f;
       }
       float top = x[0][n][0];
@@ -281,50 +282,66 @@ struct Program {
         for (int d = 0; d < DT; ++d) s.o[d][n] *= corr;
       }
     }
+    // Values of a tile that not all rows see: bytes past the sequence's end
+    // become 0 (0 * NaN is NaN in the product), and so do NaN codes.
+    unsigned nans = 0;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       u32x4 v = value(d);
-      if (edge) edge_value(s, d, v, k.have, at);
+      if (edge) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const unsigned there = held_bytes(v[w], k.have - 4 * w), bad = nan_bytes(there);
+          nans |= bad;
+          v[w] = there & ~bad;
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bf16x8 w = unpack8(v[2 * u], v[2 * u + 1], power);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s.o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, p[n][u], s.o[d][n], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if (edge && __builtin_amdgcn_ballot_w64(nans != 0) != 0) mark_nans(s, k.have, at, value);
   }
 
-  // Values of a tile that not all rows see: bytes past the sequence's end
-  // become 0 (0 * NaN is NaN in the product), and so do NaN codes, which
-  // instead make NaN of exactly the rows that see them, by a product of
-  // where they are with who sees them.
-  __device__ __forceinline__ void edge_value(State& s, int d, u32x4& v, int have, int at) const {
-    unsigned some = 0;
-    u32x4 is;
+  // The first n bytes of a word.
+  static __device__ __forceinline__ unsigned held_bytes(unsigned x, int n) {
+    return n >= 4 ? x : n <= 0 ? 0u : x & ((1u << 8 * n) - 1);
+  }
+  // 0xff where a byte is a NaN code, 0x7f or 0xff.
+  static __device__ __forceinline__ unsigned nan_bytes(unsigned x) {
+    return ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+  }
+
+  // NaN values of such a tile make NaN of exactly the rows that see them, by a product of where they are with who sees
+  // them.
+  template <class Value>
+  __device__ __forceinline__ void mark_nans(State& s, int have, int at, Value value) const {
+    asm volatile("" : "+v"(have), "+v"(at));   // (its comparisons are made here, not kept from the masks')
+    bf16x8 sees[NQ][2];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int n = min(max(have - 4 * w, 0), 4);
-      const unsigned x = v[w] & (n == 4 ? ~0u : (1u << 8 * n) - 1);
-      const unsigned high = ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // of bytes 0x7f and 0xff
-      some |= high;
-      const unsigned bytes = (high >> 7) * 0xffu;
-      v[w] = x & ~bytes;
-      is[w] = bytes & 0x38383838u;   // 1.0 in e4m3
-    }
-    if (__builtin_amdgcn_ballot_w64(some != 0) == 0) return;
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      f32x4 count = {0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 16; ++e) sees[n][e / 8][e % 8] = (bf16)(e < min(have, s.pos[n] - at + 1) ? 1.f : 0.f);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        bf16x8 sees;
+    for (int d = 0; d < DT; ++d) {
+      const u32x4 v = value(d);
+      u32x4 is;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sees[e] = (bf16)(8 * u + e < have && at + 8 * u + e <= s.pos[n] ? 1.f : 0.f);
-        count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(unpack8(is[2 * u], is[2 * u + 1], 1.f), sees, count, 0, 0, 0);
+      for (int w = 0; w < 4; ++w) is[w] = nan_bytes(held_bytes(v[w], have - 4 * w)) & 0x38383838u;   // 1.0 in e4m3
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        f32x4 count = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(unpack8(is[2 * u], is[2 * u + 1], 1.f), sees[n][u], count, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (count[i] > 0.f) s.o[d][n][i] = __builtin_nanf("");
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (count[i] > 0.f) s.o[d][n][i] = __builtin_nanf("");
     }
   }
 
@@ -508,10 +525,11 @@ struct Program {
   }
 
   __device__ __forceinline__ void segment(int pair, int keys, const wir::Segment& g) {
+    asm volatile("" : "+v"(col), "+v"(grp), "+v"(lane));
     b = pair / a.blocks;
     rb = pair % a.blocks;
     span = span_at(b);
-    walk(g.head, g.first, min(g.last, (int)(((i64)keys + wir::TILE - 1) / wir::TILE)));
+    walk(g.head, g.first, min(g.last, (keys + wir::TILE - 1) / wir::TILE));
     __syncthreads();
     if (threadIdx.x == 0 && a.programs && g.first == 0) {
       int* info = a.info + 2 * ((i64)pair * a.heads + g.head);
@@ -525,60 +543,64 @@ struct Program {
   // The pair in which item u lies, of `own` items of this lane's pairs from .. and as many as `weight` says of each,
   // and the items before the pair.  All lanes get them; false: there are no u items.
   template <class Weight>
-  __device__ __forceinline__ bool find(i64 u, i64 own, int from, int each, Weight weight, int& pair, i64& base) const {
-    const i64 upto = wave_scan(own);
+  __device__ __forceinline__ bool find(int u, int own, int from, int each, Weight weight, int& pair, int& base) const {
+    const int upto = wave_scan(own);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(u < upto);
     if (past == 0) return false;
     const int src = __builtin_ctzll(past);
-    i64 before = upto - own;
+    int before = upto - own;
     int p = from;
     if (lane == src && each > 1) {
       for (;; ++p) {
-        const i64 n = weight(p);
+        const int n = weight(p);
         if (u < before + n) break;
         before += n;
       }
     }
     pair = __builtin_amdgcn_readfirstlane(__shfl(p, src));
-    base = __shfl(before, src);
+    base = __builtin_amdgcn_readfirstlane(__shfl(before, src));
     return true;
   }
 
   __device__ __forceinline__ void run() {
+    int pair, keys;
+    wir::Segment g;
+    int u = 0, end = 0, base = 0, share = 1;   // of a share over several heads
     if (!a.programs) {   // a head's blocks, the longest first, next to one another on one XCD
       const int id = wir::remap_xcd(blockIdx.x, gridDim.x), item = id / a.blocks;
-      const int pair = item / a.heads * a.blocks + a.blocks - 1 - id % a.blocks, keys = keys_at(pair);
-      segment(pair, keys, wir::Segment{item % a.heads, 0, wir::block_units(keys), true, -1, 1});
-      return;
+      pair = item / a.heads * a.blocks + a.blocks - 1 - id % a.blocks;
+      keys = keys_at(pair);
+      g = wir::Segment{item % a.heads, 0, wir::block_units(keys), true, -1, 1};
+    } else {
+      // every wave for itself: a lane takes `each` pairs
+      const int pairs = a.batch * a.blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
+      auto units = [&](int p) { return a.heads * wir::block_units(keys_at(p)); };
+      int own = 0;
+      for (int p = from; p < to; ++p) own += units(p);
+      const int total = __builtin_amdgcn_readfirstlane(__shfl(wave_scan(own), 63));
+      if (a.least) {
+        share = wir::share_even(total, a.programs, pairs * a.heads, a.least);
+        auto parts = [&](int p) { return a.heads * wir::parts_even(wir::block_units(keys_at(p)), share); };
+        own = 0;
+        for (int p = from; p < to; ++p) own += parts(p);
+        if (!find(blockIdx.x, own, from, each, parts, pair, base)) return;
+        keys = keys_at(pair);
+        g = wir::segment_even(blockIdx.x, base, wir::block_units(keys), share);
+      } else {
+        share = wir::share_of(total, a.programs, 1);
+        u = blockIdx.x * share;
+        if (!find(u, own, from, each, units, pair, base)) return;
+        end = u + share < total ? u + share : total;
+        keys = keys_at(pair);
+        g = wir::segment_at(u, base, wir::block_units(keys), end, share);
+      }
     }
-    // every wave for itself: a lane takes `each` pairs
-    const int pairs = a.batch * a.blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
-    auto units = [&](int p) { return (i64)a.heads * wir::block_units(keys_at(p)); };
-    i64 own = 0;
-    for (int p = from; p < to; ++p) own += units(p);
-    const i64 total = __shfl(wave_scan(own), 63);
-    int pair;
-    i64 base;
-    if (a.least) {
-      const i64 share = wir::share_even(total, a.programs, pairs * a.heads, a.least);
-      auto parts = [&](int p) { return (i64)a.heads * wir::parts_even(wir::block_units(keys_at(p)), share); };
-      own = 0;
-      for (int p = from; p < to; ++p) own += parts(p);
-      if (!find(blockIdx.x, own, from, each, parts, pair, base)) return;
-      const int keys = keys_at(pair);
-      segment(pair, keys, wir::segment_even(blockIdx.x, (int)base, wir::block_units(keys), share));
-      return;
-    }
-    const i64 share = wir::share_of(total, a.programs, 1);
-    i64 u = (i64)blockIdx.x * share;
-    if (!find(u, own, from, each, units, pair, base)) return;
-    const i64 end = u + share < total ? u + share : total;
-    while (u < end) {
-      const int keys = keys_at(pair), n = wir::block_units(keys);
-      const wir::Segment g = wir::segment_at(u, base, n, end, share);
+    for (;;) {   // one segment, but for a share of several heads
       segment(pair, keys, g);
       u += g.last - g.first;
-      if (u == base + (i64)a.heads * n) base = u, ++pair;
+      if (u >= end) break;
+      if (u == base + a.heads * wir::block_units(keys)) base = u, keys = keys_at(++pair);
+      g = wir::segment_at(u, base, wir::block_units(keys), end, share);
     }
   }
 };
@@ -648,7 +670,7 @@ ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 1)
 ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2)
 JOIN_KERNEL(wir_attn_join_d64_r16, 64, 16)
 JOIN_KERNEL(wir_attn_join_d64_r32, 64, 32)

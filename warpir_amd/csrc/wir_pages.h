@@ -66,8 +66,11 @@ WIR_HD int block_keys(const Span& s, int rb, int rows_per_block, int rows, int g
 }
 
 // Its units of work: tiles, and one where there are none (its rows are written all the same).
-WIR_HD int block_units(int keys) { return imax((int)(((i64)keys + TILE - 1) / TILE), 1); }
+WIR_HD int block_units(int keys) { return imax((int)(((unsigned)keys + TILE - 1) / TILE), 1); }
 
+// All units together, and so any unit's index, have to stay below 2^30 (64-bit
+// divisions cost microseconds here).
+//
 // Division of the units of all (sequence, block) pairs, heads of a pair in
 // turn, tiles of a head in turn, over the programs.
 //
@@ -79,10 +82,7 @@ WIR_HD int block_units(int keys) { return imax((int)(((i64)keys + TILE - 1) / TI
 //
 // With fewer heads, a head's units go to parts_even(units) programs of its
 // own in equal parts, and program w's slot is w.
-WIR_HD i64 share_of(i64 total, int programs, int least) {
-  const i64 even = (total + programs - 1) / programs;
-  return even > least ? even : least;
-}
+WIR_HD int share_of(int total, int programs, int least) { return imax((total + programs - 1) / programs, least); }
 
 struct Segment {
   int head, first, last;   // tiles first .. last - 1 of the head's
@@ -91,18 +91,18 @@ struct Segment {
 };
 
 // Slot of the partial result of a segment that starts at unit u.
-WIR_HD int slot_of(i64 u, i64 share) { return (int)(2 * (u / share) + (u % share ? 1 : 0)); }
+WIR_HD int slot_of(int u, int share) { return 2 * (u / share) + (u % share ? 1 : 0); }
 
 // The segment at unit u of a pair whose units start at `base`, `units` a head; the program's share ends at `end`.
-WIR_HD Segment segment_at(i64 u, i64 base, int units, i64 end, i64 share) {
+WIR_HD Segment segment_at(int u, int base, int units, int end, int share) {
   Segment g;
-  g.head = (int)((u - base) / units);
-  g.first = (int)((u - base) % units);
-  g.last = (int)(units - g.first < end - u ? units : g.first + (end - u));
+  g.head = (u - base) / units;
+  g.first = (u - base) % units;
+  g.last = imin(units, g.first + end - u);
   g.whole = g.first == 0 && g.last == units;
-  const i64 begin = u - g.first;
+  const int begin = u - g.first;
   g.slot = slot_of(u, share);
-  g.parts = (int)((begin + units - 1) / share - begin / share) + 1;
+  g.parts = (begin + units - 1) / share - begin / share + 1;
   return g;
 }
 
@@ -110,17 +110,19 @@ WIR_HD Segment segment_at(i64 u, i64 base, int units, i64 end, i64 share) {
 WIR_HD int slot_of_part(int first, int n, bool even) { return even ? first + n : n == 0 ? first : 2 * (first / 2 + n); }
 
 // Equal parts: the share that gives all heads together at most `programs` of them (heads < programs).
-WIR_HD i64 share_even(i64 total, int programs, int heads, int least) { return share_of(total, programs - heads, least); }
-WIR_HD int parts_even(int units, i64 share) { return (int)((units + share - 1) / share); }
+WIR_HD int share_even(int total, int programs, int heads, int least) { return share_of(total, programs - heads, least); }
+WIR_HD int parts_even(int units, int share) { return (units + share - 1) / share; }
 
 // Part n of the pair's parts, which start with program `base`.
-WIR_HD Segment segment_even(int program, int base, int units, i64 share) {
+WIR_HD Segment segment_even(int program, int base, int units, int share) {
   Segment g;
   g.parts = parts_even(units, share);
   g.head = (program - base) / g.parts;
   const int n = (program - base) % g.parts;
-  g.first = (int)((i64)units * n / g.parts);
-  g.last = (int)((i64)units * (n + 1) / g.parts);
+  // the first units % parts of them have one more
+  const int each = units / g.parts, more = units % g.parts;
+  g.first = n * each + imin(n, more);
+  g.last = g.first + each + (n < more ? 1 : 0);
   g.whole = g.parts == 1;
   g.slot = program;
   return g;
