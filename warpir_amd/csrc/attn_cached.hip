@@ -240,15 +240,16 @@ struct Program {
     const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
     read();
     // vs = 2^e g; a scale that is no positive normal number is all g
-    const unsigned bits = __float_as_uint(k.vs), exponent = bits & 0x7f800000u;
+    const float ks = k.have ? k.ks : 1.f, vs = k.have ? k.vs : 1.f;
+    const unsigned bits = __float_as_uint(vs), exponent = bits & 0x7f800000u;
     const bool normal = bits < 0x7f800000u && exponent != 0;
     const float power = normal ? __uint_as_float(exponent) : 1.f;
-    const float g = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : k.vs;
+    const float g = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : vs;
     const bool plain = __builtin_amdgcn_ballot_w64(g != 1.f) == 0;
     bf16x8 p[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      float f = k.ks * s.qs[n];
+      float f = ks * s.qs[n];
       if (edge) {
         const int seen = min(k.have, s.pos[n] - at + 1);   // of the lane's tokens
 #pragma unroll
@@ -273,9 +274,18 @@ struct Program {
         for (int i = 0; i < 4; ++i) {
           const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][n][i], f, -base));
           sum[i % 2] += y;
-          // (a key that the row does not see adds nothing, whatever its scale is)
-          p[n][j / 2][j % 2 * 4 + i] = (bf16)(plain ? y : edge && x[j][n][i] == -__builtin_inff() ? 0.f : y * g);
+          x[j][n][i] = y;
         }
+      if (!plain) {   // (a key that the row does not see adds nothing, whatever its scale is)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j][n][i] = x[j][n][i] == 0.f ? 0.f : x[j][n][i] * g;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[n][j / 2][j % 2 * 4 + i] = (bf16)x[j][n][i];
       s.l[n] = s.l[n] * corr + (sum[0] + sum[1]);
       if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
 #pragma unroll
@@ -355,9 +365,8 @@ struct Program {
     const int id = wir::checked_page(page, a.pages);
     const i64 at = (i64)max(id, 0) * a.heads + head;
     k.have = id < 0 ? 0 : min(max(span.held - (t * wir::TILE + 16 * grp), 0), 16);
-    k.ks = a.k_scale[at];
+    k.ks = a.k_scale[at];   // (of page 0 where there is none: `tile` sees to it, after the loads' time)
     k.vs = a.v_scale[at];
-    if (id < 0) k.ks = k.vs = 1.f;
   }
   // A page that is none is read as page 0, and its tokens masked.
   __device__ __forceinline__ const unsigned char* key_at(int t, int page, int head) const {
