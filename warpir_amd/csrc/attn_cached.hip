@@ -224,21 +224,25 @@ struct Program {
   template <class Key, class Value, class Read>
   __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Value value, Read read) const {
     f32x4 x[4][NQ];
+    i32x8 k_of[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k_of[j] = key(j);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const i32x8 kf = key(j);
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         x[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < KC; ++u)
-          x[j][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, s.q[n][u], x[j][n], 0, 0, 0, 127, 0, 127);
+          x[j][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k_of[j], s.q[n][u], x[j][n], 0, 0, 0, 127, 0, 127);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
     const int at = t * wir::TILE + 16 * grp;   // the lane's tokens: at .. at + have - 1
     const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
     read();
+    u32x4 v[DT];   // (from LDS they come under the softmax)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) v[d] = value(d);
     // vs = 2^e g; a scale that is no positive normal number is all g
     const float ks = k.have ? k.ks : 1.f, vs = k.have ? k.vs : 1.f;
     const unsigned bits = __float_as_uint(vs), exponent = bits & 0x7f800000u;
@@ -295,25 +299,24 @@ struct Program {
     // Values of a tile that not all rows see: bytes past the sequence's end
     // become 0 (0 * NaN is NaN in the product), and so do NaN codes.
     unsigned nans = 0;
+    if (edge) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      u32x4 v = value(d);
-      if (edge) {
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const unsigned there = held_bytes(v[w], k.have - 4 * w), bad = nan_bytes(there);
+          const unsigned there = held_bytes(v[d][w], k.have - 4 * w), bad = nan_bytes(there);
           nans |= bad;
-          v[w] = there & ~bad;
+          v[d][w] = there & ~bad;
         }
-      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bf16x8 w = unpack8(v[2 * u], v[2 * u + 1], power);
+        const bf16x8 w = unpack8(v[d][2 * u], v[d][2 * u + 1], power);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s.o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, p[n][u], s.o[d][n], 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
     if (edge && __builtin_amdgcn_ballot_w64(nans != 0) != 0) mark_nans(s, k.have, at, value);
   }
 
