@@ -69,6 +69,16 @@ struct attn_args {
   int slots;                   // of partial results
 };
 
+// The arguments where the launch put them.  They fill most of the scalar registers: `fresh` makes the compiler read them
+// again in each phase instead of keeping them (spilled) through the tiles' loop, where reading a spilled one back costs
+// a vector instruction (95 of 470 a tile).
+typedef const __attribute__((address_space(4))) attn_args* args_ptr;
+__device__ __forceinline__ args_ptr fresh(args_ptr a) {
+  unsigned long long p = (unsigned long long)a;
+  asm volatile("" : "+s"(p));
+  return (args_ptr)p;
+}
+
 // (by value: a bit cast of a vector's element in place gives element 0)
 __device__ __forceinline__ unsigned bits_of(bf16 x) { return (unsigned)__builtin_bit_cast(unsigned short, x); }
 
@@ -122,14 +132,14 @@ struct Program {
     char ring[SHARED ? 2 * CHUNKS * 1024 : 16];
   };
 
-  const attn_args& a;
+  args_ptr a;
   Shared& sh;
   int lane, col, grp, wave, wr, wk;
   // the pair's
   int b, rb;
   wir::Span span;
 
-  __device__ __forceinline__ Program(const attn_args& args, Shared& shared) : a(args), sh(shared) {
+  __device__ __forceinline__ Program(args_ptr args, Shared& shared) : a(args), sh(shared) {
     lane = wir::lane_id();
     col = lane % 16;
     grp = lane / 16;
@@ -138,18 +148,18 @@ struct Program {
     wk = wave / WR;
   }
 
-  __device__ __forceinline__ int rows() const { return a.tokens * a.group; }
+  __device__ __forceinline__ int rows() const { return a->tokens * a->group; }
 
   __device__ __forceinline__ wir::Span span_at(int seq) const {
-    return wir::span_of(a.lengths[seq], a.counts ? a.counts[seq] : a.tokens, a.tokens, a.columns << a.page_shift);
+    return wir::span_of(a->lengths[seq], a->counts ? a->counts[seq] : a->tokens, a->tokens, a->columns << a->page_shift);
   }
   __device__ __forceinline__ int keys_at(int pair) const {
-    return wir::block_keys(span_at(pair / a.blocks), pair % a.blocks, BLOCK, rows(), a.group);
+    return wir::block_keys(span_at(pair / a->blocks), pair % a->blocks, BLOCK, rows(), a->group);
   }
 
   // Position that row r of the pair sees up to; -1: none.
   __device__ __forceinline__ int position(int r) const {
-    const int t = r / a.group;
+    const int t = r / a->group;
     return r < rows() && t < span.count ? max(span.start + t, -1) : -1;
   }
 
@@ -172,13 +182,13 @@ struct Program {
   __device__ __forceinline__ void begin(State& s, int head) const {
     const float c = (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));
     const int row0 = rb * BLOCK + wr * ROWS;
-    s.low = max(span.start + min(row0 / a.group, span.count), 0);
+    s.low = max(span.start + min(row0 / a->group, span.count), 0);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int r = row0 + n * 16 + col;
       s.pos[n] = position(r);
-      const int rr = r < rows() ? r : 0, t = rr / a.group;
-      const bf16* p = a.q + b * a.qb + (i64)(head * a.group + rr - t * a.group) * a.qh + t * a.qt + 16 * grp;
+      const int rr = r < rows() ? r : 0, t = rr / a->group;
+      const bf16* p = a->q + b * a->qb + (i64)(head * a->group + rr - t * a->group) * a->qh + t * a->qt + 16 * grp;
       bf16x8 x[2 * KC];
       unsigned top = 0;
 #pragma unroll
@@ -243,13 +253,12 @@ struct Program {
     u32x4 v[DT];   // (from LDS they come under the softmax)
 #pragma unroll
     for (int d = 0; d < DT; ++d) v[d] = value(d);
-    // vs = 2^e g; a scale that is no positive normal number is all g
-    const float ks = k.have ? k.ks : 1.f, vs = k.have ? k.vs : 1.f;
-    const unsigned bits = __float_as_uint(vs), exponent = bits & 0x7f800000u;
-    const bool normal = bits < 0x7f800000u && exponent != 0;
-    const float power = normal ? __uint_as_float(exponent) : 1.f;
-    const float g = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : vs;
-    const bool plain = __builtin_amdgcn_ballot_w64(g != 1.f) == 0;
+    // vs = 2^e g: 2^e goes to the values, g to the probabilities (and out of their sum again)
+    const unsigned bits = __float_as_uint(k.have ? k.vs : 1.f);
+    const float power = __uint_as_float(max(bits & 0x7f800000u, 0x00800000u));
+    const float g = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+    const float log_g = __builtin_amdgcn_logf(g), inv_g = __builtin_amdgcn_rcpf(g);
+    const float ks = k.have ? k.ks : 1.f;
     bf16x8 p[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -271,26 +280,17 @@ struct Program {
       const float base = top == -__builtin_inff() ? 0.f : top;
       const float corr = __builtin_amdgcn_exp2f(s.m[n] - base);
       s.m[n] = top;
+      const float shift = log_g - base;
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][n][i], f, -base));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][n][i], f, shift));
           sum[i % 2] += y;
-          x[j][n][i] = y;
+          p[n][j / 2][j % 2 * 4 + i] = (bf16)y;
         }
-      if (!plain) {   // (a key that the row does not see adds nothing, whatever its scale is)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[j][n][i] = x[j][n][i] == 0.f ? 0.f : x[j][n][i] * g;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[n][j / 2][j % 2 * 4 + i] = (bf16)x[j][n][i];
-      s.l[n] = s.l[n] * corr + (sum[0] + sum[1]);
+      s.l[n] = s.l[n] * corr + (sum[0] + sum[1]) * inv_g;
       if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) s.o[d][n] *= corr;
@@ -299,6 +299,12 @@ struct Program {
     // Values of a tile that not all rows see: bytes past the sequence's end
     // become 0 (0 * NaN is NaN in the product), and so do NaN codes.
     unsigned nans = 0;
+    if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u) != 0) {   // no scale: NaN
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v[d][w] = bits >= 0x7f800000u ? 0x7f7f7f7fu : v[d][w];
+    }
     if (edge) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -358,29 +364,51 @@ struct Program {
     }
   }
 
+  // Addresses of a head's pages: a lane's place in page 0, and what a page and a place in it add.
+  struct Bases {
+    const float *ks, *vs;
+    const unsigned char *k, *v;
+    const int* table;
+    int page_bytes, page_scales, shift, pages;
+  };
+  __device__ __forceinline__ Bases bases(int head) const {
+    Bases x;
+    x.ks = a->k_scale + head;
+    x.vs = a->v_scale + head;
+    x.page_scales = a->heads;
+    x.page_bytes = (a->heads * D) << a->page_shift;
+    x.shift = a->page_shift;
+    x.pages = a->pages;
+    x.table = a->table + b * a->tb;
+    x.k = a->k + (((i64)head << a->page_shift) + col % 4) * D + 16 * grp;
+    x.v = a->v + (((i64)head * D + col) << a->page_shift);
+    return x;
+  }
   // Page id of the tile's 16-token segment `seg`; -1 past the sequence.
-  __device__ __forceinline__ int page_of(int t, int seg) const {
+  __device__ __forceinline__ int page_of(const Bases& x, int t, int seg) const {
     const int at = t * wir::TILE + 16 * seg;
-    return at < span.held ? a.table[b * a.tb + (at >> a.page_shift)] : -1;
+    return at < span.held ? x.table[at >> x.shift] : -1;
   }
-  // The lane's own segment of it (its V operand and scores).
-  __device__ __forceinline__ void scales_of(Tokens& k, int t, int page, int head) const {
-    const int id = wir::checked_page(page, a.pages);
-    const i64 at = (i64)max(id, 0) * a.heads + head;
-    k.have = id < 0 ? 0 : min(max(span.held - (t * wir::TILE + 16 * grp), 0), 16);
-    k.ks = a.k_scale[at];   // (of page 0 where there is none: `tile` sees to it, after the loads' time)
-    k.vs = a.v_scale[at];
+  // (a page that is none is read as page 0, and its tokens masked)
+  static __device__ __forceinline__ i64 page_index(const Bases& x, int page) {
+    return max(wir::checked_page(page, x.pages), 0);
   }
-  // A page that is none is read as page 0, and its tokens masked.
-  __device__ __forceinline__ const unsigned char* key_at(int t, int page, int head) const {
-    const i64 at = (i64)max(wir::checked_page(page, a.pages), 0) * a.heads + head;
-    const int in_page = (t * wir::TILE + 16 * (col / 4)) & ((1 << a.page_shift) - 1);
-    return a.k + ((at << a.page_shift) + in_page + col % 4) * D + 16 * grp;
+  static __device__ __forceinline__ int in_page(const Bases& x, int t, int seg) {
+    return (t * wir::TILE + 16 * seg) & ((1 << x.shift) - 1);
   }
-  __device__ __forceinline__ const unsigned char* value_at(int t, int page, int head) const {
-    const i64 at = (i64)max(wir::checked_page(page, a.pages), 0) * a.heads + head;
-    const int in_page = (t * wir::TILE + 16 * grp) & ((1 << a.page_shift) - 1);
-    return a.v + ((at * D + col) << a.page_shift) + in_page;
+
+  // The lane's own segment of a tile (its V operand and scores).
+  __device__ __forceinline__ void scales_of(Tokens& k, const Bases& x, int t, int page) const {
+    const i64 at = page_index(x, page) * x.page_scales;
+    k.have = wir::checked_page(page, x.pages) < 0 ? 0 : min(max(span.held - (t * wir::TILE + 16 * grp), 0), 16);
+    k.ks = x.ks[at];   // (of page 0 where there is none: `tile` sees to it, after the loads' time)
+    k.vs = x.vs[at];
+  }
+  __device__ __forceinline__ const unsigned char* key_at(const Bases& x, int t, int page) const {
+    return x.k + page_index(x, page) * x.page_bytes + in_page(x, t, col / 4) * D;
+  }
+  __device__ __forceinline__ const unsigned char* value_at(const Bases& x, int t, int page) const {
+    return x.v + page_index(x, page) * x.page_bytes + in_page(x, t, grp);
   }
 
   static __device__ __forceinline__ i32x8 key_operand(const u32x4& x, const u32x4& y) {
@@ -390,13 +418,15 @@ struct Program {
   // Tiles first .. last - 1 of `head`, every WK-th from the wave's, through registers: K of the next tile is in
   // flight during the softmax and the second product, V during the next tile's first product.
   __device__ __forceinline__ void walk_registers(State& s, int head, int first, int last) const {
+    const Bases at = bases(head);
+    const i64 v_step = (i64)16 << at.shift;
     u32x4 kf[4][KC], vf[DT];
     Tokens tok;
     const unsigned char* vp;
     auto load_k = [&](int t, int page_k, int page_v) {
-      scales_of(tok, t, page_v, head);
-      const unsigned char* kp = key_at(t, page_k, head);
-      vp = value_at(t, page_v, head);
+      scales_of(tok, at, t, page_v);
+      const unsigned char* kp = key_at(at, t, page_k);
+      vp = value_at(at, t, page_v);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -404,12 +434,12 @@ struct Program {
     };
     auto load_v = [&]() {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vf[d] = *(const u32x4*)(vp + ((i64)(16 * d) << a.page_shift));
+      for (int d = 0; d < DT; ++d) vf[d] = *(const u32x4*)(vp + d * v_step);
     };
     int t = first + wk, next_k = -1, next_v = -1;
     if (t < last) {
-      load_k(t, page_of(t, col / 4), page_of(t, grp));
-      if (t + WK < last) next_k = page_of(t + WK, col / 4), next_v = page_of(t + WK, grp);
+      load_k(t, page_of(at, t, col / 4), page_of(at, t, grp));
+      if (t + WK < last) next_k = page_of(at, t + WK, col / 4), next_v = page_of(at, t + WK, grp);
       load_v();
     }
     begin(s, head);
@@ -419,7 +449,7 @@ struct Program {
            [&]() {
              if (t + WK >= last) return;
              const int page_k = next_k, page_v = next_v;
-             if (t + 2 * WK < last) next_k = page_of(t + 2 * WK, col / 4), next_v = page_of(t + 2 * WK, grp);
+             if (t + 2 * WK < last) next_k = page_of(at, t + 2 * WK, col / 4), next_v = page_of(at, t + 2 * WK, grp);
              load_k(t + WK, page_k, page_v);
            });
       if (t + WK < last) load_v();
@@ -432,22 +462,25 @@ struct Program {
     constexpr int MINE = CHUNKS / W;
     const bool mine_k = wave < W / 2;
     const int mine = wave * MINE, seg = mine_k ? col / 4 : grp;
+    const Bases at = bases(head);
+    const unsigned char* base = mine_k ? at.k : at.v;
+    const int token_bytes = mine_k ? D : 1;
     auto bring = [&](int t, int slot, int page) {
-      const unsigned char* from = mine_k ? key_at(t, page, head) : value_at(t, page, head);
+      const unsigned char* from = base + page_index(at, page) * at.page_bytes + in_page(at, t, seg) * token_bytes;
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
         const int c = mine + i;
-        const i64 off = mine_k ? (i64)(4 * (c / KC) * D + 64 * (c % KC)) : (i64)(16 * (c - 4 * KC)) << a.page_shift;
+        const int off = mine_k ? 4 * (c / KC) * D + 64 * (c % KC) : (16 * (c - 4 * KC)) << at.shift;
         wir::dma16_v(from + off, wir::lds_addr(sh.ring + (slot * CHUNKS + c) * 1024));
       }
     };
     Tokens tok;
     int next = -1, next_own = -1, slot = 0;
     if (first < last) {
-      const int page = page_of(first, seg), own = page_of(first, grp);
+      const int page = page_of(at, first, seg), own = page_of(at, first, grp);
       bring(first, 0, page);
-      scales_of(tok, first, own, head);
-      if (first + 1 < last) next = page_of(first + 1, seg), next_own = page_of(first + 1, grp);
+      scales_of(tok, at, first, own);
+      if (first + 1 < last) next = page_of(at, first + 1, seg), next_own = page_of(at, first + 1, grp);
     }
     begin(s, head);
     for (int t = first; t < last; ++t, slot ^= 1) {
@@ -457,8 +490,8 @@ struct Program {
       const Tokens now = tok;
       if (t + 1 < last) {
         bring(t + 1, slot ^ 1, next);
-        scales_of(tok, t + 1, next_own, head);
-        if (t + 2 < last) next = page_of(t + 2, seg), next_own = page_of(t + 2, grp);
+        scales_of(tok, at, t + 1, next_own);
+        if (t + 2 < last) next = page_of(at, t + 2, seg), next_own = page_of(at, t + 2, grp);
       }
       typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
       const lds_u32x4* from = (const lds_u32x4*)wir::lds(sh.ring + slot * CHUNKS * 1024) + lane;
@@ -510,11 +543,11 @@ struct Program {
         x = y = f32x4{0.f, 0.f, 0.f, 0.f};
       }
       if (slot >= 0) {
-        float* to = a.partial + ((i64)slot * BLOCK + row) * D + 8 * ch;
+        float* to = a->partial + ((i64)slot * BLOCK + row) * D + 8 * ch;
         *(f32x4*)to = x;
         *(f32x4*)(to + 4) = y;
         if (ch == 0)
-          *(f32x2*)(a.partial + (i64)a.slots * BLOCK * D + ((i64)slot * BLOCK + row) * 2) = f32x2{top, sum};
+          *(f32x2*)(a->partial + (i64)a->slots * BLOCK * D + ((i64)slot * BLOCK + row) * 2) = f32x2{top, sum};
       } else {
         put(a, b, head, rb * BLOCK + row, ch, x, y, top, sum);
       }
@@ -522,29 +555,31 @@ struct Program {
   }
 
   // 8 columns of a row's output and, with the first of them, its LSE; a row that sees nothing: 0 and -inf.
-  static __device__ __forceinline__ void put(const attn_args& a, int b, int head, int r, int ch, const f32x4& x,
+  static __device__ __forceinline__ void put(args_ptr a, int b, int head, int r, int ch, const f32x4& x,
                                              const f32x4& y, float top, float sum) {
-    const int t = r / a.group;
-    const i64 h = head * a.group + r - t * a.group;
+    const int t = r / a->group;
+    const i64 h = head * a->group + r - t * a->group;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     bf16x8 v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (bf16)(x[i] * inv), v[4 + i] = (bf16)(y[i] * inv);
-    *(bf16x8*)(a.out + b * a.ob + h * a.oh + t * a.ot + 8 * ch) = v;
+    *(bf16x8*)(a->out + b * a->ob + h * a->oh + t * a->ot + 8 * ch) = v;
     if (ch == 0)
-      a.lse[b * a.lb + h * a.lh + t * a.lt] =
+      a->lse[b * a->lb + h * a->lh + t * a->lt] =
           sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 
   __device__ __forceinline__ void segment(int pair, int keys, const wir::Segment& g) {
     asm volatile("" : "+v"(col), "+v"(grp), "+v"(lane));
-    b = pair / a.blocks;
-    rb = pair % a.blocks;
+    a = fresh(a);
+    b = pair / a->blocks;
+    rb = pair % a->blocks;
     span = span_at(b);
     walk(g.head, g.first, min(g.last, (keys + wir::TILE - 1) / wir::TILE));
     __syncthreads();
-    if (threadIdx.x == 0 && a.programs && g.first == 0) {
-      int* info = a.info + 2 * ((i64)pair * a.heads + g.head);
+    a = fresh(a);
+    if (threadIdx.x == 0 && a->programs && g.first == 0) {
+      int* info = a->info + 2 * ((i64)pair * a->heads + g.head);
       info[0] = g.slot;
       info[1] = g.parts;
     }
@@ -578,28 +613,28 @@ struct Program {
     int pair, keys;
     wir::Segment g;
     int u = 0, end = 0, base = 0, share = 1;   // of a share over several heads
-    if (!a.programs) {   // a head's blocks, the longest first, next to one another on one XCD
-      const int id = wir::remap_xcd(blockIdx.x, gridDim.x), item = id / a.blocks;
-      pair = item / a.heads * a.blocks + a.blocks - 1 - id % a.blocks;
+    if (!a->programs) {   // a head's blocks, the longest first, next to one another on one XCD
+      const int id = wir::remap_xcd(blockIdx.x, gridDim.x), item = id / a->blocks;
+      pair = item / a->heads * a->blocks + a->blocks - 1 - id % a->blocks;
       keys = keys_at(pair);
-      g = wir::Segment{item % a.heads, 0, wir::block_units(keys), true, -1, 1};
+      g = wir::Segment{item % a->heads, 0, wir::block_units(keys), true, -1, 1};
     } else {
       // every wave for itself: a lane takes `each` pairs
-      const int pairs = a.batch * a.blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
-      auto units = [&](int p) { return a.heads * wir::block_units(keys_at(p)); };
+      const int pairs = a->batch * a->blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
+      auto units = [&](int p) { return a->heads * wir::block_units(keys_at(p)); };
       int own = 0;
       for (int p = from; p < to; ++p) own += units(p);
       const int total = __builtin_amdgcn_readfirstlane(__shfl(wave_scan(own), 63));
-      if (a.least) {
-        share = wir::share_even(total, a.programs, pairs * a.heads, a.least);
-        auto parts = [&](int p) { return a.heads * wir::parts_even(wir::block_units(keys_at(p)), share); };
+      if (a->least) {
+        share = wir::share_even(total, a->programs, pairs * a->heads, a->least);
+        auto parts = [&](int p) { return a->heads * wir::parts_even(wir::block_units(keys_at(p)), share); };
         own = 0;
         for (int p = from; p < to; ++p) own += parts(p);
         if (!find(blockIdx.x, own, from, each, parts, pair, base)) return;
         keys = keys_at(pair);
         g = wir::segment_even(blockIdx.x, base, wir::block_units(keys), share);
       } else {
-        share = wir::share_of(total, a.programs, 1);
+        share = wir::share_of(total, a->programs, 1);
         u = blockIdx.x * share;
         if (!find(u, own, from, each, units, pair, base)) return;
         end = u + share < total ? u + share : total;
@@ -611,7 +646,7 @@ struct Program {
       segment(pair, keys, g);
       u += g.last - g.first;
       if (u >= end) break;
-      if (u == base + a.heads * wir::block_units(keys)) base = u, keys = keys_at(++pair);
+      if (u == base + a->heads * wir::block_units(keys)) base = u, keys = keys_at(++pair);
       g = wir::segment_at(u, base, wir::block_units(keys), end, share);
     }
   }
@@ -620,20 +655,20 @@ struct Program {
 // Partial results of a head's rows, joined in the order of their tiles:
 // program (row of the block, item).
 template <int D, int BLOCK>
-__device__ __forceinline__ void join(const attn_args& a) {
+__device__ __forceinline__ void join(args_ptr a) {
   constexpr int CH = D / 4, PER = 256 / CH;   // lanes of a row; partial results read side by side
   __shared__ float tops[256];
   __shared__ f32x4 sums[256];
   __shared__ float ls[PER];
-  const int per = min(a.tokens * a.group, BLOCK), item = blockIdx.x / per, row = blockIdx.x % per;
-  const int pair = item / a.heads, head = item - pair * a.heads, b = pair / a.blocks, rb = pair - b * a.blocks;
+  const int per = min(a->tokens * a->group, BLOCK), item = blockIdx.x / per, row = blockIdx.x % per;
+  const int pair = item / a->heads, head = item - pair * a->heads, b = pair / a->blocks, rb = pair - b * a->blocks;
   const int r = rb * BLOCK + row;
-  if (r >= a.tokens * a.group) return;
-  const int slot = a.info[2 * (i64)item], parts = a.info[2 * (i64)item + 1];
+  if (r >= a->tokens * a->group) return;
+  const int slot = a->info[2 * (i64)item], parts = a->info[2 * (i64)item + 1];
   if (parts <= 1) return;
-  const f32x2* ml = (const f32x2*)(a.partial + (i64)a.slots * BLOCK * D);
+  const f32x2* ml = (const f32x2*)(a->partial + (i64)a->slots * BLOCK * D);
   float top = -__builtin_inff();
-  for (int p = threadIdx.x; p < parts; p += 256) top = fmaxf(top, ml[(i64)wir::slot_of_part(slot, p, a.least > 0) * BLOCK + row][0]);
+  for (int p = threadIdx.x; p < parts; p += 256) top = fmaxf(top, ml[(i64)wir::slot_of_part(slot, p, a->least > 0) * BLOCK + row][0]);
   tops[threadIdx.x] = top;
   __syncthreads();
   for (int d = 128; d; d /= 2) {
@@ -647,11 +682,11 @@ __device__ __forceinline__ void join(const attn_args& a) {
   float l = 0.f;
 #pragma unroll 4
   for (int p = w; p < parts; p += PER) {
-    const i64 at = (i64)wir::slot_of_part(slot, p, a.least > 0) * BLOCK + row;
+    const i64 at = (i64)wir::slot_of_part(slot, p, a->least > 0) * BLOCK + row;
     const f32x2 y = ml[at];
     const float f = __builtin_amdgcn_exp2f(y[0] - base);
     l += f * y[1];
-    x += f * *(const f32x4*)(a.partial + at * D + 4 * ch);
+    x += f * *(const f32x4*)(a->partial + at * D + 4 * ch);
   }
   sums[threadIdx.x] = x;
   if (ch == 0) ls[w] = l;
@@ -671,12 +706,12 @@ __device__ __forceinline__ void join(const attn_args& a) {
 
 #define ATTN_KERNEL(NAME, D, NQ, WR, W, OCC)                                                                            \
   extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W), amdgpu_waves_per_eu(OCC, OCC))) \
-  NAME(const attn_args args) {                                                                                          \
+  NAME(const attn_args) {                                                                                          \
     __shared__ __attribute__((aligned(1024))) Program<D, NQ, WR, W>::Shared shared;                                     \
-    Program<D, NQ, WR, W>(args, shared).run();                                                                          \
+    Program<D, NQ, WR, W>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), shared).run();                                                                          \
   }
 #define JOIN_KERNEL(NAME, D, BLOCK) \
-  extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args args) { join<D, BLOCK>(args); }
+  extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) { join<D, BLOCK>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr()); }
 
 ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2)
