@@ -76,82 +76,32 @@ static void scales() {
   }
 }
 
-// Walks the programs as the kernel does.
+// Walks the programs as the kernels do.
 static void division() {
-  for (int it = 0; it < 20000; ++it) {
-    const int pairs = draw(1, 12), heads = draw(1, 5), programs = draw(1, 70), least = draw(1, 9);
-    std::vector<int> units(pairs);
-    for (int& n : units) n = draw(0, 9) ? draw(1, 30) : draw(1, 400);
-    int total = 0;
-    for (int n : units) total += heads * n;
-    const int share = share_of(total, programs, least);
-    CHECK(share >= least && (i64)share * programs >= total);
-    std::map<std::pair<int, int>, std::vector<int>> covered, slots;   // (pair, head) -> tiles, slots in order of tiles
-    std::map<std::pair<int, int>, std::pair<int, int>> info;          // -> (first slot, parts)
-    std::set<int> used;
-    for (int w = 0; w < programs; ++w) {
-      int u = w * share;
-      if (u >= total) break;
-      const int end = u + share < total ? u + share : total;
-      int pair = 0;
-      int base = 0;
-      while (u >= base + heads * units[pair]) base += heads * units[pair++];
-      while (u < end) {
-        const Segment g = segment_at(u, base, units[pair], end, share);
-        CHECK(g.head >= 0 && g.head < heads && g.first >= 0 && g.first < g.last && g.last <= units[pair]);
-        const std::pair<int, int> item(pair, g.head);
-        for (int t = g.first; t < g.last; ++t) covered[item].push_back(t);
-        const int slot = g.slot;
-        if (!g.whole) {
-          CHECK(slot >= 0 && slot < 2 * programs && slot / 2 == w && used.insert(slot).second);
-          slots[item].push_back(slot);
-        }
-        CHECK(g.whole == (g.parts == 1));
-        if (g.first == 0) info[item] = {slot, g.parts};
-        u += g.last - g.first;
-        if (u == base + heads * units[pair]) base = u, ++pair;
-      }
-      CHECK(u == end);
-    }
-    for (int p = 0; p < pairs; ++p)
-      for (int h = 0; h < heads; ++h) {
-        const std::pair<int, int> item(p, h);
-        CHECK((int)covered[item].size() == units[p]);
-        for (int t = 0; t < units[p]; ++t) CHECK(covered[item][t] == t);
-        CHECK(info.count(item));
-        const int parts = info[item].second;
-        if (slots[item].empty()) { CHECK(parts == 1); continue; }
-        CHECK(parts == (int)slots[item].size());
-        for (int i = 0; i < parts; ++i) CHECK(slot_of_part(info[item].first, i, false) == slots[item][i]);
-      }
-  }
-}
-
-// The same in equal parts of single heads.
-static void even_division() {
-  for (int it = 0; it < 20000; ++it) {
-    const int pairs = draw(1, 12), heads = draw(1, 5), least = draw(1, 9), programs = pairs * heads + draw(1, 90);
+  for (int it = 0; it < 40000; ++it) {
+    const int pairs = draw(1, 12), heads = draw(1, 5), least = draw(1, 9), extra = draw(1, 90);
     std::vector<int> units(pairs);
     for (int& n : units) n = draw(0, 9) ? draw(1, 30) : draw(1, 4000);
     int total = 0;
     for (int n : units) total += heads * n;
-    const int share = share_even(total, programs, pairs * heads, least);
-    int base = 0;
+    const int share = share_of(total, extra, least), width = slot_width(share);
+    std::set<int> used;
+    int programs = 0, begin = 0;
     for (int p = 0; p < pairs; ++p) {
-      const int parts = parts_even(units[p], share);
-      for (int h = 0; h < heads; ++h)
-        for (int n = 0, next = 0; n < parts; ++n) {
-          const int w = base + h * parts + n;
-          const Segment g = segment_even(w, base, units[p], share);
-          CHECK(g.head == h && g.first == next && g.last > g.first && g.last - g.first <= share);
-          CHECK(g.parts == parts && g.whole == (parts == 1) && g.slot == w);
-          CHECK(slot_of_part(base + h * parts, n, true) == w);
-          next = g.last;
-          CHECK(n + 1 < parts || next == units[p]);
+      const int parts = parts_of(units[p], share);
+      CHECK(parts >= 1 && parts <= units[p]);
+      for (int h = 0; h < heads; ++h, begin += units[p], programs += parts) {
+        CHECK(part_begin(0, units[p], parts) == 0 && part_begin(parts, units[p], parts) == units[p]);
+        for (int n = 0; n < parts; ++n) {
+          const int lo = part_begin(n, units[p], parts), hi = part_begin(n + 1, units[p], parts);
+          CHECK(hi > lo && hi - lo <= share);
+          if (parts == 1) continue;
+          const int slot = slot_of(begin + lo, width);
+          CHECK(slot >= 0 && slot < slots_for(extra) && used.insert(slot).second);
         }
-      base += heads * parts;
+      }
     }
-    CHECK(base <= programs);
+    CHECK(programs <= pairs * heads + extra && begin == total);
   }
 }
 
@@ -160,7 +110,6 @@ int main() {
   keys();
   scales();
   division();
-  even_division();
   std::puts("ok");
 }
 """

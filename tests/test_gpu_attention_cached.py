@@ -95,8 +95,8 @@ def test_long_sequences_in_many_parts(gpu, heads, hkv, tokens, d):
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
-@pytest.mark.parametrize("forced", [(16, 7, 0, 14), (16, 3, 0, 6), (128, 5, 0, 10), (32, 512, 0, 1024), (128, 0, 0, 0),
-                                    (16, 0, 0, 0), (16, 13, 1, 13), (32, 70, 1, 70), (128, 512, 2, 512), (128, 13, 9, 13)])
+@pytest.mark.parametrize("forced", [(16, 4, 7, 1), (16, 8, 3, 2), (128, 4, 5, 1), (32, 4, 512, 1), (128, 4, 0, 0),
+                                    (16, 8, 0, 0), (16, 4, 1, 1), (32, 8, 70, 1), (128, 4, 512, 2), (16, 4, 13, 9)])
 def test_every_division_gives_the_same(gpu, monkeypatch, forced):
     """Few programs that each take several heads' tiles, shares that end inside them, and no division."""
     lengths, counts = (130, 0, 400, 65), (3, 0, 3, 1)

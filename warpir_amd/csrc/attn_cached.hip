@@ -60,13 +60,12 @@ struct attn_args {
   bf16* out;                   // [B, H, T, D]
   float* lse;                  // [B, H, T]
   float* partial;              // [slots][block rows][D], then [slots][block rows][2]
-  int* info;                   // [items][2]: slot of the first partial result, how many
+  int* info;                   // [items][4]: first unit, units, parts, width of a slot
   i64 qb, qh, qt, ob, oh, ot, lb, lh, lt, tb;
   int batch, heads, group, tokens, page_shift, pages, columns;
   int blocks;                  // row blocks of a sequence and head
-  int programs;                // 0: one for each (sequence, block, head)
-  int least;                   // > 0: equal parts of single heads, of that many tiles at least
-  int slots;                   // of partial results
+  int extra;                   // programs beyond one for each (sequence, block, head) at most; 0: no division
+  int least;                   // tiles of a part at least, unless the head has fewer
 };
 
 // The arguments where the launch put them.  They fill most of the scalar registers: `fresh` makes the compiler read them
@@ -78,9 +77,6 @@ __device__ __forceinline__ args_ptr fresh(args_ptr a) {
   asm volatile("" : "+s"(p));
   return (args_ptr)p;
 }
-
-// (by value: a bit cast of a vector's element in place gives element 0)
-__device__ __forceinline__ unsigned bits_of(bf16 x) { return (unsigned)__builtin_bit_cast(unsigned short, x); }
 
 // The eight codes of two words, times a power of two, in bf16 (exact).
 __device__ __forceinline__ bf16x8 unpack8(unsigned a, unsigned b, float scale) {
@@ -153,15 +149,16 @@ struct Program {
   __device__ __forceinline__ wir::Span span_at(int seq) const {
     return wir::span_of(a->lengths[seq], a->counts ? a->counts[seq] : a->tokens, a->tokens, a->columns << a->page_shift);
   }
+  // (divisions that the plain decode step does not need are branched over: a step's whole path is a few microseconds)
+  __device__ __forceinline__ int sequence_of(int pair) const { return a->blocks == 1 ? pair : pair / a->blocks; }
+  __device__ __forceinline__ int token_of(int r) const { return a->tokens == 1 ? 0 : r / a->group; }
   __device__ __forceinline__ int keys_at(int pair) const {
-    return wir::block_keys(span_at(pair / a->blocks), pair % a->blocks, BLOCK, rows(), a->group);
+    const int seq = sequence_of(pair);
+    return wir::block_keys(span_at(seq), pair - seq * a->blocks, BLOCK, rows(), a->group);
   }
 
-  // Position that row r of the pair sees up to; -1: none.
-  __device__ __forceinline__ int position(int r) const {
-    const int t = r / a->group;
-    return r < rows() && t < span.count ? max(span.start + t, -1) : -1;
-  }
+  // Position that new token t sees up to; -1: none.
+  __device__ __forceinline__ int position_of(int t) const { return t < span.count ? max(span.start + t, -1) : -1; }
 
   // A wave's running softmax and output, and its queries as operands.
   struct State {
@@ -182,41 +179,37 @@ struct Program {
   __device__ __forceinline__ void begin(State& s, int head) const {
     const float c = (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));
     const int row0 = rb * BLOCK + wr * ROWS;
-    s.low = max(span.start + min(row0 / a->group, span.count), 0);
+    s.low = max(span.start + min(token_of(row0), span.count), 0);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int r = row0 + n * 16 + col;
-      s.pos[n] = position(r);
-      const int rr = r < rows() ? r : 0, t = rr / a->group;
+      const int rr = r < rows() ? r : 0, t = token_of(rr);
+      s.pos[n] = r < rows() ? position_of(t) : -1;
       const bf16* p = a->q + b * a->qb + (i64)(head * a->group + rr - t * a->group) * a->qh + t * a->qt + 16 * grp;
       bf16x8 x[2 * KC];
-      unsigned top = 0;
 #pragma unroll
       for (int u = 0; u < 2 * KC; ++u) x[u] = *(const bf16x8*)(p + u / 2 * 64 + u % 2 * 8);
+      float y[16 * KC], top = 0.f;
 #pragma unroll
-      for (int u = 0; u < 2 * KC; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned y = bits_of(x[u][e]) & 0x7fffu;
-          top = max(top, y < 0x7f80u ? y : 0u);
-        }
-      const float amax = over_groups(__uint_as_float(top << 16), [](float y, float z) { return fmaxf(y, z); });
-      const float scale = __uint_as_float(wir::scale_bits(__float_as_uint(amax))), inv = 1.0f / scale;
-      s.qs[n] = scale * c;
+      for (int e = 0; e < 16 * KC; ++e) {
+        y[e] = (float)x[e / 8][e % 8];
+        top = fmaxf(top, __builtin_fabsf(y[e]));
+      }
+      top = over_groups(top, [](float y, float z) { return fmaxf(y, z); });
+      // 2^e and 2^-e.  An infinite query's scores are all infinite or NaN, so its row is NaN; a NaN becomes a NaN code.
+      const unsigned scale = wir::scale_bits(__float_as_uint(top < __builtin_inff() ? top : 1.f));
+      const float inv = __uint_as_float((254u << 23) - scale);
+      s.qs[n] = top < __builtin_inff() ? __uint_as_float(scale) * c : __builtin_nanf("");
 #pragma unroll
       for (int w = 0; w < 4 * KC; ++w) {   // words of 4 values
-        float y[4], z[4];
+        float z[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[e] = (float)x[w / 2][w % 2 * 4 + e] * inv;
-          if (!(__builtin_fabsf(y[e]) < __builtin_inff())) y[e] = __builtin_nanf("");
-        }
-        unsigned hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0u, false);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], hi, true);
+        for (int e = 0; e < 4; ++e) z[e] = y[4 * w + e] * inv;
+        unsigned hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0u, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], hi, true);
         const f32x2 h0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), h1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-        z[0] = y[0] - h0[0], z[1] = y[1] - h0[1], z[2] = y[2] - h1[0], z[3] = y[3] - h1[1];
-        unsigned lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0u, false);
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], lo, true);
+        unsigned lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0] - h0[0], z[1] - h0[1], 0u, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[2] - h1[0], z[3] - h1[1], lo, true);
         s.q[n][0][w] = hi;
         if (KC == 2)
           s.q[n][1 % KC][w] = lo;
@@ -538,7 +531,7 @@ struct Program {
         x += f * *(const f32x4*)(sh.r.o + at * PITCH + 8 * ch);
         y += f * *(const f32x4*)(sh.r.o + at * PITCH + 8 * ch + 4);
       }
-      if (position(rb * BLOCK + row) < 0) {   // it took part in tiles that every row with a position sees
+      if (position_of(token_of(rb * BLOCK + row)) < 0) {   // it took part in tiles that every row with a position sees
         top = -__builtin_inff(), sum = 0.f;
         x = y = f32x4{0.f, 0.f, 0.f, 0.f};
       }
@@ -547,7 +540,7 @@ struct Program {
         *(f32x4*)to = x;
         *(f32x4*)(to + 4) = y;
         if (ch == 0)
-          *(f32x2*)(a->partial + (i64)a->slots * BLOCK * D + ((i64)slot * BLOCK + row) * 2) = f32x2{top, sum};
+          *(f32x2*)(a->partial + (i64)wir::slots_for(a->extra) * BLOCK * D + ((i64)slot * BLOCK + row) * 2) = f32x2{top, sum};
       } else {
         put(a, b, head, rb * BLOCK + row, ch, x, y, top, sum);
       }
@@ -557,7 +550,7 @@ struct Program {
   // 8 columns of a row's output and, with the first of them, its LSE; a row that sees nothing: 0 and -inf.
   static __device__ __forceinline__ void put(args_ptr a, int b, int head, int r, int ch, const f32x4& x,
                                              const f32x4& y, float top, float sum) {
-    const int t = r / a->group;
+    const int t = a->tokens == 1 ? 0 : r / a->group;
     const i64 h = head * a->group + r - t * a->group;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     bf16x8 v;
@@ -569,86 +562,67 @@ struct Program {
           sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 
-  __device__ __forceinline__ void segment(int pair, int keys, const wir::Segment& g) {
-    asm volatile("" : "+v"(col), "+v"(grp), "+v"(lane));
-    a = fresh(a);
-    b = pair / a->blocks;
-    rb = pair % a->blocks;
-    span = span_at(b);
-    walk(g.head, g.first, min(g.last, (keys + wir::TILE - 1) / wir::TILE));
-    __syncthreads();
-    a = fresh(a);
-    if (threadIdx.x == 0 && a->programs && g.first == 0) {
-      int* info = a->info + 2 * ((i64)pair * a->heads + g.head);
-      info[0] = g.slot;
-      info[1] = g.parts;
-    }
-    store(g.head, g.whole ? -1 : g.slot);
-    __syncthreads();
-  }
-
-  // The pair in which item u lies, of `own` items of this lane's pairs from .. and as many as `weight` says of each,
-  // and the items before the pair.  All lanes get them; false: there are no u items.
-  template <class Weight>
-  __device__ __forceinline__ bool find(int u, int own, int from, int each, Weight weight, int& pair, int& base) const {
-    const int upto = wave_scan(own);
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(u < upto);
-    if (past == 0) return false;
-    const int src = __builtin_ctzll(past);
-    int before = upto - own;
-    int p = from;
-    if (lane == src && each > 1) {
-      for (;; ++p) {
-        const int n = weight(p);
-        if (u < before + n) break;
-        before += n;
-      }
-    }
-    pair = __builtin_amdgcn_readfirstlane(__shfl(p, src));
-    base = __builtin_amdgcn_readfirstlane(__shfl(before, src));
-    return true;
-  }
-
   __device__ __forceinline__ void run() {
-    int pair, keys;
-    wir::Segment g;
-    int u = 0, end = 0, base = 0, share = 1;   // of a share over several heads
-    if (!a->programs) {   // a head's blocks, the longest first, next to one another on one XCD
-      const int id = wir::remap_xcd(blockIdx.x, gridDim.x), item = id / a->blocks;
-      pair = item / a->heads * a->blocks + a->blocks - 1 - id % a->blocks;
+    int pair, head, keys, first = 0, last, slot = -1;
+    if (!a->extra) {
+      int id = blockIdx.x;
+      if (a->blocks == 1) {
+        pair = id / a->heads;
+        head = id - pair * a->heads;
+      } else {   // a head's blocks, the longest first, next to one another on one XCD
+        id = wir::remap_xcd(id, gridDim.x);
+        const int item = id / a->blocks, seq = item / a->heads;
+        head = item - seq * a->heads;
+        pair = (seq + 1) * a->blocks - 1 - (id - item * a->blocks);
+      }
       keys = keys_at(pair);
-      g = wir::Segment{item % a->heads, 0, wir::block_units(keys), true, -1, 1};
+      last = wir::block_units(keys);
     } else {
       // every wave for itself: a lane takes `each` pairs
       const int pairs = a->batch * a->blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
-      auto units = [&](int p) { return a->heads * wir::block_units(keys_at(p)); };
-      int own = 0;
-      for (int p = from; p < to; ++p) own += units(p);
-      const int total = __builtin_amdgcn_readfirstlane(__shfl(wave_scan(own), 63));
-      if (a->least) {
-        share = wir::share_even(total, a->programs, pairs * a->heads, a->least);
-        auto parts = [&](int p) { return a->heads * wir::parts_even(wir::block_units(keys_at(p)), share); };
-        own = 0;
-        for (int p = from; p < to; ++p) own += parts(p);
-        if (!find(blockIdx.x, own, from, each, parts, pair, base)) return;
-        keys = keys_at(pair);
-        g = wir::segment_even(blockIdx.x, base, wir::block_units(keys), share);
-      } else {
-        share = wir::share_of(total, a->programs, 1);
-        u = blockIdx.x * share;
-        if (!find(u, own, from, each, units, pair, base)) return;
-        end = u + share < total ? u + share : total;
-        keys = keys_at(pair);
-        g = wir::segment_at(u, base, wir::block_units(keys), end, share);
+      auto units_of = [&](int p) { return wir::block_units(keys_at(p)); };
+      int units = 0, parts = 0;
+      for (int p = from; p < to; ++p) units += units_of(p);
+      const int units_to = a->heads * (pairs == 1 ? units : wave_scan(units));
+      const int share = wir::share_of(__builtin_amdgcn_readlane(units_to, pairs == 1 ? 0 : 63), a->extra, a->least);
+      for (int p = from; p < to; ++p) parts += wir::parts_of(units_of(p), share);
+      const int parts_to = a->heads * (pairs == 1 ? parts : wave_scan(parts));
+      // the program's pair, and the units and parts before it
+      const int id = blockIdx.x;
+      const unsigned long long past = __builtin_amdgcn_ballot_w64(lane < pairs && id < parts_to);
+      if (past == 0) return;
+      const int src = __builtin_ctzll(past);
+      int p = from, units_before = units_to - a->heads * units, parts_before = parts_to - a->heads * parts;
+      if (lane == src && each > 1) {
+        for (;; ++p) {
+          const int u = units_of(p), n = a->heads * wir::parts_of(u, share);
+          if (id < parts_before + n) break;
+          parts_before += n, units_before += a->heads * u;
+        }
+      }
+      pair = __builtin_amdgcn_readlane(p, src);
+      units_before = __builtin_amdgcn_readlane(units_before, src);
+      parts_before = __builtin_amdgcn_readlane(parts_before, src);
+      keys = keys_at(pair);
+      units = wir::block_units(keys);
+      parts = wir::parts_of(units, share);
+      head = (id - parts_before) / parts;
+      const int n = id - parts_before - head * parts, begin = units_before + head * units, width = wir::slot_width(share);
+      first = wir::part_begin(n, units, parts);
+      last = wir::part_begin(n + 1, units, parts);
+      if (parts > 1) slot = wir::slot_of(begin + first, width);
+      if (threadIdx.x == 0 && n == 0) {
+        int* info = a->info + 4 * ((i64)pair * a->heads + head);
+        info[0] = begin, info[1] = units, info[2] = parts, info[3] = width;
       }
     }
-    for (;;) {   // one segment, but for a share of several heads
-      segment(pair, keys, g);
-      u += g.last - g.first;
-      if (u >= end) break;
-      if (u == base + a->heads * wir::block_units(keys)) base = u, keys = keys_at(++pair);
-      g = wir::segment_at(u, base, wir::block_units(keys), end, share);
-    }
+    b = sequence_of(pair);
+    rb = pair - b * a->blocks;
+    span = span_at(b);
+    walk(head, first, min(last, (keys + wir::TILE - 1) / wir::TILE));
+    __syncthreads();
+    a = fresh(a);
+    store(head, slot);
   }
 };
 
@@ -657,32 +631,29 @@ struct Program {
 template <int D, int BLOCK>
 __device__ __forceinline__ void join(args_ptr a) {
   constexpr int CH = D / 4, PER = 256 / CH;   // lanes of a row; partial results read side by side
-  __shared__ float tops[256];
   __shared__ f32x4 sums[256];
   __shared__ float ls[PER];
-  const int per = min(a->tokens * a->group, BLOCK), item = blockIdx.x / per, row = blockIdx.x % per;
+  const int per = min(a->tokens * a->group, BLOCK), item = blockIdx.x / per, row = blockIdx.x - item * per;
+  const int* info = a->info + 4 * (i64)item;
+  const int begin = info[0], units = info[1], parts = info[2], width = info[3];
+  if (parts <= 1) return;
   const int pair = item / a->heads, head = item - pair * a->heads, b = pair / a->blocks, rb = pair - b * a->blocks;
   const int r = rb * BLOCK + row;
   if (r >= a->tokens * a->group) return;
-  const int slot = a->info[2 * (i64)item], parts = a->info[2 * (i64)item + 1];
-  if (parts <= 1) return;
-  const f32x2* ml = (const f32x2*)(a->partial + (i64)a->slots * BLOCK * D);
-  float top = -__builtin_inff();
-  for (int p = threadIdx.x; p < parts; p += 256) top = fmaxf(top, ml[(i64)wir::slot_of_part(slot, p, a->least > 0) * BLOCK + row][0]);
-  tops[threadIdx.x] = top;
-  __syncthreads();
-  for (int d = 128; d; d /= 2) {
-    if (threadIdx.x < d) tops[threadIdx.x] = fmaxf(tops[threadIdx.x], tops[threadIdx.x + d]);
-    __syncthreads();
-  }
-  top = tops[0];
+  const f32x2* ml = (const f32x2*)(a->partial + (i64)wir::slots_for(a->extra) * BLOCK * D);
+  auto place = [&](int p) { return (i64)wir::slot_of(begin + wir::part_begin(p, units, parts), width) * BLOCK + row; };
+  float top = -__builtin_inff();   // every wave for itself
+  for (int p = wir::lane_id(); p < parts; p += 64) top = fmaxf(top, ml[place(p)][0]);
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
   const float base = top == -__builtin_inff() ? 0.f : top;
   const int ch = threadIdx.x % CH, w = threadIdx.x / CH;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
 #pragma unroll 4
   for (int p = w; p < parts; p += PER) {
-    const i64 at = (i64)wir::slot_of_part(slot, p, a->least > 0) * BLOCK + row;
+    const i64 at = place(p);
     const f32x2 y = ml[at];
     const float f = __builtin_amdgcn_exp2f(y[0] - base);
     l += f * y[1];
@@ -694,6 +665,7 @@ __device__ __forceinline__ void join(args_ptr a) {
   if (threadIdx.x >= D / 8) return;
   f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
   l = 0.f;
+#pragma unroll
   for (int i = 0; i < PER; ++i) {
     lo += sums[i * CH + 2 * threadIdx.x];
     hi += sums[i * CH + 2 * threadIdx.x + 1];
@@ -714,6 +686,9 @@ __device__ __forceinline__ void join(args_ptr a) {
   extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) { join<D, BLOCK>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr()); }
 
 ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 2)
+ATTN_KERNEL(wir_attn_cached_d128_r16_w8, 128, 1, 1, 8, 2)
+ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2)

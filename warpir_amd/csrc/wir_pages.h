@@ -59,8 +59,12 @@ constexpr int TILE = 64;
 
 // Positions that some row of block rb sees: 0 .. keys - 1.
 WIR_HD int block_keys(const Span& s, int rb, int rows_per_block, int rows, int group) {
-  const int first = rb * rows_per_block / group;
-  const int last = imin((imin(rows, (rb + 1) * rows_per_block) - 1) / group, s.count - 1);
+  int first = 0, last = rows;   // tokens; one block has them all (and needs no division)
+  if (rows > rows_per_block) {
+    first = rb * rows_per_block / group;
+    last = (imin(rows, (rb + 1) * rows_per_block) - 1) / group;
+  }
+  last = imin(last, s.count - 1);
   if (first >= s.count || s.start + last < 0) return 0;
   return imin(s.start + last + 1, s.held);
 }
@@ -68,64 +72,25 @@ WIR_HD int block_keys(const Span& s, int rb, int rows_per_block, int rows, int g
 // Its units of work: tiles, and one where there are none (its rows are written all the same).
 WIR_HD int block_units(int keys) { return imax((int)(((unsigned)keys + TILE - 1) / TILE), 1); }
 
-// All units together, and so any unit's index, have to stay below 2^30 (64-bit
-// divisions cost microseconds here).
-//
-// Division of the units of all (sequence, block) pairs, heads of a pair in
-// turn, tiles of a head in turn, over the programs.
-//
-// With more heads than programs can have one each, a program takes `share`
-// consecutive units, parts of one or more heads.  One that takes part of a
-// head's units leaves a partial result in one of its two slots: the first
-// segment of its share in slot 2 * program, another one, which is then its
-// last, in 2 * program + 1.
-//
-// With fewer heads, a head's units go to parts_even(units) programs of its
-// own in equal parts, and program w's slot is w.
-WIR_HD int share_of(int total, int programs, int least) { return imax((total + programs - 1) / programs, least); }
+// Division of the work: a head's units go to parts_of(units) programs in
+// equal parts of at most `share`, in the order of (sequence, block) pairs,
+// their heads, and tiles.  `extra` bounds the programs: at most one a head and
+// `extra` more.  All units together have to stay below 2^30 (64-bit divisions
+// cost microseconds here).
+WIR_HD int share_of(int total, int extra, int least) { return imax((total + extra - 1) / extra, least); }
+WIR_HD int parts_of(int units, int share) { return (units + share - 1) / share; }
 
-struct Segment {
-  int head, first, last;   // tiles first .. last - 1 of the head's
-  bool whole;              // all of the head's
-  int slot, parts;         // of its partial result; partial results of the head
-};
-
-// Slot of the partial result of a segment that starts at unit u.
-WIR_HD int slot_of(int u, int share) { return 2 * (u / share) + (u % share ? 1 : 0); }
-
-// The segment at unit u of a pair whose units start at `base`, `units` a head; the program's share ends at `end`.
-WIR_HD Segment segment_at(int u, int base, int units, int end, int share) {
-  Segment g;
-  g.head = (u - base) / units;
-  g.first = (u - base) % units;
-  g.last = imin(units, g.first + end - u);
-  g.whole = g.first == 0 && g.last == units;
-  const int begin = u - g.first;
-  g.slot = slot_of(u, share);
-  g.parts = (begin + units - 1) / share - begin / share + 1;
-  return g;
+// First unit of part n; the first units % parts of them have one more.
+WIR_HD int part_begin(int n, int units, int parts) {
+  const int each = units / parts;
+  return n * each + imin(n, units - each * parts);
 }
 
-// Slot of a head's n-th partial result, from that of its first.
-WIR_HD int slot_of_part(int first, int n, bool even) { return even ? first + n : n == 0 ? first : 2 * (first / 2 + n); }
-
-// Equal parts: the share that gives all heads together at most `programs` of them (heads < programs).
-WIR_HD int share_even(int total, int programs, int heads, int least) { return share_of(total, programs - heads, least); }
-WIR_HD int parts_even(int units, int share) { return (units + share - 1) / share; }
-
-// Part n of the pair's parts, which start with program `base`.
-WIR_HD Segment segment_even(int program, int base, int units, int share) {
-  Segment g;
-  g.parts = parts_even(units, share);
-  g.head = (program - base) / g.parts;
-  const int n = (program - base) % g.parts;
-  // the first units % parts of them have one more
-  const int each = units / g.parts, more = units % g.parts;
-  g.first = n * each + imin(n, more);
-  g.last = g.first + each + (n < more ? 1 : 0);
-  g.whole = g.parts == 1;
-  g.slot = program;
-  return g;
-}
+// Where a partial result goes: the parts of divided heads have at least
+// share / 2 units, so no two of them start in the same such interval of all
+// units.  `begin`: the part's first unit among them.
+WIR_HD int slot_width(int share) { return imax(share / 2, 1); }
+WIR_HD int slot_of(int begin, int width) { return begin / width; }
+WIR_HD int slots_for(int extra) { return 3 * extra + 2; }
 
 }  // namespace wir

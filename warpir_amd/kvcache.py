@@ -165,25 +165,40 @@ class _AttnArgs(ctypes.Structure):
                                                  "out", "lse", "partial", "info")),
                 *((n, ctypes.c_longlong) for n in ("qb", "qh", "qt", "ob", "oh", "ot", "lb", "lh", "lt", "tb")),
                 *((n, ctypes.c_int) for n in ("batch", "heads", "group", "tokens", "page_shift", "pages", "columns",
-                                              "blocks", "programs", "least", "slots"))]
+                                              "blocks", "extra", "least"))]
 
 
 TILE = 64        # positions of a tile (csrc/wir_pages.h)
 
 
-def _attention_form(rows: int, items_of, columns: int, page: int):
-    """(rows of a block, programs, least, slots) of the kernel for ``rows`` query
+def _attention_form(rows: int, items_of, columns: int, page: int, d: int):
+    """(rows of a block, waves, extra, least) of the kernel for ``rows`` query
     rows a key/value head over a table of ``columns`` pages; ``items_of`` gives the
-    number of (sequence, block, head) for a block's rows.  Programs 0: one for
-    each of those; least 0: shares of all heads' tiles in turn, else equal
-    parts of single heads with at least that many tiles."""
+    number of (sequence, block, head) for a block's rows.  The heads' tiles are
+    divided over at most ``extra`` more programs than one for each of those, in
+    parts of at least ``least`` tiles; extra 0: no division.
+
+    A division costs a second launch and the partial results' way, ~3 us; a
+    head that is not divided is read by one CU at ~49 GB/s, against ~5 TB/s of
+    the chip, so it pays below ~105 heads and from ~150 kB of keys and values
+    in a head, or where one sequence may be far longer than the rest.  us,
+    divided / not (8 heads of D = 128 a sequence): 1 x 1000 keys 11.1 / 10.9, 1 x
+    4000 11.2 / 26.6, 4 x 2048 13.7 / 17.5, 16 x 2048 20.5 / 17.9, 32 x 512 12.8 / 9.7;
+    16 x 16 heads of D = 64, up to 2050 keys 16.6 / 13.4."""
     block = 16 if rows <= 16 else 32 if rows <= 32 else 128
-    items, programs = items_of(block), 512
-    if columns * page <= 8 * TILE or (block == 128 and items >= programs):
-        return block, 0, 0, 0
-    if items <= programs // 2:
-        return block, programs, 4, programs
-    return block, programs, 0, 2 * programs
+    items = items_of(block)
+    if block == 128:
+        return (block, 4, 0, 0) if items >= 512 else (block, 4, max(512 - items, 256), 4)
+    held = columns * page * 2 * d   # bytes of a head at most
+    if held <= 640 << 10 and held * (1 - items / 105) <= 147 << 10:
+        # eight waves a head while there is one such program for each CU
+        return block, 8 if items <= 256 and columns * page > 16 * TILE and (block, d) != (32, 128) else 4, 0, 0
+    # two programs of four waves a CU (32 sequences of up to 16000 keys, 256 heads: 384 more 96.6, 128 or 1024 over
+    # 99); with more heads, one of eight and as many more (64 sequences of up to 8192, 512 heads: 512 more of eight
+    # waves 119.6, 1536 of four 122)
+    if items <= 384 or (block, d) == (32, 128):
+        return block, 4, max(512 - items, 384), 2
+    return block, 8, 512, 2
 
 
 def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=None, lse=None,
@@ -229,16 +244,15 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     if page_table.shape[1] == 0:
         return out.zero_(), lse.fill_(float("-inf"))
     rows = tokens * group
-    block, programs, least, slots = _attention_form(rows, lambda n: batch * -(-rows // n) * heads,
-                                                    page_table.shape[1], page)
+    block, waves, extra, least = _attention_form(rows, lambda n: batch * -(-rows // n) * heads,
+                                                 page_table.shape[1], page, d)
     blocks = -(-rows // block)
     items = batch * blocks * heads
     need(fn, items * min(rows, block) < 1 << 24, "2^24 query rows or more in one call")
     need(fn, items * max(1, -(-page_table.shape[1] * page // TILE)) < 1 << 30, "2^30 tiles of keys or more in one call")
     args = _AttnArgs(*[None] * 12, *q.stride()[:3], *out.stride()[:3], *lse.stride(), page_table.stride(0), batch, heads,
-                     group, tokens, page.bit_length() - 1, cache.k.shape[0], page_table.shape[1], blocks, programs,
-                     least, slots)
-    floats = _workspace_floats(slots, block, d, items)
+                     group, tokens, page.bit_length() - 1, cache.k.shape[0], page_table.shape[1], blocks, extra, least)
+    floats = _workspace_floats(extra, block, d, items)
     if floats:
         if workspace is None:
             workspace = rec.alloc(torch.empty(floats, dtype=torch.float32, device=device))
@@ -249,10 +263,10 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     tensors = {"q": q, "k": cache.k, "v": cache.v, "k_scale": cache.k_scale, "v_scale": cache.v_scale,
                "table": page_table, "lengths": lengths, "counts": counts, "out": out, "lse": lse,
                "partial": workspace, "info": workspace}
-    past = {"info": 4 * (floats - 2 * items)}
-    launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}", (programs or items, 1, 1), (256, 1, 1),
-           args, tensors, past)
-    if programs:
+    past = {"info": 4 * (floats - 4 * items)}
+    launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}" + ("_w8" if waves == 8 else ""),
+           (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
+    if extra:
         launch(rec, device, "attn_cached.hsaco", f"wir_attn_join_d{d}_r{block}", (items * min(rows, block), 1, 1),
                (256, 1, 1), args, tensors, past)
     if rec:
@@ -260,10 +274,10 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     return out, lse
 
 
-def _workspace_floats(slots: int, block: int, d: int, items: int) -> int:
-    """A slot is a block's unnormalised rows, maxima and sums; two words of
-    every (sequence, block, head) say where its partial results are."""
-    return slots * block * (d + 2) + 2 * items if slots else 0
+def _workspace_floats(extra: int, block: int, d: int, items: int) -> int:
+    """Slots of partial results, each a block's unnormalised rows, maxima and
+    sums, and four words of every (sequence, block, head)."""
+    return (3 * extra + 2) * block * (d + 2) + 4 * items if extra else 0
 
 
 def attention_cached_workspace(q, cache: KVCache, page_table) -> int:
@@ -274,8 +288,8 @@ def attention_cached_workspace(q, cache: KVCache, page_table) -> int:
     def items(block):
         return q.shape[0] * -(-rows // block) * heads
 
-    block, _, _, slots = _attention_form(rows, items, page_table.shape[1], page)
-    return _workspace_floats(slots, block, d, items(block))
+    block, _, extra, _ = _attention_form(rows, items, page_table.shape[1], page, d)
+    return _workspace_floats(extra, block, d, items(block))
 
 
 __all__ = ["KVCache", "kv_cache_write", "kv_cache_read", "attention_cached", "attention_cached_workspace"]
