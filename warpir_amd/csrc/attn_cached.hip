@@ -5,16 +5,13 @@
 // scale for each page and head.  For query row r at position p:
 //   s_j = q . code_j * ks / sqrt(D) for j <= p,  O = sum_j softmax(s)_j vs code_j.
 //
-// First product: the codes go to v_mfma_f32_16x16x128_f8f6f4 as they are.  A
-// query row is written as 2^e (hi + lo) with two e4m3 terms, which hold bf16's
-// 8 bits of fraction (hi rounds to 4 of them, the rest has 4 more); what is
-// lost lies below 2^-19 of the row's largest value.  Two terms at twice the
-// bf16 rate cost what bf16 would, without converting K.  The scales and 2^e
-// multiply the fp32 score.
-//
-// Second product: codes times the power of two vs are exact in bf16, one
-// instruction for two values (what a scale has beside its power of two goes
-// to the probability), and probabilities are rounded to bf16 once.
+// Both products run on v_mfma_f32_16x16x32_bf16: e4m3 codes are exact in bf16,
+// also times a power of two, and one instruction converts two of them.  ks
+// multiplies the fp32 score; the power of two of vs goes to the values in
+// their conversion, what vs has beside it to the probabilities (which are
+// rounded to bf16 once).  (The first product on fp8 matrix instructions, with
+// q as the sum of two e4m3 terms, spares half the conversions, but those add
+// up with about 16 bits: scores were off by 1.4e-5 of sum |q k|.)
 //
 // Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, with 16
 // query rows (the heads that share a key/value head, and the new tokens) as
@@ -28,9 +25,10 @@
 // into registers, every byte once, with no LDS and no barrier in the loop; a
 // workgroup's waves take every WK-th tile and are joined at the end.  Bound by
 // the cache's bytes.
-// Many rows: a workgroup's waves take 32 rows each and share the tiles, which
-// LDS-DMA brings in the lanes' operand order (a fragment is 64 consecutive
-// 16-byte chunks), one tile ahead.
+// Many rows: a workgroup's waves take 32 rows each and share the tiles: each
+// wave converts its part of the next tile's codes and leaves them in LDS as
+// operands (a fragment is 64 lanes' 16 bytes in lane order), so that a code is
+// converted once for 128 rows.
 #include "wir_cdna4.h"
 #include "wir_pages.h"
 
@@ -44,7 +42,7 @@ using wir::f32x4;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) bf16x8 lds_bf16x8;
 
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -116,16 +114,19 @@ struct Program {
   static constexpr int ROWS = 16 * NQ;           // query rows of a wave
   static constexpr int BLOCK = ROWS * WR;        // and of the workgroup
   static constexpr int KC = D / 64, DT = D / 16, PITCH = D + 4;
-  static constexpr int CHUNKS = 4 * KC + DT;     // 1 KiB fragments of a tile
+  static constexpr int CHUNKS = 4 * KC + DT;     // of a tile's codes, 64 lanes' 16 bytes each
   static_assert(!SHARED || (WK == 1 && CHUNKS % (2 * W) == 0), "");
 
   struct Results {
     float o[W * ROWS * PITCH];
     float ml[W * ROWS * 2];
   };
-  union Shared {
-    Results r;
-    char ring[SHARED ? 2 * CHUNKS * 1024 : 16];
+  struct Shared {
+    union {
+      Results r;
+      char ring[SHARED ? 2 * CHUNKS * 2048 : 16];   // two tiles as operands
+    };
+    int nan_tile[2];                               // the tile there has NaN codes that not all rows see
   };
 
   args_ptr a;
@@ -162,8 +163,7 @@ struct Program {
 
   // A wave's running softmax and output, and its queries as operands.
   struct State {
-    i32x8 q[NQ][KC];      // D = 128: hi, lo of the 32 values of a lane; D = 64: both, 16 values each
-    float qs[NQ];         // 2^e log2(e) / sqrt(D)
+    bf16x8 q[NQ][2 * KC];   // in the order of K's 16-byte pieces
     int pos[NQ];
     int low;              // no row that sees anything sees less
     f32x4 o[DT][NQ];
@@ -177,7 +177,6 @@ struct Program {
   };
 
   __device__ __forceinline__ void begin(State& s, int head) const {
-    const float c = (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));
     const int row0 = rb * BLOCK + wr * ROWS;
     s.low = max(span.start + min(token_of(row0), span.count), 0);
 #pragma unroll
@@ -186,76 +185,50 @@ struct Program {
       const int rr = r < rows() ? r : 0, t = token_of(rr);
       s.pos[n] = r < rows() ? position_of(t) : -1;
       const bf16* p = a->q + b * a->qb + (i64)(head * a->group + rr - t * a->group) * a->qh + t * a->qt + 16 * grp;
-      bf16x8 x[2 * KC];
 #pragma unroll
-      for (int u = 0; u < 2 * KC; ++u) x[u] = *(const bf16x8*)(p + u / 2 * 64 + u % 2 * 8);
-      float y[16 * KC], top = 0.f;
-#pragma unroll
-      for (int e = 0; e < 16 * KC; ++e) {
-        y[e] = (float)x[e / 8][e % 8];
-        top = fmaxf(top, __builtin_fabsf(y[e]));
-      }
-      top = over_groups(top, [](float y, float z) { return fmaxf(y, z); });
-      // 2^e and 2^-e.  An infinite query's scores are all infinite or NaN, so its row is NaN; a NaN becomes a NaN code.
-      const unsigned scale = wir::scale_bits(__float_as_uint(top < __builtin_inff() ? top : 1.f));
-      const float inv = __uint_as_float((254u << 23) - scale);
-      s.qs[n] = top < __builtin_inff() ? __uint_as_float(scale) * c : __builtin_nanf("");
-#pragma unroll
-      for (int w = 0; w < 4 * KC; ++w) {   // words of 4 values
-        float z[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = y[4 * w + e] * inv;
-        unsigned hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0u, false);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], hi, true);
-        const f32x2 h0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), h1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-        unsigned lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[0] - h0[0], z[1] - h0[1], 0u, false);
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(z[2] - h1[0], z[3] - h1[1], lo, true);
-        s.q[n][0][w] = hi;
-        if (KC == 2)
-          s.q[n][1 % KC][w] = lo;
-        else
-          s.q[n][0][4 + w % 4] = lo;
-      }
+      for (int u = 0; u < 2 * KC; ++u) s.q[n][u] = *(const bf16x8*)(p + u / 2 * 64 + u % 2 * 8);
       s.m[n] = -__builtin_inff(), s.l[n] = 0.f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) s.o[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
 
-  // One tile: key(j) the K operand of tokens 16 g + 4 j .. + 3, value(d) the V words of column 16 d + col, read() once
-  // the keys are used.
-  template <class Key, class Value, class Read>
-  __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Value value, Read read) const {
+  // A lane's value scale vs = 2^e g by its bits: 2^e goes to the values, g to the probabilities (and out of their sum
+  // again).  Where the lane has no token it is 1.
+  static __device__ __forceinline__ unsigned scale_of(const Tokens& k) { return __float_as_uint(k.have ? k.vs : 1.f); }
+  static __device__ __forceinline__ float power_of(unsigned bits) {
+    return __uint_as_float(max(bits & 0x7f800000u, 0x00800000u));
+  }
+
+  // One tile: key(j, u) the K operand of tokens 16 g + 4 j .. + 3, read() what to do once the keys are used.  Through
+  // registers, value(d) gives the codes of column 16 d + col; through LDS, operand(d, u) the finished V operand, and
+  // value(d) the codes again for a tile with `nans`.
+  template <class Key, class Read, class Value, class Operand>
+  __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Read read, Value value, Operand operand,
+                                       bool nans) const {
     f32x4 x[4][NQ];
-    i32x8 k_of[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) k_of[j] = key(j);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        x[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NQ; ++n) x[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < KC; ++u)
-          x[j][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k_of[j], s.q[n][u], x[j][n], 0, 0, 0, 127, 0, 127);
+      for (int u = 0; u < 2 * KC; ++u) {
+        const bf16x8 y = key(j, u);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) x[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, s.q[n][u], x[j][n], 0, 0, 0);
       }
     }
     const int at = t * wir::TILE + 16 * grp;   // the lane's tokens: at .. at + have - 1
     const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
     read();
-    u32x4 v[DT];   // (from LDS they come under the softmax)
-#pragma unroll
-    for (int d = 0; d < DT; ++d) v[d] = value(d);
-    // vs = 2^e g: 2^e goes to the values, g to the probabilities (and out of their sum again)
-    const unsigned bits = __float_as_uint(k.have ? k.vs : 1.f);
-    const float power = __uint_as_float(max(bits & 0x7f800000u, 0x00800000u));
-    const float g = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+    const float g = __uint_as_float((scale_of(k) & 0x7fffffu) | 0x3f800000u);
     const float log_g = __builtin_amdgcn_logf(g), inv_g = __builtin_amdgcn_rcpf(g);
-    const float ks = k.have ? k.ks : 1.f;
+    // ks log2(e) / sqrt(D)
+    const float scale = (k.have ? k.ks : 1.f) * (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));
     bf16x8 p[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      float f = ks * s.qs[n];
+      float f = scale;
       if (edge) {
         const int seen = min(k.have, s.pos[n] - at + 1);   // of the lane's tokens
 #pragma unroll
@@ -289,49 +262,70 @@ struct Program {
         for (int d = 0; d < DT; ++d) s.o[d][n] *= corr;
       }
     }
-    // Values of a tile that not all rows see: bytes past the sequence's end
-    // become 0 (0 * NaN is NaN in the product), and so do NaN codes.
-    unsigned nans = 0;
-    if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u) != 0) {   // no scale: NaN
+    u32x4 v[SHARED ? 1 : DT];
+    float power = 1.f;
+    if constexpr (SHARED) {
+      if (nans) mark_nans(s, k.have, at, value);
+    } else {
+      const unsigned bits = scale_of(k);
+      power = power_of(bits);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) v[d] = value(d);
+      if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u) != 0) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v[d][w] = bits >= 0x7f800000u ? 0x7f7f7f7fu : v[d][w];
-    }
-    if (edge) {
+        for (int d = 0; d < DT; ++d) v[d] = scaled_codes(v[d], bits);
+      }
+      if (edge) {
+        const u32x4 held = held_bytes(k.have);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d) v[d] &= held;
+        if (unseen(k.have, at, s.low)) {
+          u32x4 some = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const unsigned there = held_bytes(v[d][w], k.have - 4 * w), bad = nan_bytes(there);
-          nans |= bad;
-          v[d][w] = there & ~bad;
+          for (int d = 0; d < DT; ++d) some |= nan_codes(v[d]);
+          if (__builtin_amdgcn_ballot_w64((some[0] | some[1] | some[2] | some[3]) != 0) != 0) {
+            mark_nans(s, k.have, at, [&](int d) { return v[d]; });
+#pragma unroll
+            for (int d = 0; d < DT; ++d) v[d] &= ~nan_codes(v[d]);
+          }
         }
+      }
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bf16x8 w = unpack8(v[d][2 * u], v[d][2 * u + 1], power);
+        bf16x8 w;
+        if constexpr (SHARED)
+          w = operand(d, u);
+        else
+          w = unpack8(v[d][2 * u], v[d][2 * u + 1], power);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s.o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, p[n][u], s.o[d][n], 0, 0, 0);
       }
-    if (edge && __builtin_amdgcn_ballot_w64(nans != 0) != 0) mark_nans(s, k.have, at, value);
   }
 
-  // The first n bytes of a word.
-  static __device__ __forceinline__ unsigned held_bytes(unsigned x, int n) {
-    return n >= 4 ? x : n <= 0 ? 0u : x & ((1u << 8 * n) - 1);
+  // Value codes past the sequence's end become 0 (0 * NaN is NaN in the product); those of a scale that is no number
+  // NaN.  NaN codes of a tile that not all rows see whole are marked instead.
+  static __device__ __forceinline__ u32x4 held_bytes(int n) {   // 0xff where a lane's 16 bytes hold a token
+    u32x4 m;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m[w] = n >= 4 * w + 4 ? ~0u : n <= 4 * w ? 0u : (1u << 8 * (n - 4 * w)) - 1;
+    return m;
   }
-  // 0xff where a byte is a NaN code, 0x7f or 0xff.
-  static __device__ __forceinline__ unsigned nan_bytes(unsigned x) {
-    return ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+  static __device__ __forceinline__ u32x4 nan_codes(const u32x4& v) {   // 0xff where a byte is 0x7f or 0xff
+    return ((((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
   }
-
-  // NaN values of such a tile make NaN of exactly the rows that see them, by a product of where they are with who sees
-  // them.
-  template <class Value>
-  __device__ __forceinline__ void mark_nans(State& s, int have, int at, Value value) const {
+  static __device__ __forceinline__ u32x4 scaled_codes(const u32x4& v, unsigned bits) {
+    return bits >= 0x7f800000u ? u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu} : v;
+  }
+  // Whether some held token of the tile may be seen by one row and not by another (never with one new token).
+  static __device__ __forceinline__ bool unseen(int have, int at, int low) {
+    return __builtin_amdgcn_ballot_w64(have > 0 && at + have - 1 > low) != 0;
+  }
+  // They make NaN of exactly the rows that see them, by a product of where they are with who sees them.
+  template <class Codes>
+  __device__ __forceinline__ void mark_nans(State& s, int have, int at, Codes codes) const {
     asm volatile("" : "+v"(have), "+v"(at));   // (its comparisons are made here, not kept from the masks')
     bf16x8 sees[NQ][2];
 #pragma unroll
@@ -340,10 +334,7 @@ struct Program {
       for (int e = 0; e < 16; ++e) sees[n][e / 8][e % 8] = (bf16)(e < min(have, s.pos[n] - at + 1) ? 1.f : 0.f);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const u32x4 v = value(d);
-      u32x4 is;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) is[w] = nan_bytes(held_bytes(v[w], have - 4 * w)) & 0x38383838u;   // 1.0 in e4m3
+      const u32x4 is = nan_codes(codes(d)) & 0x38383838u;   // 1.0 in e4m3
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         f32x4 count = {0.f, 0.f, 0.f, 0.f};
@@ -404,10 +395,6 @@ struct Program {
     return x.v + page_index(x, page) * x.page_bytes + in_page(x, t, grp);
   }
 
-  static __device__ __forceinline__ i32x8 key_operand(const u32x4& x, const u32x4& y) {
-    return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-  }
-
   // Tiles first .. last - 1 of `head`, every WK-th from the wave's, through registers: K of the next tile is in
   // flight during the softmax and the second product, V during the next tile's first product.
   __device__ __forceinline__ void walk_registers(State& s, int head, int first, int last) const {
@@ -438,19 +425,21 @@ struct Program {
     begin(s, head);
     for (; t < last; t += WK) {
       const Tokens now = tok;
-      tile(s, t, now, [&](int j) { return key_operand(kf[j][0], kf[j][KC - 1]); }, [&](int d) { return vf[d]; },
+      tile(s, t, now,
+           [&](int j, int u) { return unpack8(kf[j][u / 2][u % 2 * 2], kf[j][u / 2][u % 2 * 2 + 1], 1.f); },
            [&]() {
              if (t + WK >= last) return;
              const int page_k = next_k, page_v = next_v;
              if (t + 2 * WK < last) next_k = page_of(at, t + 2 * WK, col / 4), next_v = page_of(at, t + 2 * WK, grp);
              load_k(t + WK, page_k, page_v);
-           });
+           },
+           [&](int d) { return vf[d]; }, [](int, int) { return bf16x8{}; }, false);
       if (t + WK < last) load_v();
     }
   }
 
-  // The same through LDS, every tile for all waves: a wave brings CHUNKS / W of a tile's fragments, the first half of
-  // the waves K's, the others V's.  Everything asked for in one iteration is there in the next.
+  // The same through LDS, every tile for all waves.  In each iteration a wave asks for its CHUNKS / W of the next tile
+  // (the first half of the waves K's, the others V's), computes, and leaves what came as operands in the other slot.
   __device__ __forceinline__ void walk_shared(State& s, int head, int first, int last) const {
     constexpr int MINE = CHUNKS / W;
     const bool mine_k = wave < W / 2;
@@ -458,38 +447,72 @@ struct Program {
     const Bases at = bases(head);
     const unsigned char* base = mine_k ? at.k : at.v;
     const int token_bytes = mine_k ? D : 1;
-    auto bring = [&](int t, int slot, int page) {
+    u32x4 codes[MINE];
+    Tokens tok;
+    auto ask = [&](int t, int page, int own) {
       const unsigned char* from = base + page_index(at, page) * at.page_bytes + in_page(at, t, seg) * token_bytes;
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
         const int c = mine + i;
-        const int off = mine_k ? 4 * (c / KC) * D + 64 * (c % KC) : (16 * (c - 4 * KC)) << at.shift;
-        wir::dma16_v(from + off, wir::lds_addr(sh.ring + (slot * CHUNKS + c) * 1024));
+        codes[i] = *(const u32x4*)(from + (mine_k ? 4 * (c / KC) * D + 64 * (c % KC) : (16 * (c - 4 * KC)) << at.shift));
       }
+      scales_of(tok, at, t, own);
     };
-    Tokens tok;
-    int next = -1, next_own = -1, slot = 0;
-    if (first < last) {
-      const int page = page_of(at, first, seg), own = page_of(at, first, grp);
-      bring(first, 0, page);
-      scales_of(tok, at, first, own);
-      if (first + 1 < last) next = page_of(at, first + 1, seg), next_own = page_of(at, first + 1, grp);
-    }
     begin(s, head);
+    const int low = max(span.start + min(token_of(rb * BLOCK), span.count), 0);   // of all waves' rows
+    auto leave = [&](int t, int slot) {
+      float power = 1.f;
+      if (!mine_k) {
+        const unsigned bits = scale_of(tok);
+        power = power_of(bits);
+        const int first_token = t * wir::TILE + 16 * grp;
+        if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u || tok.have < 16 || first_token + 15 > low) != 0) {
+          const u32x4 held = held_bytes(tok.have);
+          u32x4 some = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < MINE; ++i) {
+            codes[i] = scaled_codes(codes[i], bits) & held;
+            some |= nan_codes(codes[i]);
+          }
+          if (unseen(tok.have, first_token, low)
+              && __builtin_amdgcn_ballot_w64((some[0] | some[1] | some[2] | some[3]) != 0) != 0) {
+            sh.nan_tile[slot] = t;
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) codes[i] &= ~nan_codes(codes[i]);
+          }
+        }
+      }
+      lds_bf16x8* to = (lds_bf16x8*)wir::lds(sh.ring + (slot * CHUNKS + mine) * 2048) + lane;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) to[(2 * i + u) * 64] = unpack8(codes[i][2 * u], codes[i][2 * u + 1], power);
+    };
+    int next = -1, next_own = -1, slot = 0;
+    if (threadIdx.x < 2) sh.nan_tile[threadIdx.x] = -1;
+    __syncthreads();
+    if (first < last) {
+      ask(first, page_of(at, first, seg), page_of(at, first, grp));
+      if (first + 1 < last) next = page_of(at, first + 1, seg), next_own = page_of(at, first + 1, grp);
+      leave(first, 0);
+    }
     for (int t = first; t < last; ++t, slot ^= 1) {
-      wir::wait_vm_barrier<0>();
-      // loaded before the wait: no later wait for them, which would count the transfers that follow
-      asm volatile("" : "+v"(tok.ks), "+v"(tok.vs), "+v"(next), "+v"(next_own));
+      __syncthreads();
       const Tokens now = tok;
       if (t + 1 < last) {
-        bring(t + 1, slot ^ 1, next);
-        scales_of(tok, at, t + 1, next_own);
+        const int page = next, own = next_own;
         if (t + 2 < last) next = page_of(at, t + 2, seg), next_own = page_of(at, t + 2, grp);
+        ask(t + 1, page, own);
       }
-      typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-      const lds_u32x4* from = (const lds_u32x4*)wir::lds(sh.ring + slot * CHUNKS * 1024) + lane;
-      tile(s, t, now, [&](int j) { return key_operand(from[j * KC * 64], from[(j * KC + KC - 1) * 64]); },
-           [&](int d) { return (u32x4)from[(4 * KC + d) * 64]; }, []() {});
+      const lds_bf16x8* from = (const lds_bf16x8*)wir::lds(sh.ring + slot * CHUNKS * 2048) + lane;
+      const bool nans = sh.nan_tile[slot] == t;
+      tile(s, t, now, [&](int j, int u) { return (bf16x8)from[(j * 2 * KC + u) * 64]; }, []() {},
+           [&](int d) {
+             const u32x4 v = *(const u32x4*)(value_at(at, t, page_of(at, t, grp)) + ((16 * d) << at.shift));
+             return scaled_codes(v, scale_of(now)) & held_bytes(now.have);
+           },
+           [&](int d, int u) { return (bf16x8)from[(8 * KC + 2 * d + u) * 64]; }, nans);
+      if (t + 1 < last) leave(t + 1, slot ^ 1);
     }
     __syncthreads();   // the ring is read: results go there
   }
