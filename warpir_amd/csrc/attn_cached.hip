@@ -126,7 +126,8 @@ struct Program {
       Results r;
       char ring[SHARED ? 2 * CHUNKS * 2048 : 16];   // two tiles as operands
     };
-    int nan_tile[2];                               // the tile there has NaN codes that not all rows see
+    int nan_from[D];   // first position with a NaN code in the column, of the tiles that not all rows see whole
+    int nan_any;
   };
 
   args_ptr a;
@@ -201,11 +202,10 @@ struct Program {
   }
 
   // One tile: key(j, u) the K operand of tokens 16 g + 4 j .. + 3, read() what to do once the keys are used.  Through
-  // registers, value(d) gives the codes of column 16 d + col; through LDS, operand(d, u) the finished V operand, and
-  // value(d) the codes again for a tile with `nans`.
+  // registers, value(d) gives the codes of column 16 d + col; through LDS, operand(d, u) the finished V operand.
   template <class Key, class Read, class Value, class Operand>
-  __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Read read, Value value, Operand operand,
-                                       bool nans) const {
+  __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Read read, Value value,
+                                       Operand operand) const {
     f32x4 x[4][NQ];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -264,9 +264,7 @@ struct Program {
     }
     u32x4 v[SHARED ? 1 : DT];
     float power = 1.f;
-    if constexpr (SHARED) {
-      if (nans) mark_nans(s, k.have, at, value);
-    } else {
+    if constexpr (!SHARED) {
       const unsigned bits = scale_of(k);
       power = power_of(bits);
 #pragma unroll
@@ -279,16 +277,7 @@ struct Program {
         const u32x4 held = held_bytes(k.have);
 #pragma unroll
         for (int d = 0; d < DT; ++d) v[d] &= held;
-        if (unseen(k.have, at, s.low)) {
-          u32x4 some = {0, 0, 0, 0};
-#pragma unroll
-          for (int d = 0; d < DT; ++d) some |= nan_codes(v[d]);
-          if (__builtin_amdgcn_ballot_w64((some[0] | some[1] | some[2] | some[3]) != 0) != 0) {
-            mark_nans(s, k.have, at, [&](int d) { return v[d]; });
-#pragma unroll
-            for (int d = 0; d < DT; ++d) v[d] &= ~nan_codes(v[d]);
-          }
-        }
+        if (unseen(k.have, at, s.low)) take_nans<DT>(v, 0, at);
       }
     }
 #pragma unroll
@@ -323,28 +312,22 @@ struct Program {
   static __device__ __forceinline__ bool unseen(int have, int at, int low) {
     return __builtin_amdgcn_ballot_w64(have > 0 && at + have - 1 > low) != 0;
   }
-  // They make NaN of exactly the rows that see them, by a product of where they are with who sees them.
-  template <class Codes>
-  __device__ __forceinline__ void mark_nans(State& s, int have, int at, Codes codes) const {
-    asm volatile("" : "+v"(have), "+v"(at));   // (its comparisons are made here, not kept from the masks')
-    bf16x8 sees[NQ][2];
+  // NaN codes out of the lane's tokens at .. of columns 16 (d + i) + col: a row that sees one of a column's is NaN there,
+  // which is so from the first of them on, so that is all `store` has to know.
+  template <int N>
+  __device__ __forceinline__ void take_nans(u32x4 (&v)[N], int d, int at) const {
+    u32x4 some = {0, 0, 0, 0};
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int i = 0; i < N; ++i) some |= nan_codes(v[i]);
+    if (__builtin_amdgcn_ballot_w64((some[0] | some[1] | some[2] | some[3]) != 0) == 0) return;
+    sh.nan_any = 1;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sees[n][e / 8][e % 8] = (bf16)(e < min(have, s.pos[n] - at + 1) ? 1.f : 0.f);
+    for (int i = 0; i < N; ++i) {
+      const u32x4 n = nan_codes(v[i]);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const u32x4 is = nan_codes(codes(d)) & 0x38383838u;   // 1.0 in e4m3
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        f32x4 count = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(unpack8(is[2 * u], is[2 * u + 1], 1.f), sees[n][u], count, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (count[i] > 0.f) s.o[d][n][i] = __builtin_nanf("");
-      }
+      for (int w = 3; w >= 0; --w)
+        if (n[w]) atomicMin(&sh.nan_from[16 * (d + i) + col], at + 4 * w + __builtin_ctz(n[w]) / 8);
+      v[i] &= ~n;
     }
   }
 
@@ -433,7 +416,7 @@ struct Program {
              if (t + 2 * WK < last) next_k = page_of(at, t + 2 * WK, col / 4), next_v = page_of(at, t + 2 * WK, grp);
              load_k(t + WK, page_k, page_v);
            },
-           [&](int d) { return vf[d]; }, [](int, int) { return bf16x8{}; }, false);
+           [&](int d) { return vf[d]; }, [](int, int) { return bf16x8{}; });
       if (t + WK < last) load_v();
     }
   }
@@ -468,18 +451,9 @@ struct Program {
         const int first_token = t * wir::TILE + 16 * grp;
         if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u || tok.have < 16 || first_token + 15 > low) != 0) {
           const u32x4 held = held_bytes(tok.have);
-          u32x4 some = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < MINE; ++i) {
-            codes[i] = scaled_codes(codes[i], bits) & held;
-            some |= nan_codes(codes[i]);
-          }
-          if (unseen(tok.have, first_token, low)
-              && __builtin_amdgcn_ballot_w64((some[0] | some[1] | some[2] | some[3]) != 0) != 0) {
-            sh.nan_tile[slot] = t;
-#pragma unroll
-            for (int i = 0; i < MINE; ++i) codes[i] &= ~nan_codes(codes[i]);
-          }
+          for (int i = 0; i < MINE; ++i) codes[i] = scaled_codes(codes[i], bits) & held;
+          if (unseen(tok.have, first_token, low)) take_nans<MINE>(codes, mine - 4 * KC, first_token);
         }
       }
       lds_bf16x8* to = (lds_bf16x8*)wir::lds(sh.ring + (slot * CHUNKS + mine) * 2048) + lane;
@@ -489,8 +463,6 @@ struct Program {
         for (int u = 0; u < 2; ++u) to[(2 * i + u) * 64] = unpack8(codes[i][2 * u], codes[i][2 * u + 1], power);
     };
     int next = -1, next_own = -1, slot = 0;
-    if (threadIdx.x < 2) sh.nan_tile[threadIdx.x] = -1;
-    __syncthreads();
     if (first < last) {
       ask(first, page_of(at, first, seg), page_of(at, first, grp));
       if (first + 1 < last) next = page_of(at, first + 1, seg), next_own = page_of(at, first + 1, grp);
@@ -505,13 +477,8 @@ struct Program {
         ask(t + 1, page, own);
       }
       const lds_bf16x8* from = (const lds_bf16x8*)wir::lds(sh.ring + slot * CHUNKS * 2048) + lane;
-      const bool nans = sh.nan_tile[slot] == t;
       tile(s, t, now, [&](int j, int u) { return (bf16x8)from[(j * 2 * KC + u) * 64]; }, []() {},
-           [&](int d) {
-             const u32x4 v = *(const u32x4*)(value_at(at, t, page_of(at, t, grp)) + ((16 * d) << at.shift));
-             return scaled_codes(v, scale_of(now)) & held_bytes(now.have);
-           },
-           [&](int d, int u) { return (bf16x8)from[(8 * KC + 2 * d + u) * 64]; }, nans);
+           [](int) { return u32x4{}; }, [&](int d, int u) { return (bf16x8)from[(8 * KC + 2 * d + u) * 64]; });
       if (t + 1 < last) leave(t + 1, slot ^ 1);
     }
     __syncthreads();   // the ring is read: results go there
@@ -554,7 +521,15 @@ struct Program {
         x += f * *(const f32x4*)(sh.r.o + at * PITCH + 8 * ch);
         y += f * *(const f32x4*)(sh.r.o + at * PITCH + 8 * ch + 4);
       }
-      if (position_of(token_of(rb * BLOCK + row)) < 0) {   // it took part in tiles that every row with a position sees
+      const int pos = position_of(token_of(rb * BLOCK + row));
+      if (sh.nan_any) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (sh.nan_from[8 * ch + i] <= pos) x[i] = __builtin_nanf("");
+          if (sh.nan_from[8 * ch + 4 + i] <= pos) y[i] = __builtin_nanf("");
+        }
+      }
+      if (pos < 0) {   // it took part in tiles that every row with a position sees
         top = -__builtin_inff(), sum = 0.f;
         x = y = f32x4{0.f, 0.f, 0.f, 0.f};
       }
@@ -586,6 +561,9 @@ struct Program {
   }
 
   __device__ __forceinline__ void run() {
+    for (int d = threadIdx.x; d < D; d += 64 * W) sh.nan_from[d] = 0x7fffffff;
+    if (threadIdx.x == 0) sh.nan_any = 0;
+    __syncthreads();
     int pair, head, keys, first = 0, last, slot = -1;
     if (!a->extra) {
       int id = blockIdx.x;
@@ -708,12 +686,12 @@ __device__ __forceinline__ void join(args_ptr a) {
 #define JOIN_KERNEL(NAME, D, BLOCK) \
   extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) { join<D, BLOCK>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr()); }
 
-ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 2)
+ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 4)
+ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 4)
 ATTN_KERNEL(wir_attn_cached_d128_r16_w8, 128, 1, 1, 8, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 3)
 ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 1)
 ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2)
