@@ -207,6 +207,7 @@ struct Program {
   __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Read read, Value value,
                                        Operand operand) const {
     f32x4 x[4][NQ];
+    if (SHARED) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -218,6 +219,7 @@ struct Program {
         for (int n = 0; n < NQ; ++n) x[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, s.q[n][u], x[j][n], 0, 0, 0);
       }
     }
+    if (SHARED) __builtin_amdgcn_s_setprio(0);
     const int at = t * wir::TILE + 16 * grp;   // the lane's tokens: at .. at + have - 1
     const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
     read();

@@ -76,6 +76,11 @@ __device__ __forceinline__ unsigned rescale(unsigned w, float ratio) {
   return pack4(a[0] * ratio, a[1] * ratio, b[0] * ratio, b[1] * ratio);
 }
 
+__device__ __forceinline__ void rescale2(unsigned* at, float ratio) {
+  const u32x2 w = *(const u32x2*)at;
+  *(u32x2*)at = u32x2{rescale(w[0], ratio), rescale(w[1], ratio)};
+}
+
 // Workgroup -> one page of one sequence and head, of K or of V.  A lane takes
 // 4 tokens x 8 columns; PASSES of 256 lanes cover the largest page.
 template <int D>
@@ -102,26 +107,35 @@ __device__ __forceinline__ void write(const kv_args& a) {
   const bool kept = lo > base;   // (the page then holds positions base .. lo - 1)
   const float was = side.scales[index];
 
-  // lane -> tokens 4 r .. 4 r + 3 of the page and columns 8 c .. 8 c + 7; neighbours in K's store order or V's
+  // lane -> tokens 4 r .. 4 r + 3 of the page and columns 8 c .. 8 c + 7: neighbours in K's store order or, for whole
+  // V pages, in V's (a few tokens then keep to few waves, and the others skip the work)
   const int groups = a.page / 4, lanes = groups * COLS;
+  const bool by_token = is_v && hi - lo >= 16;
   const bf16* x = side.x + b * side.xb + h * side.xh;
   bf16x8 val[PASSES][4];
+  unsigned had[PASSES][8];   // V words that keep some of their codes
   unsigned top = 0;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int l = p * 256 + threadIdx.x, r = is_v ? l % groups : l / COLS, c = is_v ? l / groups : l % COLS;
+    const int l = p * 256 + threadIdx.x, r = by_token ? l % groups : l / COLS, c = by_token ? l / groups : l % COLS;
+    const int pos = base + 4 * r;
+    if (l >= lanes || pos >= hi || pos + 4 <= lo) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int pos = base + 4 * r + i;
-      bf16x8 y = {};
-      if (l < lanes && pos >= lo && pos < hi) y = *(const bf16x8*)(x + (pos - s.start) * side.xt + 8 * c);
-      val[p][i] = y;
+      val[p][i] = bf16x8{};
+      if (pos + i >= lo && pos + i < hi) val[p][i] = *(const bf16x8*)(x + (pos + i - s.start) * side.xt + 8 * c);
+    }
+    if (is_v && (pos < lo || pos + 4 > hi)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) had[p][j] = codes[(8 * c + j) * groups + r];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const unsigned m = bits_of(y[j]) & 0x7fffu;
+        const unsigned m = bits_of(val[p][i][j]) & 0x7fffu;
         top = max(top, m < 0x7f80u ? m : 0u);
       }
-    }
   }
   const float enough = __uint_as_float(wir::scale_bits(group_max(top) << 16));
   const float scale = kept && was >= enough ? was : enough;
@@ -131,9 +145,21 @@ __device__ __forceinline__ void write(const kv_args& a) {
 
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int l = p * 256 + threadIdx.x, r = is_v ? l % groups : l / COLS, c = is_v ? l / groups : l % COLS;
+    const int l = p * 256 + threadIdx.x, r = by_token ? l % groups : l / COLS, c = by_token ? l / groups : l % COLS;
     const int pos = base + 4 * r;
-    if (l >= lanes || pos >= hi || (pos + 4 <= lo && !grown)) continue;
+    if (l >= lanes || pos >= hi) continue;
+    unsigned* to = codes + (8 * c * a.page + 4 * r) / 4;   // V: word j the four tokens of column 8 c + j
+    if (pos + 4 <= lo) {   // tokens that were there
+      if (!grown) continue;
+      if (is_v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j * groups] = rescale(to[j * groups], ratio);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rescale2(codes + ((4 * r + i) * D + 8 * c) / 4, ratio);
+      }
+      continue;
+    }
     float y[4][8];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -143,36 +169,29 @@ __device__ __forceinline__ void write(const kv_args& a) {
         y[i][j] = __builtin_fabsf(z) < __builtin_inff() ? z * inv : __builtin_nanf("");
       }
     if (is_v) {
-      // word j: the four tokens of column 8 c + j
       unsigned fresh = 0, old = 0;   // masks of the word's bytes
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (pos + i >= lo && pos + i < hi) fresh |= 0xffu << 8 * i;
         if (pos + i < lo) old |= 0xffu << 8 * i;
       }
-      unsigned* to = codes + (8 * c * a.page + 4 * r) / 4;
-      unsigned had[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) had[j] = fresh != ~0u ? to[j * groups] : 0u;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         unsigned w = pack4(y[0][j], y[1][j], y[2][j], y[3][j]);
         if (fresh != ~0u) {
-          const unsigned again = grown ? rescale(had[j], ratio) : had[j];
-          w = (w & fresh) | (again & old) | (had[j] & ~(fresh | old));
+          const unsigned again = grown ? rescale(had[p][j], ratio) : had[p][j];
+          w = (w & fresh) | (again & old) | (had[p][j] & ~(fresh | old));
         }
         to[j * groups] = w;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u32x2* to = (u32x2*)(codes + ((4 * r + i) * D + 8 * c) / 4);
-        if (pos + i >= lo && pos + i < hi) {
-          *to = u32x2{pack4(y[i][0], y[i][1], y[i][2], y[i][3]), pack4(y[i][4], y[i][5], y[i][6], y[i][7])};
-        } else if (pos + i < lo && grown) {
-          const u32x2 w = *to;
-          *to = u32x2{rescale(w[0], ratio), rescale(w[1], ratio)};
-        }
+        unsigned* row = codes + ((4 * r + i) * D + 8 * c) / 4;
+        if (pos + i >= lo && pos + i < hi)
+          *(u32x2*)row = u32x2{pack4(y[i][0], y[i][1], y[i][2], y[i][3]), pack4(y[i][4], y[i][5], y[i][6], y[i][7])};
+        else if (pos + i < lo && grown)
+          rescale2(row, ratio);
       }
     }
   }

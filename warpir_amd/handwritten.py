@@ -7,8 +7,9 @@ import ctypes
 import functools
 from typing import Dict, Optional, Sequence
 
+from warpir_amd import plans
 from warpir_amd.plans import Plans
-from warpir_amd.runtime import RawKernel
+from warpir_amd.runtime import RawKernel, check
 
 INT_MAX = 2 ** 31 - 1
 
@@ -104,19 +105,22 @@ class DevicePlans(Plans):
     """Plans that are replayed on the current device only: the default stream
     of another one has no handle of its own."""
 
-    def run(self, flags: int, first, *tensors):
+    _one_device = False
+
+    def run(self, flags: int, *tensors):
+        if self._one_device:   # (the common call: no more Python than this)
+            r = plans._native.run(self._table, flags, *tensors)
+            if type(r) is not int:
+                return r
+            check(r, self.what)
         import torch
 
-        if _devices() > 1 and getattr(first, "is_cuda", False) and first.device.index != torch.cuda.current_device():
+        first = tensors[0]
+        if not getattr(first, "is_cuda", False) or first.device.index != torch.cuda.current_device():
             return None
-        return super().run(flags, first, *tensors)
-
-
-@functools.lru_cache(maxsize=None)
-def _devices() -> int:
-    import torch
-
-    return torch.cuda.device_count()
+        r = super().run(flags, *tensors)
+        self._one_device = self._table is not None and torch.cuda.device_count() == 1
+        return r
 
 
 __all__ = ["check_tensor", "check_written", "need", "launch", "on", "DevicePlans", "INT_MAX"]

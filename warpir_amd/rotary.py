@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from typing import Optional, Tuple
 
@@ -44,9 +45,10 @@ def rope_table(positions: int, d: int, base: float = 10000.0, device="cuda"):
     return angle.cos().float(), angle.sin().float()
 
 
+@functools.lru_cache(maxsize=64, typed=True)
 def _flags(eps: float, interleaved) -> Optional[int]:
     """The plan's flags: interleaved and the bits of eps; None for values that are refused."""
-    if type(eps) is not float or type(interleaved) is not bool or not 0.0 <= eps < 1e30:
+    if not 0.0 <= eps < 1e30:
         return None
     return struct.unpack("I", struct.pack("f", eps))[0] << 1 | interleaved
 
@@ -111,7 +113,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
     import torch
 
     fn = "qk_norm_rope"
-    flags, done = _flags(eps, interleaved), None
+    flags, done = _flags(eps, interleaved) if type(eps) is float and type(interleaved) is bool else None, None
     if flags is not None:
         done = _forward_plans.run(flags, q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out)
         if done is not None and done is not False:
@@ -156,7 +158,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     import torch
 
     fn = "qk_norm_rope_backward"
-    flags, done = _flags(eps, interleaved), None
+    flags, done = _flags(eps, interleaved) if type(eps) is float and type(interleaved) is bool else None, None
     given = (dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions, dq, dk, dq_weight, dk_weight)
     if flags is not None and workspace is None:
         done = _backward_plans.run(flags, *given)
