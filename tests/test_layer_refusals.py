@@ -194,3 +194,47 @@ def test_empty_cache_and_table():
     assert cos.shape == (1 << 20, 32) and abs(float(cos[999999, 0]) - math.cos(999999)) < 2 ** -24
     with pytest.raises(ValueError):
         api.rope_table(0, 64, device="cpu")
+
+
+@pytest.mark.parametrize("change,error", CACHE_REFUSALS + [
+    (dict(q=_fake(3, 4, 5, 128)), "q must have shape"),
+    (dict(q=_fake(2, 4, 5, 64)), "q must have shape"),
+    (dict(q=_fake(3, 4, 5, 64, dtype=f32)), "q must be bfloat16"),
+    (dict(q=_fake(3, 4, 64, 5).transpose(2, 3)), "last dimension"),
+    (dict(q=_fake(3, 3, 5, 64)), "not a multiple of 2"),
+    (dict(q=_fake(3, 0, 5, 64)), "not a multiple of 2"),
+    (dict(counts=_fake(3, dtype=torch.int64)), "counts must be int32"),
+    (dict(out=_fake(3, 4, 4, 64)), "out must have shape"),
+    (dict(out=_fake(3, 1, 5, 64).expand(3, 4, 5, 64)), "overlap"),
+    (dict(lse=_fake(3, 4, 5)), "lse must be float32"),
+    (dict(lse=_fake(3, 4, 1, dtype=f32).expand(3, 4, 5)), "overlap"),
+    (dict(page_table=_fake(3, 1 << 10, dtype=i32), workspace=_fake(64, dtype=f32)), "workspace needs"),
+    (dict(page_table=_fake(3, 1 << 10, dtype=i32), workspace=_fake(1 << 24)), "workspace must be float32"),
+    (dict(q=_fake(3, 4, 1, 64).expand(3, 4, 1 << 23, 64), out=_fake(3, 4, 1 << 23, 64),
+          lse=_fake(3, 4, 1 << 23, dtype=f32)), "2\\^24 query rows"),
+    (dict(q=_fake(3, 4, 1, 64).expand(3, 4, 1 << 20, 64), out=_fake(3, 4, 1 << 20, 64), lse=_fake(3, 4, 1 << 20, dtype=f32),
+          page_table=_fake(3, 1 << 21, dtype=i32)), "2\\^30 tiles"),
+])
+def test_attention_cached(monkeypatch, change, error):
+    _lenient(monkeypatch)
+    a = dict(q=_fake(3, 4, 5, 64), cache=_cache(), page_table=_fake(3, 4, dtype=i32), lengths=_fake(3, dtype=i32),
+             out=_fake(3, 4, 5, 64), lse=_fake(3, 4, 5, dtype=f32))
+    with pytest.raises((ValueError, TypeError), match=error):
+        api.attention_cached(**{**a, **change})
+
+
+def test_attention_cached_asks_for_memory_last():
+    with pytest.raises(ValueError, match="no memory"):
+        api.attention_cached(_fake(3, 4, 5, 64), _cache(), _fake(3, 4, dtype=i32), _fake(3, dtype=i32))
+
+
+def test_attention_forms_hold_their_bounds():
+    """The kernels' launch: a known kernel, at least one program a head, and slots for what `extra` allows."""
+    for rows in (1, 16, 17, 32, 33, 1000):
+        for heads in (1, 7, 100, 300, 600, 5000):
+            for columns, page in ((1, 16), (8, 64), (40, 128), (4096, 64)):
+                for d in (64, 128):
+                    block, waves, extra, least = kvcache._attention_form(rows, lambda n: heads * -(-rows // n), columns, page, d)
+                    assert block in (16, 32, 128) and rows <= block or block == 128
+                    assert waves == 4 or block == 16 or (block, d) == (32, 64)
+                    assert extra >= 0 and (least > 0) == (extra > 0)
