@@ -207,7 +207,6 @@ struct Program {
   __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Read read, Value value,
                                        Operand operand) const {
     f32x4 x[4][NQ];
-    if (SHARED) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -219,7 +218,7 @@ struct Program {
         for (int n = 0; n < NQ; ++n) x[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, s.q[n][u], x[j][n], 0, 0, 0);
       }
     }
-    if (SHARED) __builtin_amdgcn_s_setprio(0);
+    if (SHARED) fragments_ahead<8 * KC>();
     const int at = t * wir::TILE + 16 * grp;   // the lane's tokens: at .. at + have - 1
     const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
     read();
@@ -227,18 +226,21 @@ struct Program {
     const float log_g = __builtin_amdgcn_logf(g), inv_g = __builtin_amdgcn_rcpf(g);
     // ks log2(e) / sqrt(D)
     const float scale = (k.have ? k.ks : 1.f) * (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));
-    bf16x8 p[NQ][2];
+    const float f = edge ? 1.f : scale;
+    if (edge) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float f = scale;
-      if (edge) {
+      for (int n = 0; n < NQ; ++n) {
         const int seen = min(k.have, s.pos[n] - at + 1);   // of the lane's tokens
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[j][n][i] = 4 * j + i < seen ? x[j][n][i] * f : -__builtin_inff();
-        f = 1.f;
+          for (int i = 0; i < 4; ++i) x[j][n][i] = 4 * j + i < seen ? x[j][n][i] * scale : -__builtin_inff();
       }
+    }
+    float corr[NQ], shift[NQ];
+    bool rescale = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
       float top = x[0][n][0];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -246,23 +248,31 @@ struct Program {
         for (int i = 0; i < 4; ++i) top = fmaxf(top, x[j][n][i]);
       top = fmaxf(over_groups(top * f, [](float y, float z) { return fmaxf(y, z); }), s.m[n]);
       const float base = top == -__builtin_inff() ? 0.f : top;
-      const float corr = __builtin_amdgcn_exp2f(s.m[n] - base);
+      corr[n] = __builtin_amdgcn_exp2f(s.m[n] - base);
+      shift[n] = log_g - base;
       s.m[n] = top;
-      const float shift = log_g - base;
+      s.l[n] *= corr[n];
+      rescale |= corr[n] != 1.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(rescale) != 0) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) s.o[d][n] *= corr[n];
+    }
+    bf16x8 p[NQ][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][n][i], f, shift));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][n][i], f, shift[n]));
           sum[i % 2] += y;
           p[n][j / 2][j % 2 * 4 + i] = (bf16)y;
         }
-      s.l[n] = s.l[n] * corr + (sum[0] + sum[1]) * inv_g;
-      if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d) s.o[d][n] *= corr;
-      }
+      s.l[n] += (sum[0] + sum[1]) * inv_g;
     }
     u32x4 v[SHARED ? 1 : DT];
     float power = 1.f;
@@ -294,6 +304,19 @@ struct Program {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s.o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, p[n][u], s.o[d][n], 0, 0, 0);
       }
+    if (SHARED) fragments_ahead<2 * DT>();
+  }
+
+  template <int N>
+  static __device__ __forceinline__ void fragments_ahead() {
+    constexpr int AHEAD = 8;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, NQ, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, NQ * AHEAD, 0);
   }
 
   // Value codes past the sequence's end become 0 (0 * NaN is NaN in the product); those of a scale that is no number
@@ -467,17 +490,14 @@ struct Program {
     int next = -1, next_own = -1, slot = 0;
     if (first < last) {
       ask(first, page_of(at, first, seg), page_of(at, first, grp));
-      if (first + 1 < last) next = page_of(at, first + 1, seg), next_own = page_of(at, first + 1, grp);
+      next = page_of(at, first + 1, seg), next_own = page_of(at, first + 1, grp);
       leave(first, 0);
     }
     for (int t = first; t < last; ++t, slot ^= 1) {
       __syncthreads();
       const Tokens now = tok;
-      if (t + 1 < last) {
-        const int page = next, own = next_own;
-        if (t + 2 < last) next = page_of(at, t + 2, seg), next_own = page_of(at, t + 2, grp);
-        ask(t + 1, page, own);
-      }
+      ask(t + 1, next, next_own);
+      next = page_of(at, t + 2, seg), next_own = page_of(at, t + 2, grp);   // (past the end -1, or pages not used)
       const lds_bf16x8* from = (const lds_bf16x8*)wir::lds(sh.ring + slot * CHUNKS * 2048) + lane;
       tile(s, t, now, [&](int j, int u) { return (bf16x8)from[(j * 2 * KC + u) * 64]; }, []() {},
            [](int) { return u32x4{}; }, [&](int d, int u) { return (bf16x8)from[(8 * KC + 2 * d + u) * 64]; });
