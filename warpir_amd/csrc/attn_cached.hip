@@ -649,52 +649,57 @@ struct Program {
   }
 };
 
-// Partial results of a head's rows, joined in the order of their tiles:
-// program (row of the block, item).
-template <int D, int BLOCK>
+// Partial results of a head's rows, joined in the order of their tiles: a
+// workgroup takes one row, its waves' lanes reading 1024 / D partial results
+// side by side, or, for launches with many rows and so few partial results
+// of each, one row a wave (ROWS = 4).
+template <int D, int BLOCK, int ROWS>
 __device__ __forceinline__ void join(args_ptr a) {
-  constexpr int CH = D / 4, PER = 256 / CH;   // lanes of a row; partial results read side by side
+  constexpr int CH = D / 4, PER = 256 / ROWS / CH;   // lanes of a row; partial results read side by side
   __shared__ f32x4 sums[256];
-  __shared__ float ls[PER];
-  const int per = min(a->tokens * a->group, BLOCK), item = blockIdx.x / per, row = blockIdx.x - item * per;
+  __shared__ float ls[ROWS * PER];
+  const int per = (min(a->tokens * a->group, BLOCK) + ROWS - 1) / ROWS;   // programs of an item
+  const int item = blockIdx.x / per, sub = ROWS == 1 ? 0 : wir::wave_id(), lane = threadIdx.x % (256 / ROWS);
+  const int row = (blockIdx.x - item * per) * ROWS + sub;
   const int* info = a->info + 4 * (i64)item;
   const int begin = info[0], units = info[1], parts = info[2], width = info[3];
   if (parts <= 1) return;
   const int pair = item / a->heads, head = item - pair * a->heads, b = pair / a->blocks, rb = pair - b * a->blocks;
   const int r = rb * BLOCK + row;
-  if (r >= a->tokens * a->group) return;
+  const bool mine = row < BLOCK && r < a->tokens * a->group;
   const f32x2* ml = (const f32x2*)(a->partial + (i64)wir::slots_for(a->extra) * BLOCK * D);
   auto place = [&](int p) { return (i64)wir::slot_of(begin + wir::part_begin(p, units, parts), width) * BLOCK + row; };
-  float top = -__builtin_inff();   // every wave for itself
-  for (int p = wir::lane_id(); p < parts; p += 64) top = fmaxf(top, ml[place(p)][0]);
+  const int ch = lane % CH, w = lane / CH;
+  float top = -__builtin_inff(), l = 0.f;
+  if (mine) {
+    for (int p = wir::lane_id(); p < parts; p += 64) top = fmaxf(top, ml[place(p)][0]);   // every wave for itself
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-  top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
-  const float base = top == -__builtin_inff() ? 0.f : top;
-  const int ch = threadIdx.x % CH, w = threadIdx.x / CH;
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
+    for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
+    const float base = top == -__builtin_inff() ? 0.f : top;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int p = w; p < parts; p += PER) {
-    const i64 at = place(p);
-    const f32x2 y = ml[at];
-    const float f = __builtin_amdgcn_exp2f(y[0] - base);
-    l += f * y[1];
-    x += f * *(const f32x4*)(a->partial + at * D + 4 * ch);
+    for (int p = w; p < parts; p += PER) {
+      const i64 at = place(p);
+      const f32x2 y = ml[at];
+      const float f = __builtin_amdgcn_exp2f(y[0] - base);
+      l += f * y[1];
+      x += f * *(const f32x4*)(a->partial + at * D + 4 * ch);
+    }
+    sums[threadIdx.x] = x;
+    if (ch == 0) ls[sub * PER + w] = l;
   }
-  sums[threadIdx.x] = x;
-  if (ch == 0) ls[w] = l;
   __syncthreads();
-  if (threadIdx.x >= D / 8) return;
+  if (lane >= D / 8 || !mine) return;
   f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
   l = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    lo += sums[i * CH + 2 * threadIdx.x];
-    hi += sums[i * CH + 2 * threadIdx.x + 1];
-    l += ls[i];
+    lo += sums[sub * (256 / ROWS) + i * CH + 2 * lane];
+    hi += sums[sub * (256 / ROWS) + i * CH + 2 * lane + 1];
+    l += ls[sub * PER + i];
   }
-  Program<D, 1, 1, 1>::put(a, b, head, r, threadIdx.x, lo, hi, top, l);
+  Program<D, 1, 1, 1>::put(a, b, head, r, lane, lo, hi, top, l);
 }
 
 }  // namespace
@@ -705,8 +710,8 @@ __device__ __forceinline__ void join(args_ptr a) {
     __shared__ __attribute__((aligned(1024))) Program<D, NQ, WR, W>::Shared shared;                                     \
     Program<D, NQ, WR, W>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), shared).run();                                                                          \
   }
-#define JOIN_KERNEL(NAME, D, BLOCK) \
-  extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) { join<D, BLOCK>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr()); }
+#define JOIN_KERNEL(NAME, D, BLOCK, ROWS) \
+  extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) { join<D, BLOCK, ROWS>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr()); }
 
 ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 4)
 ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 4)
@@ -717,9 +722,11 @@ ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 3)
 ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 1)
 ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2)
-JOIN_KERNEL(wir_attn_join_d64_r16, 64, 16)
-JOIN_KERNEL(wir_attn_join_d64_r32, 64, 32)
-JOIN_KERNEL(wir_attn_join_d64_r128, 64, 128)
-JOIN_KERNEL(wir_attn_join_d128_r16, 128, 16)
-JOIN_KERNEL(wir_attn_join_d128_r32, 128, 32)
-JOIN_KERNEL(wir_attn_join_d128_r128, 128, 128)
+JOIN_KERNEL(wir_attn_join_d64_r16, 64, 16, 1)
+JOIN_KERNEL(wir_attn_join_d64_r32, 64, 32, 1)
+JOIN_KERNEL(wir_attn_join_d64_r128, 64, 128, 1)
+JOIN_KERNEL(wir_attn_join_d64_r128_w4, 64, 128, 4)
+JOIN_KERNEL(wir_attn_join_d128_r16, 128, 16, 1)
+JOIN_KERNEL(wir_attn_join_d128_r32, 128, 32, 1)
+JOIN_KERNEL(wir_attn_join_d128_r128, 128, 128, 1)
+JOIN_KERNEL(wir_attn_join_d128_r128_w4, 128, 128, 4)

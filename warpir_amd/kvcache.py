@@ -267,8 +267,9 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}" + ("_w8" if waves == 8 else ""),
            (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
     if extra:
-        launch(rec, device, "attn_cached.hsaco", f"wir_attn_join_d{d}_r{block}", (items * min(rows, block), 1, 1),
-               (256, 1, 1), args, tensors, past)
+        many = block == 128 and items * min(rows, block) > 2048   # a row a wave, not a workgroup
+        launch(rec, device, "attn_cached.hsaco", f"wir_attn_join_d{d}_r{block}" + ("_w4" if many else ""),
+               (items * (-(-min(rows, block) // 4) if many else min(rows, block)), 1, 1), (256, 1, 1), args, tensors, past)
     if rec:
         _attention_plans.add(0, rec, out, lse)
     return out, lse
