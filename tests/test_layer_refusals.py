@@ -234,7 +234,7 @@ def test_attention_forms_hold_their_bounds():
         for heads in (1, 7, 100, 300, 600, 5000):
             for columns, page in ((1, 16), (8, 64), (40, 128), (4096, 64)):
                 for d in (64, 128):
-                    block, waves, extra, least = kvcache._attention_form(rows, lambda n: heads * -(-rows // n), columns, page, d)
-                    assert block in (16, 32, 128) and rows <= block or block == 128
+                    block, waves, extra, least = kvcache._attention_form(rows, heads, columns, page, d)
+                    assert block in (16, 32, 128) and (rows <= block or rows > 32)
                     assert waves == 4 or block == 16 or (block, d) == (32, 64)
                     assert extra >= 0 and (least > 0) == (extra > 0)

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Tuple
 
 from warpir_amd.handwritten import DevicePlans, check_tensor, check_written, launch, need
@@ -171,33 +172,52 @@ class _AttnArgs(ctypes.Structure):
 TILE = 64        # positions of a tile (csrc/wir_pages.h)
 
 
-def _attention_form(rows: int, items_of, columns: int, page: int, d: int):
-    """(rows of a block, waves, extra, least) of the kernel for ``rows`` query
-    rows a key/value head over a table of ``columns`` pages; ``items_of`` gives the
-    number of (sequence, block, head) for a block's rows.  The heads' tiles are
-    divided over at most ``extra`` more programs than one for each of those, in
-    parts of at least ``least`` tiles; extra 0: no division.
+# us of one tile of a workgroup that has a CU to itself, and of one CU's time where all are busy, by head size and rows
+# of a block: the slopes of launches of 30 to 500 tiles
+_TILE_US = {128: {16: (0.35, 0.35), 32: (0.43, 0.48), 128: (1.5, 1.2)},
+            64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (1.2, 0.77)}}
+_DIVIDED_US = {128: 1.23, 64: 0.75}   # us of a CU's time for a tile of 128 rows, divided
 
-    A division costs a second launch and the partial results' way, ~3 us; a
-    head that is not divided is read by one CU at ~49 GB/s, against ~5 TB/s of
-    the chip, so it pays below ~105 heads and from ~150 kB of keys and values
-    in a head, or where one sequence may be far longer than the rest.  us,
-    divided / not (8 heads of D = 128 a sequence): 1 x 1000 keys 11.1 / 10.9, 1 x
-    4000 11.2 / 26.6, 4 x 2048 13.7 / 17.5, 16 x 2048 20.5 / 17.9, 32 x 512 12.8 / 9.7;
-    16 x 16 heads of D = 64, up to 2050 keys 16.6 / 13.4."""
-    block = 16 if rows <= 16 else 32 if rows <= 32 else 128
-    items = items_of(block)
-    if block == 128:
-        return (block, 4, 0, 0) if items >= 512 else (block, 4, max(512 - items, 256), 4)
-    held = columns * page * 2 * d   # bytes of a head at most
-    if held <= 640 << 10 and held * (1 - items / 105) <= 147 << 10:
+
+@functools.lru_cache(maxsize=1024)
+def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
+    """(rows of a block, waves, extra, least) of the kernel for ``rows`` query
+    rows a key/value head over a table of ``columns`` pages, ``heads`` of them in all
+    sequences together.  The heads' tiles are divided over at most ``extra`` more
+    programs than one for each (sequence, block, head), in parts of at least
+    ``least`` tiles; extra 0: no division.
+
+    Up to 32 rows, one block: a division costs a second launch and the partial
+    results' way, ~3 us; a head that is not divided is read by one CU at ~49
+    GB/s, against ~5 TB/s of the chip, so it pays below ~105 heads and from ~150
+    kB of keys and values in a head, or where one sequence may be far longer
+    than the rest.  us, divided / not (8 heads of D = 128 a sequence): 1 x 1000
+    keys 11.1 / 10.9, 1 x 4000 11.2 / 26.6, 4 x 2048 13.7 / 17.5, 16 x 2048 20.5 / 17.9,
+    32 x 512 12.8 / 9.7; 16 x 16 heads of D = 64, up to 2050 keys 16.6 / 13.4.
+
+    More rows: the form with the smallest estimate for keys that fill the
+    table.  Blocks of 16 rows win while they leave CUs idle, blocks of 128 where
+    the work is much.  us, 16 / 32 / 128 rows / 128 rows divided (D = 128, H32/8): 40
+    queries over 2000 keys 17.0 / 21.2 / 59 / 24.7, 8 x 64 over 2000 52 / 43.7 / 60 / 47, 64
+    over 32000 192 / 220 / 745 / 61.5, 2 x 1000 over 8192 659 / 460 / 292 / 300."""
+    if rows > 32:
+        tiles = -(-columns * page // TILE)
+        n = {block: heads * -(-rows // block) for block in (16, 32, 128)}
+        us = {(block, 0): 6 + tiles * max(light, busy * n[block] / 256) for block, (light, busy) in _TILE_US[d].items()}
+        if d == 128:
+            us[32, 0] += 5 * ((n[32] - 1) // 256)   # (one such program a CU: the next one's start is not covered)
+        us[128, 1] = 24 + tiles * _DIVIDED_US[d] * max(n[128] / 256, 2 / tiles)
+        block, divided = min(us, key=us.get)
+        return (block, 4, max(512 - n[128], 256), 2) if divided else (block, 4, 0, 0)
+    block, held = 16 if rows <= 16 else 32, columns * page * 2 * d   # bytes of a head at most
+    if held <= 640 << 10 and held * (1 - heads / 105) <= 147 << 10:
         # eight waves a head while there is one such program for each CU
-        return block, 8 if items <= 256 and columns * page > 16 * TILE and (block, d) != (32, 128) else 4, 0, 0
+        return block, 8 if heads <= 256 and columns * page > 16 * TILE and (block, d) != (32, 128) else 4, 0, 0
     # two programs of four waves a CU (32 sequences of up to 16000 keys, 256 heads: 384 more 96.6, 128 or 1024 over
     # 99); with more heads, one of eight and as many more (64 sequences of up to 8192, 512 heads: 512 more of eight
     # waves 119.6, 1536 of four 122)
-    if items <= 384 or (block, d) == (32, 128):
-        return block, 4, max(512 - items, 384), 2
+    if heads <= 384 or (block, d) == (32, 128):
+        return block, 4, max(512 - heads, 384), 2
     return block, 8, 512, 2
 
 
@@ -244,8 +264,7 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     if page_table.shape[1] == 0:
         return out.zero_(), lse.fill_(float("-inf"))
     rows = tokens * group
-    block, waves, extra, least = _attention_form(rows, lambda n: batch * -(-rows // n) * heads,
-                                                 page_table.shape[1], page, d)
+    block, waves, extra, least = _attention_form(rows, batch * heads, page_table.shape[1], page, d)
     blocks = -(-rows // block)
     items = batch * blocks * heads
     need(fn, items * min(rows, block) < 1 << 24, "2^24 query rows or more in one call")
@@ -286,11 +305,8 @@ def attention_cached_workspace(q, cache: KVCache, page_table) -> int:
     _, heads, page, d = cache.k.shape
     rows = q.shape[2] * (q.shape[1] // heads)
 
-    def items(block):
-        return q.shape[0] * -(-rows // block) * heads
-
-    block, _, extra, _ = _attention_form(rows, items, page_table.shape[1], page, d)
-    return _workspace_floats(extra, block, d, items(block))
+    block, _, extra, _ = _attention_form(rows, q.shape[0] * heads, page_table.shape[1], page, d)
+    return _workspace_floats(extra, block, d, q.shape[0] * -(-rows // block) * heads)
 
 
 __all__ = ["KVCache", "kv_cache_write", "kv_cache_read", "attention_cached", "attention_cached_workspace"]
