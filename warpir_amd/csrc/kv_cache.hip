@@ -82,10 +82,10 @@ __device__ __forceinline__ void rescale2(unsigned* at, float ratio) {
 }
 
 // Workgroup -> one page of one sequence and head, of K or of V.  A lane takes
-// 4 tokens x 8 columns; PASSES of 256 lanes cover the largest page.
-template <int D>
+// 4 tokens x 8 columns; PASSES of 256 lanes cover a page.
+template <int D, int PASSES>
 __device__ __forceinline__ void write(const kv_args& a) {
-  constexpr int COLS = D / 8, PASSES = D == 128 ? 2 : 1;   // pages of at most 128 tokens
+  constexpr int COLS = D / 8;
   unsigned at = blockIdx.x;
   const bool is_v = at & 1;
   at >>= 1;
@@ -199,9 +199,9 @@ __device__ __forceinline__ void write(const kv_args& a) {
 
 // Workgroup -> one page's places of one sequence and head, of K or of V, as
 // dense rows; places past the sequence and those of no page become 0.
-template <int D>
+template <int D, int PASSES>
 __device__ __forceinline__ void read(const kv_args& a) {
-  constexpr int COLS = D / 8, PASSES = D == 128 ? 2 : 1;
+  constexpr int COLS = D / 8;
   unsigned at = blockIdx.x;
   const bool is_v = at & 1;
   at >>= 1;
@@ -262,7 +262,9 @@ __device__ __forceinline__ void read(const kv_args& a) {
 #define KV_KERNEL(NAME, CALL) \
   extern "C" __global__ void __launch_bounds__(256) NAME(const kv_args args) { CALL(args); }
 
-KV_KERNEL(wir_kv_write_d64, write<64>)
-KV_KERNEL(wir_kv_write_d128, write<128>)
-KV_KERNEL(wir_kv_read_d64, read<64>)
-KV_KERNEL(wir_kv_read_d128, read<128>)
+KV_KERNEL(wir_kv_write_d64, (write<64, 1>))
+KV_KERNEL(wir_kv_write_d128, (write<128, 1>))
+KV_KERNEL(wir_kv_write_d128_p128, (write<128, 2>))   // pages of 128 tokens
+KV_KERNEL(wir_kv_read_d64, (read<64, 1>))
+KV_KERNEL(wir_kv_read_d128, (read<128, 1>))
+KV_KERNEL(wir_kv_read_d128_p128, (read<128, 2>))

@@ -87,7 +87,8 @@ def _launch(fn, rec, kernel, cache, k, v, page_table, lengths, counts, slots, de
         return False
     args = _Args(*(_Side(None, None, None, *x.stride()[:3]) for x in (k, v)), None, None, None, page_table.stride(0),
                  batch, heads, tokens, cache.k.shape[2], cache.k.shape[0], page_table.shape[1], slots)
-    launch(rec, device, "kv_cache.hsaco", f"{kernel}_d{d}", (programs, 1, 1), (256, 1, 1), args,
+    name = f"{kernel}_d{d}" + ("_p128" if d == 128 and cache.k.shape[2] == 128 else "")
+    launch(rec, device, "kv_cache.hsaco", name, (programs, 1, 1), (256, 1, 1), args,
            {"k.codes": cache.k, "k.scales": cache.k_scale, "k.x": k, "v.codes": cache.v, "v.scales": cache.v_scale,
             "v.x": v, "table": page_table, "lengths": lengths, "counts": counts})
     return True
