@@ -60,6 +60,8 @@ static void keys() {
     CHECK(got == most);
     CHECK(block_units(got) == (most ? (most + TILE - 1) / TILE : 1));
   }
+  CHECK(block_tiles(0) == 0 && block_tiles(1) == 1 && block_tiles(64) == 1 && block_tiles(65) == 2);
+  CHECK(slot_of(-5, 3, 4) == 0 && slot_of(INT_MAX, 1, 4) == slots_for(4) - 1);
   CHECK(block_units(INT_MAX) == (int)(((long long)INT_MAX + 63) / 64));
 }
 
@@ -96,7 +98,8 @@ static void division() {
           const int lo = part_begin(n, units[p], parts), hi = part_begin(n + 1, units[p], parts);
           CHECK(hi > lo && hi - lo <= share);
           if (parts == 1) continue;
-          const int slot = slot_of(begin + lo, width);
+          CHECK((begin + lo) / width < slots_for(extra));   // (the bound is for lengths that change meanwhile)
+          const int slot = slot_of(begin + lo, width, extra);
           CHECK(slot >= 0 && slot < slots_for(extra) && used.insert(slot).second);
         }
       }

@@ -117,6 +117,13 @@ struct Program {
   static constexpr int CHUNKS = 4 * KC + DT;     // of a tile's codes, 64 lanes' 16 bytes each
   static_assert(!SHARED || (WK == 1 && CHUNKS % (2 * W) == 0), "");
 
+  // What the workgroup does, worked out by its first wave.  The lengths are read here and nowhere else, and every index
+  // that follows from them is bounded: a program that changes them under a running launch gets wrong rows, no more.
+  struct Plan {
+    int pair, head, first, last, slot;
+    wir::Span span;
+  };
+
   struct Results {
     float o[W * ROWS * PITCH];
     float ml[W * ROWS * 2];
@@ -128,6 +135,7 @@ struct Program {
     };
     int nan_from[D];   // first position with a NaN code in the column, of the tiles that not all rows see whole
     int nan_any;
+    Plan plan;
   };
 
   args_ptr a;
@@ -154,9 +162,8 @@ struct Program {
   // (divisions that the plain decode step does not need are branched over: a step's whole path is a few microseconds)
   __device__ __forceinline__ int sequence_of(int pair) const { return a->blocks == 1 ? pair : pair / a->blocks; }
   __device__ __forceinline__ int token_of(int r) const { return a->tokens == 1 ? 0 : r / a->group; }
-  __device__ __forceinline__ int keys_at(int pair) const {
-    const int seq = sequence_of(pair);
-    return wir::block_keys(span_at(seq), pair - seq * a->blocks, BLOCK, rows(), a->group);
+  __device__ __forceinline__ int keys_of(const wir::Span& s, int pair) const {
+    return wir::block_keys(s, pair - sequence_of(pair) * a->blocks, BLOCK, rows(), a->group);
   }
 
   // Position that new token t sees up to; -1: none.
@@ -582,67 +589,84 @@ struct Program {
           sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 
-  __device__ __forceinline__ void run() {
-    for (int d = threadIdx.x; d < D; d += 64 * W) sh.nan_from[d] = 0x7fffffff;
-    if (threadIdx.x == 0) sh.nan_any = 0;
-    __syncthreads();
-    int pair, head, keys, first = 0, last, slot = -1;
+  __device__ __forceinline__ Plan plan() const {
+    Plan w;
+    w.first = 0, w.slot = -1;
     if (!a->extra) {
       int id = blockIdx.x;
       if (a->blocks == 1) {
-        pair = id / a->heads;
-        head = id - pair * a->heads;
+        w.pair = id / a->heads;
+        w.head = id - w.pair * a->heads;
       } else {   // a head's blocks, the longest first, next to one another on one XCD
         id = wir::remap_xcd(id, gridDim.x);
         const int item = id / a->blocks, seq = item / a->heads;
-        head = item - seq * a->heads;
-        pair = (seq + 1) * a->blocks - 1 - (id - item * a->blocks);
+        w.head = item - seq * a->heads;
+        w.pair = (seq + 1) * a->blocks - 1 - (id - item * a->blocks);
       }
-      keys = keys_at(pair);
-      last = wir::block_units(keys);
-    } else {
-      // every wave for itself: a lane takes `each` pairs
-      const int pairs = a->batch * a->blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
-      auto units_of = [&](int p) { return wir::block_units(keys_at(p)); };
-      int units = 0, parts = 0;
-      for (int p = from; p < to; ++p) units += units_of(p);
-      const int units_to = a->heads * (pairs == 1 ? units : wave_scan(units));
-      const int share = wir::share_of(__builtin_amdgcn_readlane(units_to, pairs == 1 ? 0 : 63), a->extra, a->least);
-      for (int p = from; p < to; ++p) parts += wir::parts_of(units_of(p), share);
-      const int parts_to = a->heads * (pairs == 1 ? parts : wave_scan(parts));
-      // the program's pair, and the units and parts before it
-      const int id = blockIdx.x;
-      const unsigned long long past = __builtin_amdgcn_ballot_w64(lane < pairs && id < parts_to);
-      if (past == 0) return;
-      const int src = __builtin_ctzll(past);
-      int p = from, units_before = units_to - a->heads * units, parts_before = parts_to - a->heads * parts;
-      if (lane == src && each > 1) {
-        for (;; ++p) {
-          const int u = units_of(p), n = a->heads * wir::parts_of(u, share);
-          if (id < parts_before + n) break;
-          parts_before += n, units_before += a->heads * u;
-        }
-      }
-      pair = __builtin_amdgcn_readlane(p, src);
-      units_before = __builtin_amdgcn_readlane(units_before, src);
-      parts_before = __builtin_amdgcn_readlane(parts_before, src);
-      keys = keys_at(pair);
-      units = wir::block_units(keys);
-      parts = wir::parts_of(units, share);
-      head = (id - parts_before) / parts;
-      const int n = id - parts_before - head * parts, begin = units_before + head * units, width = wir::slot_width(share);
-      first = wir::part_begin(n, units, parts);
-      last = wir::part_begin(n + 1, units, parts);
-      if (parts > 1) slot = wir::slot_of(begin + first, width);
-      if (threadIdx.x == 0 && n == 0) {
-        int* info = a->info + 4 * ((i64)pair * a->heads + head);
-        info[0] = begin, info[1] = units, info[2] = parts, info[3] = width;
+      w.span = span_at(sequence_of(w.pair));
+      w.last = wir::block_tiles(keys_of(w.span, w.pair));
+      return w;
+    }
+    // a lane takes `each` pairs
+    const int pairs = a->batch * a->blocks, each = (pairs + 63) / 64, from = lane * each, to = min(from + each, pairs);
+    auto units_of = [&](int p) { return wir::block_units(keys_of(span_at(sequence_of(p)), p)); };
+    int units = 0, parts = 0;
+    for (int p = from; p < to; ++p) units += units_of(p);
+    const int units_to = a->heads * (pairs == 1 ? units : wave_scan(units));
+    const int share = wir::share_of(__builtin_amdgcn_readlane(units_to, pairs == 1 ? 0 : 63), a->extra, a->least);
+    for (int p = from; p < to; ++p) parts += wir::parts_of(units_of(p), share);
+    const int parts_to = a->heads * (pairs == 1 ? parts : wave_scan(parts));
+    // the program's pair, and the units and parts before it
+    const int id = blockIdx.x;
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(lane < pairs && id < parts_to);
+    if (past == 0) {
+      w.pair = -1;
+      return w;
+    }
+    const int src = __builtin_ctzll(past);
+    int p = from, units_before = units_to - a->heads * units, parts_before = parts_to - a->heads * parts;
+    if (lane == src) {
+      for (; p + 1 < to; ++p) {
+        const int u = units_of(p), n = a->heads * wir::parts_of(u, share);
+        if (id < parts_before + n) break;
+        parts_before += n, units_before += a->heads * u;
       }
     }
+    w.pair = __builtin_amdgcn_readlane(p, src);
+    units_before = __builtin_amdgcn_readlane(units_before, src);
+    parts_before = __builtin_amdgcn_readlane(parts_before, src);
+    w.span = span_at(sequence_of(w.pair));
+    const int keys = keys_of(w.span, w.pair);
+    units = wir::block_units(keys);
+    parts = wir::parts_of(units, share);
+    w.head = min((id - parts_before) / parts, a->heads - 1);
+    const int n = min(id - parts_before - w.head * parts, parts - 1), width = wir::slot_width(share);
+    const int begin = units_before + w.head * units;
+    w.first = wir::part_begin(n, units, parts);
+    w.last = min(wir::part_begin(n + 1, units, parts), wir::block_tiles(keys));
+    if (parts > 1) w.slot = wir::slot_of(begin + w.first, width, a->extra);
+    if (lane == 0 && n == 0) {
+      int* info = a->info + 4 * ((i64)w.pair * a->heads + w.head);
+      info[0] = begin, info[1] = units, info[2] = parts, info[3] = width;
+    }
+    return w;
+  }
+
+  __device__ __forceinline__ void run() {
+    if (wave == 0) {
+      const Plan w = plan();
+      for (int d = lane; d < D; d += 64) sh.nan_from[d] = 0x7fffffff;
+      if (lane == 0) sh.plan = w, sh.nan_any = 0;
+    }
+    __syncthreads();
+    auto read = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const int pair = read(sh.plan.pair);
+    if (pair < 0) return;
+    const int head = read(sh.plan.head), slot = read(sh.plan.slot);
     b = sequence_of(pair);
     rb = pair - b * a->blocks;
-    span = span_at(b);
-    walk(head, first, min(last, (keys + wir::TILE - 1) / wir::TILE));
+    span = wir::Span{read(sh.plan.span.start), read(sh.plan.span.count), read(sh.plan.span.held)};
+    walk(head, read(sh.plan.first), read(sh.plan.last));
     __syncthreads();
     a = fresh(a);
     store(head, slot);
@@ -662,13 +686,13 @@ __device__ __forceinline__ void join(args_ptr a) {
   const int item = blockIdx.x / per, sub = ROWS == 1 ? 0 : wir::wave_id(), lane = threadIdx.x % (256 / ROWS);
   const int row = (blockIdx.x - item * per) * ROWS + sub;
   const int* info = a->info + 4 * (i64)item;
-  const int begin = info[0], units = info[1], parts = info[2], width = info[3];
+  const int begin = info[0], units = info[1], parts = min(info[2], wir::slots_for(a->extra)), width = max(info[3], 1);
   if (parts <= 1) return;
   const int pair = item / a->heads, head = item - pair * a->heads, b = pair / a->blocks, rb = pair - b * a->blocks;
   const int r = rb * BLOCK + row;
   const bool mine = row < BLOCK && r < a->tokens * a->group;
   const f32x2* ml = (const f32x2*)(a->partial + (i64)wir::slots_for(a->extra) * BLOCK * D);
-  auto place = [&](int p) { return (i64)wir::slot_of(begin + wir::part_begin(p, units, parts), width) * BLOCK + row; };
+  auto place = [&](int p) { return (i64)wir::slot_of(begin + wir::part_begin(p, units, parts), width, a->extra) * BLOCK + row; };
   const int ch = lane % CH, w = lane / CH;
   float top = -__builtin_inff(), l = 0.f;
   if (mine) {

@@ -70,7 +70,8 @@ WIR_HD int block_keys(const Span& s, int rb, int rows_per_block, int rows, int g
 }
 
 // Its units of work: tiles, and one where there are none (its rows are written all the same).
-WIR_HD int block_units(int keys) { return imax((int)(((unsigned)keys + TILE - 1) / TILE), 1); }
+WIR_HD int block_tiles(int keys) { return (int)(((unsigned)keys + TILE - 1) / TILE); }
+WIR_HD int block_units(int keys) { return imax(block_tiles(keys), 1); }
 
 // Division of the work: a head's units go to parts_of(units) programs in
 // equal parts of at most `share`, in the order of (sequence, block) pairs,
@@ -90,7 +91,7 @@ WIR_HD int part_begin(int n, int units, int parts) {
 // share / 2 units, so no two of them start in the same such interval of all
 // units.  `begin`: the part's first unit among them.
 WIR_HD int slot_width(int share) { return imax(share / 2, 1); }
-WIR_HD int slot_of(int begin, int width) { return begin / width; }
 WIR_HD int slots_for(int extra) { return 3 * extra + 2; }
+WIR_HD int slot_of(int begin, int width, int extra) { return imin(imax(begin / width, 0), slots_for(extra) - 1); }
 
 }  // namespace wir
