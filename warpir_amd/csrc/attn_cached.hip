@@ -728,14 +728,16 @@ __device__ __forceinline__ void join(args_ptr a) {
 
 }  // namespace
 
-#define ATTN_KERNEL(NAME, D, NQ, WR, W, OCC)                                                                            \
-  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W), amdgpu_waves_per_eu(OCC, OCC))) \
-  NAME(const attn_args) {                                                                                          \
-    __shared__ __attribute__((aligned(1024))) Program<D, NQ, WR, W>::Shared shared;                                     \
-    Program<D, NQ, WR, W>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), shared).run();                                                                          \
+#define ATTN_KERNEL(NAME, D, NQ, WR, W, OCC)                                                              \
+  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W),                  \
+                                            amdgpu_waves_per_eu(OCC, OCC))) NAME(const attn_args) {       \
+    __shared__ __attribute__((aligned(1024))) Program<D, NQ, WR, W>::Shared shared;                       \
+    Program<D, NQ, WR, W>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), shared).run();                \
   }
-#define JOIN_KERNEL(NAME, D, BLOCK, ROWS) \
-  extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) { join<D, BLOCK, ROWS>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr()); }
+#define JOIN_KERNEL(NAME, D, BLOCK, ROWS)                                             \
+  extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) {           \
+    join<D, BLOCK, ROWS>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr());           \
+  }
 
 ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 4)
 ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 4)
@@ -744,7 +746,7 @@ ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 3)
 ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 1)
+ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 2)
 ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2)
 JOIN_KERNEL(wir_attn_join_d64_r16, 64, 16, 1)
 JOIN_KERNEL(wir_attn_join_d64_r32, 64, 32, 1)

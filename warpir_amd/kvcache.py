@@ -175,7 +175,7 @@ TILE = 64        # positions of a tile (csrc/wir_pages.h)
 
 # us of one tile of a workgroup that has a CU to itself, and of one CU's time where all are busy, by head size and rows
 # of a block: the slopes of launches of 30 to 500 tiles
-_TILE_US = {128: {16: (0.35, 0.35), 32: (0.43, 0.48), 128: (1.5, 1.2)},
+_TILE_US = {128: {16: (0.35, 0.35), 32: (0.55, 0.43), 128: (1.5, 1.2)},
             64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (1.2, 0.77)}}
 _DIVIDED_US = {128: 1.23, 64: 0.75}   # us of a CU's time for a tile of 128 rows, divided
 
@@ -199,14 +199,12 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
     More rows: the form with the smallest estimate for keys that fill the
     table.  Blocks of 16 rows win while they leave CUs idle, blocks of 128 where
     the work is much.  us, 16 / 32 / 128 rows / 128 rows divided (D = 128, H32/8): 40
-    queries over 2000 keys 17.0 / 21.2 / 59 / 24.7, 8 x 64 over 2000 52 / 43.7 / 60 / 47, 64
-    over 32000 192 / 220 / 745 / 61.5, 2 x 1000 over 8192 659 / 460 / 292 / 300."""
+    queries over 2000 keys 17.1 / 26.1 / 60 / 25, 8 x 64 over 2000 53.9 / 39.9 / 60 / 47, 64
+    over 32000 191 / 274 / 750 / 62, 2 x 1000 over 8192 658 / 410 / 295 / 301."""
     if rows > 32:
         tiles = -(-columns * page // TILE)
         n = {block: heads * -(-rows // block) for block in (16, 32, 128)}
         us = {(block, 0): 6 + tiles * max(light, busy * n[block] / 256) for block, (light, busy) in _TILE_US[d].items()}
-        if d == 128:
-            us[32, 0] += 5 * ((n[32] - 1) // 256)   # (one such program a CU: the next one's start is not covered)
         us[128, 1] = 24 + tiles * _DIVIDED_US[d] * max(n[128] / 256, 2 / tiles)
         block, divided = min(us, key=us.get)
         return (block, 4, max(512 - n[128], 256), 2) if divided else (block, 4, 0, 0)
