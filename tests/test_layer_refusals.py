@@ -93,6 +93,7 @@ def _lenient(monkeypatch):
     (dict(q_out=_fake(2, 4, 8, 64), k_out=_fake(1, 2, 8, 64).expand(2, 2, 8, 64)), "overlap"),
     (dict(positions=_fake(7, dtype=i32)), "positions must have shape"),
     (dict(q=_fake(1, 1, 1, 64).expand(1 << 20, 1 << 9, 1, 64), k=_fake(1, 1, 1, 64).expand(1 << 20, 1, 1, 64)), "2\\^29 rows"),
+    (dict(q=_fake(1, 1, 1, 64).expand(1 << 24, 1, 1, 64), k=_fake(1, 1, 1, 64).expand(1 << 24, 1, 1, 64)), "2\\^24 workgroups"),
 ])
 def test_norm_rope_past_the_pointers(monkeypatch, change, error):
     _lenient(monkeypatch)

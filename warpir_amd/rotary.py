@@ -77,6 +77,7 @@ def _validate(fn, q, k, q_weight, k_weight, cos, sin, positions, eps, interleave
     if not isinstance(interleaved, bool):
         raise TypeError(f"{fn}: interleaved must be a bool")
     need(fn, b * s * (h + k.shape[1]) < 1 << 29, "2^29 rows or more in one call")
+    need(fn, b * -(-s * (h + k.shape[1]) * d // 4096) < 1 << 24, "2^24 workgroups or more in one call")
     return b, h, s, d, device
 
 
@@ -125,7 +126,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
     if b * s * (h + k.shape[1]) == 0:
         return q_out, k_out
     args = _packed(q, k, q_out, k_out, None, None, q_weight, cos, sin, positions, eps)
-    rows = 4096 // d   # rows of a workgroup
+    rows = 4096 // d   # rows of a workgroup, all of one sequence
     launch(rec, device, "qk_norm_rope.hsaco", f"wir_qk_norm_rope_d{d}" + ("_inter" if interleaved else ""),
            (b * -(-s * (h + k.shape[1]) // rows), 1, 1), (256, 1, 1), args,
            {"q.x": q, "q.out": q_out, "q.w": q_weight, "k.x": k, "k.out": k_out, "k.w": k_weight, "cos": cos,
