@@ -107,6 +107,18 @@ def test_every_division_gives_the_same(gpu, monkeypatch, forced):
     _compare(_run(q, _gpu(cache), table, lengths, counts), q, cache, table, lengths, counts)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("forced", [(16, 4, 256, 2), (32, 4, 40, 1), (128, 4, 300, 2), (16, 4, 3, 1), (32, 4, 0, 0)])
+def test_every_division_of_many_blocks(gpu, monkeypatch, forced, d):
+    """Blocks that end inside a token's heads, some with nothing to see."""
+    lengths, counts = (700, 0, 90, 300), (50, 0, 7, 33)
+    cache, table = _cache(4, 2, 32, d, 23, lengths)
+    q = seeded_normal((4, 6, 50, d), 5)
+    monkeypatch.setattr(kvcache, "_attention_form", lambda *a: forced)
+    monkeypatch.setattr(kvcache, "_attention_plans", kvcache.DevicePlans("attention_cached"))
+    _compare(_run(q, _gpu(cache), table, lengths, counts), q, cache, table, lengths, counts)
+
+
 def test_more_sequences_than_threads(gpu):
     lengths = [(i * 37) % 90 for i in range(700)]
     cache, table = _cache(700, 1, 16, 64, 40, lengths)

@@ -110,8 +110,8 @@ def kv_cache_write(cache: KVCache, k, v, page_table, lengths, counts=None) -> KV
     are rounded again for the new one.  An infinity becomes NaN, which e4m3 has.
     Nothing else in the cache changes.  Tokens before position 0, past the
     table, or in a page that the cache does not have (-1) are dropped.  A page
-    that is written may belong to one sequence only: two that write it at once
-    leave a mixture of both there."""
+    that is written stands in one place of the table only: tokens that reach it
+    by two (sequences, or columns of one) leave a mixture of both there."""
     import torch
 
     fn, done = "kv_cache_write", None
@@ -177,7 +177,7 @@ TILE = 64        # positions of a tile (csrc/wir_pages.h)
 # of a block: the slopes of launches of 30 to 500 tiles
 _TILE_US = {128: {16: (0.35, 0.35), 32: (0.55, 0.43), 128: (1.5, 1.2)},
             64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (1.2, 0.77)}}
-_DIVIDED_US = {128: 1.23, 64: 0.75}   # us of a CU's time for a tile of 128 rows, divided
+_DIVIDED_US = {128: (13, 0.5, 24, 1.23), 64: (13, 0.26, 24, 0.75)}   # divided: us, and us of a CU for a tile; 16, 128
 
 
 @functools.lru_cache(maxsize=1024)
@@ -198,16 +198,19 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
 
     More rows: the form with the smallest estimate for keys that fill the
     table.  Blocks of 16 rows win while they leave CUs idle, blocks of 128 where
-    the work is much.  us, 16 / 32 / 128 rows / 128 rows divided (D = 128, H32/8): 40
-    queries over 2000 keys 17.1 / 26.1 / 60 / 25, 8 x 64 over 2000 53.9 / 39.9 / 60 / 47, 64
-    over 32000 191 / 274 / 750 / 62, 2 x 1000 over 8192 658 / 410 / 295 / 301."""
+    the work is much.  us, 16 / 32 / 128 rows / 16 divided / 128 divided (D = 128,
+    H32/8): 16 queries over 8000 keys 53.6 / 83 / 193 / 19.2 / 24.7, 40 over 2000 17.1 /
+    26 / 60 / 19.7 / 25, 8 x 64 over 2000 54 / 39.9 / 60 / - / 47, 64 over 32000 191 / 274 /
+    750 / 127 / 62, 2 x 1000 over 8192 658 / 410 / 295 / - / 301."""
     if rows > 32:
         tiles = -(-columns * page // TILE)
         n = {block: heads * -(-rows // block) for block in (16, 32, 128)}
         us = {(block, 0): 6 + tiles * max(light, busy * n[block] / 256) for block, (light, busy) in _TILE_US[d].items()}
-        us[128, 1] = 24 + tiles * _DIVIDED_US[d] * max(n[128] / 256, 2 / tiles)
+        few, few_tile, many, many_tile = _DIVIDED_US[d]
+        us[16, 1] = few + few_tile * max(n[16] * tiles / 256, 2)
+        us[128, 1] = many + many_tile * max(n[128] * tiles / 256, 2)
         block, divided = min(us, key=us.get)
-        return (block, 4, max(512 - n[128], 256), 2) if divided else (block, 4, 0, 0)
+        return (block, 4, 256 if block == 16 else max(512 - n[128], 256), 2) if divided else (block, 4, 0, 0)
     block, held = 16 if rows <= 16 else 32, columns * page * 2 * d   # bytes of a head at most
     if held <= 640 << 10 and held * (1 - heads / 105) <= 147 << 10:
         # eight waves a head while there is one such program for each CU
