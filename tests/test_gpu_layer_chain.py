@@ -9,7 +9,7 @@ from oracle.layer_ref import (angles_ref, attention_cached_ref, cache_read_ref, 
                               norm_rope_ref)
 from oracle.torch_ref import attention_bwd_ref, attention_ref, gemm_ref, rel_err, seeded_normal
 from tests.conftest import announce
-from warpir_amd import api
+from warpir_amd import api, kvcache
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,19 @@ def test_cached_attention_is_the_dense_one_on_what_the_cache_holds(gpu):
     # both round the probabilities and O to bf16 (2^-8 of sum p |v|, which is under max |v|, and of O)
     assert float((o.float() - od.float()).abs().max()) <= 4 * 2 ** -8 * float(vd.abs().max())
     assert float((lse - lsed).abs().max()) <= 2 ** -11
+
+
+def test_one_tensor_for_lengths_and_counts(gpu):
+    """Whole prompts: the results and the plans of two tensors."""
+    n = torch.tensor((90, 1, 37), dtype=torch.int32, device="cuda")
+    q, k, v = (seeded_normal((3, h, 90, 64), i).cuda() for i, h in enumerate((4, 2, 2)))
+    table = torch.arange(9, dtype=torch.int32, device="cuda").view(3, 3)
+    got = []
+    for counts in (n.clone(), n, n):
+        cache = api.KVCache.empty(9, 2, 32, 64)
+        api.kv_cache_write(cache, k, v, table, n, counts)
+        got.append((*(x.view(torch.uint8) for x in cache), *api.attention_cached(q, cache, table, n, counts)))
+    assert all(torch.equal(x, y) for other in got[1:] for x, y in zip(got[0], other))
+    own = kvcache._own(n, n)
+    assert kvcache._write_plans.run(0, k, v, *cache, table, n, own) is not False
+    assert kvcache._own(None, None) is None and kvcache._own("x", "x") == "x"

@@ -17,8 +17,8 @@ _attention_plans = DevicePlans("attention_cached")
 class KVCache(NamedTuple):
     """A paged cache of keys and values in e4m3 codes (``torch.float8_e4m3fn``)
     with one fp32 scale for each page and key/value head; a code stands for
-    ``code * scale``.  Tokens lie next to one another in a V page, since
-    attention's second product sums over them."""
+    ``code * scale`` (scales are positive).  Tokens lie next to one another in a V
+    page, since attention's second product sums over them."""
 
     k: object        # [pages, H_kv, page size, D]
     v: object        # [pages, H_kv, D, page size]
@@ -79,6 +79,12 @@ def _validate(fn, cache, page_table, lengths, counts):
     return batch, heads, page, d, device
 
 
+def _own(counts, lengths):
+    """``counts`` as a tensor of its own where it is ``lengths`` (whole prompts): a
+    call that gives one tensor twice has no plan."""
+    return counts.view_as(counts) if counts is lengths and hasattr(counts, "view_as") else counts
+
+
 def _launch(fn, rec, kernel, cache, k, v, page_table, lengths, counts, slots, device):
     batch, heads, tokens, d = k.shape
     programs = batch * slots * heads * 2
@@ -115,8 +121,8 @@ def kv_cache_write(cache: KVCache, k, v, page_table, lengths, counts=None) -> KV
     import torch
 
     fn, done = "kv_cache_write", None
-    planned = isinstance(cache, KVCache)
-    if planned:
+    counts = _own(counts, lengths)
+    if isinstance(cache, KVCache):
         done = _write_plans.run(0, k, v, *cache, page_table, lengths, counts)
         if done is not None and done is not False:
             return cache
@@ -242,6 +248,7 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     import torch
 
     fn, done = "attention_cached", None
+    counts = _own(counts, lengths)
     if isinstance(cache, KVCache) and workspace is None:
         done = _attention_plans.run(0, q, *cache, page_table, lengths, counts, out, lse)
         if done is not None and done is not False:
