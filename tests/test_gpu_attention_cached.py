@@ -119,6 +119,19 @@ def test_every_division_of_many_blocks(gpu, monkeypatch, forced, d):
     _compare(_run(q, _gpu(cache), table, lengths, counts), q, cache, table, lengths, counts)
 
 
+@pytest.mark.parametrize("batch,heads,hkv,tokens,form", [
+    (12, 32, 8, 256, (128, 4, 0, 0)), (1, 8, 1, 600, (128, 4, 0, 0)), (1, 4, 2, 333, (16, 4, 0, 0)),
+    (3, 6, 3, 500, (128, 4, 0, 0)), (40, 8, 8, 300, (32, 4, 0, 0))])
+def test_the_order_of_many_blocks(gpu, monkeypatch, batch, heads, hkv, tokens, form):
+    """Every block is computed once, whatever the order: long before short, halves that turn round, by length."""
+    lengths = [tokens + 13 * (i % 5) for i in range(batch)]
+    cache, table = _cache(batch, hkv, 64, 64, 11, lengths)
+    q = seeded_normal((batch, heads, tokens, 64), 5)
+    monkeypatch.setattr(kvcache, "_attention_form", lambda *a: form)
+    monkeypatch.setattr(kvcache, "_attention_plans", kvcache.DevicePlans("attention_cached"))
+    _compare(_run(q, _gpu(cache), table, lengths), q, cache, table, lengths)
+
+
 def test_more_sequences_than_threads(gpu):
     lengths = [(i * 37) % 90 for i in range(700)]
     cache, table = _cache(700, 1, 16, 64, 40, lengths)

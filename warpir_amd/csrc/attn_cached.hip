@@ -589,19 +589,41 @@ struct Program {
           sum == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   }
 
+  // Program -> (sequence and head, block) without a division of the work; later blocks see more keys.
+  // A head's blocks are next to one another on one XCD, the longest first.  Where all programs run at once, two a CU, the
+  // second half comes in the opposite order, so that a CU has a long and a short one; many blocks of 128 rows go block
+  // length by block length; those of one or two heads are dealt over the XCDs, for each to have long ones.  us, in turn /
+  // so, D = 128: 4 x 512 queries over 1000 keys (32/8 heads) 50.4 / 45.7, 4096 over 4096 (16/8) 116 / 109.5, 2 x 1000
+  // over 8192 (32/8) 316 / 308; 4 x 2048 over 2048 (32/8) 194 / 182, 4096 over 4096 (24/12) 178 / 140; 8000 over 8000 (8/1)
+  // 270 / 202.  Elsewhere they cost: by length just past two a CU (3 x 700 over 3000, 32/8) 151 / 156 and for blocks of 32
+  // rows (32 x 300 over up to 1000, 16/16, D = 64) 66 / 70, dealt for more heads (5 x 40 over 2000, 24/6) 27.7 / 30.5.
+  __device__ __forceinline__ void in_turn(int& item, int& block) const {
+    int id = blockIdx.x;
+    const int total = gridDim.x;
+    const int heads = a->batch * a->heads;
+    if (SHARED && total >= 768 && a->blocks >= 8) return wir::longest_first<true, 2048>(id, a->blocks, heads, block, item);
+    const bool whole = heads > 2;   // a head on one XCD
+    const int step = whole ? 8 : 1, per = total / step, half = (per + 1) / 2;
+    if (total <= 512 && id >= step * half && id < step * per) id = step * (per - 1 - (id / step - half)) + id % step;
+    if (whole) id = wir::remap_xcd(id, total);
+    item = id / a->blocks;
+    block = a->blocks - 1 - (id - item * a->blocks);
+  }
+
   __device__ __forceinline__ Plan plan() const {
     Plan w;
     w.first = 0, w.slot = -1;
     if (!a->extra) {
-      int id = blockIdx.x;
       if (a->blocks == 1) {
+        const int id = blockIdx.x;
         w.pair = id / a->heads;
         w.head = id - w.pair * a->heads;
-      } else {   // a head's blocks, the longest first, next to one another on one XCD
-        id = wir::remap_xcd(id, gridDim.x);
-        const int item = id / a->blocks, seq = item / a->heads;
+      } else {
+        int item, block;
+        in_turn(item, block);
+        const int seq = item / a->heads;
         w.head = item - seq * a->heads;
-        w.pair = (seq + 1) * a->blocks - 1 - (id - item * a->blocks);
+        w.pair = seq * a->blocks + block;
       }
       w.span = span_at(sequence_of(w.pair));
       w.last = wir::block_tiles(keys_of(w.span, w.pair));
