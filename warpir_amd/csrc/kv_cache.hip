@@ -18,6 +18,12 @@
 // columns packs either way.
 //
 // Both kernels are bound by memory (2 bytes a value in, 1 out, and back).
+// Measured (a 2 GiB copy moves 4.90 TB/s; 8 heads, D = 128, pages of 64): 8
+// prompts of up to 4096 tokens written in 19.2 us, 81 MB at 4.2 TB/s; 16
+// contexts of up to 8192 read back in 135 us, 654 MB at 4.84 TB/s; bytes moved
+// by the counters 1.00 of that.  One token for each of 64 sequences: 4.8 - 6.7
+// us, bound by its latency (table, page, store) and by V, of which a token is
+// one byte in each of D lines.
 #include <hip/hip_runtime.h>
 
 #include "wir_pages.h"
@@ -81,8 +87,9 @@ __device__ __forceinline__ void rescale2(unsigned* at, float ratio) {
   *(u32x2*)at = u32x2{rescale(w[0], ratio), rescale(w[1], ratio)};
 }
 
-// Workgroup -> one page of one sequence and head, of K or of V.  A lane takes
-// 4 tokens x 8 columns; PASSES of 256 lanes cover a page.
+// Workgroup -> one page of one sequence and head, of K or of V: a page's scale
+// needs all of its new values first, and so few stay in registers between the
+// two.  A lane takes 4 tokens x 8 columns; PASSES of 256 lanes cover a page.
 template <int D, int PASSES>
 __device__ __forceinline__ void write(const kv_args& a) {
   constexpr int COLS = D / 8;

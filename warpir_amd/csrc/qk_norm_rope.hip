@@ -14,6 +14,12 @@
 // holds values 8j..8j+7 of both halves of its row, so loads and stores are 16
 // bytes, both kinds of pairs are within a lane, and a row's sums take two or
 // three lane steps of D/16 lanes.
+//
+// Measured (a 2 GiB copy moves 4.90 TB/s): 8 x 4096 tokens, 16/16 heads, D =
+// 128: forward 110 us, 537 MB at 4.87 TB/s; backward 160 us, 805 MB at 5.03
+// TB/s, and 4.6 us for the weights' sums.  Counters there: bytes written 1.00,
+// read 1.07 and 1.04 of what the formula needs (the rest is the table).  3 x
+// 1337 tokens, 24/8 heads, D = 64, interleaved: 8.5 us; 8 rows of one token: 3.4.
 #include <hip/hip_runtime.h>
 
 namespace {
@@ -113,6 +119,8 @@ __device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float
 
 // Workgroup -> 256 / L rows of one sequence; rows run over the heads of a
 // token first, q's and then k's, so that a token's angles are read together.
+// One row a lane group and no loop: the loads of 8 waves a SIMD hide one
+// another.
 template <int D, bool INTER>
 __device__ __forceinline__ void forward(const rope_args& a) {
   constexpr int L = D / 16, ROWS = 256 / L;
