@@ -132,6 +132,50 @@ def test_the_order_of_many_blocks(gpu, monkeypatch, batch, heads, hkv, tokens, f
     _compare(_run(q, _gpu(cache), table, lengths), q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("d", [64, 128])
+def test_blocks_of_128_rows(gpu, monkeypatch, d, page):
+    """Against the oracle with pages that are none, and where NaN codes and scales lie: as blocks of 16 rows have it."""
+    lengths, counts = (700, 0, 90, 300), (50, 0, 7, 33)
+    columns = -(-704 // page) + 1
+    cache, table = _cache(4, 2, page, d, columns, lengths)
+    q = seeded_normal((4, 6, 50, d), 5)
+
+    def both(cache, table):
+        got = []
+        for form in ((128, 4, 0, 0), (16, 4, 0, 0), (128, 4, 300, 2)):
+            monkeypatch.setattr(kvcache, "_attention_form", lambda *a: form)
+            monkeypatch.setattr(kvcache, "_attention_plans", kvcache.DevicePlans("attention_cached"))
+            got.append([x.cpu() for x in _run(q, _gpu(cache), table, lengths, counts)])
+        return got
+
+    holes = table.clone()
+    holes[0, 3], holes[3, 1], holes[2, 0] = -1, 10 ** 6, -1
+    for tab in (table, holes):
+        for got in both(cache, tab):
+            _compare(got, q, cache, tab, lengths, counts)
+    clean = both(cache, table)[0]
+    last = int(table[3, 299 // page])
+    cache.k.view(torch.uint8)[last, :, 300 % page:] = 0x7f   # behind the sequence: not seen
+    cache.v.view(torch.uint8)[last, :, :, 300 % page:] = 0xff
+    for got in both(cache, table):
+        _compare(got, q, cache, table, lengths, counts)
+    assert all(torch.equal(x, y) for x, y in zip(both(cache, table)[0], clean))
+    at = 300 - 20   # seen by the last 20 new tokens
+    cache.v.view(torch.uint8)[int(table[3, at // page]), 1, d - 3, at % page] = 0x7f
+    cache.v.view(torch.uint8)[int(table[0, 0]), 0, 5, 9] = 0xff   # by all
+    cache.k.view(torch.uint8)[int(table[2, 0]), 1, 2, 7] = 0x7f
+    cache.v_scale[int(table[0, 600 // page]), 1] = math.nan
+    wide, few, parts = both(cache, table)
+    for got in (wide, parts):
+        for x, y in zip(got, few):
+            assert torch.equal(x.isnan(), y.isnan())
+    sees = torch.arange(300 - 33, 300) >= at
+    assert torch.equal(wide[0][3, 3, :33, d - 3].isnan(), sees) and not bool(wide[0][3, :3].isnan().any())
+    assert bool(wide[0][0, :3, :, 5].isnan().all()) and bool(wide[0][0, 3:].isnan().all())
+    assert bool(wide[0][2, 3:, :7].isnan().all()) and not bool(wide[0][2, :3].isnan().any())
+
+
 def test_more_sequences_than_threads(gpu):
     lengths = [(i * 37) % 90 for i in range(700)]
     cache, table = _cache(700, 1, 16, 64, 40, lengths)

@@ -5,7 +5,7 @@
 // scale for each page and head.  For query row r at position p:
 //   s_j = q . code_j * ks / sqrt(D) for j <= p,  O = sum_j softmax(s)_j vs code_j.
 //
-// Both products run on v_mfma_f32_16x16x32_bf16: e4m3 codes are exact in bf16,
+// Both products run on bf16 matrix instructions: e4m3 codes are exact in bf16,
 // also times a power of two, and one instruction converts two of them.  ks
 // multiplies the fp32 score; the power of two of vs goes to the values in
 // their conversion, what vs has beside it to the probabilities (which are
@@ -13,31 +13,36 @@
 // q as the sum of two e4m3 terms, spares half the conversions, but those add
 // up with about 16 bits: scores were off by 1.4e-5 of sum |q k|.)
 //
-// Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, with 16
+// Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, with the
 // query rows (the heads that share a key/value head, and the new tokens) as
-// the columns.  A lane then holds scores of one query row, and its 16 of a
+// the columns.  A lane then holds scores of one query row, and those of a
 // 64-token tile are turned into the second product's operand without leaving
-// the lane: the rows of K go to the matrix core in an order that gives lane
-// group g (16 lanes) the tokens 16 g .. 16 g + 15.  V pages are [D, token], so
+// the lane: the rows of K go to the matrix core in an order that gives each
+// lane group 16 tokens that follow one another.  V pages are [D, token], so
 // that operand's other side is 16 contiguous bytes of one column.
 //
-// Few rows (16 or 32 of a key/value head): K and V come from memory straight
-// into registers, every byte once, with no LDS and no barrier in the loop; a
-// workgroup's waves take every WK-th tile and are joined at the end.  Bound by
-// the cache's bytes: one token over 131072 (32/8 heads, D = 128) 45 us, 268 MB
-// at 5.9 TB/s, and 5 for the join; 64 sequences of up to 8192 113 us, 598 MB at
-// 5.3 TB/s, and 5; 16 sequences of up to 2050, 4 tokens, 16 heads of D = 64,
-// pages of 16: 11 us, 41 MB at 3.7 TB/s.  (A 2 GiB copy moves 4.90 TB/s.)
-// Many rows: a workgroup's waves take 32 rows each and share the tiles: each
-// wave converts its part of the next tile's codes and leaves them in LDS as
-// operands (a fragment is 64 lanes' 16 bytes in lane order), so that a code is
-// converted once for 128 rows.  Bound by the vector instructions of the
-// softmax: 2 x 1000 queries over 8192 keys (32/8 heads, D = 128) 291 us, 866
-// TFLOP/s, 65% of a large matrix product's 1328; there the vector ALU is busy
-// 60% and the matrix cores 36% of the time, without LDS conflicts, with two
-// waves a SIMD (the accumulators, queries and scores of 32 rows leave no room for a third).
-// Computing the next tile's scores under this one's exponentials, 64 rows a
-// wave and higher priorities for either phase changed nothing.
+// Few rows (16 or 32 of a key/value head, on 16x16x32 products): K and V come
+// from memory straight into registers, every byte once, with no LDS and no
+// barrier in the loop; a workgroup's waves take every WK-th tile and are joined
+// at the end.  Bound by the cache's bytes: one token over 131072 (32/8 heads, D
+// = 128) 45 us, 268 MB at 5.9 TB/s, and 5 for the join; 64 sequences of up to
+// 8192 113 us, 598 MB at 5.3 TB/s, and 5; 16 sequences of up to 2050, 4 tokens,
+// 16 heads of D = 64, pages of 16: 11 us, 41 MB at 3.7 TB/s.  (A 2 GiB copy moves
+// 4.90 TB/s.)
+// Many rows: a workgroup's waves take 32 rows each, on 32x32x16 products (half
+// the steps between lanes, and half the instructions to issue, of 16x16x32:
+// 5% at D = 128, 3% at 64), and share the tiles: each wave converts its part
+// of the next tile's codes and leaves them in LDS as operands (a fragment is 64
+// lanes' 16 bytes in lane order), so that a code is converted once for 128
+// rows.  2 x 1000 queries over 8192 keys (32/8 heads, D = 128): 281 us, 897
+// TFLOP/s, 68% of a large matrix product's 1328.  No one thing bounds it: taken
+// out of a copy each by itself, the next tile's loads are 10% of the time, its
+// conversion and LDS stores 10%, the softmax 14%, the barrier 1.5%, half of the
+// LDS reads 2.5%; two waves a SIMD cover each other only in part, and the
+// registers of 32 rows leave no room for a third.  The next tile's scores under
+// this one's exponentials, 64 rows a wave, 256 rows a workgroup with the halves
+// of its waves in opposite phases, loads two tiles ahead, and higher priorities
+// for either phase changed nothing.
 #include "wir_cdna4.h"
 #include "wir_pages.h"
 
@@ -50,6 +55,7 @@ using wir::f32x4;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) bf16x8 lds_bf16x8;
 
@@ -115,16 +121,16 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 
 // One of a sequence's row blocks of one head, over some of its tiles: W waves, of 16 * NQ rows each, WR side by side
-// and the others dividing the tiles.
-template <int D, int NQ, int WR, int W>
+// and the others dividing the tiles.  WIDE: a page holds whole tiles.
+template <int D, int NQ, int WR, int W, bool WIDE = false>
 struct Program {
   static constexpr int WK = W / WR;              // waves that divide the tiles
   static constexpr bool SHARED = WR > 1;         // tiles go through LDS
   static constexpr int ROWS = 16 * NQ;           // query rows of a wave
   static constexpr int BLOCK = ROWS * WR;        // and of the workgroup
   static constexpr int KC = D / 64, DT = D / 16, PITCH = D + 4;
-  static constexpr int CHUNKS = 4 * KC + DT;     // of a tile's codes, 64 lanes' 16 bytes each
-  static_assert(!SHARED || (WK == 1 && CHUNKS % (2 * W) == 0), "");
+  static constexpr int CHUNKS = D / 8;           // of a tile's codes, 64 lanes' 16 bytes each
+  static_assert(!SHARED || (WK == 1 && W == 4 && NQ == 2), "");
 
   // What the workgroup does, worked out by its first wave.  The lengths are read here and nowhere else, and every index
   // that follows from them is bounded: a program that changes them under a running launch gets wrong rows, no more.
@@ -217,11 +223,10 @@ struct Program {
     return __uint_as_float(max(bits & 0x7f800000u, 0x00800000u));
   }
 
-  // One tile: key(j, u) the K operand of tokens 16 g + 4 j .. + 3, read() what to do once the keys are used.  Through
-  // registers, value(d) gives the codes of column 16 d + col; through LDS, operand(d, u) the finished V operand.
-  template <class Key, class Read, class Value, class Operand>
-  __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Read read, Value value,
-                                       Operand operand) const {
+  // One tile: key(j, u) the K operand of tokens 16 g + 4 j .. + 3, read() what to do once the keys are used, value(d) the
+  // codes of column 16 d + col.
+  template <class Key, class Read, class Value>
+  __device__ __forceinline__ void tile(State& s, int t, const Tokens& k, Key key, Read read, Value value) const {
     f32x4 x[4][NQ];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -234,7 +239,6 @@ struct Program {
         for (int n = 0; n < NQ; ++n) x[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, s.q[n][u], x[j][n], 0, 0, 0);
       }
     }
-    if (SHARED) fragments_ahead<8 * KC>();
     const int at = t * wir::TILE + 16 * grp;   // the lane's tokens: at .. at + have - 1
     const bool edge = __builtin_amdgcn_ballot_w64(k.have < 16 || at + 15 > s.low) != 0;
     read();
@@ -290,49 +294,29 @@ struct Program {
         }
       s.l[n] += (sum[0] + sum[1]) * inv_g;
     }
-    u32x4 v[SHARED ? 1 : DT];
-    float power = 1.f;
-    if constexpr (!SHARED) {
-      const unsigned bits = scale_of(k);
-      power = power_of(bits);
+    const unsigned bits = scale_of(k);
+    const float power = power_of(bits);
+    u32x4 v[DT];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) v[d] = value(d);
-      if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u) != 0) {
+    for (int d = 0; d < DT; ++d) v[d] = value(d);
+    if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u) != 0) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) v[d] = scaled_codes(v[d], bits);
-      }
-      if (edge) {
-        const u32x4 held = held_bytes(k.have);
+      for (int d = 0; d < DT; ++d) v[d] = scaled_codes(v[d], bits);
+    }
+    if (edge) {
+      const u32x4 held = held_bytes(k.have);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) v[d] &= held;
-        if (unseen(k.have, at, s.low)) take_nans<DT>(v, 0, at);
-      }
+      for (int d = 0; d < DT; ++d) v[d] &= held;
+      if (unseen(k.have, at, s.low)) take_nans<DT>(v, col, 16, at);
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        bf16x8 w;
-        if constexpr (SHARED)
-          w = operand(d, u);
-        else
-          w = unpack8(v[d][2 * u], v[d][2 * u + 1], power);
+        const bf16x8 w = unpack8(v[d][2 * u], v[d][2 * u + 1], power);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) s.o[d][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, p[n][u], s.o[d][n], 0, 0, 0);
       }
-    if (SHARED) fragments_ahead<2 * DT>();
-  }
-
-  template <int N>
-  static __device__ __forceinline__ void fragments_ahead() {
-    constexpr int AHEAD = 8;
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
-#pragma unroll
-    for (int i = 0; i < N - AHEAD; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x8, NQ, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x8, NQ * AHEAD, 0);
   }
 
   // Value codes past the sequence's end become 0 (0 * NaN is NaN in the product); those of a scale that is no number
@@ -353,10 +337,10 @@ struct Program {
   static __device__ __forceinline__ bool unseen(int have, int at, int low) {
     return __builtin_amdgcn_ballot_w64(have > 0 && at + have - 1 > low) != 0;
   }
-  // NaN codes out of the lane's tokens at .. of columns 16 (d + i) + col: a row that sees one of a column's is NaN there,
-  // which is so from the first of them on, so that is all `store` has to know.
+  // NaN codes out of the lane's tokens at .. of columns from, from + step, ..: a row that sees one of a column's is NaN
+  // there, which is so from the first of them on, so that is all `store` has to know.
   template <int N>
-  __device__ __forceinline__ void take_nans(u32x4 (&v)[N], int d, int at) const {
+  __device__ __forceinline__ void take_nans(u32x4 (&v)[N], int from, int step, int at) const {
     u32x4 some = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < N; ++i) some |= nan_codes(v[i]);
@@ -367,7 +351,7 @@ struct Program {
       const u32x4 n = nan_codes(v[i]);
 #pragma unroll
       for (int w = 3; w >= 0; --w)
-        if (n[w]) atomicMin(&sh.nan_from[16 * (d + i) + col], at + 4 * w + __builtin_ctz(n[w]) / 8);
+        if (n[w]) atomicMin(&sh.nan_from[from + step * i], at + 4 * w + __builtin_ctz(n[w]) / 8);
       v[i] &= ~n;
     }
   }
@@ -405,10 +389,10 @@ struct Program {
     return (t * wir::TILE + 16 * seg) & ((1 << x.shift) - 1);
   }
 
-  // The lane's own segment of a tile (its V operand and scores).
-  __device__ __forceinline__ void scales_of(Tokens& k, const Bases& x, int t, int page) const {
+  // Segment `seg` of a tile, which the lane has scores of.
+  __device__ __forceinline__ void scales_of(Tokens& k, const Bases& x, int t, int seg, int page) const {
     const i64 at = page_index(x, page) * x.page_scales;
-    k.have = wir::checked_page(page, x.pages) < 0 ? 0 : min(max(span.held - (t * wir::TILE + 16 * grp), 0), 16);
+    k.have = wir::checked_page(page, x.pages) < 0 ? 0 : min(max(span.held - (t * wir::TILE + 16 * seg), 0), 16);
     k.ks = x.ks[at];   // (of page 0 where there is none: `tile` sees to it, after the loads' time)
     k.vs = x.vs[at];
   }
@@ -428,7 +412,7 @@ struct Program {
     Tokens tok;
     const unsigned char* vp;
     auto load_k = [&](int t, int page_k, int page_v) {
-      scales_of(tok, at, t, page_v);
+      scales_of(tok, at, t, grp, page_v);
       const unsigned char* kp = key_at(at, t, page_k);
       vp = value_at(at, t, page_v);
 #pragma unroll
@@ -457,66 +441,201 @@ struct Program {
              if (t + 2 * WK < last) next_k = page_of(at, t + 2 * WK, col / 4), next_v = page_of(at, t + 2 * WK, grp);
              load_k(t + WK, page_k, page_v);
            },
-           [&](int d) { return vf[d]; }, [](int, int) { return bf16x8{}; });
+           [&](int d) { return vf[d]; });
       if (t + WK < last) load_v();
     }
   }
 
-  // The same through LDS, every tile for all waves.  In each iteration a wave asks for its CHUNKS / W of the next tile
-  // (the first half of the waves K's, the others V's), computes, and leaves what came as operands in the other slot.
-  __device__ __forceinline__ void walk_shared(State& s, int head, int first, int last) const {
-    constexpr int MINE = CHUNKS / W;
-    const bool mine_k = wave < W / 2;
-    const int mine = wave * MINE, seg = mine_k ? col / 4 : grp;
-    const Bases at = bases(head);
-    const unsigned char* base = mine_k ? at.k : at.v;
-    const int token_bytes = mine_k ? D : 1;
-    u32x4 codes[MINE];
-    Tokens tok;
-    auto ask = [&](int t, int page, int own) {
-      const unsigned char* from = base + page_index(at, page) * at.page_bytes + in_page(at, t, seg) * token_bytes;
+  // Through LDS: 32 rows a wave on 32x32x16 products, every tile for all waves.  A lane has the scores of row lane % 32
+  // and, with h = lane / 32, tokens 32 j + 16 h .. + 15 of the tile for j = 0, 1: K's rows come in the order that puts
+  // those into the lane's 16 registers of product j one after another.
+  struct Rows {
+    bf16x8 q[D / 16];
+    int pos, low;
+    f32x16 o[D / 32];
+    float m, l;
+  };
+  static __device__ __forceinline__ float max_of_halves(float x) {
+    auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
+  }
+
+  __device__ __forceinline__ void begin(Rows& s, int head) const {
+    const int row0 = rb * BLOCK + wave * ROWS, r = row0 + lane % 32, rr = r < rows() ? r : 0, t = token_of(rr);
+    s.low = max(span.start + min(token_of(row0), span.count), 0);
+    s.pos = r < rows() ? position_of(t) : -1;
+    const bf16* p = a->q + b * a->qb + (i64)(head * a->group + rr - t * a->group) * a->qh + t * a->qt + lane / 32 * 16;
 #pragma unroll
-      for (int i = 0; i < MINE; ++i) {
-        const int c = mine + i;
-        codes[i] = *(const u32x4*)(from + (mine_k ? 4 * (c / KC) * D + 64 * (c % KC) : (16 * (c - 4 * KC)) << at.shift));
+    for (int u = 0; u < D / 16; ++u) s.q[u] = *(const bf16x8*)(p + u / 2 * 32 + u % 2 * 8);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s.o[d][i] = 0.f;
+    s.m = -__builtin_inff(), s.l = 0.f;
+    // (they are here before the loop, or its waits for them would count the loop's own loads)
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u) asm volatile("" : "+v"(s.q[u]));
+  }
+
+  // Reads of N fragments, a few ahead of the products that use them.
+  template <int N>
+  static __device__ __forceinline__ void fragments_ahead() {
+    constexpr int AHEAD = 8;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
+  }
+
+  // One tile, its operands at `from`: K's (j, u) and then V's (j, d, m).
+  __device__ __forceinline__ void tile(Rows& s, int t, const Tokens (&k)[2], const lds_bf16x8* from) const {
+    constexpr int U = D / 16, V = D / 32;
+    f32x16 x[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[j][i] = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        x[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(from[(j * U + u) * 64], s.q[u], x[j], 0, 0, 0);
+    fragments_ahead<2 * U>();
+    const int at = t * wir::TILE + lane / 32 * 16;   // the lane's tokens: at + 32 j .. + have[j] - 1
+    const bool edge = __builtin_amdgcn_ballot_w64(k[0].have < 16 || k[1].have < 16 || at + 47 > s.low) != 0;
+    float f[2], log_g[2], inv_g[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float g = __uint_as_float((scale_of(k[j]) & 0x7fffffu) | 0x3f800000u);
+      log_g[j] = __builtin_amdgcn_logf(g), inv_g[j] = __builtin_amdgcn_rcpf(g);
+      // ks log2(e) / sqrt(D)
+      f[j] = (k[j].have ? k[j].ks : 1.f) * (float)(1.4426950408889634 / (D == 64 ? 8.0 : 11.313708498984761));
+    }
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int seen = min(k[j].have, s.pos - (at + 32 * j) + 1);   // of the lane's tokens
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[j][i] = i < seen ? x[j][i] * f[j] : -__builtin_inff();
+        f[j] = 1.f;
       }
-      scales_of(tok, at, t, own);
+    }
+    float top[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      top[j] = x[j][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top[j] = fmaxf(top[j], x[j][i]);
+    }
+    float m = fmaxf(top[0] * f[0], top[1] * f[1]);
+    m = fmaxf(max_of_halves(m), s.m);
+    const float base = m == -__builtin_inff() ? 0.f : m, corr = __builtin_amdgcn_exp2f(s.m - base);
+    s.m = m;
+    s.l *= corr;
+    if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
+#pragma unroll
+      for (int d = 0; d < V; ++d) s.o[d] *= corr;
+    }
+    bf16x8 p[2][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float sum[2] = {0.f, 0.f};
+      const float shift = log_g[j] - base;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][i], f[j], shift));
+        sum[i % 2] += y;
+        p[j][i / 8][i % 8] = (bf16)y;
+      }
+      s.l += (sum[0] + sum[1]) * inv_g[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int d = 0; d < V; ++d)
+          s.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(from[(2 * U + 2 * (j * V + d) + m) * 64], p[j][m], s.o[d], 0, 0, 0);
+    fragments_ahead<4 * V>();
+  }
+
+  // In each iteration a wave asks for its quarter of the next tile (K or V of 32 tokens), computes, and leaves what came
+  // as operands in the other slot.  WIDE: a tile's page and addresses are the wave's, and a lane adds its place (pages of
+  // 64 tokens, this way / by lanes' own addresses: 277 / 291 us for 2 x 1000 over 8192, 308 / 334 for 2 x 2048 over 8192 at
+  // D = 64).
+  __device__ __forceinline__ void walk_shared(Rows& s, int head, int first, int last) const {
+    constexpr int MINE = CHUNKS / W, V = D / 32;
+    const bool mine_k = wave < 2;
+    const int half = wave % 2, h = lane / 32, r = lane % 32;
+    // K: row r of the operand is token 16 (r / 4 % 2) + 4 (r / 8) + r % 4, bytes 32 i + 16 h; V: column 32 i + r, token 16 h
+    const int mine_h = mine_k ? r / 4 % 2 : h, token = 16 * mine_h + (mine_k ? 4 * (r / 8) + r % 4 : 0);
+    const Bases at = bases(head);
+    const unsigned char* head_at = mine_k ? a->k + (((i64)head << at.shift) * D) : a->v + (((i64)head * D) << at.shift);
+    const int token_bytes = mine_k ? D : 1, chunk_bytes = mine_k ? 32 : 32 << at.shift;
+    // the lane's place: WIDE in a tile, else in a segment
+    const unsigned lane_at = mine_k ? ((WIDE ? 32 * half + token : token % 16) * D + 16 * h)
+                                    : (r << at.shift) + (WIDE ? 32 * half + token : 0);
+    u32x4 codes[MINE];
+    Tokens tok[2];
+    auto ask = [&](int t, const int (&page)[3]) {   // of segments h and 2 + h, and of the lane's own codes
+      const unsigned char* from;
+      if constexpr (WIDE) {
+        const int id = __builtin_amdgcn_readfirstlane(page[0]);
+        from = head_at + page_index(at, id) * at.page_bytes + in_page(at, t, 0) * token_bytes;
+        scales_of(tok[0], at, t, h, id);
+        tok[1] = tok[0];
+        tok[1].have = wir::checked_page(id, at.pages) < 0 ? 0 : min(max(span.held - (t * wir::TILE + 16 * (2 + h)), 0), 16);
+      } else {
+        from = head_at + page_index(at, page[2]) * at.page_bytes + in_page(at, t, 2 * half + mine_h) * token_bytes;
+        scales_of(tok[0], at, t, h, page[0]);
+        scales_of(tok[1], at, t, 2 + h, page[1]);
+      }
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) codes[i] = *(const u32x4*)(from + i * chunk_bytes + lane_at);
     };
-    begin(s, head);
+    auto pages_of = [&](int (&page)[3], int t) {
+      page[0] = page_of(at, t, WIDE ? 0 : h);
+      if constexpr (!WIDE) page[1] = page_of(at, t, 2 + h), page[2] = page_of(at, t, 2 * half + mine_h);
+    };
     const int low = max(span.start + min(token_of(rb * BLOCK), span.count), 0);   // of all waves' rows
     auto leave = [&](int t, int slot) {
       float power = 1.f;
       if (!mine_k) {
-        const unsigned bits = scale_of(tok);
+        const Tokens mine = {0.f, half ? tok[1].vs : tok[0].vs, half ? tok[1].have : tok[0].have};   // (not by an index)
+        const unsigned bits = scale_of(mine);
         power = power_of(bits);
-        const int first_token = t * wir::TILE + 16 * grp;
-        if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u || tok.have < 16 || first_token + 15 > low) != 0) {
-          const u32x4 held = held_bytes(tok.have);
+        const int first_token = t * wir::TILE + 32 * half + 16 * h;
+        if (__builtin_amdgcn_ballot_w64(bits >= 0x7f800000u || mine.have < 16 || first_token + 15 > low) != 0) {
+          const u32x4 held = held_bytes(mine.have);
 #pragma unroll
           for (int i = 0; i < MINE; ++i) codes[i] = scaled_codes(codes[i], bits) & held;
-          if (unseen(tok.have, first_token, low)) take_nans<MINE>(codes, mine - 4 * KC, first_token);
+          if (unseen(mine.have, first_token, low)) take_nans<MINE>(codes, r, 32, first_token);
         }
       }
-      lds_bf16x8* to = (lds_bf16x8*)wir::lds(sh.ring + (slot * CHUNKS + mine) * 2048) + lane;
+      lds_bf16x8* to = (lds_bf16x8*)wir::lds(sh.ring + (slot * CHUNKS + wave * MINE) * 2048) + lane;
 #pragma unroll
       for (int i = 0; i < MINE; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u) to[(2 * i + u) * 64] = unpack8(codes[i][2 * u], codes[i][2 * u + 1], power);
     };
-    int next = -1, next_own = -1, slot = 0;
+    static_assert(MINE == V, "");
+    int next[3] = {-1, -1, -1}, slot = 0;
     if (first < last) {
-      ask(first, page_of(at, first, seg), page_of(at, first, grp));
-      next = page_of(at, first + 1, seg), next_own = page_of(at, first + 1, grp);
-      leave(first, 0);
+      pages_of(next, first);
+      ask(first, next);
+      pages_of(next, first + 1);
     }
+    begin(s, head);
+    if (first < last) leave(first, 0);
     for (int t = first; t < last; ++t, slot ^= 1) {
       __syncthreads();
-      const Tokens now = tok;
-      ask(t + 1, next, next_own);
-      next = page_of(at, t + 2, seg), next_own = page_of(at, t + 2, grp);   // (past the end -1, or pages not used)
-      const lds_bf16x8* from = (const lds_bf16x8*)wir::lds(sh.ring + slot * CHUNKS * 2048) + lane;
-      tile(s, t, now, [&](int j, int u) { return (bf16x8)from[(j * 2 * KC + u) * 64]; }, []() {},
-           [](int) { return u32x4{}; }, [&](int d, int u) { return (bf16x8)from[(8 * KC + 2 * d + u) * 64]; });
+      const Tokens now[2] = {tok[0], tok[1]};
+      ask(t + 1, next);
+      pages_of(next, t + 2);   // (past the end -1, or pages not used)
+      tile(s, t, now, (const lds_bf16x8*)wir::lds(sh.ring + slot * CHUNKS * 2048) + lane);
       if (t + 1 < last) leave(t + 1, slot ^ 1);
     }
     __syncthreads();   // the ring is read: results go there
@@ -524,18 +643,29 @@ struct Program {
 
   // Tiles first .. last - 1 of `head` -> sh.r
   __device__ __forceinline__ void walk(int head, int first, int last) {
-    State s;
-    if constexpr (SHARED)
+    if constexpr (SHARED) {
+      Rows s;
       walk_shared(s, head, first, last);
-    else
+      const int row = wave * ROWS + lane % 32, h = lane / 32;
+      auto l = __builtin_amdgcn_permlane32_swap(__float_as_uint(s.l), __float_as_uint(s.l), false, false);
+      if (h == 0) sh.r.ml[2 * row] = s.m, sh.r.ml[2 * row + 1] = __uint_as_float(l[0]) + __uint_as_float(l[1]);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(f32x4*)(sh.r.o + row * PITCH + 32 * d + 8 * g + 4 * h) =
+              f32x4{s.o[d][4 * g], s.o[d][4 * g + 1], s.o[d][4 * g + 2], s.o[d][4 * g + 3]};
+    } else {
+      State s;
       walk_registers(s, head, first, last);
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const float sum = over_groups(s.l[n], [](float x, float y) { return x + y; });
-      const int row = wave * ROWS + n * 16 + col;
-      if (grp == 0) sh.r.ml[2 * row] = s.m[n], sh.r.ml[2 * row + 1] = sum;
+      for (int n = 0; n < NQ; ++n) {
+        const float sum = over_groups(s.l[n], [](float x, float y) { return x + y; });
+        const int row = wave * ROWS + n * 16 + col;
+        if (grp == 0) sh.r.ml[2 * row] = s.m[n], sh.r.ml[2 * row + 1] = sum;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *(f32x4*)(sh.r.o + row * PITCH + 16 * d + 4 * grp) = s.o[d][n];
+        for (int d = 0; d < DT; ++d) *(f32x4*)(sh.r.o + row * PITCH + 16 * d + 4 * grp) = s.o[d][n];
+      }
     }
   }
 
@@ -759,26 +889,28 @@ __device__ __forceinline__ void join(args_ptr a) {
 
 }  // namespace
 
-#define ATTN_KERNEL(NAME, D, NQ, WR, W, OCC)                                                              \
+#define ATTN_KERNEL(NAME, D, NQ, WR, W, OCC, WIDE)                                                        \
   extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W),                  \
                                             amdgpu_waves_per_eu(OCC, OCC))) NAME(const attn_args) {       \
-    __shared__ __attribute__((aligned(1024))) Program<D, NQ, WR, W>::Shared shared;                       \
-    Program<D, NQ, WR, W>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), shared).run();                \
+    __shared__ __attribute__((aligned(1024))) Program<D, NQ, WR, W, WIDE>::Shared shared;                 \
+    Program<D, NQ, WR, W, WIDE>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), shared).run();          \
   }
 #define JOIN_KERNEL(NAME, D, BLOCK, ROWS)                                             \
   extern "C" __global__ void __launch_bounds__(256) NAME(const attn_args) {           \
     join<D, BLOCK, ROWS>((args_ptr)__builtin_amdgcn_kernarg_segment_ptr());           \
   }
 
-ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 4)
-ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 4)
-ATTN_KERNEL(wir_attn_cached_d128_r16_w8, 128, 1, 1, 8, 2)
-ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2)
-ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 3)
-ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 2)
-ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2)
+ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 4, false)
+ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 4, false)
+ATTN_KERNEL(wir_attn_cached_d128_r16_w8, 128, 1, 1, 8, 2, false)
+ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2, false)
+ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2, false)
+ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 3, false)
+ATTN_KERNEL(wir_attn_cached_d64_r128_p64, 64, 2, 4, 4, 3, true)   // pages of 64 tokens or more
+ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2, false)
+ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 2, false)
+ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2, false)
+ATTN_KERNEL(wir_attn_cached_d128_r128_p64, 128, 2, 4, 4, 2, true)   // pages of 64 tokens or more
 JOIN_KERNEL(wir_attn_join_d64_r16, 64, 16, 1)
 JOIN_KERNEL(wir_attn_join_d64_r32, 64, 32, 1)
 JOIN_KERNEL(wir_attn_join_d64_r128, 64, 128, 1)

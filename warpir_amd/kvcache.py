@@ -181,8 +181,8 @@ TILE = 64        # positions of a tile (csrc/wir_pages.h)
 
 # us of one tile of a workgroup that has a CU to itself, and of one CU's time where all are busy, by head size and rows
 # of a block: the slopes of launches of 30 to 500 tiles
-_TILE_US = {128: {16: (0.35, 0.35), 32: (0.55, 0.43), 128: (1.5, 1.2)},
-            64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (1.2, 0.77)}}
+_TILE_US = {128: {16: (0.35, 0.35), 32: (0.55, 0.43), 128: (1.35, 1.1)},
+            64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (0.96, 0.62)}}
 _DIVIDED_US = {128: (13, 0.5, 24, 1.23), 64: (13, 0.26, 24, 0.75)}   # divided: us, and us of a CU for a tile; 16, 128
 
 
@@ -206,12 +206,13 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
     table.  Blocks of 16 rows win while they leave CUs idle, blocks of 128 where
     the work is much.  us, 16 / 32 / 128 rows / 16 divided / 128 divided (D = 128,
     H32/8): 16 queries over 8000 keys 53.6 / 83 / 193 / 19.2 / 24.7, 40 over 2000 17.1 /
-    26 / 60 / 19.7 / 25, 8 x 64 over 2000 54 / 39.9 / 60 / - / 47, 64 over 32000 191 / 274 /
-    750 / 127 / 62, 2 x 1000 over 8192 658 / 410 / 295 / - / 301."""
+    26 / 60 / 19.7 / 25, 8 x 64 over 2000 54 / 41.8 / 54 / - / 50, 64 over 32000 193 / 296 /
+    649 / 111 / 68, 2 x 1000 over 8192 665 / 430 / 278 / - / 293."""
     if rows > 32:
         tiles = -(-columns * page // TILE)
         n = {block: heads * -(-rows // block) for block in (16, 32, 128)}
-        us = {(block, 0): 6 + tiles * max(light, busy * n[block] / 256) for block, (light, busy) in _TILE_US[d].items()}
+        each = {block: x / 256 if x > 512 else -(-x // 256) for block, x in n.items()}   # programs of a CU
+        us = {(block, 0): 6 + tiles * max(light, busy * each[block]) for block, (light, busy) in _TILE_US[d].items()}
         few, few_tile, many, many_tile = _DIVIDED_US[d]
         us[16, 1] = few + few_tile * max(n[16] * tiles / 256, 2)
         us[128, 1] = many + many_tile * max(n[128] * tiles / 256, 2)
@@ -292,7 +293,8 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
                "table": page_table, "lengths": lengths, "counts": counts, "out": out, "lse": lse,
                "partial": workspace, "info": workspace}
     past = {"info": 4 * (floats - 4 * items)}
-    launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}" + ("_w8" if waves == 8 else ""),
+    kind = "_w8" if waves == 8 else "_p64" if block == 128 and page >= TILE else ""
+    launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}{kind}",
            (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
     if extra:
         many = block == 128 and items * min(rows, block) > 2048   # a row a wave, not a workgroup
