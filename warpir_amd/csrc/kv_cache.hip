@@ -57,14 +57,43 @@ struct kv_args {
 
 __device__ __forceinline__ unsigned bits_of(bf16 x) { return (unsigned)__builtin_bit_cast(unsigned short, x); }
 
-// Maximum over a workgroup of 256 (x: finite values' bits, ordered as unsigned).
-__device__ __forceinline__ unsigned group_max(unsigned x) {
-  __shared__ unsigned part[4];
+// Maximum over a page's threads: each `lanes` (32 or 64) of a wave, or not PACKED the workgroup's 256 (x: finite values'
+// bits, ordered as unsigned).
+template <bool PACKED>
+__device__ __forceinline__ unsigned page_max(unsigned x, int lanes) {
 #pragma unroll
-  for (int m = 32; m; m >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, m));
+  for (int m = 32; m; m >>= 1)
+    if (!PACKED || m < lanes) x = max(x, (unsigned)__shfl_xor((int)x, m));
+  if (PACKED) return x;
+  __shared__ unsigned part[4];
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
   __syncthreads();
   return max(max(part[0], part[1]), max(part[2], part[3]));
+}
+
+// A workgroup's page of one sequence and head, of K or of V.  PACKED: pages of 32 or 64 lanes, several to a workgroup,
+// which has threads idle otherwise (us, one a workgroup / packed, pages of 16: 51 x 309 tokens, 12 heads of D = 64, written
+// 32.8 / 16.7; 8 x up to 4096, 8 heads of D = 128 39 / 26.7; 16 x up to 8192 of D = 64 read 123 / 70.  Pages of 128 lanes
+// are no faster packed: 26.4 / 27.0).
+struct Unit {
+  unsigned b, slot, h;
+  int lane;
+  bool is_v, any;
+};
+template <int D, bool PACKED>
+__device__ __forceinline__ Unit unit_of(const kv_args& a, int lanes) {
+  const unsigned first = PACKED ? threadIdx.x / (unsigned)lanes : 0;
+  unsigned at = PACKED ? blockIdx.x * (256 / (unsigned)lanes) + first : blockIdx.x;
+  Unit u;
+  u.lane = threadIdx.x - first * lanes;
+  u.is_v = at & 1;
+  at >>= 1;
+  u.h = at % (unsigned)a.heads;
+  at /= (unsigned)a.heads;
+  u.slot = at % (unsigned)a.slots, u.b = at / (unsigned)a.slots;
+  u.any = !PACKED || u.b < (unsigned)a.batch;
+  if (PACKED && !u.any) u.b = 0;
+  return u;
 }
 
 // Two codes in the low or high half of a word.  An infinity becomes NaN, which e4m3 has and infinity not.
@@ -87,36 +116,34 @@ __device__ __forceinline__ void rescale2(unsigned* at, float ratio) {
   *(u32x2*)at = u32x2{rescale(w[0], ratio), rescale(w[1], ratio)};
 }
 
-// Workgroup -> one page of one sequence and head, of K or of V: a page's scale
-// needs all of its new values first, and so few stay in registers between the
-// two.  A lane takes 4 tokens x 8 columns; PASSES of 256 lanes cover a page.
-template <int D, int PASSES>
+// Workgroup -> one page of one sequence and head, of K or of V, or several: a
+// page's scale needs all of its new values first, and so few stay in registers
+// between the two.  A lane takes 4 tokens x 8 columns; PASSES of 256 lanes
+// cover a page.
+template <int D, int PASSES, bool PACKED>
 __device__ __forceinline__ void write(const kv_args& a) {
   constexpr int COLS = D / 8;
-  unsigned at = blockIdx.x;
-  const bool is_v = at & 1;
-  at >>= 1;
-  const unsigned h = at % (unsigned)a.heads;
-  at /= (unsigned)a.heads;
-  const unsigned slot = at % (unsigned)a.slots, b = at / (unsigned)a.slots;
+  const int groups = a.page / 4, lanes = groups * COLS;
+  const Unit u = unit_of<D, PACKED>(a, lanes);
+  const unsigned h = u.h, slot = u.slot, b = u.b;
+  const bool is_v = u.is_v;
   const kv_side& side = is_v ? a.v : a.k;
 
   const wir::Span s = wir::span_of(a.lengths[b], a.counts ? a.counts[b] : a.tokens, a.tokens, a.columns * a.page);
-  const int place = wir::first_new(s) / a.page + (int)slot;
-  if (place >= a.columns) return;
+  const int place = min(wir::first_new(s) / a.page + (int)slot, a.columns);
   const int base = place * a.page;   // position of the page's first token
-  const int lo = max(wir::first_new(s), base), hi = min(s.held, base + a.page);
-  if (lo >= hi) return;
-  const int id = wir::checked_page(a.table[b * a.tb + place], a.pages);
-  if (id < 0) return;
-  const i64 index = (i64)id * a.heads + h;
+  const int lo = max(wir::first_new(s), base);
+  int hi = min(s.held, base + a.page), id = -1;
+  if (u.any && place < a.columns && lo < hi) id = wir::checked_page(a.table[b * a.tb + place], a.pages);
+  if (!PACKED && id < 0) return;
+  if (PACKED && id < 0) hi = 0;   // no tokens
+  const i64 index = (i64)max(id, 0) * a.heads + h;
   unsigned* codes = (unsigned*)(side.codes + index * a.page * D);
   const bool kept = lo > base;   // (the page then holds positions base .. lo - 1)
   const float was = side.scales[index];
 
   // lane -> tokens 4 r .. 4 r + 3 of the page and columns 8 c .. 8 c + 7: neighbours in K's store order or, for whole
   // V pages, in V's (a few tokens then keep to few waves, and the others skip the work)
-  const int groups = a.page / 4, lanes = groups * COLS;
   const bool by_token = is_v && hi - lo >= 16;
   const bf16* x = side.x + b * side.xb + h * side.xh;
   bf16x8 val[PASSES][4];
@@ -124,7 +151,7 @@ __device__ __forceinline__ void write(const kv_args& a) {
   unsigned top = 0;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int l = p * 256 + threadIdx.x, r = by_token ? l % groups : l / COLS, c = by_token ? l / groups : l % COLS;
+    const int l = p * 256 + u.lane, r = by_token ? l % groups : l / COLS, c = by_token ? l / groups : l % COLS;
     const int pos = base + 4 * r;
     if (l >= lanes || pos >= hi || pos + 4 <= lo) continue;
 #pragma unroll
@@ -144,15 +171,15 @@ __device__ __forceinline__ void write(const kv_args& a) {
         top = max(top, m < 0x7f80u ? m : 0u);
       }
   }
-  const float enough = __uint_as_float(wir::scale_bits(group_max(top) << 16));
+  const float enough = __uint_as_float(wir::scale_bits(page_max<PACKED>(top, lanes) << 16));
   const float scale = kept && was >= enough ? was : enough;
   const bool grown = kept && !(scale == was);
   const float inv = 1.0f / scale, ratio = was / scale;
-  if (threadIdx.x == 0) side.scales[index] = scale;
+  if (u.lane == 0 && (!PACKED || id >= 0)) side.scales[index] = scale;
 
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int l = p * 256 + threadIdx.x, r = by_token ? l % groups : l / COLS, c = by_token ? l / groups : l % COLS;
+    const int l = p * 256 + u.lane, r = by_token ? l % groups : l / COLS, c = by_token ? l / groups : l % COLS;
     const int pos = base + 4 * r;
     if (l >= lanes || pos >= hi) continue;
     unsigned* to = codes + (8 * c * a.page + 4 * r) / 4;   // V: word j the four tokens of column 8 c + j
@@ -204,17 +231,17 @@ __device__ __forceinline__ void write(const kv_args& a) {
   }
 }
 
-// Workgroup -> one page's places of one sequence and head, of K or of V, as
-// dense rows; places past the sequence and those of no page become 0.
-template <int D, int PASSES>
+// Workgroup -> one page's places of one sequence and head, of K or of V, or
+// several, as dense rows; places past the sequence and those of no page
+// become 0.
+template <int D, int PASSES, bool PACKED>
 __device__ __forceinline__ void read(const kv_args& a) {
   constexpr int COLS = D / 8;
-  unsigned at = blockIdx.x;
-  const bool is_v = at & 1;
-  at >>= 1;
-  const unsigned h = at % (unsigned)a.heads;
-  at /= (unsigned)a.heads;
-  const unsigned slot = at % (unsigned)a.slots, b = at / (unsigned)a.slots;
+  const int groups = a.page / 4, lanes = groups * COLS;
+  const Unit u = unit_of<D, PACKED>(a, lanes);
+  if (!u.any) return;
+  const unsigned h = u.h, slot = u.slot, b = u.b;
+  const bool is_v = u.is_v;
   const kv_side& side = is_v ? a.v : a.k;
   const int held = wir::span_of(a.lengths[b], 0, 0, a.columns * a.page).held;
   const int base = (int)slot * a.page;
@@ -224,11 +251,10 @@ __device__ __forceinline__ void read(const kv_args& a) {
   const i64 index = (i64)(id < 0 ? 0 : id) * a.heads + h;
   const unsigned* codes = (const unsigned*)(side.codes + index * a.page * D);
   const float scale = side.scales[index];
-  const int groups = a.page / 4, lanes = groups * COLS;
   bf16* x = side.x + b * side.xb + h * side.xh;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int l = p * 256 + threadIdx.x, r = is_v ? l % groups : l / COLS, c = is_v ? l / groups : l % COLS;
+    const int l = p * 256 + u.lane, r = is_v ? l % groups : l / COLS, c = is_v ? l / groups : l % COLS;
     if (l >= lanes || base + 4 * r >= a.tokens) continue;
     // word (i, u): columns 4 u .. of token i (K), or w[j]: tokens of column j (V)
     unsigned w[8] = {};
@@ -269,9 +295,13 @@ __device__ __forceinline__ void read(const kv_args& a) {
 #define KV_KERNEL(NAME, CALL) \
   extern "C" __global__ void __launch_bounds__(256) NAME(const kv_args args) { CALL(args); }
 
-KV_KERNEL(wir_kv_write_d64, (write<64, 1>))
-KV_KERNEL(wir_kv_write_d128, (write<128, 1>))
-KV_KERNEL(wir_kv_write_d128_p128, (write<128, 2>))   // pages of 128 tokens
-KV_KERNEL(wir_kv_read_d64, (read<64, 1>))
-KV_KERNEL(wir_kv_read_d128, (read<128, 1>))
-KV_KERNEL(wir_kv_read_d128_p128, (read<128, 2>))
+KV_KERNEL(wir_kv_write_d64, (write<64, 1, false>))
+KV_KERNEL(wir_kv_write_d64_packed, (write<64, 1, true>))     // pages of 16 and 32 tokens
+KV_KERNEL(wir_kv_write_d128, (write<128, 1, false>))
+KV_KERNEL(wir_kv_write_d128_packed, (write<128, 1, true>))   // pages of 16
+KV_KERNEL(wir_kv_write_d128_p128, (write<128, 2, false>))    // pages of 128
+KV_KERNEL(wir_kv_read_d64, (read<64, 1, false>))
+KV_KERNEL(wir_kv_read_d64_packed, (read<64, 1, true>))
+KV_KERNEL(wir_kv_read_d128, (read<128, 1, false>))
+KV_KERNEL(wir_kv_read_d128_packed, (read<128, 1, true>))
+KV_KERNEL(wir_kv_read_d128_p128, (read<128, 2, false>))

@@ -93,8 +93,11 @@ def _launch(fn, rec, kernel, cache, k, v, page_table, lengths, counts, slots, de
         return False
     args = _Args(*(_Side(None, None, None, *x.stride()[:3]) for x in (k, v)), None, None, None, page_table.stride(0),
                  batch, heads, tokens, cache.k.shape[2], cache.k.shape[0], page_table.shape[1], slots)
-    name = f"{kernel}_d{d}" + ("_p128" if d == 128 and cache.k.shape[2] == 128 else "")
-    launch(rec, device, "kv_cache.hsaco", name, (programs, 1, 1), (256, 1, 1), args,
+    lanes = cache.k.shape[2] // 4 * (d // 8)   # of a page: 4 tokens x 8 columns each
+    kind = "_packed" if lanes <= 64 else "_p128" if lanes > 256 else ""
+    if lanes <= 64:   # pages of a workgroup (csrc/kv_cache.hip)
+        programs = -(-programs * lanes // 256)
+    launch(rec, device, "kv_cache.hsaco", f"{kernel}_d{d}{kind}", (programs, 1, 1), (256, 1, 1), args,
            {"k.codes": cache.k, "k.scales": cache.k_scale, "k.x": k, "v.codes": cache.v, "v.scales": cache.v_scale,
             "v.x": v, "table": page_table, "lengths": lengths, "counts": counts})
     return True
