@@ -34,15 +34,17 @@
 // 5% at D = 128, 3% at 64), and share the tiles: each wave converts its part
 // of the next tile's codes and leaves them in LDS as operands (a fragment is 64
 // lanes' 16 bytes in lane order), so that a code is converted once for 128
-// rows.  2 x 1000 queries over 8192 keys (32/8 heads, D = 128): 281 us, 897
-// TFLOP/s, 68% of a large matrix product's 1328.  No one thing bounds it: taken
-// out of a copy each by itself, the next tile's loads are 10% of the time, its
-// conversion and LDS stores 10%, the softmax 14%, the barrier 1.5%, half of the
-// LDS reads 2.5%; two waves a SIMD cover each other only in part, and the
-// registers of 32 rows leave no room for a third.  The next tile's scores under
-// this one's exponentials, 64 rows a wave, 256 rows a workgroup with the halves
-// of its waves in opposite phases, loads two tiles ahead, and higher priorities
-// for either phase changed nothing.
+// rows.  2 x 1000 queries over 8192 keys (32/8 heads, D = 128): 278 us, 907
+// TFLOP/s, 68% of a large matrix product's 1328, with the matrix cores busy 42%
+// and the vector ALU 56% of the cycles at 2.1 GHz, to which the card's power
+// holds it (on 16x16x32 products 2.3 GHz, and 16% more cycles).  No one thing
+// bounds it: taken out of a copy each by itself, the next tile's loads are 10%
+// of the time, its conversion and LDS stores 10%, the softmax 14%, the barrier
+// 1.5%, half of the LDS reads 2.5%; two waves a SIMD cover each other only in
+// part, and the registers of 32 rows leave no room for a third.  The next tile's
+// scores under this one's exponentials, 64 rows a wave, 256 rows a workgroup
+// with the halves of its waves in opposite phases, loads two tiles ahead, and
+// higher priorities for either phase changed nothing.
 #include "wir_cdna4.h"
 #include "wir_pages.h"
 
