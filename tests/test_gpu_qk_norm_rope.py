@@ -15,7 +15,7 @@ import torch
 from oracle.layer_ref import angles_ref, norm_rope_bwd_ref, norm_rope_ref
 from oracle.torch_ref import seeded_normal
 from tests.conftest import announce
-from warpir_amd import api
+from warpir_amd import api, plans, rotary
 
 pytestmark = pytest.mark.gpu
 
@@ -114,6 +114,27 @@ def test_outputs_given_in_place_and_strided(gpu):
     assert again[0] is gq and again[2] is own[0] and all(torch.equal(x, y) for x, y in zip(again, grads))
     got = api.qk_norm_rope(q, k, qw, kw, *table, q_out=q, k_out=k)
     assert got[0] is q and all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_in_place_and_one_weight_by_their_plans(gpu):
+    """The results of calls with tensors of their own, and the tensors that were given."""
+    q, k, w, _ = _inputs(2, 4, 2, 19, 64, True, False)
+    table = api.rope_table(32, 64)
+    want = api.qk_norm_rope(q, k, w, w.clone(), *table)
+    gq, gk = torch.randn_like(want[0]), torch.randn_like(want[1])
+    grads = api.qk_norm_rope_backward(gq, gk, q, k, w, w.clone(), *table)
+    held = [[plans.native().size(p._table) for p in (rotary._forward_plans, rotary._backward_plans)]]
+    for _ in range(3):
+        x, y = q.clone(), k.clone()
+        got = api.qk_norm_rope(x, y, w, w, *table, q_out=x, k_out=y)
+        assert got[0] is x and got[1] is y and all(torch.equal(a, b) for a, b in zip(got, want))
+        for over in ((gq, gk), (q, k)):
+            at = [t.clone() for t in (gq, gk, q, k)]
+            dq, dk = at[:2] if over[0] is gq else at[2:]
+            got = api.qk_norm_rope_backward(*at, w, w, *table, dq=dq, dk=dk)
+            assert got[0] is dq and got[1] is dk and all(torch.equal(a, b) for a, b in zip(got, grads))
+        held.append([plans.native().size(p._table) for p in (rotary._forward_plans, rotary._backward_plans)])
+    assert all(a < b for a, b in zip(*held[:2])) and held[1] == held[2] == held[3]
 
 
 def test_positions_outside_the_table_and_special_rows(gpu):

@@ -101,6 +101,19 @@ def test_norm_rope_past_the_pointers(monkeypatch, change, error):
         api.qk_norm_rope(**_rope(**change))
 
 
+def test_one_tensor_for_two_results():
+    one = _fake(2, 2, 8, 64)
+    with pytest.raises(ValueError, match="q_out and k_out are one tensor"):
+        api.qk_norm_rope(**_rope(q=_fake(2, 2, 8, 64)), q_out=one, k_out=one)
+    with pytest.raises(ValueError, match="dq and dk are one tensor"):
+        api.qk_norm_rope_backward(one, one, **_rope(q=_fake(2, 2, 8, 64)), dq=one, dk=one)
+    w = _fake(64, dtype=f32)
+    with pytest.raises(ValueError, match="dq_weight and dk_weight are one tensor"):
+        api.qk_norm_rope_backward(one, one, **_rope(q=_fake(2, 2, 8, 64)), dq_weight=w, dk_weight=w)
+    with pytest.raises(ValueError, match="k and v are one tensor"):
+        api.kv_cache_read(None, None, None, 8, k=one, v=one)
+
+
 def test_norm_rope_backward_past_the_pointers(monkeypatch):
     _lenient(monkeypatch)
     g = dict(dq_out=_fake(2, 4, 8, 64), dk_out=_fake(2, 2, 8, 64), dq=_fake(2, 4, 8, 64), dk=_fake(2, 2, 8, 64),

@@ -59,6 +59,12 @@ def check_written(fn: str, name: str, t) -> None:
         span = stride * (size - 1) + span
 
 
+def own(t, other):
+    """``t`` as a tensor of its own where it is ``other``: a call that gives one
+    tensor twice has no plan."""
+    return t.view_as(t) if t is other and hasattr(t, "view_as") else t
+
+
 @functools.lru_cache(maxsize=None)
 def _kernel(filename: str, symbol: str, device: int) -> RawKernel:
     return RawKernel(filename, symbol)   # (a code object is loaded for one device)
@@ -123,4 +129,4 @@ class DevicePlans(Plans):
         return r
 
 
-__all__ = ["check_tensor", "check_written", "need", "launch", "on", "DevicePlans", "INT_MAX"]
+__all__ = ["check_tensor", "check_written", "need", "own", "launch", "on", "DevicePlans", "INT_MAX"]

@@ -6,7 +6,7 @@ import ctypes
 import functools
 from typing import NamedTuple, Tuple
 
-from warpir_amd.handwritten import DevicePlans, check_tensor, check_written, launch, need
+from warpir_amd.handwritten import DevicePlans, check_tensor, check_written, launch, need, own
 
 PAGE_SIZES = (16, 32, 64, 128)
 _write_plans = DevicePlans("kv_cache_write")
@@ -79,12 +79,6 @@ def _validate(fn, cache, page_table, lengths, counts):
     return batch, heads, page, d, device
 
 
-def _own(counts, lengths):
-    """``counts`` as a tensor of its own where it is ``lengths`` (whole prompts): a
-    call that gives one tensor twice has no plan."""
-    return counts.view_as(counts) if counts is lengths and hasattr(counts, "view_as") else counts
-
-
 def _launch(fn, rec, kernel, cache, k, v, page_table, lengths, counts, slots, device):
     batch, heads, tokens, d = k.shape
     programs = batch * slots * heads * 2
@@ -124,7 +118,8 @@ def kv_cache_write(cache: KVCache, k, v, page_table, lengths, counts=None) -> KV
     import torch
 
     fn, done = "kv_cache_write", None
-    counts = _own(counts, lengths)
+    if counts is lengths:
+        counts = own(counts, lengths)
     if isinstance(cache, KVCache):
         done = _write_plans.run(0, k, v, *cache, page_table, lengths, counts)
         if done is not None and done is not False:
@@ -150,6 +145,7 @@ def kv_cache_read(cache: KVCache, page_table, lengths, tokens: int, k=None, v=No
     import torch
 
     fn, done = "kv_cache_read", None
+    need(fn, k is None or k is not v, "k and v are one tensor")
     if isinstance(cache, KVCache) and type(tokens) is int:
         done = _read_plans.run(tokens, *cache, page_table, lengths, k, v)
         if done is not None and done is not False:
@@ -252,7 +248,8 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     import torch
 
     fn, done = "attention_cached", None
-    counts = _own(counts, lengths)
+    if counts is lengths:
+        counts = own(counts, lengths)
     if isinstance(cache, KVCache) and workspace is None:
         done = _attention_plans.run(0, q, *cache, page_table, lengths, counts, out, lse)
         if done is not None and done is not False:

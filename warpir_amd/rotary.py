@@ -7,7 +7,7 @@ import functools
 import struct
 from typing import Optional, Tuple
 
-from warpir_amd.handwritten import INT_MAX, DevicePlans, check_tensor, check_written, launch, need
+from warpir_amd.handwritten import INT_MAX, DevicePlans, check_tensor, check_written, launch, need, own
 
 _forward_plans = DevicePlans("qk_norm_rope")
 _backward_plans = DevicePlans("qk_norm_rope_backward")
@@ -115,16 +115,23 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
 
     fn = "qk_norm_rope"
     flags, done = _flags(eps, interleaved) if type(eps) is float and type(interleaved) is bool else None, None
+    given = None
+    if q_out is not None or k_out is not None:
+        need(fn, q_out is not k_out, "q_out and k_out are one tensor")
+        given = q_out, k_out
+        q_out, k_out = own(q_out, q), own(k_out, k)
+    if k_weight is q_weight:
+        k_weight = own(k_weight, q_weight)
     if flags is not None:
         done = _forward_plans.run(flags, q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out)
         if done is not None and done is not False:
-            return done
+            return _results(given, done)
     b, h, s, d, device = _validate(fn, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     rec = _forward_plans.recording(done, q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out)
     q_out = _output(fn, "q_out", q_out, q, rec)
     k_out = _output(fn, "k_out", k_out, k, rec)
     if b * s * (h + k.shape[1]) == 0:
-        return q_out, k_out
+        return _results(given, (q_out, k_out))
     args = _packed(q, k, q_out, k_out, None, None, q_weight, cos, sin, positions, eps)
     rows = 4096 // d   # rows of a workgroup, all of one sequence
     launch(rec, device, "qk_norm_rope.hsaco", f"wir_qk_norm_rope_d{d}" + ("_inter" if interleaved else ""),
@@ -133,7 +140,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
             "sin": sin, "pos": positions})
     if rec:
         _forward_plans.add(flags, rec, q_out, k_out)
-    return q_out, k_out
+    return _results(given, (q_out, k_out))
+
+
+def _results(given, done):
+    """The tensors that the caller gave, where it did."""
+    return done if given is None else tuple(x if g is None else g for g, x in zip(given, done))
 
 
 def _output(fn, name, out, like, rec):
@@ -153,22 +165,30 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     those of its outputs (``dq_out``, ``dk_out``, bf16, shaped as ``q`` and ``k``, any
     row-aligned layout) and its inputs; ``dq`` and ``dk`` are bf16, the weights'
     gradients fp32 sums over all rows, added in an order that the shapes fix.
-    ``dq`` and ``dk`` may be ``dq_out`` and ``dk_out`` themselves.
+    ``dq`` and ``dk`` may be ``dq_out`` and ``dk_out`` themselves, or ``q`` and ``k``.
     ``workspace`` holds the workgroups' partial sums (fp32, at least
     ``1025 * D`` elements, allocated if omitted)."""
     import torch
 
     fn = "qk_norm_rope_backward"
     flags, done = _flags(eps, interleaved) if type(eps) is float and type(interleaved) is bool else None, None
-    given = (dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions, dq, dk, dq_weight, dk_weight)
+    given = None
+    if dq is not None or dk is not None or dq_weight is not None or dk_weight is not None:
+        need(fn, dq is None or dq is not dk, "dq and dk are one tensor")
+        need(fn, dq_weight is None or dq_weight is not dk_weight, "dq_weight and dk_weight are one tensor")
+        given = dq, dk, dq_weight, dk_weight
+        dq, dk = own(own(dq, dq_out), q), own(own(dk, dk_out), k)
+    if k_weight is q_weight:
+        k_weight = own(k_weight, q_weight)
+    tensors = (dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions, dq, dk, dq_weight, dk_weight)
     if flags is not None and workspace is None:
-        done = _backward_plans.run(flags, *given)
+        done = _backward_plans.run(flags, *tensors)
         if done is not None and done is not False:
-            return done
+            return _results(given, done)
     b, h, s, d, device = _validate(fn, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     check_tensor(fn, "dq_out", dq_out, q.dtype, q.shape, device)
     check_tensor(fn, "dk_out", dk_out, k.dtype, k.shape, device)
-    rec = _backward_plans.recording(done, *given)
+    rec = _backward_plans.recording(done, *tensors)
     dq = _output(fn, "dq", dq, q, rec)
     dk = _output(fn, "dk", dk, k, rec)
     weights = []
@@ -181,7 +201,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     if b * s * (h + hk) == 0:
         for w in weights:
             w.zero_()
-        return (dq, dk, *weights)
+        return _results(given, (dq, dk, *weights))
     args = _packed(q, k, dq, dk, dq_out, dk_out, q_weight, cos, sin, positions, eps)
     args.q.blocks, args.k.blocks = _blocks(b * s * h, b * s * hk, d)
     floats = (args.q.blocks + args.k.blocks) * d
@@ -198,7 +218,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
            {"partial": workspace, "q": weights[0], "k": weights[1]})
     if rec:
         _backward_plans.add(flags, rec, dq, dk, *weights)
-    return (dq, dk, *weights)
+    return _results(given, (dq, dk, *weights))
 
 
 def _blocks(q_rows: int, k_rows: int, d: int) -> Tuple[int, int]:
