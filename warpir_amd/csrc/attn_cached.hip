@@ -903,7 +903,9 @@ __device__ __forceinline__ void join(args_ptr a) {
   }
 
 ATTN_KERNEL(wir_attn_cached_d64_r16, 64, 1, 1, 4, 4, false)
+ATTN_KERNEL(wir_attn_cached_d64_r16_w2, 64, 1, 1, 2, 4, false)
 ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 4, false)
+ATTN_KERNEL(wir_attn_cached_d128_r16_w2, 128, 1, 1, 2, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r16_w8, 128, 1, 1, 8, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2, false)

@@ -219,8 +219,13 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
         return (block, 4, 256 if block == 16 else max(512 - n[128], 256), 2) if divided else (block, 4, 0, 0)
     block, held = 16 if rows <= 16 else 32, columns * page * 2 * d   # bytes of a head at most
     if held <= 640 << 10 and held * (1 - heads / 105) <= 147 << 10:
-        # eight waves a head while there is one such program for each CU
-        return block, 8 if heads <= 256 and columns * page > 16 * TILE and (block, d) != (32, 128) else 4, 0, 0
+        # eight waves a head while there is one such program for each CU, two where many heads are short (us, two / four
+        # waves, 32/8 heads of D = 128: 1024 sequences of up to 200 keys 67 / 92, 128 of up to 1000 32.0 / 32.3; 8192 heads of
+        # D = 64 and up to 100 keys 22 / 32; but 512 sequences of up to 2500 249 / 242)
+        short = columns * page <= 16 * TILE
+        if block == 16 and heads >= 1024 and short:
+            return block, 2, 0, 0
+        return block, 8 if heads <= 256 and not short and (block, d) != (32, 128) else 4, 0, 0
     # two programs of four waves a CU (32 sequences of up to 16000 keys, 256 heads: 384 more 96.6, 128 or 1024 over
     # 99); with more heads, one of eight and as many more (64 sequences of up to 8192, 512 heads: 512 more of eight
     # waves 119.6, 1536 of four 122)
@@ -293,7 +298,7 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
                "table": page_table, "lengths": lengths, "counts": counts, "out": out, "lse": lse,
                "partial": workspace, "info": workspace}
     past = {"info": 4 * (floats - 4 * items)}
-    kind = "_w8" if waves == 8 else "_p64" if block == 128 and page >= TILE else ""
+    kind = f"_w{waves}" if waves != 4 else "_p64" if block == 128 and page >= TILE else ""
     launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}{kind}",
            (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
     if extra:
