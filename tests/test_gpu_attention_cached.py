@@ -96,7 +96,7 @@ def test_long_sequences_in_many_parts(gpu, heads, hkv, tokens, d):
 
 
 @pytest.mark.parametrize("forced", [(16, 4, 7, 1), (16, 8, 3, 2), (128, 4, 5, 1), (32, 4, 512, 1), (128, 4, 0, 0),
-                                    (16, 8, 0, 0), (16, 2, 0, 0), (16, 4, 1, 1), (32, 8, 70, 1), (128, 4, 512, 2), (16, 4, 13, 9)])
+                                    (16, 8, 0, 0), (16, 2, 0, 0), (32, 2, 0, 0), (16, 4, 1, 1), (32, 8, 70, 1), (128, 4, 512, 2), (16, 4, 13, 9)])
 def test_every_division_gives_the_same(gpu, monkeypatch, forced):
     """Few programs that each take several heads' tiles, shares that end inside them, and no division."""
     lengths, counts = (130, 0, 400, 65), (3, 0, 3, 1)
@@ -176,11 +176,11 @@ def test_blocks_of_128_rows(gpu, monkeypatch, d, page):
     assert bool(wide[0][2, 3:, :7].isnan().all()) and not bool(wide[0][2, :3].isnan().any())
 
 
-@pytest.mark.parametrize("batch,d", [(700, 64), (1100, 64), (1100, 128)])
-def test_more_sequences_than_threads(gpu, batch, d):
+@pytest.mark.parametrize("batch,heads,d", [(700, 2, 64), (1100, 2, 64), (1100, 2, 128), (800, 20, 64), (800, 20, 128)])
+def test_more_sequences_than_threads(gpu, batch, heads, d):
     lengths = [(i * 37) % 90 for i in range(batch)]
     cache, table = _cache(batch, 1, 16, d, 40, lengths)
-    q = seeded_normal((batch, 2, 1, d), 5)
+    q = seeded_normal((batch, heads, 1, d), 5)
     _compare(_run(q, _gpu(cache), table, lengths), q, cache, table, lengths)
 
 

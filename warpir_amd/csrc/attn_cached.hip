@@ -907,11 +907,13 @@ ATTN_KERNEL(wir_attn_cached_d64_r16_w2, 64, 1, 1, 2, 4, false)
 ATTN_KERNEL(wir_attn_cached_d64_r16_w8, 64, 1, 1, 8, 4, false)
 ATTN_KERNEL(wir_attn_cached_d128_r16_w2, 128, 1, 1, 2, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r16_w8, 128, 1, 1, 8, 2, false)
+ATTN_KERNEL(wir_attn_cached_d64_r32_w2, 64, 2, 1, 2, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 3, false)
 ATTN_KERNEL(wir_attn_cached_d64_r128_p64, 64, 2, 4, 4, 3, true)   // pages of 64 tokens or more
 ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2, false)
+ATTN_KERNEL(wir_attn_cached_d128_r32_w2, 128, 2, 1, 2, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r128_p64, 128, 2, 4, 4, 2, true)   // pages of 64 tokens or more

@@ -219,11 +219,12 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
         return (block, 4, 256 if block == 16 else max(512 - n[128], 256), 2) if divided else (block, 4, 0, 0)
     block, held = 16 if rows <= 16 else 32, columns * page * 2 * d   # bytes of a head at most
     if held <= 640 << 10 and held * (1 - heads / 105) <= 147 << 10:
-        # eight waves a head while there is one such program for each CU, two where many heads are short (us, two / four
-        # waves, 32/8 heads of D = 128: 1024 sequences of up to 200 keys 67 / 92, 128 of up to 1000 32.0 / 32.3; 8192 heads of
-        # D = 64 and up to 100 keys 22 / 32; but 512 sequences of up to 2500 249 / 242)
+        # eight waves a head while there is one such program for each CU, two where more heads than four fill the CUs
+        # with are short (us, two / four waves, 32/8 heads of D = 128: 1024 sequences of up to 200 keys 67 / 92, 128 of up to
+        # 1000 32.0 / 32.3, 100 of up to 300 13.1 / 15.3; with 8 tokens 512 of up to 1000 164 / 180, 128 of 1000 47.5 / 55;
+        # but 512 of up to 2500 249 / 242, and with 8 tokens 80 of up to 1000 41 / 37)
         short = columns * page <= 16 * TILE
-        if block == 16 and heads >= 1024 and short:
+        if heads >= 768 and short:
             return block, 2, 0, 0
         return block, 8 if heads <= 256 and not short and (block, d) != (32, 128) else 4, 0, 0
     # two programs of four waves a CU (32 sequences of up to 16000 keys, 256 heads: 384 more 96.6, 128 or 1024 over
