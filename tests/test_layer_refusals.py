@@ -228,6 +228,8 @@ def test_empty_cache_and_table():
           lse=_fake(3, 4, 1 << 23, dtype=f32)), "2\\^24 query rows"),
     (dict(q=_fake(3, 4, 1, 64).expand(3, 4, 1 << 20, 64), out=_fake(3, 4, 1 << 20, 64), lse=_fake(3, 4, 1 << 20, dtype=f32),
           page_table=_fake(3, 1 << 21, dtype=i32)), "2\\^30 tiles"),
+    (dict(q=_fake(1, 2, 1, 64).expand(1 << 22, 2, 1, 64), out=_fake(1 << 22, 2, 1, 64), lse=_fake(1 << 22, 2, 1, dtype=f32),
+          page_table=_fake(1 << 22, 1000, dtype=i32), lengths=_fake(1 << 22, dtype=i32)), "2\\^32 threads"),
 ])
 def test_attention_cached(monkeypatch, change, error):
     _lenient(monkeypatch)

@@ -284,6 +284,7 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     blocks = -(-rows // block)
     items = batch * blocks * heads
     need(fn, items * min(rows, block) < 1 << 24, "2^24 query rows or more in one call")
+    need(fn, (items + extra) * waves < 1 << 26, "2^32 threads or more in one call")
     need(fn, items * max(1, -(-page_table.shape[1] * page // TILE)) < 1 << 30, "2^30 tiles of keys or more in one call")
     args = _AttnArgs(*[None] * 12, *q.stride()[:3], *out.stride()[:3], *lse.stride(), page_table.stride(0), batch, heads,
                      group, tokens, page.bit_length() - 1, cache.k.shape[0], page_table.shape[1], blocks, extra, least)
