@@ -842,7 +842,7 @@ struct Program {
 // of each, one row a wave (ROWS = 4).
 template <int D, int BLOCK, int ROWS>
 __device__ __forceinline__ void join(args_ptr a) {
-  constexpr int CH = D / 4, PER = 256 / ROWS / CH;   // lanes of a row; partial results read side by side
+  constexpr int CH = D / 4, PER = 256 / ROWS / CH, EARLY = 4;   // lanes of a row; partial results read side by side
   __shared__ f32x4 sums[256];
   __shared__ float ls[ROWS * PER];
   const int per = (min(a->tokens * a->group, BLOCK) + ROWS - 1) / ROWS;   // programs of an item
@@ -859,19 +859,33 @@ __device__ __forceinline__ void join(args_ptr a) {
   const int ch = lane % CH, w = lane / CH;
   float top = -__builtin_inff(), l = 0.f;
   if (mine) {
+    // the first partial results are on their way while their maxima are compared
+    f32x4 early[EARLY];
+    f32x2 early_ml[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) {
+      const i64 at = place(min(w + i * PER, parts - 1));
+      early_ml[i] = ml[at];
+      early[i] = *(const f32x4*)(a->partial + at * D + 4 * ch);
+    }
     for (int p = wir::lane_id(); p < parts; p += 64) top = fmaxf(top, ml[place(p)][0]);   // every wave for itself
 #pragma unroll
     for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
     top = over_groups(top, [](float x, float y) { return fmaxf(x, y); });
     const float base = top == -__builtin_inff() ? 0.f : top;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = w; p < parts; p += PER) {
-      const i64 at = place(p);
-      const f32x2 y = ml[at];
+    auto add = [&](const f32x2& y, const f32x4& z) {
       const float f = __builtin_amdgcn_exp2f(y[0] - base);
       l += f * y[1];
-      x += f * *(const f32x4*)(a->partial + at * D + 4 * ch);
+      x += f * z;
+    };
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i)
+      if (w + i * PER < parts) add(early_ml[i], early[i]);
+#pragma unroll 4
+    for (int p = w + EARLY * PER; p < parts; p += PER) {
+      const i64 at = place(p);
+      add(ml[at], *(const f32x4*)(a->partial + at * D + 4 * ch));
     }
     sums[threadIdx.x] = x;
     if (ch == 0) ls[sub * PER + w] = l;
