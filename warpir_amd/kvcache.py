@@ -250,7 +250,9 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
 
     The keys of a sequence are divided over the chip by its lengths as they
     are on the GPU; partial results go through ``workspace`` (fp32, as many
-    elements as ``attention_cached_workspace`` says, allocated if omitted)."""
+    elements as ``attention_cached_workspace`` says, allocated if omitted), which
+    one call at a time may use: two streams, or two graphs that run at once,
+    need one each."""
     import torch
 
     fn, done = "attention_cached", None

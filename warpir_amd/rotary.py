@@ -167,7 +167,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     gradients fp32 sums over all rows, added in an order that the shapes fix.
     ``dq`` and ``dk`` may be ``dq_out`` and ``dk_out`` themselves, or ``q`` and ``k``.
     ``workspace`` holds the workgroups' partial sums (fp32, at least
-    ``1025 * D`` elements, allocated if omitted)."""
+    ``1025 * D`` elements, allocated if omitted); one call at a time may use it."""
     import torch
 
     fn = "qk_norm_rope_backward"
