@@ -108,7 +108,7 @@ def test_every_division_gives_the_same(gpu, monkeypatch, forced):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("forced", [(16, 4, 256, 2), (32, 4, 40, 1), (128, 4, 300, 2), (16, 4, 3, 1), (32, 4, 0, 0)])
+@pytest.mark.parametrize("forced", [(16, 4, 256, 2), (128, 8, 0, 0), (32, 4, 40, 1), (128, 4, 300, 2), (16, 4, 3, 1), (32, 4, 0, 0)])
 def test_every_division_of_many_blocks(gpu, monkeypatch, forced, d):
     """Blocks that end inside a token's heads, some with nothing to see."""
     lengths, counts = (700, 0, 90, 300), (50, 0, 7, 33)
@@ -121,7 +121,7 @@ def test_every_division_of_many_blocks(gpu, monkeypatch, forced, d):
 
 @pytest.mark.parametrize("batch,heads,hkv,tokens,form", [
     (12, 32, 8, 256, (128, 4, 0, 0)), (1, 8, 1, 600, (128, 4, 0, 0)), (1, 4, 2, 333, (16, 4, 0, 0)),
-    (3, 6, 3, 500, (128, 4, 0, 0)), (40, 8, 8, 300, (32, 4, 0, 0))])
+    (3, 6, 3, 500, (128, 4, 0, 0)), (3, 6, 3, 500, (128, 8, 0, 0)), (40, 8, 8, 300, (32, 4, 0, 0))])
 def test_the_order_of_many_blocks(gpu, monkeypatch, batch, heads, hkv, tokens, form):
     """Every block is computed once, whatever the order: long before short, halves that turn round, by length."""
     lengths = [tokens + 13 * (i % 5) for i in range(batch)]
@@ -143,7 +143,7 @@ def test_blocks_of_128_rows(gpu, monkeypatch, d, page):
 
     def both(cache, table):
         got = []
-        for form in ((128, 4, 0, 0), (16, 4, 0, 0), (128, 4, 300, 2)):
+        for form in ((128, 4, 0, 0), (16, 4, 0, 0), (128, 4, 300, 2), (128, 8, 0, 0)):
             monkeypatch.setattr(kvcache, "_attention_form", lambda *a: form)
             monkeypatch.setattr(kvcache, "_attention_plans", kvcache.DevicePlans("attention_cached"))
             got.append([x.cpu() for x in _run(q, _gpu(cache), table, lengths, counts)])
@@ -166,8 +166,8 @@ def test_blocks_of_128_rows(gpu, monkeypatch, d, page):
     cache.v.view(torch.uint8)[int(table[0, 0]), 0, 5, 9] = 0xff   # by all
     cache.k.view(torch.uint8)[int(table[2, 0]), 1, 2, 7] = 0x7f
     cache.v_scale[int(table[0, 600 // page]), 1] = math.nan
-    wide, few, parts = both(cache, table)
-    for got in (wide, parts):
+    wide, few, parts, groups = both(cache, table)
+    for got in (wide, parts, groups):
         for x, y in zip(got, few):
             assert torch.equal(x.isnan(), y.isnan())
     sees = torch.arange(300 - 33, 300) >= at

@@ -252,5 +252,5 @@ def test_attention_forms_hold_their_bounds():
                 for d in (64, 128):
                     block, waves, extra, least = kvcache._attention_form(rows, heads, columns, page, d)
                     assert block in (16, 32, 128) and (rows <= block or rows > 32)
-                    assert waves == 4 or block == 16 or (block, d) == (32, 64) or (block, waves) == (32, 2)
+                    assert waves == 4 or block == 16 or (block, d) == (32, 64) or (block, waves) in ((32, 2), (128, 8))
                     assert extra >= 0 and (least > 0) == (extra > 0)

@@ -34,7 +34,9 @@
 // 5% at D = 128, 3% at 64), and share the tiles: each wave converts its part
 // of the next tile's codes and leaves them in LDS as operands (a fragment is 64
 // lanes' 16 bytes in lane order), so that a code is converted once for 128
-// rows.  2 x 1000 queries over 8192 keys (32/8 heads, D = 128): 278 us, 907
+// rows.  (Eight waves, for launches of one block a CU: two such groups divide the
+// tiles and are joined at the end; 1 x 1000 queries over 8192 keys 180 -> 156 us.)
+// 2 x 1000 queries over 8192 keys (32/8 heads, D = 128): 278 us, 907
 // TFLOP/s, 68% of a large matrix product's 1328, with the matrix cores busy 42%
 // and the vector ALU 56% of the cycles at 2.1 GHz, to which the card's power
 // holds it (on 16x16x32 products 2.3 GHz, and 16% more cycles).  No one thing
@@ -132,7 +134,7 @@ struct Program {
   static constexpr int BLOCK = ROWS * WR;        // and of the workgroup
   static constexpr int KC = D / 64, DT = D / 16, PITCH = D + 4;
   static constexpr int CHUNKS = D / 8;           // of a tile's codes, 64 lanes' 16 bytes each
-  static_assert(!SHARED || (WK == 1 && W == 4 && NQ == 2), "");
+  static_assert(!SHARED || (WR == 4 && NQ == 2), "");
 
   // What the workgroup does, worked out by its first wave.  The lengths are read here and nowhere else, and every index
   // that follows from them is bounded: a program that changes them under a running launch gets wrong rows, no more.
@@ -148,7 +150,7 @@ struct Program {
   struct Shared {
     union {
       Results r;
-      char ring[SHARED ? 2 * CHUNKS * 2048 : 16];   // two tiles as operands
+      char ring[SHARED ? WK * 2 * CHUNKS * 2048 : 16];   // two tiles as operands, for each that divide the tiles
     };
     int nan_from[D];   // first position with a NaN code in the column, of the tiles that not all rows see whole
     int nan_any;
@@ -463,7 +465,7 @@ struct Program {
   }
 
   __device__ __forceinline__ void begin(Rows& s, int head) const {
-    const int row0 = rb * BLOCK + wave * ROWS, r = row0 + lane % 32, rr = r < rows() ? r : 0, t = token_of(rr);
+    const int row0 = rb * BLOCK + wr * ROWS, r = row0 + lane % 32, rr = r < rows() ? r : 0, t = token_of(rr);
     s.low = max(span.start + min(token_of(row0), span.count), 0);
     s.pos = r < rows() ? position_of(t) : -1;
     const bf16* p = a->q + b * a->qb + (i64)(head * a->group + rr - t * a->group) * a->qh + t * a->qt + lane / 32 * 16;
@@ -569,9 +571,9 @@ struct Program {
   // 64 tokens, this way / by lanes' own addresses: 277 / 291 us for 2 x 1000 over 8192, 308 / 334 for 2 x 2048 over 8192 at
   // D = 64).
   __device__ __forceinline__ void walk_shared(Rows& s, int head, int first, int last) const {
-    constexpr int MINE = CHUNKS / W, V = D / 32;
-    const bool mine_k = wave < 2;
-    const int half = wave % 2, h = lane / 32, r = lane % 32;
+    constexpr int MINE = CHUNKS / WR, V = D / 32;
+    const bool mine_k = wr < 2;
+    const int half = wr % 2, h = lane / 32, r = lane % 32;
     // K: row r of the operand is token 16 (r / 4 % 2) + 4 (r / 8) + r % 4, bytes 32 i + 16 h; V: column 32 i + r, token 16 h
     const int mine_h = mine_k ? r / 4 % 2 : h, token = 16 * mine_h + (mine_k ? 4 * (r / 8) + r % 4 : 0);
     const Bases at = bases(head);
@@ -580,6 +582,7 @@ struct Program {
     // the lane's place: WIDE in a tile, else in a segment
     const unsigned lane_at = mine_k ? ((WIDE ? 32 * half + token : token % 16) * D + 16 * h)
                                     : (r << at.shift) + (WIDE ? 32 * half + token : 0);
+    char* ring = sh.ring + wk * 2 * CHUNKS * 2048;
     u32x4 codes[MINE];
     Tokens tok[2];
     auto ask = [&](int t, const int (&page)[3]) {   // of segments h and 2 + h, and of the lane's own codes
@@ -617,7 +620,7 @@ struct Program {
           if (unseen(mine.have, first_token, low)) take_nans<MINE>(codes, r, 32, first_token);
         }
       }
-      lds_bf16x8* to = (lds_bf16x8*)wir::lds(sh.ring + (slot * CHUNKS + wave * MINE) * 2048) + lane;
+      lds_bf16x8* to = (lds_bf16x8*)wir::lds(ring + (slot * CHUNKS + wr * MINE) * 2048) + lane;
 #pragma unroll
       for (int i = 0; i < MINE; ++i)
 #pragma unroll
@@ -625,20 +628,22 @@ struct Program {
     };
     static_assert(MINE == V, "");
     int next[3] = {-1, -1, -1}, slot = 0;
-    if (first < last) {
-      pages_of(next, first);
-      ask(first, next);
-      pages_of(next, first + 1);
+    const int start = first + wk;
+    if (start < last) {
+      pages_of(next, start);
+      ask(start, next);
+      pages_of(next, start + WK);
     }
     begin(s, head);
-    if (first < last) leave(first, 0);
-    for (int t = first; t < last; ++t, slot ^= 1) {
+    if (start < last) leave(start, 0);
+    for (int t = start; t < last + wk; t += WK, slot ^= 1) {   // (as often for all waves)
       __syncthreads();
+      if (WK > 1 && t >= last) break;
       const Tokens now[2] = {tok[0], tok[1]};
-      ask(t + 1, next);
-      pages_of(next, t + 2);   // (past the end -1, or pages not used)
-      tile(s, t, now, (const lds_bf16x8*)wir::lds(sh.ring + slot * CHUNKS * 2048) + lane);
-      if (t + 1 < last) leave(t + 1, slot ^ 1);
+      ask(t + WK, next);
+      pages_of(next, t + 2 * WK);   // (past the end -1, or pages not used)
+      tile(s, t, now, (const lds_bf16x8*)wir::lds(ring + slot * CHUNKS * 2048) + lane);
+      if (t + WK < last) leave(t + WK, slot ^ 1);
     }
     __syncthreads();   // the ring is read: results go there
   }
@@ -925,11 +930,15 @@ ATTN_KERNEL(wir_attn_cached_d64_r32_w2, 64, 2, 1, 2, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r32_w8, 64, 2, 1, 8, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r32, 64, 2, 1, 4, 2, false)
 ATTN_KERNEL(wir_attn_cached_d64_r128, 64, 2, 4, 4, 3, false)
+ATTN_KERNEL(wir_attn_cached_d64_r128_w8, 64, 2, 4, 8, 2, false)
+ATTN_KERNEL(wir_attn_cached_d64_r128_w8_p64, 64, 2, 4, 8, 2, true)
 ATTN_KERNEL(wir_attn_cached_d64_r128_p64, 64, 2, 4, 4, 3, true)   // pages of 64 tokens or more
 ATTN_KERNEL(wir_attn_cached_d128_r16, 128, 1, 1, 4, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r32_w2, 128, 2, 1, 2, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r32, 128, 2, 1, 4, 2, false)
 ATTN_KERNEL(wir_attn_cached_d128_r128, 128, 2, 4, 4, 2, false)
+ATTN_KERNEL(wir_attn_cached_d128_r128_w8, 128, 2, 4, 8, 2, false)
+ATTN_KERNEL(wir_attn_cached_d128_r128_w8_p64, 128, 2, 4, 8, 2, true)
 ATTN_KERNEL(wir_attn_cached_d128_r128_p64, 128, 2, 4, 4, 2, true)   // pages of 64 tokens or more
 JOIN_KERNEL(wir_attn_join_d64_r16, 64, 16, 1)
 JOIN_KERNEL(wir_attn_join_d64_r32, 64, 32, 1)

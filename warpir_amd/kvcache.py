@@ -180,8 +180,8 @@ TILE = 64        # positions of a tile (csrc/wir_pages.h)
 
 # us of one tile of a workgroup that has a CU to itself, and of one CU's time where all are busy, by head size and rows
 # of a block: the slopes of launches of 30 to 500 tiles
-_TILE_US = {128: {16: (0.35, 0.35), 32: (0.55, 0.43), 128: (1.35, 1.1)},
-            64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (0.96, 0.62)}}
+_TILE_US = {128: {16: (0.35, 0.35), 32: (0.55, 0.43), 128: (1.2, 1.1)},
+            64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (0.85, 0.62)}}
 _DIVIDED_US = {128: (13, 0.5, 24, 1.23), 64: (13, 0.26, 24, 0.75)}   # divided: us, and us of a CU for a tile; 16, 128
 
 
@@ -216,7 +216,11 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
         us[16, 1] = few + few_tile * max(n[16] * tiles / 256, 2)
         us[128, 1] = many + many_tile * max(n[128] * tiles / 256, 2)
         block, divided = min(us, key=us.get)
-        return (block, 4, 256 if block == 16 else max(512 - n[128], 256), 2) if divided else (block, 4, 0, 0)
+        if divided:
+            return block, 4, 256 if block == 16 else max(512 - n[128], 256), 2
+        # a CU's only block of 128 rows: its tiles divided over two groups of four waves (us, 1 x 1000 queries over 8192 keys
+        # 180 / 156, 1909 over 1914, 16/16 heads, 52 / 44)
+        return block, 8 if block == 128 and n[128] <= 256 else 4, 0, 0
     block, held = 16 if rows <= 16 else 32, columns * page * 2 * d   # bytes of a head at most
     if held <= 640 << 10 and held * (1 - heads / 105) <= 147 << 10:
         # eight waves a head while there is one such program for each CU, two where more heads than four fill the CUs
@@ -302,7 +306,7 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
                "table": page_table, "lengths": lengths, "counts": counts, "out": out, "lse": lse,
                "partial": workspace, "info": workspace}
     past = {"info": 4 * (floats - 4 * items)}
-    kind = f"_w{waves}" if waves != 4 else "_p64" if block == 128 and page >= TILE else ""
+    kind = ("" if waves == 4 else f"_w{waves}") + ("_p64" if block == 128 and page >= TILE else "")
     launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}{kind}",
            (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
     if extra:
