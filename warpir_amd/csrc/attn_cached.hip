@@ -737,7 +737,7 @@ struct Program {
 
   // Program -> (sequence and head, block) without a division of the work; later blocks see more keys.
   // A head's blocks are next to one another on one XCD, the longest first.  Where all programs run at once, two a CU, the
-  // second half comes in the opposite order, so that a CU has a long and a short one; many blocks of 128 rows go block
+  // second ones come in the opposite order, so that a CU has a long and a short one; many blocks of 128 rows go block
   // length by block length; those of one or two heads are dealt over the XCDs, for each to have long ones.  us, in turn /
   // so, D = 128: 4 x 512 queries over 1000 keys (32/8 heads) 50.4 / 45.7, 4096 over 4096 (16/8) 116 / 109.5, 2 x 1000
   // over 8192 (32/8) 316 / 308; 4 x 2048 over 2048 (32/8) 194 / 182, 4096 over 4096 (24/12) 178 / 140; 8000 over 8000 (8/1)
@@ -749,7 +749,7 @@ struct Program {
     const int heads = a->batch * a->heads;
     if (SHARED && total >= 768 && a->blocks >= 8) return wir::longest_first<true, 2048>(id, a->blocks, heads, block, item);
     const bool whole = heads > 2;   // a head on one XCD
-    const int step = whole ? 8 : 1, per = total / step, half = (per + 1) / 2;
+    const int step = whole ? 8 : 1, per = total / step, half = min(256 / step, per);   // (the first on every CU)
     if (total <= 512 && id >= step * half && id < step * per) id = step * (per - 1 - (id / step - half)) + id % step;
     if (whole) id = wir::remap_xcd(id, total);
     item = id / a->blocks;
