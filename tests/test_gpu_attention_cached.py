@@ -121,7 +121,7 @@ def test_every_division_of_many_blocks(gpu, monkeypatch, forced, d):
 
 @pytest.mark.parametrize("batch,heads,hkv,tokens,form", [
     (12, 32, 8, 256, (128, 4, 0, 0)), (1, 8, 1, 600, (128, 4, 0, 0)), (1, 4, 2, 333, (16, 4, 0, 0)),
-    (3, 6, 3, 500, (128, 4, 0, 0)), (3, 6, 3, 500, (128, 8, 0, 0)), (40, 8, 8, 300, (32, 4, 0, 0))])
+    (3, 6, 3, 500, (128, 4, 0, 0)), (3, 6, 3, 500, (128, 8, 0, 0)), (4, 8, 4, 300, (128, 4, 0, 0)), (40, 8, 8, 300, (32, 4, 0, 0))])
 def test_the_order_of_many_blocks(gpu, monkeypatch, batch, heads, hkv, tokens, form):
     """Every block is computed once, whatever the order: long before short, halves that turn round, by length."""
     lengths = [tokens + 13 * (i % 5) for i in range(batch)]

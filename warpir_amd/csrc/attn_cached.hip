@@ -736,24 +736,35 @@ struct Program {
   }
 
   // Program -> (sequence and head, block) without a division of the work; later blocks see more keys.
-  // A head's blocks are next to one another on one XCD, the longest first.  Where all programs run at once, two a CU, the
-  // second ones come in the opposite order, so that a CU has a long and a short one; many blocks of 128 rows go block
-  // length by block length; those of one or two heads are dealt over the XCDs, for each to have long ones.  us, in turn /
-  // so, D = 128: 4 x 512 queries over 1000 keys (32/8 heads) 50.4 / 45.7, 4096 over 4096 (16/8) 116 / 109.5, 2 x 1000
-  // over 8192 (32/8) 316 / 308; 4 x 2048 over 2048 (32/8) 194 / 182, 4096 over 4096 (24/12) 178 / 140; 8000 over 8000 (8/1)
-  // 270 / 202.  Elsewhere they cost: by length just past two a CU (3 x 700 over 3000, 32/8) 151 / 156 and for blocks of 32
-  // rows (32 x 300 over up to 1000, 16/16, D = 64) 66 / 70, dealt for more heads (5 x 40 over 2000, 24/6) 27.7 / 30.5.
+  // A head's blocks are next to one another on one XCD, the longest first, and a sequence's heads on all of them.  Where
+  // all programs run at once, two a CU, the second ones come in the opposite order, so that a CU has a long and a short
+  // one; many blocks of 128 rows go block length by block length; those of one or two heads are dealt over the XCDs, for
+  // each to have long ones.  us, the blocks in turn with consecutive heads on an XCD / so, D = 128: 4096 queries over
+  // 4096 keys (16/8 heads) 111 / 103, 2 x 1000 over 8192 (32/8) 285 / 281; 4 x 2048 over 2048 (32/8) 192 / 180, 4096 over
+  // 4096 (24/12) 167 / 135; 8000 over 8000 (8/1) 245 / 180; 8 x 200 over up to 3000 (32/8) 104 / 77, 12 x 1024 over up to
+  // 2048 (16/8) 163 / 142.  Elsewhere they cost: by length just past two a CU (3 x 700 over 3000, 32/8) 143 / 146 and where
+  // a head has few blocks (64 x 100 over 2000, 32/8) 327 / 351, dealt for more heads (5 x 40 over 2000, 24/6) 30.7 / 31.9.
   __device__ __forceinline__ void in_turn(int& item, int& block) const {
     int id = blockIdx.x;
     const int total = gridDim.x;
     const int heads = a->batch * a->heads;
-    if (SHARED && total >= 768 && a->blocks >= 8) return wir::longest_first<true, 2048>(id, a->blocks, heads, block, item);
+    if (SHARED && total >= 768 && a->blocks >= 8) {
+      wir::longest_first<true, 2048>(id, a->blocks, heads, block, item);
+      if (heads % 8 == 0 && total <= 2048) item = item % (heads / 8) * 8 + item / (heads / 8);   // (one range of heads)
+      return;
+    }
     const bool whole = heads > 2;   // a head on one XCD
     const int step = whole ? 8 : 1, per = total / step, half = min(256 / step, per);   // (the first on every CU)
     if (total <= 512 && id >= step * half && id < step * per) id = step * (per - 1 - (id / step - half)) + id % step;
-    if (whole) id = wir::remap_xcd(id, total);
+    const bool spread = whole && heads % 8 == 0;
+    const int xcd = id % 8;
+    if (spread)
+      id /= 8;
+    else if (whole)
+      id = wir::remap_xcd(id, total);
     item = id / a->blocks;
     block = a->blocks - 1 - (id - item * a->blocks);
+    if (spread) item = 8 * item + xcd;
   }
 
   __device__ __forceinline__ Plan plan() const {
