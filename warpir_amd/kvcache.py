@@ -181,7 +181,7 @@ TILE = 64        # positions of a tile (csrc/wir_pages.h)
 # us of one tile of a workgroup that has a CU to itself, and of one CU's time where all are busy, by head size and rows
 # of a block: the slopes of launches of 30 to 500 tiles
 _TILE_US = {128: {16: (0.35, 0.35), 32: (0.55, 0.43), 128: (1.2, 1.1)},
-            64: {16: (0.22, 0.125), 32: (0.29, 0.21), 128: (0.85, 0.62)}}
+            64: {16: (0.22, 0.125), 32: (0.29, 0.18), 128: (0.85, 0.62)}}
 _DIVIDED_US = {128: (13, 0.5, 24, 1.23), 64: (13, 0.26, 24, 0.75)}   # divided: us, and us of a CU for a tile; 16, 128
 
 
@@ -211,7 +211,9 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
         tiles = -(-columns * page // TILE)
         n = {block: heads * -(-rows // block) for block in (16, 32, 128)}
         each = {block: x / 256 if x > 512 else -(-x // 256) for block, x in n.items()}   # programs of a CU
-        us = {(block, 0): 6 + tiles * max(light, busy * each[block]) for block, (light, busy) in _TILE_US[d].items()}
+        starts = {block: (6 if d == 128 else 3) * max(x / 512 - 1, 0) for block, x in n.items()}   # of later programs
+        us = {(block, 0): 6 + starts[block] + tiles * max(light, busy * each[block])
+              for block, (light, busy) in _TILE_US[d].items()}
         few, few_tile, many, many_tile = _DIVIDED_US[d]
         us[16, 1] = few + few_tile * max(n[16] * tiles / 256, 2)
         us[128, 1] = many + many_tile * max(n[128] * tiles / 256, 2)
