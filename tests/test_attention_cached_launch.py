@@ -1,0 +1,91 @@
+"""What ``attention_cached`` launches, on the CPU: calls of any size that the
+kernels can take are launched, within the bounds of a launch."""
+import warnings
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from warpir_amd import api, handwritten, kvcache
+
+pytestmark = pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+f32, i32, e4 = torch.float32, torch.int32, torch.float8_e4m3fn
+
+
+class _NoPlans(handwritten.DevicePlans):
+    def run(self, flags, *tensors):
+        return None
+
+
+def _fake(*shape, dtype=torch.bfloat16):
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        with FakeTensorMode():
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The launches of a call on fake tensors: (kernel, workgroups, threads of one, arguments)."""
+    seen = []
+    real = handwritten.check_tensor
+
+    def check(*a, **k):
+        try:
+            real(*a, **k)
+        except ValueError as e:
+            if "no memory" not in str(e):
+                raise
+
+    def launch(rec, device, filename, symbol, grid, block, args, tensors, offsets=None):
+        assert grid[1:] == block[1:] == (1, 1)
+        seen.append((symbol, grid[0], block[0], args))
+
+    monkeypatch.setattr(kvcache, "check_tensor", check)
+    monkeypatch.setattr(kvcache, "launch", launch)
+    monkeypatch.setattr(kvcache, "_attention_plans", _NoPlans("none"))
+    return seen
+
+
+def _call(b, h, hk, t, columns, page, d):
+    q, table = _fake(b, h, t, d), _fake(b, columns, dtype=i32)
+    cache = api.KVCache(_fake(8, hk, page, d, dtype=e4), _fake(8, hk, d, page, dtype=e4), _fake(8, hk, dtype=f32),
+                        _fake(8, hk, dtype=f32))
+    workspace = _fake(max(1, api.attention_cached_workspace(q, cache, table)), dtype=f32)
+    api.attention_cached(q, cache, table, _fake(b, dtype=i32), out=_fake(b, h, t, d), lse=_fake(b, h, t, dtype=f32),
+                         workspace=workspace)
+
+
+@pytest.mark.parametrize("b,h,hk,t,columns,page,d", [
+    (32, 64, 8, 8192, 128, 64, 128),     # 2^24 query rows
+    (8, 64, 8, 32768, 512, 64, 128),
+    (128, 128, 16, 1024, 16, 64, 128),   # divided, a row a wave in the join
+    (64, 64, 8, 4096, 64, 64, 64),
+    (200, 64, 8, 20000, 400, 64, 128),
+    (20000, 128, 8, 16, 40, 64, 128),    # 2^25 rows in blocks of 128
+    (8192, 64, 8, 1, 16384, 64, 128),    # 2^30 tiles in a table for a million tokens
+    (65536, 32, 8, 1, 400, 64, 64),      # half a million heads of one block
+    (4096, 64, 1, 64, 80, 64, 128),
+])
+def test_large_calls_are_launched(launches, b, h, hk, t, columns, page, d):
+    _call(b, h, hk, t, columns, page, d)
+    symbol, grid, threads, args = launches[0]
+    items = b * hk * args.blocks
+    assert grid == items + args.extra and grid * threads < 1 << 32
+    assert len(launches) == (2 if args.extra else 1)
+    for symbol, grid, threads, args in launches[1:]:
+        assert grid * threads < 1 << 32 and items * -(-columns * page // 64) < 1 << 30
+
+
+def test_what_cannot_be_divided_is_not():
+    """The sums of a division and the grid of its join have to hold for every form."""
+    for rows in (1, 8, 16, 32, 64, 1000, 100000):
+        for heads in (1, 100, 1 << 16, 1 << 20, 1 << 23):
+            for columns, page in ((4, 16), (400, 64), (16384, 64), (1 << 21, 128)):
+                for d in (64, 128):
+                    block, waves, extra, least = kvcache._attention_form(rows, heads, columns, page, d)
+                    items = heads * -(-rows // block)
+                    if extra:
+                        assert items * -(-columns * page // 64) < 1 << 30
+                        assert kvcache._join_grid(items, rows, block)[0] < 1 << 24 and least > 0
+                    assert (block, waves) == kvcache._fastest_form(rows, heads, columns, page, d)[:2]

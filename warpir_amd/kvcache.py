@@ -191,7 +191,27 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
     rows a key/value head over a table of ``columns`` pages, ``heads`` of them in all
     sequences together.  The heads' tiles are divided over at most ``extra`` more
     programs than one for each (sequence, block, head), in parts of at least
-    ``least`` tiles; extra 0: no division.
+    ``least`` tiles; extra 0: no division.  A division adds up the tiles in 32 bits
+    and joins rows in a launch of its own: where either is past its bound the
+    form's kernel runs undivided."""
+    block, waves, extra, least = _fastest_form(rows, heads, columns, page, d)
+    items = heads * -(-rows // block)
+    if extra and (items * max(1, -(-columns * page // TILE)) >= 1 << 30 or
+                  _join_grid(items, rows, block)[0] >= 1 << 24):
+        return block, waves, 0, 0
+    return block, waves, extra, least
+
+
+def _join_grid(items: int, rows: int, block: int):
+    """(workgroups of 256, whether a wave takes a row) of the launch that joins ``items`` blocks' partial results."""
+    each = min(rows, block)
+    if block == 128 and items * each > 2048:
+        return items * -(-each // 4), True
+    return items * each, False
+
+
+def _fastest_form(rows: int, heads: int, columns: int, page: int, d: int):
+    """The form of ``_attention_form`` by time.
 
     Up to 32 rows, one block: a division costs a second launch and the partial
     results' way, ~3 us; a head that is not divided is read by one CU at ~49
@@ -258,7 +278,10 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     are on the GPU; partial results go through ``workspace`` (fp32, as many
     elements as ``attention_cached_workspace`` says, allocated if omitted), which
     one call at a time may use: two streams, or two graphs that run at once,
-    need one each."""
+    need one each.
+
+    Refused are 2^24 query rows (T * H / H_kv) or more a key/value head of a
+    sequence, and launches of 2^32 threads or more."""
     import torch
 
     fn, done = "attention_cached", None
@@ -273,7 +296,7 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     h, tokens = q.shape[1:3]
     need(fn, h > 0 and h % heads == 0, f"{h} query heads are not a multiple of {heads} key/value heads")
     group = h // heads
-    need(fn, tokens * group <= 1 << 30, "more than 2^30 query rows a key/value head")
+    need(fn, tokens * group < 1 << 24, "2^24 query rows or more a key/value head of a sequence")
     rec = _attention_plans.recording(done, q, *cache, page_table, lengths, counts, out, lse)
     if out is None:
         out = rec.alloc(torch.empty(q.shape, dtype=q.dtype, device=device))
@@ -291,9 +314,9 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     block, waves, extra, least = _attention_form(rows, batch * heads, page_table.shape[1], page, d)
     blocks = -(-rows // block)
     items = batch * blocks * heads
-    need(fn, items * min(rows, block) < 1 << 24, "2^24 query rows or more in one call")
     need(fn, (items + extra) * waves < 1 << 26, "2^32 threads or more in one call")
-    need(fn, items * max(1, -(-page_table.shape[1] * page // TILE)) < 1 << 30, "2^30 tiles of keys or more in one call")
+    # (no bound of the kernels: were the table full, the launch would take the best part of an hour)
+    need(fn, blocks * -(-page_table.shape[1] * page // TILE) < 1 << 30, "2^30 tiles of keys or more a key/value head")
     args = _AttnArgs(*[None] * 12, *q.stride()[:3], *out.stride()[:3], *lse.stride(), page_table.stride(0), batch, heads,
                      group, tokens, page.bit_length() - 1, cache.k.shape[0], page_table.shape[1], blocks, extra, least)
     floats = _workspace_floats(extra, block, d, items)
@@ -312,9 +335,9 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}{kind}",
            (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
     if extra:
-        many = block == 128 and items * min(rows, block) > 2048   # a row a wave, not a workgroup
-        launch(rec, device, "attn_cached.hsaco", f"wir_attn_join_d{d}_r{block}" + ("_w4" if many else ""),
-               (items * (-(-min(rows, block) // 4) if many else min(rows, block)), 1, 1), (256, 1, 1), args, tensors, past)
+        grid, many = _join_grid(items, rows, block)
+        launch(rec, device, "attn_cached.hsaco", f"wir_attn_join_d{d}_r{block}" + ("_w4" if many else ""), (grid, 1, 1),
+               (256, 1, 1), args, tensors, past)
     if rec:
         _attention_plans.add(0, rec, out, lse)
     return out, lse
