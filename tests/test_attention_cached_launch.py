@@ -89,3 +89,12 @@ def test_what_cannot_be_divided_is_not():
                         assert items * -(-columns * page // 64) < 1 << 30
                         assert kvcache._join_grid(items, rows, block)[0] < 1 << 24 and least > 0
                     assert (block, waves) == kvcache._fastest_form(rows, heads, columns, page, d)[:2]
+
+
+@pytest.mark.parametrize("b,h,hk,t,columns,d", [
+    (64, 32, 8, 300, 7, 128), (64, 64, 4, 300, 7, 64), (500, 64, 4, 64, 2, 128), (500, 64, 4, 40, 10, 128),
+    (100, 128, 16, 1000, 16, 128), (256, 128, 8, 272, 6, 64), (200, 32, 8, 64, 4, 128), (500, 16, 16, 64, 2, 64)])
+def test_blocks_that_fill_the_chip_are_not_divided(b, h, hk, t, columns, d):
+    """Every program of a division adds up all blocks' tiles: 2 to 6 times these launches' time, undivided."""
+    block, waves, extra, least = kvcache._attention_form(t * h // hk, b * hk, columns, 64, d)
+    assert b * hk * -(-t * h // hk // block) > 512 and extra == 0

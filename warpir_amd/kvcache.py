@@ -235,8 +235,13 @@ def _fastest_form(rows: int, heads: int, columns: int, page: int, d: int):
         us = {(block, 0): 6 + starts[block] + tiles * max(light, busy * each[block])
               for block, (light, busy) in _TILE_US[d].items()}
         few, few_tile, many, many_tile = _DIVIDED_US[d]
-        us[16, 1] = few + few_tile * max(n[16] * tiles / 256, 2)
-        us[128, 1] = many + many_tile * max(n[128] * tiles / 256, 2)
+        # (past two programs a CU a division only adds to the starts, which these leave out, and to what each program
+        # adds up; us, divided / not: 64 x 300 queries over 400 keys (32/8 heads, D = 128) 356 / 198, 500 x 64 over 100 (64/4)
+        # 2577 / 423, 100 x 1000 over 1000 (128/16) 24700 / 5250; D = 64: 64 x 300 over 400 (64/4) 770 / 204)
+        if n[16] <= 512:
+            us[16, 1] = few + few_tile * max(n[16] * tiles / 256, 2)
+        if n[128] <= 512:
+            us[128, 1] = many + many_tile * max(n[128] * tiles / 256, 2)
         block, divided = min(us, key=us.get)
         if divided:
             return block, 4, 256 if block == 16 else max(512 - n[128], 256), 2
