@@ -98,3 +98,11 @@ def test_blocks_that_fill_the_chip_are_not_divided(b, h, hk, t, columns, d):
     """Every program of a division adds up all blocks' tiles: 2 to 6 times these launches' time, undivided."""
     block, waves, extra, least = kvcache._attention_form(t * h // hk, b * hk, columns, 64, d)
     assert b * hk * -(-t * h // hk // block) > 512 and extra == 0
+
+
+@pytest.mark.parametrize("b,h,hk,t,d", [(1024, 32, 8, 1, 128), (96, 32, 8, 1, 128), (512, 32, 8, 8, 128),
+                                        (512, 16, 16, 1, 64), (100, 32, 8, 8, 64), (40, 32, 32, 1, 128)])
+def test_heads_that_fill_the_chip_are_not_divided_for_the_width_of_the_table(b, h, hk, t, d):
+    """Short sequences in a table for long ones: a division took up to ten times the time of the narrow table's form."""
+    for columns in (1, 16, 512, 16384):
+        assert kvcache._attention_form(t * h // hk, b * hk, columns, 64, d)[2] == 0

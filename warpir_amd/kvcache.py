@@ -192,8 +192,8 @@ def _attention_form(rows: int, heads: int, columns: int, page: int, d: int):
     sequences together.  The heads' tiles are divided over at most ``extra`` more
     programs than one for each (sequence, block, head), in parts of at least
     ``least`` tiles; extra 0: no division.  A division adds up the tiles in 32 bits
-    and joins rows in a launch of its own: where either is past its bound the
-    form's kernel runs undivided."""
+    (2^30 of them at most) and joins rows in a launch of its own: past either's
+    bound the form's kernel runs undivided."""
     block, waves, extra, least = _fastest_form(rows, heads, columns, page, d)
     items = heads * -(-rows // block)
     if extra and (items * max(1, -(-columns * page // TILE)) >= 1 << 30 or
@@ -258,6 +258,12 @@ def _fastest_form(rows: int, heads: int, columns: int, page: int, d: int):
         if heads >= 768 and short:
             return block, 2, 0, 0
         return block, 8 if heads <= 256 and not short and (block, d) != (32, 128) else 4, 0, 0
+    # more heads than 512 fill the chip by themselves, and every program of a division adds up all sequences' tiles: the
+    # kernel runs undivided.  us, divided / not (32/8 heads, D = 128, lengths from 1 to the named, in a table of 32768):
+    # 1024 sequences of 200 keys 536 / 145, of 4000 1047 / 739, 96 of 200 28.8 / 15.2, of 8192 166 / 160; with 8 tokens 512 of
+    # 1000 278 / 177; 16/16 heads, D = 64: 512 of 1000 230 / 117.  (One of 32000 among 511 of 200: 198 / 238.)
+    if heads > 512:
+        return block, 4 if (block, d) == (32, 128) else 8, 0, 0
     # two programs of four waves a CU (32 sequences of up to 16000 keys, 256 heads: 384 more 96.6, 128 or 1024 over
     # 99); with more heads, one of eight and as many more (64 sequences of up to 8192, 512 heads: 512 more of eight
     # waves 119.6, 1536 of four 122)
