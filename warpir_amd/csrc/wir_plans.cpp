@@ -19,6 +19,7 @@
 // tensors); the Python path then does, with its own checks and errors, and
 // leaves a plan after False only.  The interpreter
 // lock guards the tables; it is released around the launches only.
+// meets() says which of a call's tensors share memory (handwritten.apart).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -28,6 +29,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstring>
 #include <memory>
 #include <string>
@@ -301,6 +303,89 @@ PyObject* add(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
+// The bytes of a tensor: blocks of `block` bytes at every sum of multiples of
+// the strides (bytes; ascending).
+struct Bytes {
+  long long at, block = 1;
+  int n = 0;
+  long long sizes[8], strides[8];
+
+  // Bytes from the first to the last of the dimensions below `top`.
+  long long span(int top) const {
+    long long x = block;
+    for (int i = 0; i < top; ++i) x += (sizes[i] - 1) * strides[i];
+    return x;
+  }
+};
+
+bool bytes_of(const at::Tensor& t, Bytes& b) {
+  b.at = (long long)(uintptr_t)t.data_ptr();
+  b.block = t.element_size();
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) == 1 || t.stride(d) == 0) continue;
+    int i = b.n++;
+    const long long stride = t.stride(d) * t.element_size();
+    for (; i > 0 && b.strides[i - 1] > stride; --i) b.sizes[i] = b.sizes[i - 1], b.strides[i] = b.strides[i - 1];
+    b.sizes[i] = t.size(d), b.strides[i] = stride;
+  }
+  while (b.n && b.strides[0] == b.block) {   // a run of the innermost dimensions is one block
+    b.block *= b.sizes[0];
+    --b.n;
+    for (int i = 0; i < b.n; ++i) b.sizes[i] = b.sizes[i + 1], b.strides[i] = b.strides[i + 1];
+  }
+  return b.at != 0;
+}
+
+long long floor_div(long long a, long long b) { return a / b - (a % b < 0); }   // b > 0
+
+// Whether the first `na` dimensions of a and `nb` of b, from the addresses x
+// and y on, have a byte in common.  Dimensions of one stride are walked by the
+// difference of their indices, and only where the rest may meet, so that views
+// of one buffer take a step or two a dimension.  After `left` steps: true.
+bool meet(const Bytes& a, int na, long long x, const Bytes& b, int nb, long long y, int& left) {
+  const long long sa = a.span(na), sb = b.span(nb);
+  if (x + sa <= y || y + sb <= x) return false;
+  if ((!na && !nb) || --left < 0) return true;
+  const long long ta = na ? a.strides[na - 1] : 0, tb = nb ? b.strides[nb - 1] : 0, step = std::max(ta, tb);
+  const int ia = ta == step, ib = tb == step;   // of which tensors the dimension is
+  // x + k step against y, for k from -(b's indices) to a's
+  const long long lo = ib ? 1 - b.sizes[nb - 1] : 0, hi = ia ? a.sizes[na - 1] - 1 : 0;
+  const long long from = std::max(lo, floor_div(y - x - a.span(na - ia), step) + 1);
+  const long long to = std::min(hi, floor_div(y + b.span(nb - ib) - x - 1, step));
+  for (long long k = from; k <= to; ++k)
+    if (meet(a, na - ia, x + k * step, b, nb - ib, y, left)) return true;
+  return false;
+}
+
+// meets(strict, a0, b0, a1, b1, ...) -> the first pair of tensors that have
+// memory in common, or -1; of pairs past the first `strict` ones those that are
+// one and the same layout at one address do not count.  What is no plain
+// tensor (None too) meets nothing.
+PyObject* meets(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const long strict = nargs ? PyLong_AsLong(args[0]) : 0;
+  if (strict == -1 && PyErr_Occurred()) return nullptr;
+  for (Py_ssize_t i = 0; 2 * i + 2 < nargs; ++i) {
+    PyObject *p = args[2 * i + 1], *q = args[2 * i + 2];
+    if (!THPVariable_CheckExact(p) || !THPVariable_CheckExact(q)) continue;
+    const at::Tensor &t = THPVariable_Unpack(p), &u = THPVariable_Unpack(q);
+    if (!t.defined() || !u.defined() || !t.has_storage() || !u.has_storage() || t.layout() != at::kStrided ||
+        u.layout() != at::kStrided || t.dim() > 8 || u.dim() > 8 || t.numel() == 0 || u.numel() == 0 ||
+        t.device() != u.device())
+      continue;
+    if (i >= strict && t.data_ptr() == u.data_ptr() && t.scalar_type() == u.scalar_type() && t.sizes() == u.sizes()) {
+      bool same = true;
+      for (int64_t d = 0; d < t.dim(); ++d) same &= t.size(d) == 1 || t.stride(d) == u.stride(d);
+      if (same) continue;
+    }
+    Bytes a, b;
+    int left = 10000;
+    if (bytes_of(t, a) && bytes_of(u, b) && meet(a, a.n, a.at, b, b.n, b.at, left)) return PyLong_FromSsize_t(i);
+  }
+  return PyLong_FromLong(-1);
+  END_HANDLE_TH_ERRORS
+}
+
 // size(table): the number of plans held.
 PyObject* size(PyObject*, PyObject* capsule) {
   Table* table = table_of(capsule);
@@ -323,6 +408,7 @@ PyObject* init(PyObject*, PyObject* args) {
 
 PyMethodDef methods[] = {{"run", (PyCFunction)(void (*)(void))run, METH_FASTCALL, nullptr},
                          {"add", add, METH_VARARGS, nullptr},
+                         {"meets", (PyCFunction)(void (*)(void))meets, METH_FASTCALL, nullptr},
                          {"size", size, METH_O, nullptr},
                          {"table", new_table, METH_NOARGS, nullptr},
                          {"init", init, METH_VARARGS, nullptr},

@@ -59,6 +59,23 @@ def check_written(fn: str, name: str, t) -> None:
         span = stride * (size - 1) + span
 
 
+def apart(fn: str, names: Sequence[str], strict: int, *tensors) -> None:
+    """Refuse pairs of ``tensors`` (named by ``names``) that have memory in common:
+    a kernel's workgroups write one while others read or write the other.  Past
+    the first ``strict`` pairs one layout at one address is no such pair: a row is
+    read and written by the same lanes.  None has no memory."""
+    mod = plans._native
+    if mod is None:
+        import torch
+
+        if not torch.cuda.is_available():
+            return   # (nothing runs)
+        mod = plans.native()
+    first = mod.meets(strict, *tensors)
+    if first >= 0:
+        raise ValueError(f"{fn}: {names[2 * first]} and {names[2 * first + 1]} have memory in common")
+
+
 def own(t, other):
     """``t`` as a tensor of its own where it is ``other``: a call that gives one
     tensor twice has no plan."""
@@ -129,4 +146,4 @@ class DevicePlans(Plans):
         return r
 
 
-__all__ = ["check_tensor", "check_written", "need", "own", "launch", "on", "DevicePlans", "INT_MAX"]
+__all__ = ["apart", "check_tensor", "check_written", "need", "own", "launch", "on", "DevicePlans", "INT_MAX"]

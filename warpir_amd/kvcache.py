@@ -6,7 +6,7 @@ import ctypes
 import functools
 from typing import NamedTuple, Tuple
 
-from warpir_amd.handwritten import DevicePlans, check_tensor, check_written, launch, need, own
+from warpir_amd.handwritten import DevicePlans, apart, check_tensor, check_written, launch, need, own
 
 PAGE_SIZES = (16, 32, 64, 128)
 _write_plans = DevicePlans("kv_cache_write")
@@ -121,6 +121,7 @@ def kv_cache_write(cache: KVCache, k, v, page_table, lengths, counts=None) -> KV
     if counts is lengths:
         counts = own(counts, lengths)
     if isinstance(cache, KVCache):
+        need(fn, cache.k_scale is not cache.v_scale, "cache.k_scale and cache.v_scale are one tensor")
         done = _write_plans.run(0, k, v, *cache, page_table, lengths, counts)
         if done is not None and done is not False:
             return cache
@@ -146,6 +147,8 @@ def kv_cache_read(cache: KVCache, page_table, lengths, tokens: int, k=None, v=No
 
     fn, done = "kv_cache_read", None
     need(fn, k is None or k is not v, "k and v are one tensor")
+    if k is not None and v is not None:
+        apart(fn, ("k", "v"), 1, k, v)
     if isinstance(cache, KVCache) and type(tokens) is int:
         done = _read_plans.run(tokens, *cache, page_table, lengths, k, v)
         if done is not None and done is not False:
@@ -289,13 +292,15 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     are on the GPU; partial results go through ``workspace`` (fp32, as many
     elements as ``attention_cached_workspace`` says, allocated if omitted), which
     one call at a time may use: two streams, or two graphs that run at once,
-    need one each.
+    need one each.  ``out`` may be ``q`` itself.
 
     Refused are 2^24 query rows (T * H / H_kv) or more a key/value head of a
     sequence, and launches of 2^32 threads or more."""
     import torch
 
     fn, done = "attention_cached", None
+    if out is not None:   # (its own rows of q a workgroup reads before it writes them)
+        apart(fn, ("out", "lse", "out", "q"), 1, out, lse, out, q)
     if counts is lengths:
         counts = own(counts, lengths)
     if isinstance(cache, KVCache) and workspace is None:

@@ -7,7 +7,7 @@ import functools
 import struct
 from typing import Optional, Tuple
 
-from warpir_amd.handwritten import INT_MAX, DevicePlans, check_tensor, check_written, launch, need, own
+from warpir_amd.handwritten import INT_MAX, DevicePlans, apart, check_tensor, check_written, launch, need, own
 
 _forward_plans = DevicePlans("qk_norm_rope")
 _backward_plans = DevicePlans("qk_norm_rope_backward")
@@ -99,6 +99,12 @@ def _packed(q, k, q_out, k_out, dq, dk, q_weight, cos, sin, positions, eps):
                  q.shape[0], q.shape[2], cos.shape[0], flags, eps)
 
 
+# what a given output and another tensor of the call must not share, with the pairs that may be one tensor last
+_FORWARD_PAIRS = ("q_out", "k_out", "q_out", "k", "k_out", "q", "q_out", "q", "k_out", "k")
+_BACKWARD_PAIRS = ("dq", "dk", "dq", "dk_out", "dq", "k", "dk", "dq_out", "dk", "q", "dq_weight", "dk_weight",
+                   "dq", "dq_out", "dq", "q", "dk", "dk_out", "dk", "k")
+
+
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float = 1e-6, interleaved: bool = False,
                  q_out=None, k_out=None) -> Tuple[object, object]:
     """The RMS norm of every head of ``q`` ``[B, H, S, D]`` and ``k`` ``[B, H_kv, S, D]``
@@ -110,7 +116,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
     rotation turns pairs ``(i, i + D / 2)``, or ``(2 i, 2 i + 1)`` with
     ``interleaved``.  ``positions`` is int32 or int64, ``[S]`` or ``[B, S]`` (default
     ``0 .. S - 1``); the rows of a position outside the table become NaN.
-    The outputs may be ``q`` and ``k`` themselves."""
+    ``q_out`` may be ``q`` itself and ``k_out`` ``k``; memory that an output shares
+    otherwise with the other or with an input is refused."""
     import torch
 
     fn = "qk_norm_rope"
@@ -118,6 +125,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
     given = None
     if q_out is not None or k_out is not None:
         need(fn, q_out is not k_out, "q_out and k_out are one tensor")
+        apart(fn, _FORWARD_PAIRS, 3, q_out, k_out, q_out, k, k_out, q, q_out, q, k_out, k)
         given = q_out, k_out
         q_out, k_out = own(q_out, q), own(k_out, k)
     if k_weight is q_weight:
@@ -165,7 +173,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     those of its outputs (``dq_out``, ``dk_out``, bf16, shaped as ``q`` and ``k``, any
     row-aligned layout) and its inputs; ``dq`` and ``dk`` are bf16, the weights'
     gradients fp32 sums over all rows, added in an order that the shapes fix.
-    ``dq`` and ``dk`` may be ``dq_out`` and ``dk_out`` themselves, or ``q`` and ``k``.
+    ``dq`` may be ``dq_out`` or ``q`` itself and ``dk`` ``dk_out`` or ``k``; memory that
+    they share otherwise with one another or with those is refused.
     ``workspace`` holds the workgroups' partial sums (fp32, at least
     ``1025 * D`` elements, allocated if omitted); one call at a time may use it."""
     import torch
@@ -176,6 +185,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     if dq is not None or dk is not None or dq_weight is not None or dk_weight is not None:
         need(fn, dq is None or dq is not dk, "dq and dk are one tensor")
         need(fn, dq_weight is None or dq_weight is not dk_weight, "dq_weight and dk_weight are one tensor")
+        apart(fn, _BACKWARD_PAIRS, 6, dq, dk, dq, dk_out, dq, k, dk, dq_out, dk, q, dq_weight, dk_weight,
+              dq, dq_out, dq, q, dk, dk_out, dk, k)
         given = dq, dk, dq_weight, dk_weight
         dq, dk = own(own(dq, dq_out), q), own(own(dk, dk_out), k)
     if k_weight is q_weight:
