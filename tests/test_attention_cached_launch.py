@@ -1,5 +1,7 @@
 """What ``attention_cached`` launches, on the CPU: calls of any size that the
 kernels can take are launched, within the bounds of a launch."""
+import os
+import re
 import warnings
 
 import pytest
@@ -7,6 +9,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from warpir_amd import api, handwritten, kvcache
+from warpir_amd.runtime import PKG_DIR
 
 pytestmark = pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
 f32, i32, e4 = torch.float32, torch.int32, torch.float8_e4m3fn
@@ -106,3 +109,37 @@ def test_heads_that_fill_the_chip_are_not_divided_for_the_width_of_the_table(b, 
     """Short sequences in a table for long ones: a division took up to ten times the time of the narrow table's form."""
     for columns in (1, 16, 512, 16384):
         assert kvcache._attention_form(t * h // hk, b * hk, columns, 64, d)[2] == 0
+
+
+def test_every_form_has_its_kernels_and_its_workspace():
+    """Names that attn_cached.hip defines, with the waves and rows that it gives them; a slot for every partial result."""
+    with open(os.path.join(PKG_DIR, "csrc", "attn_cached.hip")) as f:
+        source = f.read()
+    attention = {m[0]: [int(x) for x in m[1:6]] for m in
+                 re.findall(r"^ATTN_KERNEL\((\w+), (\d+), (\d+), (\d+), (\d+), (\d+), \w+\)", source, re.M)}
+    join = {m[0]: [int(x) for x in m[1:]] for m in re.findall(r"^JOIN_KERNEL\((\w+), (\d+), (\d+), (\d+)\)", source, re.M)}
+    assert len(attention) > 15 and len(join) > 5
+    used = set()
+    for d in (64, 128):
+        for rows in (1, 2, 5, 8, 16, 17, 24, 32, 33, 40, 64, 100, 128, 129, 200, 256, 400, 700, 1000, 2048, 5000, 20000):
+            for heads in (1, 2, 4, 7, 8, 16, 32, 60, 100, 104, 106, 200, 256, 257, 300, 384, 385, 512, 513, 600, 768, 1100, 5000):
+                for columns, page in ((1, 16), (4, 16), (2, 128), (8, 64), (20, 32), (40, 128), (300, 64), (4096, 64)):
+                    block, waves, extra, least = kvcache._attention_form(rows, heads, columns, page, d)
+                    items = heads * -(-rows // block)
+                    grid, many = kvcache._join_grid(items, rows, block)
+                    names = kvcache._attention_kernels(block, waves, extra, d, page, many)
+                    used.update(names)
+                    _, nq, wr, w, _ = attention[names[0]]
+                    assert attention[names[0]][0] == d and (w, 16 * nq * wr) == (waves, block)
+                    assert rows <= block or rows > 32   # up to 32 rows: one block
+                    assert len(names) == 1 + (extra > 0) and (least > 0) == (extra > 0)
+                    floats = kvcache._workspace_floats(extra, block, d, items)
+                    if not extra:
+                        assert floats == 0
+                        continue
+                    assert join[names[1]] == [d, block, 4 if many else 1]
+                    assert grid * (4 if many else 1) >= items * min(rows, block)
+                    # wir_pages.h: slots_for(extra) = 3 extra + 2 partial results, a row of each D values, a maximum and a sum
+                    assert floats >= (3 * extra + 2) * block * (d + 2) + 4 * items
+                    assert (floats - 4 * items) % 4 == 0
+    assert used == set(attention) | set(join)

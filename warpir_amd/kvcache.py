@@ -213,6 +213,13 @@ def _join_grid(items: int, rows: int, block: int):
     return items * each, False
 
 
+def _attention_kernels(block: int, waves: int, extra: int, d: int, page: int, many: bool):
+    """Names of the launches of a form: attention and, where heads are divided, the join."""
+    kind = ("" if waves == 4 else f"_w{waves}") + ("_p64" if block == 128 and page >= TILE else "")
+    names = [f"wir_attn_cached_d{d}_r{block}{kind}"]
+    return names + [f"wir_attn_join_d{d}_r{block}" + ("_w4" if many else "")] if extra else names
+
+
 def _fastest_form(rows: int, heads: int, columns: int, page: int, d: int):
     """The form of ``_attention_form`` by time.
 
@@ -347,13 +354,11 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
                "table": page_table, "lengths": lengths, "counts": counts, "out": out, "lse": lse,
                "partial": workspace, "info": workspace}
     past = {"info": 4 * (floats - 4 * items)}
-    kind = ("" if waves == 4 else f"_w{waves}") + ("_p64" if block == 128 and page >= TILE else "")
-    launch(rec, device, "attn_cached.hsaco", f"wir_attn_cached_d{d}_r{block}{kind}",
-           (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
+    grid, many = _join_grid(items, rows, block)
+    names = _attention_kernels(block, waves, extra, d, page, many)
+    launch(rec, device, "attn_cached.hsaco", names[0], (items + extra, 1, 1), (64 * waves, 1, 1), args, tensors, past)
     if extra:
-        grid, many = _join_grid(items, rows, block)
-        launch(rec, device, "attn_cached.hsaco", f"wir_attn_join_d{d}_r{block}" + ("_w4" if many else ""), (grid, 1, 1),
-               (256, 1, 1), args, tensors, past)
+        launch(rec, device, "attn_cached.hsaco", names[1], (grid, 1, 1), (256, 1, 1), args, tensors, past)
     if rec:
         _attention_plans.add(0, rec, out, lse)
     return out, lse
