@@ -27,8 +27,11 @@
 // at the end.  Bound by the cache's bytes: one token over 131072 (32/8 heads, D
 // = 128) 45 us, 268 MB at 5.9 TB/s, and 5 for the join; 64 sequences of up to
 // 8192 113 us, 598 MB at 5.3 TB/s, and 5; 16 sequences of up to 2050, 4 tokens,
-// 16 heads of D = 64, pages of 16: 11 us, 41 MB at 3.7 TB/s.  (A 2 GiB copy moves
-// 4.90 TB/s.)
+// 16 heads of D = 64, pages of 16: 11 us, 41 MB at 3.7 TB/s.  (Reading 4 GiB
+// alone goes at 7.1 TB/s.)  32 rows at D = 128 need 11 registers more than the 256
+// that two programs a CU leave: four 8-byte loads, a 4-byte load and store of
+// scratch memory in each tile.  One program without them is slower: 8 x 64
+// queries over 2000 keys (32/8 heads) 46.0 us, so 42.5; 4 x 8 over 8000 32.2, so 28.9.
 // Many rows: a workgroup's waves take 32 rows each, on 32x32x16 products (half
 // the steps between lanes, and half the instructions to issue, of 16x16x32:
 // 5% at D = 128, 3% at 64), and share the tiles: each wave converts its part
@@ -568,8 +571,8 @@ struct Program {
 
   // In each iteration a wave asks for its quarter of the next tile (K or V of 32 tokens), computes, and leaves what came
   // as operands in the other slot.  WIDE: a tile's page and addresses are the wave's, and a lane adds its place (pages of
-  // 64 tokens, this way / by lanes' own addresses: 277 / 291 us for 2 x 1000 over 8192, 308 / 334 for 2 x 2048 over 8192 at
-  // D = 64).
+  // 64 tokens, 32/8 heads, this way / by lanes' own addresses: 277 / 291 us for 2 x 1000 over 8192, 308 / 334 for 2 x 2048
+  // over 8192 at D = 64).
   __device__ __forceinline__ void walk_shared(Rows& s, int head, int first, int last) const {
     constexpr int MINE = CHUNKS / WR, V = D / 32;
     const bool mine_k = wr < 2;

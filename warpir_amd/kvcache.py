@@ -241,7 +241,9 @@ def _fastest_form(rows: int, heads: int, columns: int, page: int, d: int):
         tiles = -(-columns * page // TILE)
         n = {block: heads * -(-rows // block) for block in (16, 32, 128)}
         each = {block: x / 256 if x > 512 else -(-x // 256) for block, x in n.items()}   # programs of a CU
-        starts = {block: (6 if d == 128 else 3) * max(x / 512 - 1, 0) for block, x in n.items()}   # of later programs
+        # of later programs (beside their tiles; by launches of 512 to 16384 blocks of 16 / 32 / 128 rows with one tile
+        # each: 3.7 / 6.9 / 8.5 us for 512 at D = 128, 1.7 / 4.1 / 4.2 at 64)
+        starts = {block: (6 if d == 128 else 3) * max(x / 512 - 1, 0) for block, x in n.items()}
         us = {(block, 0): 6 + starts[block] + tiles * max(light, busy * each[block])
               for block, (light, busy) in _TILE_US[d].items()}
         few, few_tile, many, many_tile = _DIVIDED_US[d]
@@ -295,8 +297,10 @@ def attention_cached(q, cache: KVCache, page_table, lengths, counts=None, out=No
     sees no key (also ``t >= counts[b]``, or a position below 0) gives O = 0 and
     LSE = -inf.
 
-    The keys of a sequence are divided over the chip by its lengths as they
-    are on the GPU; partial results go through ``workspace`` (fp32, as many
+    The kernel is chosen by the shapes and the table's width, so the table
+    should have the columns that the sequences may fill.  Where few heads leave
+    CUs idle, the keys are divided over the chip by the lengths as they are on
+    the GPU; partial results go through ``workspace`` (fp32, as many
     elements as ``attention_cached_workspace`` says, allocated if omitted), which
     one call at a time may use: two streams, or two graphs that run at once,
     need one each.  ``out`` may be ``q`` itself.
