@@ -117,7 +117,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
     ``interleaved``.  ``positions`` is int32 or int64, ``[S]`` or ``[B, S]`` (default
     ``0 .. S - 1``); the rows of a position outside the table become NaN.
     ``q_out`` may be ``q`` itself and ``k_out`` ``k``; memory that an output shares
-    otherwise with the other or with an input is refused."""
+    otherwise with the other, ``q`` or ``k`` is refused."""
     import torch
 
     fn = "qk_norm_rope"
