@@ -16,9 +16,11 @@ import math
 from typing import Optional, Tuple
 
 from warpir_amd import kernels
+from warpir_amd.int8 import gemm_int8, quantize_int8
 from warpir_amd.kvcache import KVCache, attention_cached, attention_cached_workspace, kv_cache_read, kv_cache_write
+from warpir_amd.packed import attention_packed, attention_packed_backward
 from warpir_amd.plans import Plans, Recording
-from warpir_amd.rotary import qk_norm_rope, qk_norm_rope_backward, rope_table
+from warpir_amd.rotary import qk_norm_rope, qk_norm_rope_backward, rope_axes, rope_axes_backward, rope_table
 from warpir_amd.runtime import GL, RawKernel
 
 # Plans of the calls below, by flags: gemm 0; attention_forward and
@@ -701,4 +703,6 @@ def _kv_tile(variant: str) -> int:
 
 __all__ = ["gemm", "gemm_split_k", "splitk_count", "gemm_variant", "attention_forward", "attention_backward",
            "attention_flops", "attention_backward_flops", "rope_table", "qk_norm_rope", "qk_norm_rope_backward",
-           "KVCache", "kv_cache_write", "kv_cache_read", "attention_cached", "attention_cached_workspace"]
+           "KVCache", "kv_cache_write", "kv_cache_read", "attention_cached", "attention_cached_workspace",
+           "rope_axes", "rope_axes_backward", "attention_packed", "attention_packed_backward",
+           "quantize_int8", "gemm_int8"]

@@ -1,0 +1,142 @@
+// wir_packed.h -- what the kernels over packed sequences (attn_packed.hip,
+// attn_packed_bwd.hip) share: which rows a workgroup takes, and products whose
+// tile may hold infinities or NaN in places that not all rows see.
+#pragma once
+#include "wir_cdna4.h"
+
+namespace wir {
+
+typedef long long i64;
+
+// Rows of a workgroup, and of one of its four waves.
+constexpr int PACKED_WAVES = 4, PACKED_ROWS = 128;
+
+// A workgroup's rows: row0 .. of the sequence of `len` tokens from token `start`
+// on.  `rest`: of the tokens behind the last sequence instead.
+struct Rows {
+  int start, len, row0;
+  bool rest;
+};
+
+// offsets[i], within the tokens.  Every index that follows from the offsets is
+// bounded: offsets that do not ascend give wrong rows, no more.
+__device__ __forceinline__ int packed_offset(const int* offsets, int i, int batch, int tokens) {
+  return i > batch ? tokens : min(max(offsets[i], 0), tokens);
+}
+
+// Block x of all sequences' blocks of PACKED_ROWS rows.  Sequence i's blocks are
+// numbered from offsets[i] / PACKED_ROWS + i on: that leaves each at least as
+// many numbers as it has blocks, needs no sum over the sequences' blocks and no
+// length on the host; tokens / PACKED_ROWS + batch + 1 numbers hold all, the last
+// ones those of the tokens behind the last sequence (i = batch).  The lanes look
+// at 64 sequences at a time: one round of loads up to 63 sequences, two up to 4095.
+__device__ __forceinline__ Rows packed_block(const int* offsets, int batch, int tokens, int x) {
+  const int lane = lane_id();
+  int lo = 0, n = batch + 1;   // the sequence is one of lo .. lo + n - 1
+  for (;;) {
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    const int from = packed_offset(offsets, min(i, batch), batch, tokens);
+    const bool here = lane * step < n && from / PACKED_ROWS + i <= x;
+    const int last = max(63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(here) | 1), 0);
+    if (step > 1) {
+      lo += last * step;
+      n = min(step, n - last * step);
+      continue;
+    }
+    const int to = packed_offset(offsets, min(i, batch) + 1, batch, tokens);
+    Rows r;
+    r.start = __builtin_amdgcn_readlane(from, last);
+    r.len = __builtin_amdgcn_readlane(to, last) - r.start;
+    const int seq = lo + last;
+    r.row0 = (x - r.start / PACKED_ROWS - seq) * PACKED_ROWS;
+    r.rest = seq == batch;
+    return r;
+  }
+}
+
+// Program -> (block, head).  The programs of one XCD are of few heads, so that
+// a head's keys and values stay in its L2.
+__device__ __forceinline__ void packed_program(int blocks, int heads, int& x, int& head) {
+  const int id = remap_xcd(blockIdx.x, blocks * heads);
+  head = id / blocks;
+  x = id - head * blocks;
+}
+
+// One head of one sequence as a tensor of its own: rows past its end read as zeros and are not stored.
+template <typename T>
+__device__ __forceinline__ gl<T> packed_head(T* data, i64 head_stride, i64 row_stride, int head, int start, int len,
+                                             int cols) {
+  return gl<T>{data + head * head_stride + (i64)start * row_stride, 1, 1, len, cols, 0, 0, row_stride};
+}
+
+// Keep (row, col) for col <= row (CAUSAL; TRANSPOSED: row <= col) and col < cols; elsewhere -inf.
+template <bool CAUSAL, bool TRANSPOSED, int MS, int R, int C>
+__device__ __forceinline__ void packed_mask(RTile<MS, R, C>& t, int row0, int col0, int cols) {
+  const int lane = lane_id(), lr = lane % MS, lh = lane / MS;
+#pragma unroll
+  for (int cb = 0; cb < t.CB; ++cb)
+#pragma unroll
+    for (int rb = 0; rb < t.RB; ++rb)
+#pragma unroll
+      for (int i = 0; i < MF<MS>::CREGS; ++i) {
+        const int row = row0 + rb * MS + lr, col = col0 + cb * MS + ccol<MS>(i, lh);
+        const bool keep = col < cols && (!CAUSAL || (TRANSPOSED ? row <= col : col <= row));
+        t.f[cb][rb][i] = keep ? t.f[cb][rb][i] : -__builtin_inff();
+      }
+}
+
+// Whether a wave's tile holds a NaN.
+template <int MS, int R, int C>
+__device__ __forceinline__ bool has_nan(const RTile<MS, R, C>& t) {
+  bool any = false;
+#pragma unroll
+  for (int cb = 0; cb < t.CB; ++cb)
+#pragma unroll
+    for (int rb = 0; rb < t.RB; ++rb)
+#pragma unroll
+      for (int i = 0; i < MF<MS>::CREGS; ++i) any |= t.f[cb][rb][i] != t.f[cb][rb][i];
+  return __builtin_amdgcn_ballot_w64(any) != 0;
+}
+
+// A product a @ b over a tile b (K rows, C columns) whose rows not all rows of
+// `a` see: a is 0 where it does not see, but 0 times an infinity or NaN is NaN.
+// clear_odd makes those values of b 0 for the product and notes for each of its
+// columns the first (LAST: the last) position that holds one: they rule the
+// results of the rows that see that position.
+template <int D>
+struct Odd {
+  int at[3][D];   // NaN, +infinity, -infinity
+};
+
+constexpr int NOWHERE = 0x7fffffff;
+
+template <bool LAST, int D>
+__device__ __forceinline__ void no_odd(__attribute__((address_space(3))) Odd<D>* odd) {
+  for (int i = threadIdx.x; i < 3 * D; i += 64 * PACKED_WAVES) (&odd->at[0][0])[i] = LAST ? -1 : NOWHERE;
+}
+
+template <bool LAST, class TB>
+__device__ __forceinline__ void clear_odd(char* b_base, int pos0, __attribute__((address_space(3))) Odd<TB::COLS>* odd) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+#pragma unroll 1
+  for (int i = threadIdx.x; i < TB::ROWS * TB::CPR; i += 64 * PACKED_WAVES) {
+    const int row = i / TB::CPR, chunk = i % TB::CPR;
+    auto* p = (__attribute__((address_space(3))) u16x8*)(lds(b_base) + TB::chunk_off(row, chunk));
+    u16x8 w = *p;
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) any |= (w[j] & 0x7f80) == 0x7f80;
+    if (!any) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if ((w[j] & 0x7f80) != 0x7f80) continue;
+      int* at = (int*)&odd->at[w[j] & 0x7f ? 0 : w[j] & 0x8000 ? 2 : 1][chunk * 8 + j];
+      if (LAST) atomicMax(at, pos0 + row);
+      else atomicMin(at, pos0 + row);
+      w[j] = 0;
+    }
+    *p = w;
+  }
+}
+
+}  // namespace wir

@@ -1,0 +1,130 @@
+"""Products in 8-bit integers: tokens' codes and scales, and the product of two
+matrices of them (``csrc/gemm_int8.hip``)."""
+from __future__ import annotations
+
+import ctypes
+from typing import Tuple
+
+from warpir_amd.handwritten import DevicePlans, apart, check_tensor, check_written, launch, need
+
+_quantize_plans = DevicePlans("quantize_int8")
+_gemm_plans = DevicePlans("gemm_int8")
+
+MAX_WIDTH = 131056   # 2^7 * 2^7 * 131056 < 2^31: a sum of that many products fits
+
+
+class _QuantizeArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("codes", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("xs", ctypes.c_longlong), ("cs", ctypes.c_longlong), ("rows", ctypes.c_int), ("width", ctypes.c_int)]
+
+
+class _Args(ctypes.Structure):
+    _fields_ = [*((n, ctypes.c_void_p) for n in ("a", "b", "a_scale", "b_scale", "out")),
+                *((n, ctypes.c_longlong) for n in ("as_", "bs", "os")), *((n, ctypes.c_int) for n in "mnk")]
+
+
+def _pitch(t) -> int:
+    """Elements from a row to the next."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def quantize_int8(x, codes=None, scale=None) -> Tuple[object, object]:
+    """The rows of ``x`` ``[M, K]`` (bf16, K a multiple of 16, 16-byte aligned rows) in
+    8-bit integers: ``(codes, scale)``, int8 ``[M, K]`` and fp32 ``[M]``.  A row's scale is
+    its largest magnitude over 127 (2^-126 at least), its codes the integers
+    nearest to ``x / scale``, ties to even: -127 to 127.  The scale of a row with an
+    infinity or NaN is NaN, and its codes are 0.  Made for ``gemm_int8``: of tokens,
+    and of a weight's channels where they are rows."""
+    import torch
+
+    fn, done = "quantize_int8", None
+    if codes is not None:
+        apart(fn, ("codes", "scale", "codes", "x"), 2, codes, scale, codes, x)
+    done = _quantize_plans.run(0, x, codes, scale)
+    if done is not None and done is not False:
+        return done
+    check_tensor(fn, "x", x, torch.bfloat16, (None, None), None)
+    (rows, width), device = x.shape, x.device
+    need(fn, width % 16 == 0 and 0 < width <= MAX_WIDTH, f"K must be a multiple of 16 up to {MAX_WIDTH}, got {width}")
+    need(fn, rows < 1 << 24, "2^24 rows or more in one call")
+    rec = _quantize_plans.recording(done, x, codes, scale)
+    if codes is None:
+        codes = rec.alloc(torch.empty(rows, width, dtype=torch.int8, device=device))
+    if scale is None:
+        scale = rec.alloc(torch.empty(rows, dtype=torch.float32, device=device))
+    check_tensor(fn, "codes", codes, torch.int8, (rows, width), device)
+    check_tensor(fn, "scale", scale, torch.float32, (rows,), device, rows=False)
+    need(fn, rows <= 1 or scale.stride(0) == 1, "scale must be contiguous")
+    check_written(fn, "codes", codes)
+    if rows == 0:
+        return codes, scale
+    name, each = _quantize_form(width)
+    launch(rec, device, "gemm_int8.hsaco", f"wir_quantize_int8_{name}", (-(-rows // each), 1, 1), (256, 1, 1),
+           _QuantizeArgs(None, None, None, _pitch(x), _pitch(codes), rows, width), {"x": x, "codes": codes, "scale": scale})
+    if rec:
+        _quantize_plans.add(0, rec, codes, scale)
+    return codes, scale
+
+
+def _quantize_form(width: int) -> Tuple[str, int]:
+    """(kernel, rows of a workgroup): a wave a row up to 1024 values, four past that, each lane with one, two or
+    four times 16 values in registers."""
+    if width <= 1024:
+        return "w1", 4
+    return "w4" if width <= 4096 else "w4_n2" if width <= 8192 else "w4_n4", 1
+
+
+def gemm_int8(a, b, a_scale, b_scale, out=None):
+    """``out[m, n] = sum_k a[m, k] b[n, k] * a_scale[m] * b_scale[n]`` (bf16 ``[M, N]``) of
+    int8 ``a`` ``[M, K]`` (tokens, as ``quantize_int8`` gives them) and ``b`` ``[N, K]`` (a
+    weight, channel by channel), scales fp32 ``[M]`` and ``[N]``.  K is a multiple of 16
+    up to 131056, rows are 16-byte aligned; M and N are any.  The sum is exact in
+    32-bit integers; it is converted, scaled and rounded to bf16 once each."""
+    import torch
+
+    fn, done = "gemm_int8", None
+    if out is not None:
+        apart(fn, ("out", "a", "out", "b", "out", "a_scale", "out", "b_scale"), 4, out, a, out, b, out, a_scale, out, b_scale)
+    done = _gemm_plans.run(0, a, b, a_scale, b_scale, out)
+    if done is not None and done is not False:
+        return done
+    check_tensor(fn, "a", a, torch.int8, (None, None), None)
+    (m, k), device = a.shape, a.device
+    check_tensor(fn, "b", b, torch.int8, (None, k), device)
+    n = b.shape[0]
+    need(fn, k % 16 == 0 and k <= MAX_WIDTH, f"K must be a multiple of 16 up to {MAX_WIDTH}, got {k}")
+    for name, s, rows in (("a_scale", a_scale, m), ("b_scale", b_scale, n)):
+        check_tensor(fn, name, s, torch.float32, (rows,), device, rows=False)
+        need(fn, rows <= 1 or s.stride(0) == 1, f"{name} must be contiguous")
+    for name, t in (("a", a), ("b", b)):
+        need(fn, _pitch(t) < 1 << 23, f"{name}'s rows are 2^23 bytes or more apart")
+    need(fn, max(m, n) < 1 << 30, "2^30 rows or more in one call")
+    rec = _gemm_plans.recording(done, a, b, a_scale, b_scale, out)
+    if out is None:
+        out = rec.alloc(torch.empty(m, n, dtype=torch.bfloat16, device=device))
+    check_tensor(fn, "out", out, torch.bfloat16, (m, n), device, rows=False)
+    need(fn, n <= 1 or m == 0 or out.stride(1) == 1, "out's last dimension must be contiguous")
+    check_written(fn, "out", out)
+    if m == 0 or n == 0:
+        return out
+    if k == 0:
+        return out.zero_()
+    variant, tile = _gemm_form(m, n, k)
+    programs = -(-m // tile) * -(-n // tile)
+    need(fn, programs < 1 << 24, "2^24 workgroups or more in one call")
+    launch(rec, device, "gemm_int8.hsaco", f"wir_gemm_int8_{variant}", (programs, 1, 1), (256, 1, 1),
+           _Args(*[None] * 5, _pitch(a), _pitch(b), _pitch(out), m, n, k),
+           {"a": a, "b": b, "a_scale": a_scale, "b_scale": b_scale, "out": out})
+    if rec:
+        _gemm_plans.add(0, rec, out)
+    return out
+
+
+def _gemm_form(m: int, n: int, k: int):
+    for tile in (256, 128):
+        if -(-m // tile) * -(-n // tile) >= 256:
+            return str(tile), tile
+    return "64", 64
+
+
+__all__ = ["quantize_int8", "gemm_int8"]

@@ -1,0 +1,179 @@
+"""Attention over packed sequences of different lengths and its gradients
+(``csrc/attn_packed.hip``, ``csrc/attn_packed_bwd.hip``)."""
+from __future__ import annotations
+
+import ctypes
+from typing import Tuple
+
+from warpir_amd.handwritten import INT_MAX, DevicePlans, apart, check_tensor, check_written, launch, need, own
+
+_forward_plans = DevicePlans("attention_packed")
+_backward_plans = DevicePlans("attention_packed_backward")
+
+ROWS = 128   # query rows, or keys, of a workgroup (csrc/wir_packed.h)
+
+
+class _Args(ctypes.Structure):
+    _fields_ = [*((n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "offsets")),
+                *((n, ctypes.c_longlong) for n in ("qh", "qt", "kh", "kt", "vh", "vt", "oh", "ot", "lh", "lt")),
+                *((n, ctypes.c_int) for n in ("batch", "tokens", "heads", "group", "blocks", "flags"))]
+
+
+class _GradArgs(ctypes.Structure):
+    _fields_ = [*((n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "d_o", "lse", "offsets", "dq", "dk", "dv", "stats")),
+                *((n, ctypes.c_longlong) for n in ("qh", "qt", "kh", "kt", "vh", "vt", "oh", "ot", "gh", "gt", "lh", "lt",
+                                                   "dqh", "dqt", "dkh", "dkt", "dvh", "dvt")),
+                *((n, ctypes.c_int) for n in ("batch", "tokens", "heads", "group", "blocks", "flags"))]
+
+
+def _validate(fn, q, k, v, offsets, causal):
+    """(heads, key/value heads, tokens, D, batch, blocks, device)"""
+    import torch
+
+    bf16, device = torch.bfloat16, getattr(q, "device", None)
+    check_tensor(fn, "q", q, bf16, (None,) * 3, None)
+    heads, tokens, d = q.shape
+    need(fn, d in (64, 128), f"the head size must be 64 or 128, got {d}")
+    check_tensor(fn, "k", k, bf16, (None, tokens, d), device)
+    check_tensor(fn, "v", v, bf16, k.shape, device)
+    shared = k.shape[0]
+    need(fn, shared > 0 and heads > 0 and heads % shared == 0,
+         f"{heads} query heads are not a multiple of {shared} key/value heads")
+    check_tensor(fn, "offsets", offsets, torch.int32, (None,), device, rows=False)
+    batch = offsets.shape[0] - 1
+    need(fn, batch >= 0, "offsets must hold the end of each sequence behind a first 0")
+    need(fn, batch == 0 or offsets.stride(0) == 1, "offsets must be contiguous")
+    if not isinstance(causal, bool):
+        raise TypeError(f"{fn}: causal must be a bool")
+    need(fn, tokens + batch <= INT_MAX - 2 * ROWS, "2^31 tokens or more in one call")
+    blocks = tokens // ROWS + batch + 1
+    need(fn, blocks * heads < 1 << 24, "2^24 workgroups or more in one call")
+    return heads, shared, tokens, d, batch, blocks, device
+
+
+def _by_token(heads, tokens, d, device, rec):
+    """[H, T, D], a token's heads next to one another: as a projection reads it."""
+    import torch
+
+    return rec.alloc(torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=device).transpose(0, 1))
+
+
+def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) -> Tuple[object, object]:
+    """Attention over packed sequences: ``q`` ``[H, T, D]``, ``k`` and ``v`` ``[H_kv, T, D]``
+    (bf16, D = 64 or 128, H a multiple of H_kv; any 16-byte aligned rows, so
+    views of a fused projection are read as they lie).  Returns ``(O, LSE)``,
+    bf16 ``[H, T, D]`` and fp32 ``[H, T]`` (natural log) as ``api.attention_forward``.
+
+    Sequence ``i`` is tokens ``offsets[i] .. offsets[i + 1] - 1`` (int32, ascending from
+    0, on the GPU; sequences may be empty); its tokens see one another, with
+    ``causal`` only those up to their own.  Tokens behind ``offsets[-1]`` belong to no
+    sequence: a given ``out`` or ``lse`` keeps what it has there, an allocated one
+    holds 0 and -inf.  In a captured graph the offsets may change between
+    replays.  What a row does not see does not reach it, be it infinite or NaN.
+
+    An allocated ``O`` lies token by token, so that ``O.transpose(0, 1).reshape(T, H * D)``
+    is the next product's operand as it is.  ``out`` may be ``q`` itself."""
+    import torch
+
+    fn, done, given = "attention_packed", None, None
+    if out is not None or lse is not None:
+        apart(fn, ("out", "lse", "out", "k", "out", "v", "out", "q"), 3, out, lse, out, k, out, v, out, q)
+        given = out, lse
+        out = own(out, q)
+    planned = type(causal) is bool
+    if planned:
+        done = _forward_plans.run(causal, q, k, v, offsets, out, lse)
+        if done is not None and done is not False:
+            return _results(given, done)
+    heads, shared, tokens, d, batch, blocks, device = _validate(fn, q, k, v, offsets, causal)
+    rec = _forward_plans.recording(done, q, k, v, offsets, out, lse)
+    flags = (1 if out is None else 0) | (2 if lse is None else 0)
+    if out is None:
+        out = _by_token(heads, tokens, d, device, rec)
+    if lse is None:
+        lse = rec.alloc(torch.empty(heads, tokens, dtype=torch.float32, device=device))
+    check_tensor(fn, "out", out, torch.bfloat16, q.shape, device)
+    check_tensor(fn, "lse", lse, torch.float32, q.shape[:2], device, rows=False)
+    for name, x in (("out", out), ("lse", lse)):
+        check_written(fn, name, x)
+    if tokens == 0:
+        return _results(given, (out, lse))
+    args = _Args(*[None] * 6, *(s for x in (q, k, v, out) for s in x.stride()[:2]), *lse.stride(), batch, tokens, heads,
+                 heads // shared, blocks, flags)
+    launch(rec, device, "attn_packed.hsaco", f"wir_attn_packed_d{d}" + ("_causal" if causal else ""),
+           (blocks * heads, 1, 1), (256, 1, 1), args,
+           {"q": q, "k": k, "v": v, "out": out, "lse": lse, "offsets": offsets})
+    if rec:
+        _forward_plans.add(causal, rec, out, lse)
+    return _results(given, (out, lse))
+
+
+def _results(given, done):
+    """The tensors that the caller gave, where it did."""
+    return done if given is None else tuple(x if g is None else g for g, x in zip(given, done))
+
+
+# what a given gradient and another tensor of the call must not share; past the first ones, pairs that may be one tensor
+_BACKWARD_PAIRS = ("dq", "dk", "dq", "dv", "dk", "dv", "dq", "q", "dq", "k", "dq", "v", "dq", "o", "dq", "do",
+                   "dk", "q", "dk", "v", "dk", "o", "dk", "do", "dv", "q", "dv", "k", "dv", "o", "dv", "do",
+                   "dk", "k", "dv", "v")
+
+
+def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True, dq=None, dk=None, dv=None,
+                              workspace=None) -> Tuple[object, object, object]:
+    """Gradients ``(dq, dk, dv)`` (bf16) of ``attention_packed`` from its inputs, its
+    outputs ``o`` and ``lse`` and the gradient ``do`` of ``o`` (bf16 ``[H, T, D]``, any
+    row-aligned layout); ``causal`` as in the forward.  The sums over a
+    key/value head's query heads are in 32 bits, in an order that the lengths fix.
+
+    Tokens behind ``offsets[-1]`` get no gradient: given tensors keep what they
+    have there, allocated ones (which lie token by token) hold 0.  ``dk`` may be
+    ``k`` itself and ``dv`` ``v``; other shared memory is refused.  ``workspace`` holds two
+    numbers for each query head and token (fp32, at least ``2 * H * T`` elements,
+    allocated if omitted); one call at a time may use it."""
+    import torch
+
+    fn, done, given = "attention_packed_backward", None, None
+    if dq is not None or dk is not None or dv is not None:
+        apart(fn, _BACKWARD_PAIRS, 16, dq, dk, dq, dv, dk, dv, dq, q, dq, k, dq, v, dq, o, dq, do,
+              dk, q, dk, v, dk, o, dk, do, dv, q, dv, k, dv, o, dv, do, dk, k, dv, v)
+        given = dq, dk, dv
+        dk, dv = own(dk, k), own(dv, v)
+    tensors = (q, k, v, o, lse, do, offsets, dq, dk, dv)
+    if type(causal) is bool and workspace is None:
+        done = _backward_plans.run(causal, *tensors)
+        if done is not None and done is not False:
+            return _results(given, done)
+    heads, shared, tokens, d, batch, blocks, device = _validate(fn, q, k, v, offsets, causal)
+    for name, x in (("o", o), ("do", do)):
+        check_tensor(fn, name, x, torch.bfloat16, q.shape, device)
+    check_tensor(fn, "lse", lse, torch.float32, q.shape[:2], device, rows=False)
+    rec = _backward_plans.recording(done, *tensors)
+    flags, grads = 0, []
+    for i, (name, x, like) in enumerate((("dq", dq, q), ("dk", dk, k), ("dv", dv, v))):
+        if x is None:
+            flags |= 1 << i
+            x = _by_token(like.shape[0], tokens, d, device, rec)
+        check_tensor(fn, name, x, torch.bfloat16, like.shape, device)
+        check_written(fn, name, x)
+        grads.append(x)
+    floats = 2 * heads * tokens
+    if workspace is None:
+        workspace = rec.alloc(torch.empty(floats, dtype=torch.float32, device=device))
+    check_tensor(fn, "workspace", workspace, torch.float32, (None,), device)
+    need(fn, workspace.numel() >= floats, f"workspace needs {floats} elements")
+    if tokens == 0:
+        return _results(given, tuple(grads))
+    args = _GradArgs(*[None] * 11, *(s for x in (q, k, v, o, do, lse, *grads) for s in x.stride()[:2]), batch, tokens, heads,
+                     heads // shared, blocks, flags)
+    names = {"q": q, "k": k, "v": v, "o": o, "d_o": do, "lse": lse, "offsets": offsets, "dq": grads[0], "dk": grads[1],
+             "dv": grads[2], "stats": workspace}
+    for kernel, programs in (("dq", heads), ("dkdv", shared)):
+        launch(rec, device, "attn_packed_bwd.hsaco", f"wir_attn_packed_{kernel}_d{d}" + ("_causal" if causal else ""),
+               (blocks * programs, 1, 1), (256, 1, 1), args, names)
+    if rec:
+        _backward_plans.add(causal, rec, *grads)
+    return _results(given, tuple(grads))
+
+
+__all__ = ["attention_packed", "attention_packed_backward"]

@@ -1,5 +1,6 @@
-"""Head norms with position rotation: what lies between a fused projection
-(``api.gemm``) and attention (``csrc/qk_norm_rope.hip``)."""
+"""What lies between a fused projection (``api.gemm``) and attention: head norms
+with position rotation (``csrc/qk_norm_rope.hip``), and the rotation alone by
+positions with several axes (``csrc/rope_axes.hip``)."""
 from __future__ import annotations
 
 import ctypes
@@ -11,6 +12,7 @@ from warpir_amd.handwritten import INT_MAX, DevicePlans, apart, check_tensor, ch
 
 _forward_plans = DevicePlans("qk_norm_rope")
 _backward_plans = DevicePlans("qk_norm_rope_backward")
+_axes_plans = DevicePlans("rope_axes")
 
 
 class _Side(ctypes.Structure):
@@ -243,4 +245,109 @@ def _blocks(q_rows: int, k_rows: int, d: int) -> Tuple[int, int]:
     return each[0], each[1]
 
 
-__all__ = ["rope_table", "qk_norm_rope", "qk_norm_rope_backward"]
+class _AxesSide(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                *((n, ctypes.c_longlong) for n in ("xb", "xh", "xs", "ob", "oh", "os"))]
+
+
+class _AxesArgs(ctypes.Structure):
+    _fields_ = [("q", _AxesSide), ("k", _AxesSide), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+                ("pos", ctypes.c_void_p), *((n, ctypes.c_longlong) for n in ("pa", "pb", "ps", "cs", "ss")),
+                *((n, ctypes.c_int) for n in ("q_heads", "k_heads", "batch", "seq", "table_rows", "pairs")),
+                ("ends", ctypes.c_int * 3), ("flags", ctypes.c_int)]
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _sections(fn: str, sections, interleaved, back: bool):
+    """(flags of the plan, pairs, first pairs of axes 1 to 3, whether an axis ends inside four pairs)"""
+    need(fn, 1 <= len(sections) <= 4 and all(type(n) is int and n >= 0 for n in sections),
+         f"sections must be 1 to 4 numbers of pairs, got {sections}")
+    if not isinstance(interleaved, bool):
+        raise TypeError(f"{fn}: interleaved must be a bool")
+    pairs = sum(sections)
+    need(fn, 0 < pairs <= 64 and pairs % 8 == 0, f"the sections must add up to 8, 16, .. D / 2 pairs, got {pairs}")
+    ends = [min(sum(sections[:i]), pairs) if i < len(sections) else pairs for i in (1, 2, 3)]
+    flags = len(sections) << 32 | pairs << 24 | ends[0] << 17 | ends[1] << 10 | ends[2] << 3 | back << 1 | interleaved
+    return flags, pairs, ends, any(n % 4 for n in ends)
+
+
+def _rotate_axes(fn, plans, back, names, q, k, cos, sin, positions, sections, interleaved, q_out, k_out):
+    import torch
+
+    done = None
+    key, pairs, ends, inside = _sections(fn, tuple(sections), interleaved, back)
+    given = None
+    if q_out is not None or k_out is not None:
+        need(fn, q_out is not k_out, f"{names[2]} and {names[3]} are one tensor")
+        apart(fn, (names[2], names[3], names[2], names[1], names[3], names[0], names[2], names[0], names[3], names[1]), 3,
+              q_out, k_out, q_out, k, k_out, q, q_out, q, k_out, k)
+        given = q_out, k_out
+        q_out, k_out = own(q_out, q), own(k_out, k)
+    done = plans.run(key, q, k, cos, sin, positions, q_out, k_out)
+    if done is not None and done is not False:
+        return _results(given, done)
+    bf16, device = torch.bfloat16, getattr(q, "device", None)
+    check_tensor(fn, names[0], q, bf16, (None,) * 4, None)
+    b, h, s, d = q.shape
+    need(fn, d in (64, 128), f"the head size must be 64 or 128, got {d}")
+    need(fn, pairs <= d // 2, f"{pairs} pairs do not fit a head of {d}")
+    check_tensor(fn, names[1], k, bf16, (b, None, s, d), device)
+    check_tensor(fn, "cos", cos, torch.float32, (None, pairs), device)
+    check_tensor(fn, "sin", sin, torch.float32, (cos.shape[0], pairs), device)
+    need(fn, 0 < cos.shape[0] <= INT_MAX, "the table has no rows")
+    shape = (len(sections), s) if getattr(positions, "dim", lambda: 3)() == 2 else (len(sections), b, s)
+    check_tensor(fn, "positions", positions, (torch.int32, torch.int64), shape, device, rows=False)
+    heads = h + k.shape[1]
+    need(fn, b * s * heads < 1 << 29, "2^29 rows or more in one call")
+    need(fn, b * -(-s * heads * d // 4096) < 1 << 24, "2^24 workgroups or more in one call")
+    rec = plans.recording(done, q, k, cos, sin, positions, q_out, k_out)
+    q_out = _output(fn, names[2], q_out, q, rec)
+    k_out = _output(fn, names[3], k_out, k, rec)
+    if b * s * heads == 0:
+        return _results(given, (q_out, k_out))
+    pa, *where = positions.stride()
+    pb, ps = where if len(where) == 2 else (0, where[0])
+    flags = (1 if positions.dtype == torch.int64 else 0) | (2 if back else 0) | (4 if inside else 0)
+    args = _AxesArgs(_AxesSide(None, None, *q.stride()[:3], *q_out.stride()[:3]),
+                     _AxesSide(None, None, *k.stride()[:3], *k_out.stride()[:3]), None, None, None, pa, pb, ps,
+                     cos.stride(0), sin.stride(0), h, k.shape[1], b, s, cos.shape[0], pairs, (ctypes.c_int * 3)(*ends), flags)
+    rows = 4096 // d   # rows of a workgroup, all of one sequence
+    launch(rec, device, "rope_axes.hsaco", f"wir_rope_axes_d{d}" + ("_inter" if interleaved else ""),
+           (b * -(-s * heads // rows), 1, 1), (256, 1, 1), args,
+           {"q.x": q, "q.out": q_out, "k.x": k, "k.out": k_out, "cos": cos, "sin": sin, "pos": positions})
+    if rec:
+        plans.add(key, rec, q_out, k_out)
+    return _results(given, (q_out, k_out))
+
+
+def rope_axes(q, k, cos, sin, positions, sections, interleaved: bool = False, q_out=None,
+              k_out=None) -> Tuple[object, object]:
+    """The rotation of every head of ``q`` ``[B, H, S, D]`` and ``k`` ``[B, H_kv, S, D]`` (bf16,
+    D = 64 or 128; views of a fused projection are read as they lie) by
+    positions with several axes, in one launch; returns ``(q_out, k_out)``, bf16.
+
+    ``sections`` says how many pairs of a head turn by each axis, one after
+    another: 1 to 4 numbers that add up to R = 8, 16, .. D / 2 pairs.
+    ``positions`` is int32 or int64 ``[axes, S]`` or ``[axes, B, S]``, and ``cos``, ``sin`` are
+    ``[positions, R]`` fp32, column i of them pair i's (``rope_table(n, 2 * R)`` for
+    frequencies that go on through the axes, ``torch.cat`` of one table for each axis
+    along the columns for frequencies of its own).  The pairs are ``(i, i + R)``, or ``(2 i, 2 i + 1)``
+    with ``interleaved``; values from 2 R on are passed through.  The pairs of
+    an axis whose position is outside the table become NaN.
+
+    Packed sequences are one with B = 1 and the positions of each of them.
+    ``q_out`` may be ``q`` itself and ``k_out`` ``k``; memory that an output shares
+    otherwise with the other, ``q`` or ``k`` is refused."""
+    return _rotate_axes("rope_axes", _axes_plans, False, ("q", "k", "q_out", "k_out"), q, k, cos, sin, positions,
+                        sections, interleaved, q_out, k_out)
+
+
+def rope_axes_backward(dq_out, dk_out, cos, sin, positions, sections, interleaved: bool = False, dq=None,
+                       dk=None) -> Tuple[object, object]:
+    """Gradients ``(dq, dk)`` of ``rope_axes`` (bf16) from those of its outputs: the
+    rotation back.  ``dq`` may be ``dq_out`` itself and ``dk`` ``dk_out``."""
+    return _rotate_axes("rope_axes_backward", _axes_plans, True, ("dq_out", "dk_out", "dq", "dk"), dq_out, dk_out, cos,
+                        sin, positions, sections, interleaved, dq, dk)
+
+
+__all__ = ["rope_table", "qk_norm_rope", "qk_norm_rope_backward", "rope_axes", "rope_axes_backward"]
