@@ -47,15 +47,17 @@ def quantize_int8(x, codes=None, scale=None) -> Tuple[object, object]:
     (rows, width), device = x.shape, x.device
     need(fn, width % 16 == 0 and 0 < width <= MAX_WIDTH, f"K must be a multiple of 16 up to {MAX_WIDTH}, got {width}")
     need(fn, rows < 1 << 24, "2^24 rows or more in one call")
+    if codes is not None:
+        check_tensor(fn, "codes", codes, torch.int8, (rows, width), device)
+        check_written(fn, "codes", codes)
+    if scale is not None:
+        check_tensor(fn, "scale", scale, torch.float32, (rows,), device, rows=False)
+        need(fn, rows <= 1 or scale.stride(0) == 1, "scale must be contiguous")
     rec = _quantize_plans.recording(done, x, codes, scale)
     if codes is None:
         codes = rec.alloc(torch.empty(rows, width, dtype=torch.int8, device=device))
     if scale is None:
         scale = rec.alloc(torch.empty(rows, dtype=torch.float32, device=device))
-    check_tensor(fn, "codes", codes, torch.int8, (rows, width), device)
-    check_tensor(fn, "scale", scale, torch.float32, (rows,), device, rows=False)
-    need(fn, rows <= 1 or scale.stride(0) == 1, "scale must be contiguous")
-    check_written(fn, "codes", codes)
     if rows == 0:
         return codes, scale
     name, each = _quantize_form(width)
@@ -99,12 +101,13 @@ def gemm_int8(a, b, a_scale, b_scale, out=None):
     for name, t in (("a", a), ("b", b)):
         need(fn, _pitch(t) < 1 << 23, f"{name}'s rows are 2^23 bytes or more apart")
     need(fn, max(m, n) < 1 << 30, "2^30 rows or more in one call")
+    if out is not None:
+        check_tensor(fn, "out", out, torch.bfloat16, (m, n), device, rows=False)
+        need(fn, n <= 1 or m == 0 or out.stride(1) == 1, "out's last dimension must be contiguous")
+        check_written(fn, "out", out)
     rec = _gemm_plans.recording(done, a, b, a_scale, b_scale, out)
     if out is None:
         out = rec.alloc(torch.empty(m, n, dtype=torch.bfloat16, device=device))
-    check_tensor(fn, "out", out, torch.bfloat16, (m, n), device, rows=False)
-    need(fn, n <= 1 or m == 0 or out.stride(1) == 1, "out's last dimension must be contiguous")
-    check_written(fn, "out", out)
     if m == 0 or n == 0:
         return out
     if k == 0:

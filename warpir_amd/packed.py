@@ -88,14 +88,16 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
     heads, shared, tokens, d, batch, blocks, device = _validate(fn, q, k, v, offsets, causal)
     rec = _forward_plans.recording(done, q, k, v, offsets, out, lse)
     flags = (1 if out is None else 0) | (2 if lse is None else 0)
+    if out is not None:
+        check_tensor(fn, "out", out, torch.bfloat16, q.shape, device)
+        check_written(fn, "out", out)
+    if lse is not None:
+        check_tensor(fn, "lse", lse, torch.float32, q.shape[:2], device, rows=False)
+        check_written(fn, "lse", lse)
     if out is None:
         out = _by_token(heads, tokens, d, device, rec)
     if lse is None:
         lse = rec.alloc(torch.empty(heads, tokens, dtype=torch.float32, device=device))
-    check_tensor(fn, "out", out, torch.bfloat16, q.shape, device)
-    check_tensor(fn, "lse", lse, torch.float32, q.shape[:2], device, rows=False)
-    for name, x in (("out", out), ("lse", lse)):
-        check_written(fn, name, x)
     if tokens == 0:
         return _results(given, (out, lse))
     args = _Args(*[None] * 6, *(s for x in (q, k, v, out) for s in x.stride()[:2]), *lse.stride(), batch, tokens, heads,
@@ -148,20 +150,22 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
     for name, x in (("o", o), ("do", do)):
         check_tensor(fn, name, x, torch.bfloat16, q.shape, device)
     check_tensor(fn, "lse", lse, torch.float32, q.shape[:2], device, rows=False)
+    floats, flags = 2 * heads * tokens, 0
+    for name, x, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if x is not None:
+            check_tensor(fn, name, x, torch.bfloat16, like.shape, device)
+            check_written(fn, name, x)
+    if workspace is not None:
+        check_tensor(fn, "workspace", workspace, torch.float32, (None,), device)
+        need(fn, workspace.numel() >= floats, f"workspace needs {floats} elements")
     rec = _backward_plans.recording(done, *tensors)
-    flags, grads = 0, []
-    for i, (name, x, like) in enumerate((("dq", dq, q), ("dk", dk, k), ("dv", dv, v))):
-        if x is None:
+    grads = [dq, dk, dv]
+    for i, like in enumerate((q, k, v)):
+        if grads[i] is None:
             flags |= 1 << i
-            x = _by_token(like.shape[0], tokens, d, device, rec)
-        check_tensor(fn, name, x, torch.bfloat16, like.shape, device)
-        check_written(fn, name, x)
-        grads.append(x)
-    floats = 2 * heads * tokens
+            grads[i] = _by_token(like.shape[0], tokens, d, device, rec)
     if workspace is None:
         workspace = rec.alloc(torch.empty(floats, dtype=torch.float32, device=device))
-    check_tensor(fn, "workspace", workspace, torch.float32, (None,), device)
-    need(fn, workspace.numel() >= floats, f"workspace needs {floats} elements")
     if tokens == 0:
         return _results(given, tuple(grads))
     args = _GradArgs(*[None] * 11, *(s for x in (q, k, v, o, do, lse, *grads) for s in x.stride()[:2]), batch, tokens, heads,

@@ -260,7 +260,7 @@ class _AxesArgs(ctypes.Structure):
 @functools.lru_cache(maxsize=256, typed=True)
 def _sections(fn: str, sections, interleaved, back: bool):
     """(flags of the plan, pairs, first pairs of axes 1 to 3, whether an axis ends inside four pairs)"""
-    need(fn, 1 <= len(sections) <= 4 and all(type(n) is int and n >= 0 for n in sections),
+    need(fn, 1 <= len(sections) <= 4 and min(sections) >= 0,
          f"sections must be 1 to 4 numbers of pairs, got {sections}")
     if not isinstance(interleaved, bool):
         raise TypeError(f"{fn}: interleaved must be a bool")
@@ -275,6 +275,8 @@ def _rotate_axes(fn, plans, back, names, q, k, cos, sin, positions, sections, in
     import torch
 
     done = None
+    if not isinstance(sections, (tuple, list)) or any(type(n) is not int for n in sections):
+        raise TypeError(f"{fn}: sections must be 1 to 4 numbers of pairs, got {sections!r}")
     key, pairs, ends, inside = _sections(fn, tuple(sections), interleaved, back)
     given = None
     if q_out is not None or k_out is not None:
@@ -300,9 +302,11 @@ def _rotate_axes(fn, plans, back, names, q, k, cos, sin, positions, sections, in
     heads = h + k.shape[1]
     need(fn, b * s * heads < 1 << 29, "2^29 rows or more in one call")
     need(fn, b * -(-s * heads * d // 4096) < 1 << 24, "2^24 workgroups or more in one call")
+    for name, x, like in ((names[2], q_out, q), (names[3], k_out, k)):   # (both before either is allocated)
+        if x is not None:
+            _output(fn, name, x, like, None)
     rec = plans.recording(done, q, k, cos, sin, positions, q_out, k_out)
-    q_out = _output(fn, names[2], q_out, q, rec)
-    k_out = _output(fn, names[3], k_out, k, rec)
+    q_out, k_out = (_output(fn, "", None, like, rec) if x is None else x for x, like in ((q_out, q), (k_out, k)))
     if b * s * heads == 0:
         return _results(given, (q_out, k_out))
     pa, *where = positions.stride()
