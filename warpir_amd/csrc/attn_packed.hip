@@ -51,22 +51,23 @@ __device__ __forceinline__ bool forward_block(const fwd_args& a, const wir::Rows
   const int wave = wir::wave_id(), lane = wir::lane_id();
   const int row0 = r.row0 + wave * 32;
   const int kv = head / a.group;
-  const auto K = wir::packed_head(const_cast<bf16*>(a.k), a.kh, a.kt, kv, r.start, r.len, D);
-  const auto V = wir::packed_head(const_cast<bf16*>(a.v), a.vh, a.vt, kv, r.start, r.len, D);
-  const auto Q = wir::packed_head(const_cast<bf16*>(a.q), a.qh, a.qt, head, r.start, r.len, D);
+  wir::HeadTiles<TK> K;
+  wir::HeadTiles<TV> V;
+  K.init(a.k + kv * a.kh + r.start * a.kt, a.kt, r.len);
+  V.init(a.v + kv * a.vh + r.start * a.vt, a.vt, r.len);
   const int keys = CAUSAL ? min(r.len, r.row0 + ROWS) : r.len, tiles = (keys + TILE - 1) / TILE;
   auto load = [&](int t) {
     char* at = smem + t % 2 * TK::BYTES;
-    wir::Loader<TK, WAVES>::template load<false>(at, K, 0, 0, t * TILE, 0, wave);
-    wir::Loader<TV, WAVES>::template load<false>(at + 2 * TK::BYTES, V, 0, 0, t * TILE, 0, wave);
+    K.load(at, t, wave);
+    V.load(at + 2 * TK::BYTES, t, wave);
   };
   wir::RowFrags<32, 1, D / 16> q;
-  wir::load_row_frags_global(q, Q, 0, 0, row0, 0);
+  wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
   wir::RTile<32, 32, D> o;
   float m = -__builtin_inff(), l = 0.f;
   wir::fill(o, 0.f);
   auto* odd = (__attribute__((address_space(3))) wir::Odd<D>*)wir::lds(smem + 4 * TK::BYTES);
-  if (CAUSAL && careful) wir::no_odd<false>(odd);
+  if (careful) wir::no_odd<false, WAVES>(odd);
   load(0);
   for (int t = 0; t < tiles; ++t) {
     char *kt = smem + t % 2 * TK::BYTES, *vt = kt + 2 * TK::BYTES;
@@ -77,7 +78,10 @@ __device__ __forceinline__ bool forward_block(const fwd_args& a, const wir::Rows
     wir::RTile<32, 32, TILE> s;
     wir::mma_ABt_frags<32, 32, TILE, TK, D / 16>(s, q, kt, 0);
     const bool edge = CAUSAL ? col0 + TILE - 1 > row0 : col0 + TILE > r.len;
-    if (edge) wir::packed_mask<CAUSAL, false>(s, row0, col0, r.len);
+    if (edge) {
+      wir::seldom();
+      wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
+    }
     float top = s.f[0][0][0];
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb)
@@ -99,9 +103,9 @@ __device__ __forceinline__ bool forward_block(const fwd_args& a, const wir::Rows
       }
     l = l * corr.v[0] + (sum[0] + sum[1]);
     wir::row_scale(o, o, corr);
-    if (CAUSAL && careful) {
+    if (careful) {
       wir::barrier();
-      wir::clear_odd<false, TV>(vt, col0, odd);
+      wir::clear_odd<false, WAVES, TV>(vt, col0, odd);
       wir::barrier();
     }
     wir::mma_rAB<32, 32, TILE, D, TV>(o, p, vt, 0);
@@ -110,12 +114,12 @@ __device__ __forceinline__ bool forward_block(const fwd_args& a, const wir::Rows
   wir::RVec<32, 32> inv;
   inv.v[0] = 1.0f / l;
   wir::row_apply(o, o, inv, [](float x, float s) { return x * s; });
-  if (CAUSAL && !careful) {
+  if (!careful) {
     // an infinite or NaN value that not all of a tile's rows see
     int* flag = (int*)(smem + 4 * TK::BYTES);
     if (threadIdx.x == 0) *flag = 0;
     wir::wait_vm_barrier<0>();
-    if (wir::has_nan(o)) *flag = 1;
+    if (wir::has_nan(o, row0 + lane % 32 < r.len)) *flag = 1;
     wir::barrier();
     const bool odd = *flag;
     wir::barrier();
@@ -123,8 +127,8 @@ __device__ __forceinline__ bool forward_block(const fwd_args& a, const wir::Rows
   } else {
     wir::wait_vm_barrier<0>();   // the tiles are read: their LDS takes the output
   }
-  if (CAUSAL && careful) {
-    const int row = row0 + lane % 32;
+  if (careful) {
+    const int row = CAUSAL ? row0 + lane % 32 : r.len - 1;   // the last position that the row sees
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll

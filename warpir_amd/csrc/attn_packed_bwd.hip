@@ -24,7 +24,7 @@ struct bwd_args {
   bf16* dq;
   bf16* dk;
   bf16* dv;
-  float* stats;        // [2][H][T]: the LSE in log2 units, D_p
+  float* stats;        // [2][H][T]: -LSE sqrt(D) and -D_p, what the scores of the dK/dV kernels begin with
   i64 qh, qt, kh, kt, vh, vt, oh, ot, gh, gt, lh, lt, dqh, dqt, dkh, dkt, dvh, dvt;
   int batch, tokens, heads, group, blocks;
   int flags;           // rows behind the last sequence become 0 in dq: 1, dk: 2, dv: 4
@@ -35,13 +35,13 @@ constexpr int WAVES = wir::PACKED_WAVES, ROWS = wir::PACKED_ROWS;
 template <int D>
 struct Scale {
   static constexpr double inv_sqrt = D == 64 ? 0.125 : 0.08838834764831845;
-  static constexpr float s = (float)inv_sqrt, c = (float)(1.4426950408889634 * inv_sqrt);
+  static constexpr float root = D == 64 ? 8.0f : 11.313708498984761f, s = (float)inv_sqrt, c = (float)(1.4426950408889634 * inv_sqrt);
 };
 
 __device__ __forceinline__ void zero_rest(bf16* x, i64 head_stride, i64 row_stride, const wir::Rows& r, int head, int d) {
   const int rows = min(r.len - r.row0, ROWS);
   x += head * head_stride + (i64)(r.start + r.row0) * row_stride;
-  for (int i = threadIdx.x; i < rows * (d / 8); i += 256)
+  for (int i = threadIdx.x; i < rows * (d / 8); i += blockDim.x)
     *(wir::bf16x8*)(x + i / (d / 8) * row_stride + i % (d / 8) * 8) = wir::bf16x8{};
 }
 
@@ -66,31 +66,32 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
   constexpr float c = Scale<D>::c;
   const int wave = wir::wave_id(), lane = wir::lane_id();
   const int row0 = r.row0 + wave * 32, kv = head / a.group;
-  const auto K = wir::packed_head(const_cast<bf16*>(a.k), a.kh, a.kt, kv, r.start, r.len, D);
-  const auto V = wir::packed_head(const_cast<bf16*>(a.v), a.vh, a.vt, kv, r.start, r.len, D);
+  wir::HeadTiles<TK> K;
+  wir::HeadTiles<TV> V;
+  K.init(a.k + kv * a.kh + r.start * a.kt, a.kt, r.len);
+  V.init(a.v + kv * a.vh + r.start * a.vt, a.vt, r.len);
   const int keys = CAUSAL ? min(r.len, r.row0 + ROWS) : r.len, tiles = (keys + KT - 1) / KT;
   auto load = [&](int t) {
     char* at = smem + t % 2 * TK::BYTES;
-    wir::Loader<TK, WAVES>::template load<false>(at, K, 0, 0, t * KT, 0, wave);
-    wir::Loader<TV, WAVES>::template load<false>(at + 2 * TK::BYTES, V, 0, 0, t * KT, 0, wave);
+    K.load(at, t, wave);
+    V.load(at + 2 * TK::BYTES, t, wave);
   };
   auto* odd = (__attribute__((address_space(3))) wir::Odd<D>*)wir::lds(smem + 4 * TK::BYTES);
-  if (CAUSAL && careful) wir::no_odd<false>(odd);
+  if (careful) wir::no_odd<false, WAVES>(odd);
   wir::RowFrags<32, 1, D / 16> q, d_o, o;
-  wir::load_row_frags_global(q, wir::packed_head(const_cast<bf16*>(a.q), a.qh, a.qt, head, r.start, r.len, D), 0, 0, row0, 0);
-  wir::load_row_frags_global(d_o, wir::packed_head(const_cast<bf16*>(a.d_o), a.gh, a.gt, head, r.start, r.len, D), 0, 0,
-                             row0, 0);
-  wir::load_row_frags_global(o, wir::packed_head(const_cast<bf16*>(a.o), a.oh, a.ot, head, r.start, r.len, D), 0, 0, row0, 0);
+  wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
+  wir::packed_rows(d_o, a.d_o + head * a.gh + r.start * a.gt, a.gt, row0, r.len);
+  wir::packed_rows(o, a.o + head * a.oh + r.start * a.ot, a.ot, row0, r.len);
   const int row = row0 + lane % 32;
-  float lse = row < r.len ? a.lse[head * a.lh + (i64)(r.start + row) * a.lt] : 0.f;
+  float lse = a.lse[head * a.lh + (r.start + min(row, r.len - 1)) * a.lt];
   wir::RVec<32, 32> dots;
   wir::row_dot(dots, d_o, o);
-  lse *= 1.4426950408889634f;
   if (lane < 32 && row < r.len) {
     float* to = a.stats + (i64)head * a.tokens + r.start + row;
-    to[0] = lse;
-    to[(i64)a.heads * a.tokens] = dots.v[0];
+    to[0] = -lse * Scale<D>::root;
+    to[(i64)a.heads * a.tokens] = -dots.v[0];
   }
+  lse *= 1.4426950408889634f;
   wir::RTile<32, 32, D> acc;
   wir::fill(acc, 0.f);
   load(0);
@@ -104,7 +105,10 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
     wir::BTile<32, 32, KT> ds;
     wir::mma_ABt_frags<32, 32, KT, TK, D / 16>(s, q, kt, 0);
     const bool edge = CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len;
-    if (edge) wir::packed_mask<CAUSAL, false>(s, row0, col0, r.len);
+    if (edge) {
+      wir::seldom();
+      wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
+    }
     wir::mma_ABt_frags<32, 32, KT, TV, D / 16>(dp, d_o, vt, 0);
 #pragma unroll
     for (int cb = 0; cb < KT / 32; ++cb)
@@ -115,21 +119,22 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
         s.f[cb][0][i] = p;
       }
     if (edge) {   // (a value that a row does not see may be NaN)
+      wir::seldom();
 #pragma unroll
       for (int cb = 0; cb < KT / 32; ++cb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp.f[cb][0][i] = s.f[cb][0][i] == 0.f ? 0.f : dp.f[cb][0][i];
     }
     wir::to_bf16(ds, dp);
-    if (CAUSAL && careful) {
+    if (careful) {
       wir::barrier();
-      wir::clear_odd<false, TK>(kt, col0, odd);
+      wir::clear_odd<false, WAVES, TK>(kt, col0, odd);
       wir::barrier();
     }
     wir::mma_rAB<32, 32, KT, D, TK>(acc, ds, kt, 0);
   }
-  if (CAUSAL && !careful) {
-    if (any_wave(wir::has_nan(acc), smem + 4 * TK::BYTES)) return true;
+  if (!careful) {
+    if (any_wave(wir::has_nan(acc, row < r.len), smem + 4 * TK::BYTES)) return true;
   } else {
     wir::wait_vm_barrier<0>();
   }
@@ -137,14 +142,14 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
   for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc.f[cb][0][i] *= Scale<D>::s;
-  if (CAUSAL && careful) {
+  if (careful) {
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
         const int first = min(odd->at[0][d], min(odd->at[1][d], odd->at[2][d]));
-        acc.f[cb][0][i] = row >= first ? __builtin_nanf("") : acc.f[cb][0][i];
+        acc.f[cb][0][i] = (CAUSAL ? row : r.len - 1) >= first ? __builtin_nanf("") : acc.f[cb][0][i];
       }
   }
   wir::store_tile_staged<true>(wir::packed_head(a.dq, a.dqh, a.dqt, head, r.start, r.len, D), acc, 0, 0, row0, 0,
@@ -180,25 +185,25 @@ __device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r
   const int wave = wir::wave_id(), lane = wir::lane_id();
   const int row0 = r.row0 + wave * 32;
   const int first = CAUSAL ? r.row0 / QT : 0, tiles = (r.len + QT - 1) / QT;
+  wir::HeadTiles<T> Q, G;
+  Q.init(a.q + r.start * a.qt, a.qt, r.len);
+  G.init(a.d_o + r.start * a.gt, a.gt, r.len);
   auto load = [&](int head, int t, int slot) {
     char* at = smem + slot * T::BYTES;
-    const i64 stat = (i64)head * a.tokens + r.start;
-    wir::Loader<T, WAVES>::template load<false>(
-        at, wir::packed_head(const_cast<bf16*>(a.q), a.qh, a.qt, head, r.start, r.len, D), 0, 0, t * QT, 0, wave);
-    wir::Loader<T, WAVES>::template load<false>(
-        at + 2 * T::BYTES, wir::packed_head(const_cast<bf16*>(a.d_o), a.gh, a.gt, head, r.start, r.len, D), 0, 0, t * QT, 0,
-        wave);
-    wir::VecLoader<QT, WAVES>::template load<false>(
-        smem + VEC + slot * QT * 4, wir::gl<float>{a.stats + stat, 1, 1, r.len, 1, 0, 0, 1}, 0, 0, t * QT, wave);
-    wir::VecLoader<QT, WAVES>::template load<false>(
-        smem + VEC + (2 + slot) * QT * 4,
-        wir::gl<float>{a.stats + (i64)a.heads * a.tokens + stat, 1, 1, r.len, 1, 0, 0, 1}, 0, 0, t * QT, wave);
+    Q.base = (const char*)(a.q + head * a.qh + r.start * a.qt);
+    G.base = (const char*)(a.d_o + head * a.gh + r.start * a.gt);
+    Q.load(at, t, wave);
+    G.load(at + 2 * T::BYTES, t, wave);
+    if (wave < 2 && lane < QT) {   // a wave each for the LSEs and the D_p
+      const float* from = a.stats + ((i64)(wave * a.heads + head) * a.tokens + r.start);
+      wir::dma4_v(from + min(t * QT + lane, r.len - 1), wir::lds_addr(smem + VEC + (2 * wave + slot) * QT * 4));
+    }
   };
   auto* odd = (__attribute__((address_space(3))) wir::Odd<D>*)wir::lds(smem + ODD);
-  if (CAUSAL && careful) wir::no_odd<true>(odd), wir::no_odd<true>(odd + 1);
+  if (careful) wir::no_odd<true, WAVES>(odd), wir::no_odd<true, WAVES>(odd + 1);
   wir::RowFrags<32, 1, D / 16> k, v;
-  wir::load_row_frags_global(k, wir::packed_head(const_cast<bf16*>(a.k), a.kh, a.kt, kv, r.start, r.len, D), 0, 0, row0, 0);
-  wir::load_row_frags_global(v, wir::packed_head(const_cast<bf16*>(a.v), a.vh, a.vt, kv, r.start, r.len, D), 0, 0, row0, 0);
+  wir::packed_rows(k, a.k + kv * a.kh + r.start * a.kt, a.kt, row0, r.len);
+  wir::packed_rows(v, a.v + kv * a.vh + r.start * a.vt, a.vt, row0, r.len);
   wir::RTile<32, 32, D> dk, dv;
   wir::fill(dk, 0.f);
   wir::fill(dv, 0.f);
@@ -224,26 +229,29 @@ __device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r
       for (int cb = 0; cb < QT / 32; ++cb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s.f[cb][0][i], c, -lse.v[cb][i]));
-          dp.f[cb][0][i] = p * (dp.f[cb][0][i] - dots.v[cb][i]);
+          const float p = __builtin_amdgcn_exp2f((s.f[cb][0][i] + lse.v[cb][i]) * c);
+          dp.f[cb][0][i] = p * (dp.f[cb][0][i] + dots.v[cb][i]);
           s.f[cb][0][i] = p;
         }
-      if (CAUSAL && col0 < row0 + 31) {   // (a query that does not see the row may hold NaN)
+      // (a query that does not see the row may hold NaN; past the end the last one stands again)
+      if ((CAUSAL && col0 < row0 + 31) || col0 + QT > r.len) {
+        wir::seldom();
 #pragma unroll
         for (int cb = 0; cb < QT / 32; ++cb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const bool seen = row0 + lane % 32 <= col0 + cb * 32 + wir::ccol<32>(i, lane / 32);
+            const int col = col0 + cb * 32 + wir::ccol<32>(i, lane / 32);
+            const bool seen = (!CAUSAL || row0 + lane % 32 <= col) && col < r.len;
             s.f[cb][0][i] = seen ? s.f[cb][0][i] : 0.f;
             dp.f[cb][0][i] = seen ? dp.f[cb][0][i] : 0.f;
           }
       }
       wir::to_bf16(pb, s);
       wir::to_bf16(ds, dp);
-      if (CAUSAL && careful) {
+      if (careful) {
         wir::barrier();
-        wir::clear_odd<true, T>(qt, col0, odd);
-        wir::clear_odd<true, T>(dot, col0, odd + 1);
+        wir::clear_odd<true, WAVES, T>(qt, col0, odd);
+        wir::clear_odd<true, WAVES, T>(dot, col0, odd + 1);
         wir::barrier();
       }
       wir::mma_rAB<32, 32, QT, D, T>(dv, pb, dot, 0);
@@ -251,8 +259,8 @@ __device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r
     }
     head = head1, t = t1, slot ^= 1;
   }
-  if (CAUSAL && !careful) {
-    const bool nan = wir::has_nan(dk) || wir::has_nan(dv);
+  if (!careful) {
+    const bool in = row0 + lane % 32 < r.len, nan = wir::has_nan(dk, in) || wir::has_nan(dv, in);
     if (any_wave(nan, smem + ODD)) return true;
   } else {
     wir::wait_vm_barrier<0>();
@@ -261,8 +269,8 @@ __device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r
   for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk.f[cb][0][i] *= Scale<D>::s;
-  if (CAUSAL && careful) {
-    const int row = row0 + lane % 32;
+  if (careful) {
+    const int row = CAUSAL ? row0 + lane % 32 : 0;   // the first query that sees it
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
@@ -281,6 +289,238 @@ __device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r
   return false;
 }
 
+// The same with eight waves, of which two share 32 keys: one takes the scores of
+// a tile's first 32 queries and dV, the other those of its last 32 and dK.  A
+// wave then has one sum of 64 registers instead of two, so that two waves a
+// SIMD hide one another.  They hand each other the half of P and of dS that the
+// other needs through LDS: in the time of one tile a wave takes the product of
+// tile t and the scores of tile t + 1, in opposite orders.  The operands of both
+// are one stream of LDS reads that runs AHEAD products before their use.
+template <int D, bool CAUSAL>
+struct Paired {
+  static constexpr int NW = 8, QT = 64, AHEAD = 5, KS = D / 16, CB = D / 32;
+  static constexpr int SCORES = 2 * KS, PRODUCTS = QT / 16 * CB;   // products of a wave for a tile
+  typedef wir::STile<QT, D, wir::BOTH> T;
+  typedef __attribute__((address_space(3))) wir::bf16x8 lds_bf16x8;
+  typedef __attribute__((address_space(3))) wir::bf16x4 lds_bf16x4;
+  typedef __attribute__((address_space(3))) wir::i16x4 lds_i16x4;
+  typedef __attribute__((address_space(3))) wir::f32x4 lds_f32x4;
+  typedef __attribute__((address_space(3))) wir::Odd<D> lds_odd;
+  // LDS: three slots of a Q and a dO tile, what the waves hand on (twice), the tiles' statistics, notes of what is odd
+  static constexpr int SLOT = 2 * T::BYTES, HANDED = 3 * SLOT, VEC = HANDED + 2 * NW * 2048, ODD = VEC + 3 * 2 * QT * 4,
+                       BYTES = ODD + 2 * sizeof(wir::Odd<D>);
+  static_assert(D == 128, "the swizzle's addresses below are those of 16 chunks a row");
+
+  struct At {
+    int head, t;
+  };
+
+  const bwd_args& a;
+  const wir::Rows& r;
+  char* smem;
+  int wave, lane, role, row0, first, tiles;
+  wir::HeadTiles<T, NW> Q, G;
+  unsigned row_at, tr_at;          // the lane's places in a tile, as operands of the scores and of the product
+  wir::RowFrags<32, 1, KS> k, v;
+  wir::RTile<32, 32, D> acc;       // dV or dK
+  wir::RTile<32, 32, 32> s, dp;
+  wir::BTile<32, 32, 32> keep;
+  wir::BTile<32, 32, QT> x;
+
+  __device__ __forceinline__ Paired(const bwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
+
+  __device__ __forceinline__ At after(At i) const { return i.t + 1 < tiles ? At{i.head, i.t + 1} : At{i.head + 1, first}; }
+
+  __device__ __forceinline__ void load(At i, int slot) {
+    char* at = smem + slot * SLOT;
+    Q.base = (const char*)(a.q + i.head * a.qh + r.start * a.qt);
+    G.base = (const char*)(a.d_o + i.head * a.gh + r.start * a.gt);
+    Q.load(at, i.t, wave);
+    G.load(at + T::BYTES, i.t, wave);
+    if (wave < 2) {   // a wave each for the two statistics
+      const float* from = a.stats + ((i64)(wave * a.heads + i.head) * a.tokens + r.start);
+      wir::dma4_v(from + min(i.t * QT + lane, r.len - 1), wir::lds_addr(smem + VEC + (2 * slot + wave) * QT * 4));
+    }
+  }
+
+  // The scores' sums begin with the statistics: p = exp2(c (q . k - LSE sqrt(D))), dP - D_p = dO . v - D_p.
+  __device__ __forceinline__ void begin_scores(int slot) {
+    const auto* vec = (lds_f32x4*)wir::lds(smem + VEC + 2 * slot * QT * 4 + role * 128 + lane / 32 * 16);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const wir::f32x4 x0 = vec[2 * g], x1 = vec[QT / 4 + 2 * g];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s.f[0][0][4 * g + j] = x0[j], dp.f[0][0][4 * g + j] = x1[j];
+    }
+  }
+
+  __device__ __forceinline__ void begin_product(int turn) {
+    const auto* from = (lds_bf16x4*)wir::lds(smem + HANDED + (turn * NW + (wave ^ 4)) * 2048) + lane;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const wir::bf16x4 other = from[g * 64];
+      x.f[0][0][g] = role ? other : keep.f[0][0][g];
+      x.f[1][0][g] = role ? keep.f[0][0][g] : other;
+    }
+  }
+
+  __device__ __forceinline__ wir::bf16x8 score_operand(unsigned at, int i) const {
+    return *(lds_bf16x8*)((at ^ (i / 2 * 32)) + i % 2 * T::BYTES);
+  }
+  __device__ __forceinline__ void score(const wir::bf16x8& b, int i) {
+    if (i % 2 == 0) s.f[0][0] = wir::MF<32>::mma(b, k.f[0][i / 2], s.f[0][0]);
+    else dp.f[0][0] = wir::MF<32>::mma(b, v.f[0][i / 2], dp.f[0][0]);
+  }
+
+  __device__ __forceinline__ wir::bf16x8 product_operand(unsigned at, int i) const {
+    const int q = 2 * (i / CB), cb = i % CB, rows = q * 8 * D * 2;   // (two groups of eight rows)
+    const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((at ^ (cb * 64)) + rows));
+    const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((at ^ (cb * 64 + 32)) + rows + 8 * D * 2));
+    return wir::cat(__builtin_bit_cast(wir::bf16x4, lo), __builtin_bit_cast(wir::bf16x4, hi));
+  }
+  __device__ __forceinline__ void product(const wir::bf16x8& b, int i) {
+    const int q = 2 * (i / CB), cb = i % CB;
+    acc.f[cb][0] = wir::MF<32>::mma(b, wir::cat(x.f[q / 4][0][q % 4], x.f[(q + 1) / 4][0][(q + 1) % 4]), acc.f[cb][0]);
+  }
+
+  // P and dS of the wave's half of a tile: one it keeps, one it hands on.
+  __device__ __forceinline__ void finish_scores(At i, int turn) {
+    constexpr float c = Scale<D>::c;
+    const int col0 = i.t * QT + role * 32;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      s.f[0][0][n] = __builtin_amdgcn_exp2f(s.f[0][0][n] * c);
+      dp.f[0][0][n] *= s.f[0][0][n];
+    }
+    // (a query that does not see the row may hold NaN; past the end the last one stands again)
+    if ((CAUSAL && col0 < row0 + 31) || col0 + 32 > r.len) {
+      wir::seldom();
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        const int col = col0 + wir::ccol<32>(n, lane / 32);
+        const bool seen = (!CAUSAL || row0 + lane % 32 <= col) && col < r.len;
+        s.f[0][0][n] = seen ? s.f[0][0][n] : 0.f;
+        dp.f[0][0][n] = seen ? dp.f[0][0][n] : 0.f;
+      }
+    }
+    wir::BTile<32, 32, 32> pb, ds;
+    wir::to_bf16(pb, s);
+    wir::to_bf16(ds, dp);
+    auto* to = (lds_bf16x4*)wir::lds(smem + HANDED + (turn * NW + wave) * 2048) + lane;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      to[g * 64] = role ? pb.f[0][0][g] : ds.f[0][0][g];
+      keep.f[0][0][g] = role ? ds.f[0][0][g] : pb.f[0][0][g];
+    }
+  }
+
+  // The product of the tile in `slot` (PRODUCT) and the scores of tile i in `slot1` (SCORE), ROLE 1's scores first.
+  template <int ROLE, bool PRODUCT, bool SCORE>
+  __device__ __forceinline__ void stream(int slot, At i, int slot1, int turn) {
+    constexpr int N0 = ROLE ? (SCORE ? SCORES : 0) : (PRODUCT ? PRODUCTS : 0);
+    constexpr int N = N0 + (ROLE ? (PRODUCT ? PRODUCTS : 0) : (SCORE ? SCORES : 0));
+    const unsigned product_at = tr_at + slot * SLOT, score_at = row_at + slot1 * SLOT;
+    wir::bf16x8 ring[AHEAD + 1];
+    auto read = [&](auto at) {
+      constexpr int n = decltype(at)::value;
+      if constexpr ((n >= N0) == (ROLE == 1)) ring[n % (AHEAD + 1)] = product_operand(product_at, n >= N0 ? n - N0 : n);
+      else ring[n % (AHEAD + 1)] = score_operand(score_at, n >= N0 ? n - N0 : n);
+    };
+    if (PRODUCT) begin_product(turn);
+    if (SCORE) begin_scores(slot1);
+    __builtin_amdgcn_s_setprio(1);
+    wir::static_for<0, AHEAD>(read);
+    wir::static_for<0, N>([&](auto at) {
+      constexpr int n = decltype(at)::value;
+      if constexpr (n + AHEAD < N) read(wir::ic<n + AHEAD>{});
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr ((n >= N0) == (ROLE == 1)) product(ring[n % (AHEAD + 1)], n >= N0 ? n - N0 : n);
+      else score(ring[n % (AHEAD + 1)], n >= N0 ? n - N0 : n);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (SCORE && n == (ROLE ? N0 : N) - 1) {
+        __builtin_amdgcn_s_setprio(0);
+        finish_scores(i, turn ^ 1);
+        __builtin_amdgcn_s_setprio(1);
+      }
+    });
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  // All tiles of a wave (a loop for each role: one with both in it moves the sums between registers).
+  template <int ROLE>
+  __device__ __forceinline__ void walk(At now, int end, bool careful, lds_odd* odd) {
+    At next = after(now);
+    load(now, 0);
+    wir::wait_vm_barrier<0>();
+    if (next.head < end) load(next, 1);
+    stream<ROLE, false, true>(0, now, 0, 1);
+    int slot = 0, turn = 0;
+    auto settle = [&](At third, int slot2) {
+      wir::wait_vm_barrier<0>();
+      if (third.head < end) load(third, slot2);
+      if (careful) {
+        wir::clear_odd<true, NW, T>(smem + slot * SLOT, now.t * QT, odd);
+        wir::clear_odd<true, NW, T>(smem + slot * SLOT + T::BYTES, now.t * QT, odd + 1);
+        wir::barrier();
+      }
+    };
+    while (next.head < end) {
+      const At third = after(next);
+      const int slot1 = slot == 2 ? 0 : slot + 1;
+      settle(third, slot1 == 2 ? 0 : slot1 + 1);
+      stream<ROLE, true, true>(slot, next, slot1, turn);
+      now = next, next = third, slot = slot1, turn ^= 1;
+    }
+    settle(next, 0);
+    stream<ROLE, true, false>(slot, next, 0, turn);
+  }
+
+  __device__ __forceinline__ bool run(int kv, bool careful) {
+    wave = wir::wave_id(), lane = wir::lane_id();
+    role = wave / 4;   // (waves w and w + 4 are on one SIMD)
+    row0 = r.row0 + wave % 4 * 32;
+    first = CAUSAL ? r.row0 / QT : 0, tiles = (r.len + QT - 1) / QT;
+    Q.init(a.q + r.start * a.qt, a.qt, r.len);
+    G.init(a.d_o + r.start * a.gt, a.gt, r.len);
+    const int group = lane % 16;   // of the transposed reads
+    row_at = wir::lds_addr(smem) + T::chunk_off(role * 32 + lane % 32, lane / 32);
+    tr_at = wir::lds_addr(smem) + (role ? 0 : T::BYTES) + T::elem_off(lane / 32 * 4 + group / 4, lane % 32 / 16 * 16 + 4 * (group % 4));
+    auto* odd = (lds_odd*)wir::lds(smem + ODD);
+    if (careful) wir::no_odd<true, NW>(odd), wir::no_odd<true, NW>(odd + 1);
+    wir::packed_rows(k, a.k + kv * a.kh + r.start * a.kt, a.kt, row0, r.len);
+    wir::packed_rows(v, a.v + kv * a.vh + r.start * a.vt, a.vt, row0, r.len);
+    wir::fill(acc, 0.f);
+    const At now{kv * a.group, first};
+    if (role == 0) walk<0>(now, now.head + a.group, careful, odd);
+    else walk<1>(now, now.head + a.group, careful, odd);
+    const int row = row0 + lane % 32;
+    if (!careful) {
+      if (any_wave(wir::has_nan(acc, row < r.len), smem + ODD)) return true;
+    } else {
+      wir::wait_vm_barrier<0>();
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int n = 0; n < 16; ++n) acc.f[cb][0][n] *= role ? Scale<D>::s : 1.f;
+    if (careful) {
+      const auto* mine = odd + (role ? 0 : 1);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const int d = cb * 32 + wir::ccol<32>(n, lane / 32);
+          const int until = max(mine->at[0][d], max(mine->at[1][d], mine->at[2][d]));
+          acc.f[cb][0][n] = (CAUSAL ? row : 0) <= until ? __builtin_nanf("") : acc.f[cb][0][n];
+        }
+    }
+    const auto out = role ? wir::packed_head(a.dk, a.dkh, a.dkt, kv, r.start, r.len, D)
+                          : wir::packed_head(a.dv, a.dvh, a.dvt, kv, r.start, r.len, D);
+    wir::store_tile_staged<true>(out, acc, 0, 0, row0, 0, smem + wave * 32 * D * 2);
+    return false;
+  }
+};
+
 template <int D, int QT, bool CAUSAL>
 __device__ __forceinline__ void dkdv_kernel(const bwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[4 * QT * D * 2 + 16 * QT + 2 * sizeof(wir::Odd<D>)];
@@ -297,7 +537,28 @@ __device__ __forceinline__ void dkdv_kernel(const bwd_args& a) {
   while (dkdv_block<D, QT, CAUSAL>(a, r, kv, smem, careful)) careful = true;
 }
 
+template <int D, bool CAUSAL>
+__device__ __forceinline__ void dkdv_kernel8(const bwd_args& a) {
+  __shared__ __attribute__((aligned(1024))) char smem[Paired<D, CAUSAL>::BYTES];
+  int x, kv;
+  wir::packed_program(a.blocks, a.heads / a.group, x, kv);   // a sequence's longest block is its first
+  const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
+  if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
+  if (r.rest) {
+    if (a.flags & 2) zero_rest(a.dk, a.dkh, a.dkt, r, kv, D);
+    if (a.flags & 4) zero_rest(a.dv, a.dvh, a.dvt, r, kv, D);
+    return;
+  }
+  Paired<D, CAUSAL> p(a, r, smem);
+  bool careful = false;
+  while (p.run(kv, careful)) careful = true;
+}
+
 }  // namespace
+
+#define PACKED_KERNEL8(NAME, CALL)                                                                             \
+  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) \
+  NAME(const bwd_args args) { CALL(args); }
 
 #define PACKED_KERNEL(NAME, CALL, WAVES_A_SIMD)                                                         \
   extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256),                      \
@@ -310,5 +571,5 @@ PACKED_KERNEL(wir_attn_packed_dq_d128, (dq_kernel<128, 32, false>), 2)
 PACKED_KERNEL(wir_attn_packed_dq_d128_causal, (dq_kernel<128, 32, true>), 2)
 PACKED_KERNEL(wir_attn_packed_dkdv_d64, (dkdv_kernel<64, 32, false>), 2)
 PACKED_KERNEL(wir_attn_packed_dkdv_d64_causal, (dkdv_kernel<64, 32, true>), 2)
-PACKED_KERNEL(wir_attn_packed_dkdv_d128, (dkdv_kernel<128, 64, false>), 1)
-PACKED_KERNEL(wir_attn_packed_dkdv_d128_causal, (dkdv_kernel<128, 64, true>), 1)
+PACKED_KERNEL8(wir_attn_packed_dkdv_d128, (dkdv_kernel8<128, false>))
+PACKED_KERNEL8(wir_attn_packed_dkdv_d128_causal, (dkdv_kernel8<128, true>))

@@ -69,8 +69,51 @@ __device__ __forceinline__ gl<T> packed_head(T* data, i64 head_stride, i64 row_s
   return gl<T>{data + head * head_stride + (i64)start * row_stride, 1, 1, len, cols, 0, 0, row_stride};
 }
 
-// Keep (row, col) for col <= row (CAUSAL; TRANSPOSED: row <= col) and col < cols; elsewhere -inf.
-template <bool CAUSAL, bool TRANSPOSED, int MS, int R, int C>
+// The tiles of one head of one sequence, loaded into LDS by NW waves.
+// Lane l of a wave's j-th load moves a 16-byte chunk of row row + j * EVERY; the
+// swizzles repeat within EVERY rows, so the chunk's place in the row is the
+// same for every j.  Rows past the sequence's end read its last row (no branch,
+// no address of another sequence): whoever uses the tile masks them.
+template <class Tile, int NW = PACKED_WAVES>
+struct HeadTiles {
+  static constexpr int LOADS = Tile::ROWS * Tile::CPR / 64 / NW, EVERY = Tile::ROWS / LOADS;
+  static_assert(EVERY % 16 == 0, "the swizzles repeat every 16 rows");
+  const char* base;
+  unsigned row, chunk, pitch;   // the lane's row and bytes in it, bytes from a row to the next
+  int len;
+
+  __device__ __forceinline__ void init(const bf16* x, i64 row_stride, int rows) {
+    const int p = threadIdx.x, c = p % Tile::CPR;   // (wave w's chunks start at 64 w)
+    row = p / Tile::CPR;
+    chunk = (c ^ swz<Tile::CPR, Tile::ROLE>(row)) * 16;
+    pitch = (unsigned)row_stride * 2;
+    base = (const char*)x;
+    len = rows;
+  }
+
+  __device__ __forceinline__ void load(char* tile, int t, int wave) const {
+    const char* from = base + (i64)(t * Tile::ROWS) * pitch;
+    const unsigned end = (unsigned)min(len - 1 - t * Tile::ROWS, Tile::ROWS - 1);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      dma16_s(from, min(row + j * EVERY, end) * pitch + chunk, lds_addr(tile + (wave + j * NW) * 1024));
+  }
+};
+
+// A wave's 32 rows from row0 on of one head of one sequence as operands; past the sequence's end its last row.
+template <int KS>
+__device__ __forceinline__ void packed_rows(RowFrags<32, 1, KS>& fr, const bf16* x, i64 row_stride, int row0, int len) {
+  const int lane = lane_id();
+  const bf16* from = x + (i64)min(row0 + lane % 32, len - 1) * row_stride + lane / 32 * 8;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) fr.f[0][ks] = *(const bf16x8*)(from + ks * 16);
+}
+
+// In a branch that few tiles take: keeps the compiler from computing it for all of them and selecting.
+__device__ __forceinline__ void seldom() { asm volatile(""); }
+
+// Keep (row, col) for col <= row (CAUSAL), or for col < cols; elsewhere -inf.
+template <bool CAUSAL, int MS, int R, int C>
 __device__ __forceinline__ void packed_mask(RTile<MS, R, C>& t, int row0, int col0, int cols) {
   const int lane = lane_id(), lr = lane % MS, lh = lane / MS;
 #pragma unroll
@@ -80,14 +123,13 @@ __device__ __forceinline__ void packed_mask(RTile<MS, R, C>& t, int row0, int co
 #pragma unroll
       for (int i = 0; i < MF<MS>::CREGS; ++i) {
         const int row = row0 + rb * MS + lr, col = col0 + cb * MS + ccol<MS>(i, lh);
-        const bool keep = col < cols && (!CAUSAL || (TRANSPOSED ? row <= col : col <= row));
-        t.f[cb][rb][i] = keep ? t.f[cb][rb][i] : -__builtin_inff();
+        t.f[cb][rb][i] = (CAUSAL ? col <= row : col < cols) ? t.f[cb][rb][i] : -__builtin_inff();
       }
 }
 
-// Whether a wave's tile holds a NaN.
+// Whether a wave's tile holds a NaN, in the lanes whose row is `in`.
 template <int MS, int R, int C>
-__device__ __forceinline__ bool has_nan(const RTile<MS, R, C>& t) {
+__device__ __forceinline__ bool has_nan(const RTile<MS, R, C>& t, bool in) {
   bool any = false;
 #pragma unroll
   for (int cb = 0; cb < t.CB; ++cb)
@@ -95,7 +137,7 @@ __device__ __forceinline__ bool has_nan(const RTile<MS, R, C>& t) {
     for (int rb = 0; rb < t.RB; ++rb)
 #pragma unroll
       for (int i = 0; i < MF<MS>::CREGS; ++i) any |= t.f[cb][rb][i] != t.f[cb][rb][i];
-  return __builtin_amdgcn_ballot_w64(any) != 0;
+  return __builtin_amdgcn_ballot_w64(any && in) != 0;
 }
 
 // A product a @ b over a tile b (K rows, C columns) whose rows not all rows of
@@ -110,16 +152,16 @@ struct Odd {
 
 constexpr int NOWHERE = 0x7fffffff;
 
-template <bool LAST, int D>
+template <bool LAST, int NW, int D>
 __device__ __forceinline__ void no_odd(__attribute__((address_space(3))) Odd<D>* odd) {
-  for (int i = threadIdx.x; i < 3 * D; i += 64 * PACKED_WAVES) (&odd->at[0][0])[i] = LAST ? -1 : NOWHERE;
+  for (int i = threadIdx.x; i < 3 * D; i += 64 * NW) (&odd->at[0][0])[i] = LAST ? -1 : NOWHERE;
 }
 
-template <bool LAST, class TB>
+template <bool LAST, int NW, class TB>
 __device__ __forceinline__ void clear_odd(char* b_base, int pos0, __attribute__((address_space(3))) Odd<TB::COLS>* odd) {
   typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 #pragma unroll 1
-  for (int i = threadIdx.x; i < TB::ROWS * TB::CPR; i += 64 * PACKED_WAVES) {
+  for (int i = threadIdx.x; i < TB::ROWS * TB::CPR; i += 64 * NW) {
     const int row = i / TB::CPR, chunk = i % TB::CPR;
     auto* p = (__attribute__((address_space(3))) u16x8*)(lds(b_base) + TB::chunk_off(row, chunk));
     u16x8 w = *p;

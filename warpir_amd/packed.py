@@ -46,6 +46,8 @@ def _validate(fn, q, k, v, offsets, causal):
     if not isinstance(causal, bool):
         raise TypeError(f"{fn}: causal must be a bool")
     need(fn, tokens + batch <= INT_MAX - 2 * ROWS, "2^31 tokens or more in one call")
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        need(fn, tokens < 2 or x.stride(1) < 1 << 23, f"{name}'s tokens are 2^23 elements or more apart")
     blocks = tokens // ROWS + batch + 1
     need(fn, blocks * heads < 1 << 24, "2^24 workgroups or more in one call")
     return heads, shared, tokens, d, batch, blocks, device
@@ -149,6 +151,7 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
     heads, shared, tokens, d, batch, blocks, device = _validate(fn, q, k, v, offsets, causal)
     for name, x in (("o", o), ("do", do)):
         check_tensor(fn, name, x, torch.bfloat16, q.shape, device)
+    need(fn, tokens < 2 or do.stride(1) < 1 << 23, "do's tokens are 2^23 elements or more apart")
     check_tensor(fn, "lse", lse, torch.float32, q.shape[:2], device, rows=False)
     floats, flags = 2 * heads * tokens, 0
     for name, x, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
@@ -174,7 +177,7 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
              "dv": grads[2], "stats": workspace}
     for kernel, programs in (("dq", heads), ("dkdv", shared)):
         launch(rec, device, "attn_packed_bwd.hsaco", f"wir_attn_packed_{kernel}_d{d}" + ("_causal" if causal else ""),
-               (blocks * programs, 1, 1), (256, 1, 1), args, names)
+               (blocks * programs, 1, 1), (512 if kernel == "dkdv" and d == 128 else 256, 1, 1), args, names)
     if rec:
         _backward_plans.add(causal, rec, *grads)
     return _results(given, tuple(grads))
