@@ -78,7 +78,7 @@ def _attend(**change):
     (dict(offsets=[0, 30]), "offsets must be a torch.Tensor"),
     (dict(causal=1), "causal must be a bool"),
     (dict(q=_fake(1, 1, 64).expand(1 << 12, 1 << 20, 64), k=_fake(1, 1, 64).expand(1, 1 << 20, 64),
-          v=_fake(1, 1, 64).expand(1, 1 << 20, 64)), "2\\^24 workgroups"),
+          v=_fake(1, 1, 64).expand(1, 1 << 20, 64)), "2\\^32 threads"),
     (dict(q=_fake(1, 1, 64).expand(1, (1 << 31) - 1, 64), k=_fake(1, 1, 64).expand(1, (1 << 31) - 1, 64),
           v=_fake(1, 1, 64).expand(1, (1 << 31) - 1, 64)), "2\\^31 tokens"),
 ])

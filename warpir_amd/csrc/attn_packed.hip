@@ -21,10 +21,8 @@ struct fwd_args {
   const int* offsets;  // [batch + 1]
   i64 qh, qt, kh, kt, vh, vt, oh, ot, lh, lt;
   int batch, tokens, heads, group, blocks;
-  int flags;           // 1: rows behind the last sequence become 0 in out, 2: -inf in lse
+  int flags;           // 1: rows behind the last sequence become 0 in out, 2: -inf in lse, 4: two heads a workgroup
 };
-
-constexpr int WAVES = wir::PACKED_WAVES, ROWS = wir::PACKED_ROWS, TILE = 64;
 
 template <int D>
 struct Scale {
@@ -32,67 +30,88 @@ struct Scale {
   static constexpr float c = (float)(1.4426950408889634 * inv_sqrt);
 };
 
-__device__ __forceinline__ void fill_rest(const fwd_args& a, const wir::Rows& r, int head, int d) {
-  const int rows = min(r.len - r.row0, ROWS);
-  bf16* out = a.out + head * a.oh + (i64)(r.start + r.row0) * a.ot;
-  if (a.flags & 1)
-    for (int i = threadIdx.x; i < rows * (d / 8); i += 256)
-      *(wir::bf16x8*)(out + i / (d / 8) * a.ot + i % (d / 8) * 8) = wir::bf16x8{};
-  if ((a.flags & 2) && (int)threadIdx.x < rows)
-    a.lse[head * a.lh + (i64)(r.start + r.row0 + threadIdx.x) * a.lt] = -__builtin_inff();
-}
-
-// One block of 128 query rows, 32 a wave.  Returns whether a result is NaN (only then may CAREFUL give another).
+// A workgroup: two groups of four waves, 32 query rows a wave.  The groups take
+// 128 rows each, of two heads that share a key/value head where there are two
+// (flags & 4), or else one behind the other, and the same tiles of 64 keys.
+// Waves w and w + 4 are on one SIMD and work in opposite phases: in the time of
+// one tile t either takes the products of P(t - 1) with V(t - 1) and of Q with
+// K(t), and a softmax, the first group that of t behind them, the second that
+// of t - 1 before, so that one's matrix instructions run under the other's
+// exponentials.
 template <int D, bool CAUSAL>
-__device__ __forceinline__ bool forward_block(const fwd_args& a, const wir::Rows& r, int head, char* smem, bool careful) {
+struct Forward {
+  static constexpr int NW = 8, TILE = 64, AHEAD = D == 128 ? 5 : 3, KS = D / 16, CB = D / 32;
+  static constexpr int SCORES = 2 * KS, PRODUCTS = TILE / 16 * CB;   // products of a wave for a tile
   typedef wir::STile<TILE, D, wir::ROWREAD> TK;
   typedef wir::STile<TILE, D, wir::TRREAD> TV;
-  constexpr float c = Scale<D>::c;
-  const int wave = wir::wave_id(), lane = wir::lane_id();
-  const int row0 = r.row0 + wave * 32;
-  const int kv = head / a.group;
-  wir::HeadTiles<TK> K;
-  wir::HeadTiles<TV> V;
-  K.init(a.k + kv * a.kh + r.start * a.kt, a.kt, r.len);
-  V.init(a.v + kv * a.vh + r.start * a.vt, a.vt, r.len);
-  const int keys = CAUSAL ? min(r.len, r.row0 + ROWS) : r.len, tiles = (keys + TILE - 1) / TILE;
-  auto load = [&](int t) {
-    char* at = smem + t % 2 * TK::BYTES;
-    K.load(at, t, wave);
-    V.load(at + 2 * TK::BYTES, t, wave);
-  };
-  wir::RowFrags<32, 1, D / 16> q;
-  wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
+  typedef __attribute__((address_space(3))) wir::bf16x8 lds_bf16x8;
+  typedef __attribute__((address_space(3))) wir::i16x4 lds_i16x4;
+  typedef __attribute__((address_space(3))) wir::Odd<D> lds_odd;
+  static constexpr int ODD = 4 * TK::BYTES, BYTES = ODD + sizeof(wir::Odd<D>);   // LDS: two tiles of K, two of V, notes
+  // A row's probabilities are 2^(c s - m), m within 2^16 of its largest score so far: a sum past that asks for a new m.
+  static constexpr float LIMIT = 65536.f;
+
+  const fwd_args& a;
+  const wir::Rows& r;
+  char* smem;
+  int wave, lane, head, row0, tiles, mine;
+  wir::HeadTiles<TK, NW> K;
+  wir::HeadTiles<TV, NW> V;
+  unsigned row_at, tr_at;          // the lane's places in a tile, as operands of the scores and of the product
+  wir::RowFrags<32, 1, KS> q;
   wir::RTile<32, 32, D> o;
-  float m = -__builtin_inff(), l = 0.f;
-  wir::fill(o, 0.f);
-  auto* odd = (__attribute__((address_space(3))) wir::Odd<D>*)wir::lds(smem + 4 * TK::BYTES);
-  if (careful) wir::no_odd<false, WAVES>(odd);
-  load(0);
-  for (int t = 0; t < tiles; ++t) {
-    char *kt = smem + t % 2 * TK::BYTES, *vt = kt + 2 * TK::BYTES;
-    const int col0 = t * TILE;
-    wir::wait_vm_barrier<0>();
-    if (t + 1 < tiles) load(t + 1);
-    if (CAUSAL && !careful && col0 > row0 + 31) continue;   // no row of the wave sees the tile
-    wir::RTile<32, 32, TILE> s;
-    wir::mma_ABt_frags<32, 32, TILE, TK, D / 16>(s, q, kt, 0);
-    const bool edge = CAUSAL ? col0 + TILE - 1 > row0 : col0 + TILE > r.len;
-    if (edge) {
-      wir::seldom();
-      wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
-    }
-    float top = s.f[0][0][0];
-#pragma unroll
-    for (int cb = 0; cb < 2; ++cb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s.f[cb][0][i]);
-    top = fmaxf(wir::lane_group_reduce<32>(top, wir::OpMax()) * c, m);
-    wir::RVec<32, 32> corr;
-    corr.v[0] = __builtin_amdgcn_exp2f(m - top);
-    m = top;
+  wir::RTile<32, 32, TILE> s;
+  wir::BTile<32, 32, TILE> p;
+  float m, l;                      // l: of the lane's half of the columns
+
+  __device__ __forceinline__ Forward(const fwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
+
+  __device__ __forceinline__ wir::bf16x8 score_operand(unsigned at, int i) const {
+    return *(lds_bf16x8*)((at ^ (i / 2 * 32)) + i % 2 * 32 * D * 2);
+  }
+  __device__ __forceinline__ void score(const wir::bf16x8& b, int i) {
+    s.f[i % 2][0] = wir::MF<32>::mma(b, q.f[0][i / 2], i < 2 ? wir::f32x16{} : s.f[i % 2][0]);
+  }
+  __device__ __forceinline__ wir::bf16x8 product_operand(unsigned at, int i) const {
+    const int rows = i / CB * 16 * D * 2, cb = i % CB;   // (two groups of eight rows)
+    const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((at ^ (cb * 64)) + rows));
+    const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((at ^ (cb * 64)) + rows + 8 * D * 2));
+    return wir::cat(__builtin_bit_cast(wir::bf16x4, lo), __builtin_bit_cast(wir::bf16x4, hi));
+  }
+  __device__ __forceinline__ void product(const wir::bf16x8& b, int i) {
+    const int g = 2 * (i / CB), cb = i % CB;
+    o.f[cb][0] = wir::MF<32>::mma(b, wir::cat(p.f[g / 4][0][g % 4], p.f[g / 4][0][g % 4 + 1]), o.f[cb][0]);
+  }
+
+  // The product of tile t - 1 (PRODUCT) and the scores of tile t (SCORE): one stream of LDS reads, AHEAD products before
+  // their use.
+  template <bool PRODUCT, bool SCORE>
+  __device__ __forceinline__ void stream(int t) {
+    constexpr int N0 = PRODUCT ? PRODUCTS : 0, N = N0 + (SCORE ? SCORES : 0);
+    const unsigned product_at = tr_at + (t + 1) % 2 * TV::BYTES, score_at = row_at + t % 2 * TK::BYTES;
+    wir::bf16x8 ring[AHEAD + 1];
+    auto read = [&](auto at) {
+      constexpr int n = decltype(at)::value;
+      if constexpr (n < N0) ring[n % (AHEAD + 1)] = product_operand(product_at, n);
+      else ring[n % (AHEAD + 1)] = score_operand(score_at, n - N0);
+    };
+    __builtin_amdgcn_s_setprio(1);
+    wir::static_for<0, AHEAD>(read);
+    wir::static_for<0, N>([&](auto at) {
+      constexpr int n = decltype(at)::value;
+      if constexpr (n + AHEAD < N) read(wir::ic<n + AHEAD>{});
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (n < N0) product(ring[n % (AHEAD + 1)], n);
+      else score(ring[n % (AHEAD + 1)], n - N0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  // p and the lane's sum of it, with m as it is.
+  __device__ __forceinline__ float exponentials() {
+    constexpr float c = Scale<D>::c;
     float sum[2] = {0.f, 0.f};
-    wir::BTile<32, 32, TILE> p;
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
@@ -101,73 +120,158 @@ __device__ __forceinline__ bool forward_block(const fwd_args& a, const wir::Rows
         sum[i % 2] += x;
         p.f[cb][0][i / 4][i % 4] = (bf16)x;   // (the product's operand; the sum has the value itself)
       }
-    l = l * corr.v[0] + (sum[0] + sum[1]);
-    wir::row_scale(o, o, corr);
-    if (careful) {
-      wir::barrier();
-      wir::clear_odd<false, WAVES, TV>(vt, col0, odd);
-      wir::barrier();
+    return sum[0] + sum[1];
+  }
+
+  __device__ __forceinline__ void softmax(int t) {
+    constexpr float c = Scale<D>::c;
+    const int col0 = t * TILE;
+    if (CAUSAL ? col0 + TILE - 1 > row0 : col0 + TILE > r.len) {
+      wir::seldom();
+      wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
     }
-    wir::mma_rAB<32, 32, TILE, D, TV>(o, p, vt, 0);
-  }
-  l = wir::lane_group_reduce<32>(l, wir::OpAdd());
-  wir::RVec<32, 32> inv;
-  inv.v[0] = 1.0f / l;
-  wir::row_apply(o, o, inv, [](float x, float s) { return x * s; });
-  if (!careful) {
-    // an infinite or NaN value that not all of a tile's rows see
-    int* flag = (int*)(smem + 4 * TK::BYTES);
-    if (threadIdx.x == 0) *flag = 0;
-    wir::wait_vm_barrier<0>();
-    if (wir::has_nan(o, row0 + lane % 32 < r.len)) *flag = 1;
-    wir::barrier();
-    const bool odd = *flag;
-    wir::barrier();
-    if (odd) return true;
-  } else {
-    wir::wait_vm_barrier<0>();   // the tiles are read: their LDS takes the output
-  }
-  if (careful) {
-    const int row = CAUSAL ? row0 + lane % 32 : r.len - 1;   // the last position that the row sees
+    float sum = exponentials();   // (not a number before the first tile, whose m is -inf)
+    if (__builtin_amdgcn_ballot_w64(!(sum <= LIMIT)) != 0) {
+      wir::seldom();
+      float top = s.f[0][0][0];
 #pragma unroll
-    for (int cb = 0; cb < D / 32; ++cb)
+      for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
-        const bool nan = row >= odd->at[0][d], up = row >= odd->at[1][d], down = row >= odd->at[2][d];
-        const float x = o.f[cb][0][i];
-        o.f[cb][0][i] = nan || (up && down) ? __builtin_nanf("") : up ? x + __builtin_inff() : down ? x - __builtin_inff() : x;
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s.f[cb][0][i]);
+      // (a row's results do not depend on what the wave's other rows ask for)
+      const float asked = wir::lane_group_reduce<32>(sum <= LIMIT ? 0.f : 1.f, wir::OpMax());
+      top = fmaxf(wir::lane_group_reduce<32>(top, wir::OpMax()) * c, m);
+      top = asked != 0.f ? top : m;
+      const float corr = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= corr;
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) o.f[cb][0] *= corr;
+      sum = exponentials();
+    }
+    l += sum;
+  }
+
+  // All tiles of a wave, its own `mine` and those that only others need.
+  template <int ROLE>
+  __device__ __forceinline__ void walk(bool careful, lds_odd* odd) {
+    auto settle = [&](int t) {   // tile t of K and t - 1 of V have come; the next ones are asked for
+      wir::wait_vm_barrier<0>();
+      if (t + 1 < tiles) K.load(smem + (t + 1) % 2 * TK::BYTES, t + 1, wave);
+      if (t < tiles) V.load(smem + (2 + t % 2) * TK::BYTES, t, wave);
+      if (careful && t > 0) {
+        wir::clear_odd<false, NW, TV>(smem + (2 + (t - 1) % 2) * TK::BYTES, (t - 1) * TILE, odd);
+        wir::barrier();
       }
+    };
+    int t = 0;
+    if (mine > 0) {
+      settle(0);
+      stream<false, true>(0);
+      if (ROLE == 0) softmax(0);
+      for (t = 1; t < mine; ++t) {
+        settle(t);
+        if (ROLE == 1) softmax(t - 1);
+        stream<true, true>(t);
+        if (ROLE == 0) softmax(t);
+      }
+      settle(t);
+      if (ROLE == 1) softmax(t - 1);
+      stream<true, false>(t);
+      ++t;
+    }
+    for (; t <= tiles; ++t) settle(t);
   }
-  const auto O = wir::packed_head(a.out, a.oh, a.ot, head, r.start, r.len, D);
-  wir::store_tile_staged<true>(O, o, 0, 0, row0, 0, smem + wave * 32 * D * 2);
-  const int row = row0 + lane;
-  if (lane < 32 && row < r.len)
-    a.lse[head * a.lh + (i64)(r.start + row) * a.lt] = (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
-  return false;
+
+  // Returns whether a result is NaN the first time (only then may `careful` give another).
+  __device__ __forceinline__ bool run(int head0, bool careful) {
+    wave = wir::wave_id(), lane = wir::lane_id();
+    const int second = wave / 4, two = a.flags & 4;   // (the group)
+    head = head0 + (two ? second : 0);
+    row0 = r.row0 + wave % 4 * 32 + (two ? 0 : second * 128);
+    const int kv = head0 / a.group, end = CAUSAL ? min(r.len, r.row0 + (two ? 128 : 256)) : r.len;
+    tiles = (end + TILE - 1) / TILE;
+    // (in the careful pass all waves clear all tiles, and so none stays behind)
+    mine = row0 >= r.len ? 0 : CAUSAL ? min(tiles, (row0 + 31) / TILE + 1) : tiles;
+    K.init(a.k + kv * a.kh + r.start * a.kt, a.kt, r.len);
+    V.init(a.v + kv * a.vh + r.start * a.vt, a.vt, r.len);
+    const int part = lane % 16;   // of the transposed reads
+    row_at = wir::lds_addr(smem) + TK::chunk_off(lane % 32, lane / 32);
+    tr_at = wir::lds_addr(smem) + 2 * TK::BYTES + TV::elem_off(lane / 32 * 4 + part / 4, lane % 32 / 16 * 16 + 4 * (part % 4));
+    auto* odd = (lds_odd*)wir::lds(smem + ODD);
+    if (careful) wir::no_odd<false, NW>(odd);
+    K.load(smem, 0, wave);
+    wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
+    m = -__builtin_inff(), l = 0.f;
+    wir::fill(o, 0.f);
+    if (second == 0) walk<0>(careful, odd);
+    else walk<1>(careful, odd);
+    l = wir::lane_group_reduce<32>(l, wir::OpAdd());
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) o.f[cb][0] *= inv;
+    if (!careful) {   // an infinite or NaN value that not all of a tile's rows see
+      if (wir::any_wave(wir::has_nan(o, row0 + lane % 32 < r.len), smem + ODD)) return true;
+    } else {
+      wir::wait_vm_barrier<0>();   // the tiles are read: their LDS takes the output
+      const int row = CAUSAL ? row0 + lane % 32 : r.len - 1;   // the last position that the row sees
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
+          const bool nan = row >= odd->at[0][d], up = row >= odd->at[1][d], down = row >= odd->at[2][d];
+          const float x = o.f[cb][0][i];
+          o.f[cb][0][i] = nan || (up && down) ? __builtin_nanf("") : up ? x + __builtin_inff() : down ? x - __builtin_inff() : x;
+        }
+    }
+    const auto O = wir::packed_head(a.out, a.oh, a.ot, head, r.start, r.len, D);
+    wir::store_tile_staged<true>(O, o, 0, 0, row0, 0, smem + wave * 32 * D * 2);
+    const int row = row0 + lane;
+    if (lane < 32 && row < r.len)
+      a.lse[head * a.lh + (r.start + row) * a.lt] = (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    return false;
+  }
+};
+
+__device__ __forceinline__ void fill_rest(const fwd_args& a, const wir::Rows& r, int head, int d, int most) {
+  const int rows = min(r.len - r.row0, most);
+  bf16* out = a.out + head * a.oh + (i64)(r.start + r.row0) * a.ot;
+  if (a.flags & 1)
+    for (int i = threadIdx.x; i < rows * (d / 8); i += blockDim.x)
+      *(wir::bf16x8*)(out + i / (d / 8) * a.ot + i % (d / 8) * 8) = wir::bf16x8{};
+  if ((a.flags & 2) && (int)threadIdx.x < rows)
+    a.lse[head * a.lh + (r.start + r.row0 + (int)threadIdx.x) * a.lt] = -__builtin_inff();
 }
 
 template <int D, bool CAUSAL>
 __device__ __forceinline__ void forward(const fwd_args& a) {
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE * D * 2 + sizeof(wir::Odd<D>)];
+  __shared__ __attribute__((aligned(1024))) char smem[Forward<D, CAUSAL>::BYTES];
   int x, head;
-  wir::packed_program(a.blocks, a.heads, x, head);
+  const int two = a.flags & 4;
+  wir::packed_program(a.blocks, two ? a.heads / 2 : a.heads, x, head);
+  if (two) head *= 2;
   if (CAUSAL) x = a.blocks - 1 - x;   // a sequence's longest block first
-  const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
+  const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x, two ? 128 : 256);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
-  if (r.rest) return fill_rest(a, r, head, D);
+  if (r.rest) {
+    fill_rest(a, r, head, D, two ? 128 : 256);
+    if (two) fill_rest(a, r, head + 1, D, 128);
+    return;
+  }
+  Forward<D, CAUSAL> f(a, r, smem);
   bool careful = false;
-  while (forward_block<D, CAUSAL>(a, r, head, smem, careful)) careful = true;
+  while (f.run(head, careful)) careful = true;
 }
 
 }  // namespace
 
 #define PACKED_KERNEL(NAME, D, CAUSAL, WAVES_A_SIMD)                                                    \
-  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256),                      \
+  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(512, 512),                      \
                                             amdgpu_waves_per_eu(WAVES_A_SIMD, WAVES_A_SIMD)))           \
   NAME(const fwd_args args) { forward<D, CAUSAL>(args); }
 
-PACKED_KERNEL(wir_attn_packed_d64, 64, false, 3)
-PACKED_KERNEL(wir_attn_packed_d64_causal, 64, true, 3)
+PACKED_KERNEL(wir_attn_packed_d64, 64, false, 4)
+PACKED_KERNEL(wir_attn_packed_d64_causal, 64, true, 4)
 PACKED_KERNEL(wir_attn_packed_d128, 128, false, 2)
 PACKED_KERNEL(wir_attn_packed_d128_causal, 128, true, 2)

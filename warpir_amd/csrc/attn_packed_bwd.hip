@@ -45,19 +45,6 @@ __device__ __forceinline__ void zero_rest(bf16* x, i64 head_stride, i64 row_stri
     *(wir::bf16x8*)(x + i / (d / 8) * row_stride + i % (d / 8) * 8) = wir::bf16x8{};
 }
 
-// The workgroup's answer to "is there a NaN in a wave's results", after which the tiles' LDS is free.
-__device__ __forceinline__ bool any_wave(bool mine, char* flag_at) {
-  auto* flag = (__attribute__((address_space(3))) int*)wir::lds(flag_at);
-  wir::wait_vm_barrier<0>();
-  if (threadIdx.x == 0) *flag = 0;
-  wir::barrier();
-  if (mine) *flag = 1;
-  wir::barrier();
-  const bool any = *flag;
-  wir::barrier();
-  return any;
-}
-
 // dQ of one block of 128 query rows, 32 a wave.
 template <int D, int KT, bool CAUSAL>
 __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, int head, char* smem, bool careful) {
@@ -134,7 +121,7 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
     wir::mma_rAB<32, 32, KT, D, TK>(acc, ds, kt, 0);
   }
   if (!careful) {
-    if (any_wave(wir::has_nan(acc, row < r.len), smem + 4 * TK::BYTES)) return true;
+    if (wir::any_wave(wir::has_nan(acc, row < r.len), smem + 4 * TK::BYTES)) return true;
   } else {
     wir::wait_vm_barrier<0>();
   }
@@ -261,7 +248,7 @@ __device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r
   }
   if (!careful) {
     const bool in = row0 + lane % 32 < r.len, nan = wir::has_nan(dk, in) || wir::has_nan(dv, in);
-    if (any_wave(nan, smem + ODD)) return true;
+    if (wir::any_wave(nan, smem + ODD)) return true;
   } else {
     wir::wait_vm_barrier<0>();
   }
@@ -495,7 +482,7 @@ struct Paired {
     else walk<1>(now, now.head + a.group, careful, odd);
     const int row = row0 + lane % 32;
     if (!careful) {
-      if (any_wave(wir::has_nan(acc, row < r.len), smem + ODD)) return true;
+      if (wir::any_wave(wir::has_nan(acc, row < r.len), smem + ODD)) return true;
     } else {
       wir::wait_vm_barrier<0>();
     }

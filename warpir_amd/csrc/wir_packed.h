@@ -24,19 +24,19 @@ __device__ __forceinline__ int packed_offset(const int* offsets, int i, int batc
   return i > batch ? tokens : min(max(offsets[i], 0), tokens);
 }
 
-// Block x of all sequences' blocks of PACKED_ROWS rows.  Sequence i's blocks are
-// numbered from offsets[i] / PACKED_ROWS + i on: that leaves each at least as
-// many numbers as it has blocks, needs no sum over the sequences' blocks and no
-// length on the host; tokens / PACKED_ROWS + batch + 1 numbers hold all, the last
-// ones those of the tokens behind the last sequence (i = batch).  The lanes look
+// Block x of all sequences' blocks of `rows` rows (a power of two).  Sequence
+// i's blocks are numbered from offsets[i] / rows + i on: that leaves each at
+// least as many numbers as it has blocks, needs no sum over the sequences'
+// blocks and no length on the host; tokens / rows + batch + 1 numbers hold all,
+// the last ones those of the tokens behind the last sequence (i = batch).  The lanes look
 // at 64 sequences at a time: one round of loads up to 63 sequences, two up to 4095.
-__device__ __forceinline__ Rows packed_block(const int* offsets, int batch, int tokens, int x) {
+__device__ __forceinline__ Rows packed_block(const int* offsets, int batch, int tokens, int x, int rows = PACKED_ROWS) {
   const int lane = lane_id();
   int lo = 0, n = batch + 1;   // the sequence is one of lo .. lo + n - 1
   for (;;) {
     const int step = (n + 63) / 64, i = lo + lane * step;
     const int from = packed_offset(offsets, min(i, batch), batch, tokens);
-    const bool here = lane * step < n && from / PACKED_ROWS + i <= x;
+    const bool here = lane * step < n && from / rows + i <= x;
     const int last = max(63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(here) | 1), 0);
     if (step > 1) {
       lo += last * step;
@@ -48,7 +48,7 @@ __device__ __forceinline__ Rows packed_block(const int* offsets, int batch, int 
     r.start = __builtin_amdgcn_readlane(from, last);
     r.len = __builtin_amdgcn_readlane(to, last) - r.start;
     const int seq = lo + last;
-    r.row0 = (x - r.start / PACKED_ROWS - seq) * PACKED_ROWS;
+    r.row0 = (x - r.start / rows - seq) * rows;
     r.rest = seq == batch;
     return r;
   }
@@ -138,6 +138,19 @@ __device__ __forceinline__ bool has_nan(const RTile<MS, R, C>& t, bool in) {
 #pragma unroll
       for (int i = 0; i < MF<MS>::CREGS; ++i) any |= t.f[cb][rb][i] != t.f[cb][rb][i];
   return __builtin_amdgcn_ballot_w64(any && in) != 0;
+}
+
+// The workgroup's answer to "is there a NaN in a wave's results", after which the tiles' LDS is free.
+__device__ __forceinline__ bool any_wave(bool mine, char* flag_at) {
+  auto* flag = (__attribute__((address_space(3))) int*)lds(flag_at);
+  wait_vm_barrier<0>();
+  if (threadIdx.x == 0) *flag = 0;
+  barrier();
+  if (mine) *flag = 1;
+  barrier();
+  const bool any = *flag;
+  barrier();
+  return any;
 }
 
 // A product a @ b over a tile b (K rows, C columns) whose rows not all rows of

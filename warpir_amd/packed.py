@@ -27,7 +27,7 @@ class _GradArgs(ctypes.Structure):
 
 
 def _validate(fn, q, k, v, offsets, causal):
-    """(heads, key/value heads, tokens, D, batch, blocks, device)"""
+    """(heads, key/value heads, tokens, D, batch, device)"""
     import torch
 
     bf16, device = torch.bfloat16, getattr(q, "device", None)
@@ -48,9 +48,8 @@ def _validate(fn, q, k, v, offsets, causal):
     need(fn, tokens + batch <= INT_MAX - 2 * ROWS, "2^31 tokens or more in one call")
     for name, x in (("q", q), ("k", k), ("v", v)):
         need(fn, tokens < 2 or x.stride(1) < 1 << 23, f"{name}'s tokens are 2^23 elements or more apart")
-    blocks = tokens // ROWS + batch + 1
-    need(fn, blocks * heads < 1 << 24, "2^24 workgroups or more in one call")
-    return heads, shared, tokens, d, batch, blocks, device
+    need(fn, (tokens // ROWS + batch + 1) * heads < 1 << 23, "2^32 threads or more in one call")
+    return heads, shared, tokens, d, batch, device
 
 
 def _by_token(heads, tokens, d, device, rec):
@@ -87,7 +86,7 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
         done = _forward_plans.run(causal, q, k, v, offsets, out, lse)
         if done is not None and done is not False:
             return _results(given, done)
-    heads, shared, tokens, d, batch, blocks, device = _validate(fn, q, k, v, offsets, causal)
+    heads, shared, tokens, d, batch, device = _validate(fn, q, k, v, offsets, causal)
     rec = _forward_plans.recording(done, q, k, v, offsets, out, lse)
     flags = (1 if out is None else 0) | (2 if lse is None else 0)
     if out is not None:
@@ -102,10 +101,13 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
         lse = rec.alloc(torch.empty(heads, tokens, dtype=torch.float32, device=device))
     if tokens == 0:
         return _results(given, (out, lse))
+    # a workgroup's 256 rows: 128 each of two heads that share keys and values, or of one head
+    two = heads // shared % 2 == 0
+    blocks = tokens // (128 if two else 256) + batch + 1
     args = _Args(*[None] * 6, *(s for x in (q, k, v, out) for s in x.stride()[:2]), *lse.stride(), batch, tokens, heads,
-                 heads // shared, blocks, flags)
+                 heads // shared, blocks, flags | (4 if two else 0))
     launch(rec, device, "attn_packed.hsaco", f"wir_attn_packed_d{d}" + ("_causal" if causal else ""),
-           (blocks * heads, 1, 1), (256, 1, 1), args,
+           (blocks * (heads // 2 if two else heads), 1, 1), (512, 1, 1), args,
            {"q": q, "k": k, "v": v, "out": out, "lse": lse, "offsets": offsets})
     if rec:
         _forward_plans.add(causal, rec, out, lse)
@@ -148,7 +150,7 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
         done = _backward_plans.run(causal, *tensors)
         if done is not None and done is not False:
             return _results(given, done)
-    heads, shared, tokens, d, batch, blocks, device = _validate(fn, q, k, v, offsets, causal)
+    heads, shared, tokens, d, batch, device = _validate(fn, q, k, v, offsets, causal)
     for name, x in (("o", o), ("do", do)):
         check_tensor(fn, name, x, torch.bfloat16, q.shape, device)
     need(fn, tokens < 2 or do.stride(1) < 1 << 23, "do's tokens are 2^23 elements or more apart")
@@ -171,6 +173,7 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
         workspace = rec.alloc(torch.empty(floats, dtype=torch.float32, device=device))
     if tokens == 0:
         return _results(given, tuple(grads))
+    blocks = tokens // ROWS + batch + 1
     args = _GradArgs(*[None] * 11, *(s for x in (q, k, v, o, do, lse, *grads) for s in x.stride()[:2]), batch, tokens, heads,
                      heads // shared, blocks, flags)
     names = {"q": q, "k": k, "v": v, "o": o, "d_o": do, "lse": lse, "offsets": offsets, "dq": grads[0], "dk": grads[1],
