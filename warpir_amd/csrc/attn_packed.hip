@@ -30,17 +30,18 @@ struct Scale {
   static constexpr float c = (float)(1.4426950408889634 * inv_sqrt);
 };
 
-// A workgroup: two groups of four waves, 32 query rows a wave.  The groups take
-// 128 rows each, of two heads that share a key/value head where there are two
-// (flags & 4), or else one behind the other, and the same tiles of 64 keys.
-// Waves w and w + 4 are on one SIMD and work in opposite phases: in the time of
-// one tile t either takes the products of P(t - 1) with V(t - 1) and of Q with
-// K(t), and a softmax, the first group that of t behind them, the second that
-// of t - 1 before, so that one's matrix instructions run under the other's
-// exponentials.
-template <int D, bool CAUSAL>
+// A workgroup: a group of four waves, 32 query rows a wave, that share tiles of
+// 64 keys; in the time of one tile t a wave takes the products of P(t - 1) with
+// V(t - 1) and of Q with K(t), and the softmax of t.
+//
+// NW = 8: two such groups with the same tiles, of two heads that share a
+// key/value head where there are two (flags & 4), or else of 128 rows each one
+// behind the other.  Waves w and w + 4 are on one SIMD and work in opposite
+// phases, the second group's softmax is that of t - 1 before its products, so
+// that one's matrix instructions run under the other's exponentials.
+template <int D, bool CAUSAL, int NW>
 struct Forward {
-  static constexpr int NW = 8, TILE = 64, AHEAD = D == 128 ? 5 : 3, KS = D / 16, CB = D / 32;
+  static constexpr int TILE = 64, AHEAD = 5, KS = D / 16, CB = D / 32;
   static constexpr int SCORES = 2 * KS, PRODUCTS = TILE / 16 * CB;   // products of a wave for a tile
   typedef wir::STile<TILE, D, wir::ROWREAD> TK;
   typedef wir::STile<TILE, D, wir::TRREAD> TV;
@@ -186,7 +187,7 @@ struct Forward {
   // Returns whether a result is NaN the first time (only then may `careful` give another).
   __device__ __forceinline__ bool run(int head0, bool careful) {
     wave = wir::wave_id(), lane = wir::lane_id();
-    const int second = wave / 4, two = a.flags & 4;   // (the group)
+    const int second = wave / 4, two = NW == 4 || a.flags & 4;   // (the group; NW = 4: there is one)
     head = head0 + (two ? second : 0);
     row0 = r.row0 + wave % 4 * 32 + (two ? 0 : second * 128);
     const int kv = head0 / a.group, end = CAUSAL ? min(r.len, r.row0 + (two ? 128 : 256)) : r.len;
@@ -204,7 +205,7 @@ struct Forward {
     wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
     m = -__builtin_inff(), l = 0.f;
     wir::fill(o, 0.f);
-    if (second == 0) walk<0>(careful, odd);
+    if (NW == 4 || second == 0) walk<0>(careful, odd);
     else walk<1>(careful, odd);
     l = wir::lane_group_reduce<32>(l, wir::OpAdd());
     const float inv = 1.0f / l;
@@ -244,34 +245,36 @@ __device__ __forceinline__ void fill_rest(const fwd_args& a, const wir::Rows& r,
     a.lse[head * a.lh + (r.start + r.row0 + (int)threadIdx.x) * a.lt] = -__builtin_inff();
 }
 
-template <int D, bool CAUSAL>
+template <int D, bool CAUSAL, int NW>
 __device__ __forceinline__ void forward(const fwd_args& a) {
-  __shared__ __attribute__((aligned(1024))) char smem[Forward<D, CAUSAL>::BYTES];
+  __shared__ __attribute__((aligned(1024))) char smem[Forward<D, CAUSAL, NW>::BYTES];
   int x, head;
-  const int two = a.flags & 4;
+  const int two = NW == 8 && a.flags & 4, rows = NW == 4 || two ? 128 : 256;
   wir::packed_program(a.blocks, two ? a.heads / 2 : a.heads, x, head);
   if (two) head *= 2;
   if (CAUSAL) x = a.blocks - 1 - x;   // a sequence's longest block first
-  const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x, two ? 128 : 256);
+  const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x, rows);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
   if (r.rest) {
-    fill_rest(a, r, head, D, two ? 128 : 256);
+    fill_rest(a, r, head, D, rows);
     if (two) fill_rest(a, r, head + 1, D, 128);
     return;
   }
-  Forward<D, CAUSAL> f(a, r, smem);
+  Forward<D, CAUSAL, NW> f(a, r, smem);
   bool careful = false;
   while (f.run(head, careful)) careful = true;
 }
 
 }  // namespace
 
-#define PACKED_KERNEL(NAME, D, CAUSAL, WAVES_A_SIMD)                                                    \
-  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(512, 512),                      \
+#define PACKED_KERNEL(NAME, D, CAUSAL, NW, WAVES_A_SIMD)                                                \
+  extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64 * NW, 64 * NW),              \
                                             amdgpu_waves_per_eu(WAVES_A_SIMD, WAVES_A_SIMD)))           \
-  NAME(const fwd_args args) { forward<D, CAUSAL>(args); }
+  NAME(const fwd_args args) { forward<D, CAUSAL, NW>(args); }
 
-PACKED_KERNEL(wir_attn_packed_d64, 64, false, 4)
-PACKED_KERNEL(wir_attn_packed_d64_causal, 64, true, 4)
-PACKED_KERNEL(wir_attn_packed_d128, 128, false, 2)
-PACKED_KERNEL(wir_attn_packed_d128_causal, 128, true, 2)
+PACKED_KERNEL(wir_attn_packed_d64, 64, false, 4, 3)
+PACKED_KERNEL(wir_attn_packed_d64_causal, 64, true, 4, 3)
+PACKED_KERNEL(wir_attn_packed_d128, 128, false, 4, 2)
+PACKED_KERNEL(wir_attn_packed_d128_causal, 128, true, 4, 2)
+PACKED_KERNEL(wir_attn_packed_d128_w8, 128, false, 8, 2)
+PACKED_KERNEL(wir_attn_packed_d128_w8_causal, 128, true, 8, 2)

@@ -36,6 +36,7 @@ __device__ __forceinline__ Rows packed_block(const int* offsets, int batch, int 
   for (;;) {
     const int step = (n + 63) / 64, i = lo + lane * step;
     const int from = packed_offset(offsets, min(i, batch), batch, tokens);
+    const int to = packed_offset(offsets, min(i, batch) + 1, batch, tokens);
     const bool here = lane * step < n && from / rows + i <= x;
     const int last = max(63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(here) | 1), 0);
     if (step > 1) {
@@ -43,7 +44,6 @@ __device__ __forceinline__ Rows packed_block(const int* offsets, int batch, int 
       n = min(step, n - last * step);
       continue;
     }
-    const int to = packed_offset(offsets, min(i, batch) + 1, batch, tokens);
     Rows r;
     r.start = __builtin_amdgcn_readlane(from, last);
     r.len = __builtin_amdgcn_readlane(to, last) - r.start;

@@ -101,17 +101,30 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
         lse = rec.alloc(torch.empty(heads, tokens, dtype=torch.float32, device=device))
     if tokens == 0:
         return _results(given, (out, lse))
-    # a workgroup's 256 rows: 128 each of two heads that share keys and values, or of one head
-    two = heads // shared % 2 == 0
-    blocks = tokens // (128 if two else 256) + batch + 1
+    waves, two = _forward_form(heads // shared, tokens, batch, d)
+    blocks = tokens // (256 if waves == 8 and not two else 128) + batch + 1
     args = _Args(*[None] * 6, *(s for x in (q, k, v, out) for s in x.stride()[:2]), *lse.stride(), batch, tokens, heads,
                  heads // shared, blocks, flags | (4 if two else 0))
-    launch(rec, device, "attn_packed.hsaco", f"wir_attn_packed_d{d}" + ("_causal" if causal else ""),
-           (blocks * (heads // 2 if two else heads), 1, 1), (512, 1, 1), args,
+    launch(rec, device, "attn_packed.hsaco", f"wir_attn_packed_d{d}" + ("_w8" if waves == 8 else "") + ("_causal" if causal else ""),
+           (blocks * (heads // 2 if two else heads), 1, 1), (64 * waves, 1, 1), args,
            {"q": q, "k": k, "v": v, "out": out, "lse": lse, "offsets": offsets})
     if rec:
         _forward_plans.add(causal, rec, out, lse)
     return _results(given, (out, lse))
+
+
+def _forward_form(group: int, tokens: int, batch: int, d: int) -> Tuple[int, bool]:
+    """(waves of a workgroup, whether it takes two heads) of the forward.  Eight
+    waves are two groups of four with the same tiles: two heads that share keys
+    and values, or 256 rows of one head.  They pay at D = 128 in long sequences;
+    the lengths are on the GPU, so their average decides.  us, four / eight waves,
+    batches of 32768 tokens in sequences of 128, 256, 512, 1024, 2048, 4096:
+    32/8 heads, not causal 290 / 327, 240 / 257, 359 / 334, 558 / 532, 976 / 949, 1840
+    / 1750; causal 284 / 338, 208 / 225, 260 / 263, 368 / 371, 589 / 587, 1024 / 992;
+    16/16 heads, not causal 170 / 157, 139 / 213, 192 / 200, 283 / 285, 506 / 494, 932 / 893."""
+    average = tokens / max(batch, 1)
+    two = group % 2 == 0
+    return (8, two) if d == 128 and average >= (512 if two else 2048) else (4, False)
 
 
 def _results(given, done):
