@@ -13,7 +13,7 @@ using wir::bf16;
 using wir::bf16x8;
 
 typedef long long i64;
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
@@ -151,15 +151,75 @@ __device__ __forceinline__ i32x16 mma(bf16x8 a, bf16x8 b, i32x16 c) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
-// Output tiles of BM x BN, a wave's part WM x WN.
-template <int BM, int BN, int WM, int WN>
+// float(acc) * a_scale * b_scale of four columns that follow one another
+__device__ __forceinline__ f32x4 scales_at(const float* s, int at, int n) {
+  f32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = s[min(at + i, n - 1)];
+  return v;
+}
+
+// A wave's part of the output by way of `stage` in LDS, V values a store, the lanes next to one another.
+template <int V, int R, int C>
+__device__ __forceinline__ void store_narrow(const gemm_args& g, const wir::RTile<32, R, C>& t, int row0, int col0, char* stage) {
+  typedef bf16 vec __attribute__((ext_vector_type(V)));
+  typedef __attribute__((address_space(3))) vec lds_vec;
+  typedef __attribute__((address_space(3))) wir::bf16x4 lds_bf16x4;
+  constexpr int PITCH = C + 4, EACH = C / V;   // (rows are two banks apart)
+  auto* s = (__attribute__((address_space(3))) bf16*)wir::lds(stage);
+  const int lane = wir::lane_id(), lr = lane % 32, lh = lane / 32;
+#pragma unroll
+  for (int rb = 0; rb < R / 32; ++rb) {
+#pragma unroll
+    for (int cb = 0; cb < C / 32; ++cb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        wir::bf16x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (bf16)t.f[cb][rb][4 * q + i];
+        *(lds_bf16x4*)(s + lr * PITCH + cb * 32 + wir::ccol<32>(4 * q, lh)) = v;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int it = 0; it < 32 * EACH / 64; ++it) {
+      const int i = it * 64 + lane, row = row0 + rb * 32 + i / EACH, col = col0 + i % EACH * V;
+      const vec v = *(lds_vec*)(s + i / EACH * PITCH + i % EACH * V);
+      if (row < g.m && col < g.n) *(vec*)(g.out + (i64)row * g.os + col) = v;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// In the widest stores that the output's rows and the number of columns are whole multiples of.
+template <int R, int C>
+__device__ __forceinline__ void store_rows(const gemm_args& g, const wir::RTile<32, R, C>& t, int row0, int col0, char* stage) {
+  const int whole = g.n | (int)g.os | (int)((size_t)g.out >> 1);   // (in values)
+  if (((int)g.os | (int)((size_t)g.out >> 1)) % 8 == 0)
+    wir::store_tile_staged<true>(wir::gl<bf16>{g.out, 1, 1, g.m, g.n, 0, 0, g.os}, t, 0, 0, row0, col0, stage);
+  else if (whole % 4 == 0)
+    store_narrow<4>(g, t, row0, col0, stage);
+  else if (whole % 2 == 0)
+    store_narrow<2>(g, t, row0, col0, stage);
+  else
+    store_narrow<1>(g, t, row0, col0, stage);
+}
+
+// Output tiles of BM x BN, a wave's part WM x WN, over a ring of S tiles of 128
+// bytes of each row.
+//
+// WHOLE: a wave's operands of the next tile are read while this one's products
+// run, from registers.  Without (parts whose operands do not fit twice): a
+// quarter of a tile ahead, and the last quarter's products run behind the
+// barrier that the next tile needs, under the reads of its first operands.
+template <int BM, int BN, int WM, int WN, int S, bool WHOLE>
 __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
   constexpr int NW = BM / WM * (BN / WN), RB = WM / 32, CB = WN / 32;
   typedef Codes<BM, NW> CA;
   typedef Codes<BN, NW> CBt;
-  constexpr int SLOT = CA::T::BYTES + CBt::T::BYTES;
-  static_assert(NW * WM * WN * 2 <= 2 * SLOT, "the output goes through the tiles' LDS");
-  __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+  constexpr int SLOT = CA::T::BYTES + CBt::T::BYTES, EACH = CA::EACH + CBt::EACH;
+  constexpr int STAGE = (WM * WN > 32 * (WN + 4) ? WM * WN : 32 * (WN + 4)) * 2;   // bytes of a wave's output on its way
+  static_assert(NW * STAGE <= S * SLOT, "the output goes through the tiles' LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[S * SLOT];
   const int nx = (g.n + BN - 1) / BN, ny = (g.m + BM - 1) / BM;
   int x, y;
   wir::grouped_tile<8>(wir::remap_xcd(blockIdx.x, nx * ny), nx, ny, x, y);
@@ -170,8 +230,8 @@ __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
   a.init(g.a, g.as, y * BM, g.m, wave);
   b.init(g.b, g.bs, x * BN, g.n, wave);
   const int steps = (g.k + 127) / 128;
-  auto load = [&](int t) {
-    char* at = smem + t % 2 * SLOT;
+  auto load = [&](int t, int slot) {
+    char* at = smem + slot * SLOT;
     a.load(at, t * 128, g.k, wave);
     b.load(at + CA::T::BYTES, t * 128, g.k, wave);
   };
@@ -180,41 +240,176 @@ __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
   for (int c = 0; c < CB; ++c)
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[c][r] = i32x16{};
-  load(0);
-  for (int t = 0; t < steps; ++t) {
-    char *at = smem + t % 2 * SLOT, *bt = at + CA::T::BYTES;
-    wir::wait_vm_barrier<0>();
-    if (t + 1 < steps) load(t + 1);
+  constexpr int SETS = WHOLE ? 8 : 2;
+  bf16x8 fa[SETS][RB], fb[SETS][CB];
+  // (the swizzle repeats every 16 rows: a step along the row is an exclusive or, blocks of 32 rows are offsets)
+  const unsigned a_at = wir::lds_addr(smem) + CA::T::chunk_off(row0 + lane % 32, lane / 32);
+  const unsigned b_at = wir::lds_addr(smem) + CA::T::BYTES + CBt::T::chunk_off(col0 + lane % 32, lane / 32);
+  typedef __attribute__((address_space(3))) bf16x8 lds_bf16x8;
+  auto read = [&](int slot, int ks, int set) {
+    const unsigned at = (a_at ^ ks * 32) + slot * SLOT, bt = (b_at ^ ks * 32) + slot * SLOT;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      bf16x8 fa[RB], fb[CB];
+    for (int r = 0; r < RB; ++r) fa[set][r] = *(lds_bf16x8*)(at + r * 32 * 128);
 #pragma unroll
-      for (int r = 0; r < RB; ++r) fa[r] = wir::row_operand<typename CA::T, 32>(at, row0 + r * 32, ks);
+    for (int c = 0; c < CB; ++c) fb[set][c] = *(lds_bf16x8*)(bt + c * 32 * 128);
+  };
+  auto products = [&](int set) {
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int c = 0; c < CB; ++c) fb[c] = wir::row_operand<typename CBt::T, 32>(bt, col0 + c * 32, ks);
+    for (int c = 0; c < CB; ++c)
 #pragma unroll
-      for (int c = 0; c < CB; ++c)
+      for (int r = 0; r < RB; ++r) acc[c][r] = mma(fb[set][c], fa[set][r], acc[c][r]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  // Tile t + 1 has come, t + 2 .. t + S - 1 may be on their way; nobody reads tile t's slot any more: t + S goes there.
+  auto settle = [&](int t, int slot) {
+    if (t + S <= steps) wir::wait_vm_barrier<(S - 2) * EACH>();
+    else wir::wait_vm_barrier<0>();
+    if (t + S < steps) load(t + S, slot);
+  };
 #pragma unroll
-        for (int r = 0; r < RB; ++r) acc[c][r] = mma(fb[c], fa[r], acc[c][r]);
+  for (int t = 0; t < S; ++t)
+    if (t < steps) load(t, t);
+  if (steps >= S) wir::wait_vm_barrier<(S - 1) * EACH>();
+  else wir::wait_vm_barrier<0>();
+  int slot = 0;
+  if (WHOLE) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) read(0, ks, ks);
+    auto step = [&](int t, int set) {
+      const int next = slot == S - 1 ? 0 : slot + 1;
+      settle(t, slot);
+      if (t + 1 < steps) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) read(next, ks, (4 - set) + ks);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) products(set + ks);
+      __builtin_amdgcn_sched_barrier(0);
+      slot = next;
+    };
+    int t = 0;
+    for (; t + 2 <= steps; t += 2) {
+      step(t, 0);
+      step(t + 1, 4);
+    }
+    if (t < steps) step(t, 0);
+  } else {
+    read(0, 0, 0);
+    for (int t = 0; t < steps; ++t) {
+      const int next = slot == S - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int ks = 0; ks < 3; ++ks) {
+        read(slot, ks + 1, (ks + 1) % 2);
+        __builtin_amdgcn_sched_barrier(0);
+        products(ks % 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(t, slot);
+      if (t + 1 < steps) read(next, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      products(1);
+      __builtin_amdgcn_sched_barrier(0);
+      slot = next;
     }
   }
-  wir::wait_vm_barrier<0>();
+  if (WHOLE) wir::barrier();   // (the last tile's reads: the LDS takes the output)
   // a lane holds row lane % 32 of each block of rows, 16 columns of each block of columns
   const int lh = lane / 32;
   wir::RTile<32, WM, WN> out;
 #pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const float sa = g.a_scale[min(y * BM + row0 + r * 32 + lane % 32, g.m - 1)];
+  for (int c = 0; c < CB; ++c)
 #pragma unroll
-    for (int c = 0; c < CB; ++c)
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 sb = scales_at(g.b_scale, x * BN + col0 + c * 32 + wir::ccol<32>(4 * q, lh), g.n);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float sb = g.b_scale[min(x * BN + col0 + c * 32 + wir::ccol<32>(i, lh), g.n - 1)];
-        out.f[c][r][i] = (float)acc[c][r][i] * sa * sb;
+      for (int r = 0; r < RB; ++r) {
+        const float sa = g.a_scale[min(y * BM + row0 + r * 32 + lane % 32, g.m - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out.f[c][r][4 * q + i] = (float)acc[c][r][4 * q + i] * sa * sb[i];
       }
+    }
+  store_rows(g, out, y * BM + row0, x * BN + col0, smem + wave * STAGE);
+}
+
+// Few tokens, M <= 16 MT: a workgroup takes CH channels, its W waves every W-th
+// 128 bytes of their rows and of the tokens' (each through a ring of S tiles of
+// its own in LDS, without a barrier), and the waves' sums are added at the end.
+template <int MT, int CH, int W, int S>
+__device__ __forceinline__ void gemm_few(const gemm_args& g) {
+  constexpr int CT = (CH + 15) / 16;
+  typedef Codes<CH, 1> CB;
+  typedef Codes<16 * MT, 1> CA;
+  typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
+  typedef __attribute__((address_space(3))) int lds_int;
+  constexpr int SLOT = CB::T::BYTES + CA::T::BYTES, EACH = CB::EACH + CA::EACH, SUMS = CT * MT * 1024;
+  static_assert(CT * 16 * 128 <= SLOT && SUMS <= S * SLOT, "operands of channels past CH are read, and dropped");
+  __shared__ __attribute__((aligned(1024))) char smem[W * S * SLOT];
+  const int wave = wir::wave_id(), lane = wir::lane_id();
+  const int channel0 = wir::remap_xcd(blockIdx.x, gridDim.x) * CH;
+  char* own = smem + wave * S * SLOT;
+  CB b;
+  CA a;
+  b.init(g.b, g.bs, channel0, g.n, 0);
+  a.init(g.a, g.as, 0, g.m, 0);
+  const int steps = (g.k + 127) / 128, mine = steps > wave ? (steps - wave + W - 1) / W : 0;
+  auto load = [&](int t, int slot) {
+    const int k = (wave + t * W) * 128;
+    b.load(own + slot * SLOT, k, g.k, 0);
+    a.load(own + slot * SLOT + CB::T::BYTES, k, g.k, 0);
+  };
+  i32x4 acc[CT][MT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[c][i] = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t)
+    if (t < mine) load(t, t);
+  // the lane's 16 bytes of a 16 x 64 operand (the swizzle repeats every 16 rows)
+  const unsigned b_at = wir::lds_addr(own) + CB::T::chunk_off(lane % 16, lane / 16);
+  const unsigned a_at = wir::lds_addr(own) + CB::T::BYTES + CA::T::chunk_off(lane % 16, lane / 16);
+  int slot = 0;
+  for (int t = 0; t < mine; ++t) {
+    // (the slot that is loaded now was read in the step before: those reads have returned)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + S - 1 < mine) {
+      load(t + S - 1, slot == 0 ? S - 1 : slot - 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * EACH) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i32x4 fb[CT], fa[MT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) fb[c] = *(lds_i32x4*)((b_at ^ h * 64) + slot * SLOT + c * 2048);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fa[i] = *(lds_i32x4*)((a_at ^ h * 64) + slot * SLOT + i * 2048);
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[c][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[c], fa[i], acc[c][i], 0, 0, 0);
+    }
+    slot = slot == S - 1 ? 0 : slot + 1;
   }
-  wir::store_tile_staged<true>(wir::gl<bf16>{g.out, 1, 1, g.m, g.n, 0, 0, g.os}, out, 0, 0, y * BM + row0, x * BN + col0,
-                               smem + wave * WM * WN * 2);
+  // a lane holds token lane % 16, channels 4 (lane / 16) .. + 3
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *((lds_i32x4*)wir::lds(own + (c * MT + i) * 1024) + lane) = acc[c][i];
+  wir::barrier();
+  for (int i = threadIdx.x; i < CT * MT * 256; i += 64 * W) {
+    const int token = i / (16 * CT), channel = i % (16 * CT), n = channel0 + channel;
+    if (token >= g.m || channel >= CH || n >= g.n) continue;
+    const int tile = channel / 16 * MT + token / 16, at = (channel % 16 / 4 * 16 + token % 16) * 4 + channel % 4;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += *((lds_int*)wir::lds(smem + w * S * SLOT + tile * 1024) + at);
+    g.out[token * g.os + n] = (bf16)((float)sum * g.a_scale[token] * g.b_scale[n]);
+  }
 }
 
 }  // namespace
@@ -232,6 +427,22 @@ QUANTIZE_KERNEL(wir_quantize_int8_w4_n4, 4, 4)
                                             amdgpu_waves_per_eu(WAVES_A_SIMD, WAVES_A_SIMD)))           \
   NAME(const gemm_args args) { gemm_tiled<__VA_ARGS__>(args); }
 
-GEMM_KERNEL(wir_gemm_int8_256, 256, 1, 256, 256, 128, 128)
-GEMM_KERNEL(wir_gemm_int8_128, 256, 2, 128, 128, 64, 64)
-GEMM_KERNEL(wir_gemm_int8_64, 256, 2, 64, 64, 32, 32)
+GEMM_KERNEL(wir_gemm_int8_256, 512, 2, 256, 256, 128, 64, 2, false)
+GEMM_KERNEL(wir_gemm_int8_256x128, 512, 2, 256, 128, 64, 64, 3, true)
+GEMM_KERNEL(wir_gemm_int8_128_w4, 256, 2, 128, 128, 64, 64, 2, false)
+GEMM_KERNEL(wir_gemm_int8_128, 512, 2, 128, 128, 64, 32, 3, true)
+GEMM_KERNEL(wir_gemm_int8_128x64, 256, 2, 128, 64, 64, 32, 3, true)
+GEMM_KERNEL(wir_gemm_int8_64, 256, 2, 64, 64, 32, 32, 4, true)
+
+#define FEW_KERNEL(NAME, MT, CH, W, S) \
+  extern "C" __global__ void __launch_bounds__(64 * W) NAME(const gemm_args args) { gemm_few<MT, CH, W, S>(args); }
+
+FEW_KERNEL(wir_gemm_int8_few16_c16, 1, 16, 8, 4)
+FEW_KERNEL(wir_gemm_int8_few16_c24, 1, 24, 8, 4)
+FEW_KERNEL(wir_gemm_int8_few16_c32, 1, 32, 8, 2)
+FEW_KERNEL(wir_gemm_int8_few16_c64, 1, 64, 8, 2)
+FEW_KERNEL(wir_gemm_int8_few32_c16, 2, 16, 8, 3)
+FEW_KERNEL(wir_gemm_int8_few32_c24, 2, 24, 8, 2)
+FEW_KERNEL(wir_gemm_int8_few32_c32, 2, 32, 4, 2)
+FEW_KERNEL(wir_gemm_int8_few64_c16, 4, 16, 4, 3)
+FEW_KERNEL(wir_gemm_int8_few64_c32, 4, 32, 4, 3)

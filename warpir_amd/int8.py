@@ -3,6 +3,7 @@ matrices of them (``csrc/gemm_int8.hip``)."""
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Tuple
 
 from warpir_amd.handwritten import DevicePlans, apart, check_tensor, check_written, launch, need
@@ -112,10 +113,10 @@ def gemm_int8(a, b, a_scale, b_scale, out=None):
         return out
     if k == 0:
         return out.zero_()
-    variant, tile = _gemm_form(m, n, k)
-    programs = -(-m // tile) * -(-n // tile)
-    need(fn, programs < 1 << 24, "2^24 workgroups or more in one call")
-    launch(rec, device, "gemm_int8.hsaco", f"wir_gemm_int8_{variant}", (programs, 1, 1), (256, 1, 1),
+    variant, bm, bn, threads = _gemm_form(m, n, k)
+    programs = -(-m // bm) * -(-n // bn)
+    need(fn, programs * threads < 1 << 32, "2^32 threads or more in one call")
+    launch(rec, device, "gemm_int8.hsaco", f"wir_gemm_int8_{variant}", (programs, 1, 1), (threads, 1, 1),
            _Args(*[None] * 5, _pitch(a), _pitch(b), _pitch(out), m, n, k),
            {"a": a, "b": b, "a_scale": a_scale, "b_scale": b_scale, "out": out})
     if rec:
@@ -123,11 +124,52 @@ def gemm_int8(a, b, a_scale, b_scale, out=None):
     return out
 
 
-def _gemm_form(m: int, n: int, k: int):
-    for tile in (256, 128):
-        if -(-m // tile) * -(-n // tile) >= 256:
-            return str(tile), tile
-    return "64", 64
+# Tiles: rows and columns of a workgroup's output, its threads, how many workgroups a CU holds, and the time of a product
+# in microseconds: fixed + per_m * M N / 1e6 + steps of 128 along K * step, where a launch of P programs on 256 CUs, R
+# rounds of them and a rest r (of 1), has
+#   step = light + busy * r                                  R = 0, or one whole round
+#        = full * R, plus the same line from light to full for the rest.
+# Least-squares fits (rms 5-9% in log time) to 43 products from 65 x 640 x 1680 to 8192 x 7816 x 7648; the tile with the
+# smallest estimate was within 1.3% (geometric mean; 17% at worst) of the fastest.
+_TILES = {
+    "256": (256, 256, 512, 1, (8.55, 1.448, 0.194, 2.027, 0.416)),
+    "256x128": (256, 128, 512, 1, (5.67, 0.937, 0.0, 1.133, 0.551)),
+    "128_w4": (128, 128, 256, 2, (4.97, 0.692, 0.399, 1.196, 0.443)),
+    "128": (128, 128, 512, 1, (3.82, 0.613, 0.0, 0.677, 0.684)),
+    "128x64": (128, 64, 256, 2, (3.89, 0.488, 0.260, 0.810, 0.511)),
+    "64": (64, 64, 256, 2, (3.65, 0.324, 0.203, 0.526, 0.696)),
+}
+
+
+def _estimate(tile: str, m: int, n: int, k: int) -> float:
+    bm, bn, _, held, (fixed, light, busy, full, per_mn) = _TILES[tile]
+    rounds, rest = divmod(-(-m // bm) * -(-n // bn), 256 * held)
+    rest /= 256 * held
+    if rounds == 0 or (rounds == 1 and rest == 0):
+        step = light + busy * (rounds + rest)
+    else:
+        step = full * rounds + (light + (full - light) * rest if rest else 0.0)
+    return fixed + -(-k // 128) * step + per_mn * 1e-6 * m * n
+
+
+@functools.lru_cache(maxsize=1024)
+def _gemm_form(m: int, n: int, k: int) -> Tuple[str, int, int, int]:
+    """(kernel, rows and columns of a workgroup's output, its threads).
+
+    Up to 64 tokens the weight's bytes count, and the tokens' that every
+    workgroup reads again: each takes 16 to 64 channels, so that as many as 256
+    CUs have one, and its waves divide K.  us, 16 / 24 / 32 / 64 channels a
+    workgroup, 16 tokens: N = 4096, K = 4096 6.2 / 6.6 / 6.7 / 8.8, 6144 x 4096 8.8 / 7.4 /
+    7.8 / 9.3, 8192 x 8192 16.1 / 18.3 / 13.6 / 16.9, 32768 x 4096 36.8 / 35.0 / 33.3 / 29.5 (64 x 64
+    tiles 14.8, 15.1, 27.2, 31.9); 64 tokens, 16 / 32 channels: 4096 x 4096 8.4 / 10.0, 8192 x 8192
+    25.3 / 19.1 (tiles 15.4, 27.2)."""
+    if m <= 64:
+        rows = 16 if m <= 16 else 32 if m <= 32 else 64
+        columns = 16 if n <= 4096 else 24 if n <= 6144 and rows < 64 else 64 if n >= 16384 and rows == 16 else 32
+        waves = 4 if rows == 64 or (rows, columns) == (32, 32) else 8
+        return f"few{rows}_c{columns}", rows, columns, 64 * waves
+    tile = min(_TILES, key=lambda t: _estimate(t, m, n, k))
+    return (tile, *_TILES[tile][:3])
 
 
 __all__ = ["quantize_int8", "gemm_int8"]
