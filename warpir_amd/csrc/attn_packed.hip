@@ -5,30 +5,12 @@
 // products (bf16):
 //   s_j = q_p . k_j / sqrt(D) for j <= p (causal) or every j of the sequence,
 //   O_p = sum_j softmax(s)_j v_j,  LSE_p = ln sum_j exp s_j.
-#include "wir_packed.h"
+#include "wir_packed_args.h"
 
 namespace {
 
 using wir::bf16;
 using wir::i64;
-
-struct fwd_args {
-  const bf16* q;       // [H, T, D]
-  const bf16* k;       // [H_kv, T, D]
-  const bf16* v;
-  bf16* out;           // [H, T, D]
-  float* lse;          // [H, T]
-  const int* offsets;  // [batch + 1]
-  i64 qh, qt, kh, kt, vh, vt, oh, ot, lh, lt;
-  int batch, tokens, heads, group, blocks;
-  int flags;           // 1: rows behind the last sequence become 0 in out, 2: -inf in lse, 4: two heads a workgroup
-};
-
-template <int D>
-struct Scale {
-  static constexpr double inv_sqrt = D == 64 ? 0.125 : 0.08838834764831845;
-  static constexpr float c = (float)(1.4426950408889634 * inv_sqrt);
-};
 
 // A workgroup: a group of four waves, 32 query rows a wave, that share tiles of
 // 64 keys; in the time of one tile t a wave takes the products of P(t - 1) with
@@ -52,7 +34,7 @@ struct Forward {
   // A row's probabilities are 2^(c s - m), m within 2^16 of its largest score so far: a sum past that asks for a new m.
   static constexpr float LIMIT = 65536.f;
 
-  const fwd_args& a;
+  const wir::packed_fwd_args& a;
   const wir::Rows& r;
   char* smem;
   int wave, lane, head, row0, tiles, mine;
@@ -65,7 +47,7 @@ struct Forward {
   wir::BTile<32, 32, TILE> p;
   float m, l;                      // l: of the lane's half of the columns
 
-  __device__ __forceinline__ Forward(const fwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
+  __device__ __forceinline__ Forward(const wir::packed_fwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
 
   __device__ __forceinline__ wir::bf16x8 score_operand(unsigned at, int i) const {
     return *(lds_bf16x8*)((at ^ (i / 2 * 32)) + i % 2 * 32 * D * 2);
@@ -111,7 +93,7 @@ struct Forward {
 
   // p and the lane's sum of it, with m as it is.
   __device__ __forceinline__ float exponentials() {
-    constexpr float c = Scale<D>::c;
+    constexpr float c = wir::PackedScale<D>::c;
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb)
@@ -125,7 +107,7 @@ struct Forward {
   }
 
   __device__ __forceinline__ void softmax(int t) {
-    constexpr float c = Scale<D>::c;
+    constexpr float c = wir::PackedScale<D>::c;
     const int col0 = t * TILE;
     if (CAUSAL ? col0 + TILE - 1 > row0 : col0 + TILE > r.len) {
       wir::seldom();
@@ -235,18 +217,8 @@ struct Forward {
   }
 };
 
-__device__ __forceinline__ void fill_rest(const fwd_args& a, const wir::Rows& r, int head, int d, int most) {
-  const int rows = min(r.len - r.row0, most);
-  bf16* out = a.out + head * a.oh + (i64)(r.start + r.row0) * a.ot;
-  if (a.flags & 1)
-    for (int i = threadIdx.x; i < rows * (d / 8); i += blockDim.x)
-      *(wir::bf16x8*)(out + i / (d / 8) * a.ot + i % (d / 8) * 8) = wir::bf16x8{};
-  if ((a.flags & 2) && (int)threadIdx.x < rows)
-    a.lse[head * a.lh + (r.start + r.row0 + (int)threadIdx.x) * a.lt] = -__builtin_inff();
-}
-
 template <int D, bool CAUSAL, int NW>
-__device__ __forceinline__ void forward(const fwd_args& a) {
+__device__ __forceinline__ void forward(const wir::packed_fwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[Forward<D, CAUSAL, NW>::BYTES];
   int x, head;
   const int two = NW == 8 && a.flags & 4, rows = NW == 4 || two ? 128 : 256;
@@ -256,8 +228,8 @@ __device__ __forceinline__ void forward(const fwd_args& a) {
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x, rows);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
   if (r.rest) {
-    fill_rest(a, r, head, D, rows);
-    if (two) fill_rest(a, r, head + 1, D, 128);
+    wir::packed_fill_rest(a, r, head, D, rows);
+    if (two) wir::packed_fill_rest(a, r, head + 1, D, 128);
     return;
   }
   Forward<D, CAUSAL, NW> f(a, r, smem);
@@ -270,7 +242,7 @@ __device__ __forceinline__ void forward(const fwd_args& a) {
 #define PACKED_KERNEL(NAME, D, CAUSAL, NW, WAVES_A_SIMD)                                                \
   extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64 * NW, 64 * NW),              \
                                             amdgpu_waves_per_eu(WAVES_A_SIMD, WAVES_A_SIMD)))           \
-  NAME(const fwd_args args) { forward<D, CAUSAL, NW>(args); }
+  NAME(const wir::packed_fwd_args args) { forward<D, CAUSAL, NW>(args); }
 
 PACKED_KERNEL(wir_attn_packed_d64, 64, false, 4, 3)
 PACKED_KERNEL(wir_attn_packed_d64_causal, 64, true, 4, 3)

@@ -6,51 +6,21 @@
 //   dQ_p = sum_j dS_pj k_j / sqrt(D),
 //   dK_j = sum_p dS_pj q_p / sqrt(D),  dV_j = sum_p P_pj dO_p,
 // the last two over the query heads that share a key/value head as well.
-#include "wir_packed.h"
+#include "wir_packed_args.h"
 
 namespace {
 
 using wir::bf16;
 using wir::i64;
 
-struct bwd_args {
-  const bf16* q;       // [H, T, D], as o, d_o and dq
-  const bf16* k;       // [H_kv, T, D], as v, dk and dv
-  const bf16* v;
-  const bf16* o;
-  const bf16* d_o;
-  const float* lse;    // [H, T]
-  const int* offsets;  // [batch + 1]
-  bf16* dq;
-  bf16* dk;
-  bf16* dv;
-  float* stats;        // [2][H][T]: -LSE sqrt(D) and -D_p, what the scores of the dK/dV kernels begin with
-  i64 qh, qt, kh, kt, vh, vt, oh, ot, gh, gt, lh, lt, dqh, dqt, dkh, dkt, dvh, dvt;
-  int batch, tokens, heads, group, blocks;
-  int flags;           // rows behind the last sequence become 0 in dq: 1, dk: 2, dv: 4
-};
-
 constexpr int WAVES = wir::PACKED_WAVES, ROWS = wir::PACKED_ROWS;
-
-template <int D>
-struct Scale {
-  static constexpr double inv_sqrt = D == 64 ? 0.125 : 0.08838834764831845;
-  static constexpr float root = D == 64 ? 8.0f : 11.313708498984761f, s = (float)inv_sqrt, c = (float)(1.4426950408889634 * inv_sqrt);
-};
-
-__device__ __forceinline__ void zero_rest(bf16* x, i64 head_stride, i64 row_stride, const wir::Rows& r, int head, int d) {
-  const int rows = min(r.len - r.row0, ROWS);
-  x += head * head_stride + (i64)(r.start + r.row0) * row_stride;
-  for (int i = threadIdx.x; i < rows * (d / 8); i += blockDim.x)
-    *(wir::bf16x8*)(x + i / (d / 8) * row_stride + i % (d / 8) * 8) = wir::bf16x8{};
-}
 
 // dQ of one block of 128 query rows, 32 a wave.
 template <int D, int KT, bool CAUSAL>
-__device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, int head, char* smem, bool careful) {
+__device__ __forceinline__ bool dq_block(const wir::packed_bwd_args& a, const wir::Rows& r, int head, char* smem, bool careful) {
   typedef wir::STile<KT, D, wir::BOTH> TK;
   typedef wir::STile<KT, D, wir::ROWREAD> TV;
-  constexpr float c = Scale<D>::c;
+  constexpr float c = wir::PackedScale<D>::c;
   const int wave = wir::wave_id(), lane = wir::lane_id();
   const int row0 = r.row0 + wave * 32, kv = head / a.group;
   wir::HeadTiles<TK> K;
@@ -75,7 +45,7 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
   wir::row_dot(dots, d_o, o);
   if (lane < 32 && row < r.len) {
     float* to = a.stats + (i64)head * a.tokens + r.start + row;
-    to[0] = -lse * Scale<D>::root;
+    to[0] = -lse * wir::PackedScale<D>::root;
     to[(i64)a.heads * a.tokens] = -dots.v[0];
   }
   lse *= 1.4426950408889634f;
@@ -128,7 +98,7 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
 #pragma unroll
   for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc.f[cb][0][i] *= Scale<D>::s;
+    for (int i = 0; i < 16; ++i) acc.f[cb][0][i] *= wir::PackedScale<D>::s;
   if (careful) {
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb)
@@ -145,7 +115,7 @@ __device__ __forceinline__ bool dq_block(const bwd_args& a, const wir::Rows& r, 
 }
 
 template <int D, int KT, bool CAUSAL>
-__device__ __forceinline__ void dq_kernel(const bwd_args& a) {
+__device__ __forceinline__ void dq_kernel(const wir::packed_bwd_args& a) {
   constexpr int STAGE = WAVES * 32 * D * 2, TILES = 4 * KT * D * 2;
   static_assert(STAGE <= TILES, "the output goes through the tiles' LDS");
   __shared__ __attribute__((aligned(1024))) char smem[TILES + sizeof(wir::Odd<D>)];
@@ -155,7 +125,7 @@ __device__ __forceinline__ void dq_kernel(const bwd_args& a) {
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
   if (r.rest) {
-    if (a.flags & 1) zero_rest(a.dq, a.dqh, a.dqt, r, head, D);
+    if (a.flags & 1) wir::packed_zero_rest(a.dq, a.dqh, a.dqt, r, head, D, ROWS);
     return;
   }
   bool careful = false;
@@ -164,9 +134,9 @@ __device__ __forceinline__ void dq_kernel(const bwd_args& a) {
 
 // dK and dV of one block of 128 keys, 32 a wave, over the tiles of QT queries of the group's heads one after another.
 template <int D, int QT, bool CAUSAL>
-__device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r, int kv, char* smem, bool careful) {
+__device__ __forceinline__ bool dkdv_block(const wir::packed_bwd_args& a, const wir::Rows& r, int kv, char* smem, bool careful) {
   typedef wir::STile<QT, D, wir::BOTH> T;
-  constexpr float c = Scale<D>::c;
+  constexpr float c = wir::PackedScale<D>::c;
   static_assert(WAVES * 32 * D * 2 <= 4 * T::BYTES, "the outputs go through the tiles' LDS");
   constexpr int VEC = 4 * T::BYTES, ODD = VEC + 4 * QT * 4;
   const int wave = wir::wave_id(), lane = wir::lane_id();
@@ -255,7 +225,7 @@ __device__ __forceinline__ bool dkdv_block(const bwd_args& a, const wir::Rows& r
 #pragma unroll
   for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dk.f[cb][0][i] *= Scale<D>::s;
+    for (int i = 0; i < 16; ++i) dk.f[cb][0][i] *= wir::PackedScale<D>::s;
   if (careful) {
     const int row = CAUSAL ? row0 + lane % 32 : 0;   // the first query that sees it
 #pragma unroll
@@ -302,7 +272,7 @@ struct Paired {
     int head, t;
   };
 
-  const bwd_args& a;
+  const wir::packed_bwd_args& a;
   const wir::Rows& r;
   char* smem;
   int wave, lane, role, row0, first, tiles;
@@ -314,7 +284,7 @@ struct Paired {
   wir::BTile<32, 32, 32> keep;
   wir::BTile<32, 32, QT> x;
 
-  __device__ __forceinline__ Paired(const bwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
+  __device__ __forceinline__ Paired(const wir::packed_bwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
 
   __device__ __forceinline__ At after(At i) const { return i.t + 1 < tiles ? At{i.head, i.t + 1} : At{i.head + 1, first}; }
 
@@ -372,7 +342,7 @@ struct Paired {
 
   // P and dS of the wave's half of a tile: one it keeps, one it hands on.
   __device__ __forceinline__ void finish_scores(At i, int turn) {
-    constexpr float c = Scale<D>::c;
+    constexpr float c = wir::PackedScale<D>::c;
     const int col0 = i.t * QT + role * 32;
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
@@ -489,7 +459,7 @@ struct Paired {
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-      for (int n = 0; n < 16; ++n) acc.f[cb][0][n] *= role ? Scale<D>::s : 1.f;
+      for (int n = 0; n < 16; ++n) acc.f[cb][0][n] *= role ? wir::PackedScale<D>::s : 1.f;
     if (careful) {
       const auto* mine = odd + (role ? 0 : 1);
 #pragma unroll
@@ -509,15 +479,15 @@ struct Paired {
 };
 
 template <int D, int QT, bool CAUSAL>
-__device__ __forceinline__ void dkdv_kernel(const bwd_args& a) {
+__device__ __forceinline__ void dkdv_kernel(const wir::packed_bwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[4 * QT * D * 2 + 16 * QT + 2 * sizeof(wir::Odd<D>)];
   int x, kv;
   wir::packed_program(a.blocks, a.heads / a.group, x, kv);   // a sequence's longest block is its first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
   if (r.rest) {
-    if (a.flags & 2) zero_rest(a.dk, a.dkh, a.dkt, r, kv, D);
-    if (a.flags & 4) zero_rest(a.dv, a.dvh, a.dvt, r, kv, D);
+    if (a.flags & 2) wir::packed_zero_rest(a.dk, a.dkh, a.dkt, r, kv, D, ROWS);
+    if (a.flags & 4) wir::packed_zero_rest(a.dv, a.dvh, a.dvt, r, kv, D, ROWS);
     return;
   }
   bool careful = false;
@@ -525,15 +495,15 @@ __device__ __forceinline__ void dkdv_kernel(const bwd_args& a) {
 }
 
 template <int D, bool CAUSAL>
-__device__ __forceinline__ void dkdv_kernel8(const bwd_args& a) {
+__device__ __forceinline__ void dkdv_kernel8(const wir::packed_bwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[Paired<D, CAUSAL>::BYTES];
   int x, kv;
   wir::packed_program(a.blocks, a.heads / a.group, x, kv);   // a sequence's longest block is its first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
   if (r.rest) {
-    if (a.flags & 2) zero_rest(a.dk, a.dkh, a.dkt, r, kv, D);
-    if (a.flags & 4) zero_rest(a.dv, a.dvh, a.dvt, r, kv, D);
+    if (a.flags & 2) wir::packed_zero_rest(a.dk, a.dkh, a.dkt, r, kv, D, ROWS);
+    if (a.flags & 4) wir::packed_zero_rest(a.dv, a.dvh, a.dvt, r, kv, D, ROWS);
     return;
   }
   Paired<D, CAUSAL> p(a, r, smem);
@@ -545,12 +515,12 @@ __device__ __forceinline__ void dkdv_kernel8(const bwd_args& a) {
 
 #define PACKED_KERNEL8(NAME, CALL)                                                                             \
   extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) \
-  NAME(const bwd_args args) { CALL(args); }
+  NAME(const wir::packed_bwd_args args) { CALL(args); }
 
 #define PACKED_KERNEL(NAME, CALL, WAVES_A_SIMD)                                                         \
   extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256),                      \
                                             amdgpu_waves_per_eu(WAVES_A_SIMD, WAVES_A_SIMD)))           \
-  NAME(const bwd_args args) { CALL(args); }
+  NAME(const wir::packed_bwd_args args) { CALL(args); }
 
 PACKED_KERNEL(wir_attn_packed_dq_d64, (dq_kernel<64, 32, false>), 3)
 PACKED_KERNEL(wir_attn_packed_dq_d64_causal, (dq_kernel<64, 32, true>), 3)

@@ -70,20 +70,20 @@ __device__ __forceinline__ gl<T> packed_head(T* data, i64 head_stride, i64 row_s
 }
 
 // The tiles of one head of one sequence, loaded into LDS by NW waves.
-// Lane l of a wave's j-th load moves a 16-byte chunk of row row + j * EVERY; the
-// swizzles repeat within EVERY rows, so the chunk's place in the row is the
-// same for every j.  Rows past the sequence's end read its last row (no branch,
+// A lane's j-th load moves a 16-byte chunk of row row + j * EVERY (row < EVERY, a
+// power of two, and the swizzles are exclusive ors of a row's bits, so that
+// the two parts' swizzles are taken one after the other).  Rows past the sequence's end read its last row (no branch,
 // no address of another sequence): whoever uses the tile masks them.
 template <class Tile, int NW = PACKED_WAVES>
 struct HeadTiles {
   static constexpr int LOADS = Tile::ROWS * Tile::CPR / 64 / NW, EVERY = Tile::ROWS / LOADS;
-  static_assert(EVERY % 16 == 0, "the swizzles repeat every 16 rows");
+  static_assert((EVERY & (EVERY - 1)) == 0, "");
   const char* base;
   unsigned row, chunk, pitch;   // the lane's row and bytes in it, bytes from a row to the next
   int len;
 
   __device__ __forceinline__ void init(const bf16* x, i64 row_stride, int rows) {
-    const int p = threadIdx.x, c = p % Tile::CPR;   // (wave w's chunks start at 64 w)
+    const int p = NW == 1 ? lane_id() : threadIdx.x, c = p % Tile::CPR;   // (wave w's chunks start at 64 w)
     row = p / Tile::CPR;
     chunk = (c ^ swz<Tile::CPR, Tile::ROLE>(row)) * 16;
     pitch = (unsigned)row_stride * 2;
@@ -96,7 +96,7 @@ struct HeadTiles {
     const unsigned end = (unsigned)min(len - 1 - t * Tile::ROWS, Tile::ROWS - 1);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
-      dma16_s(from, min(row + j * EVERY, end) * pitch + chunk, lds_addr(tile + (wave + j * NW) * 1024));
+      dma16_s(from, min(row + j * EVERY, end) * pitch + (chunk ^ swz<Tile::CPR, Tile::ROLE>(j * EVERY) * 16), lds_addr(tile + (wave + j * NW) * 1024));
   }
 };
 
@@ -174,7 +174,7 @@ template <bool LAST, int NW, class TB>
 __device__ __forceinline__ void clear_odd(char* b_base, int pos0, __attribute__((address_space(3))) Odd<TB::COLS>* odd) {
   typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 #pragma unroll 1
-  for (int i = threadIdx.x; i < TB::ROWS * TB::CPR; i += 64 * NW) {
+  for (int i = NW == 1 ? lane_id() : threadIdx.x; i < TB::ROWS * TB::CPR; i += 64 * NW) {
     const int row = i / TB::CPR, chunk = i % TB::CPR;
     auto* p = (__attribute__((address_space(3))) u16x8*)(lds(b_base) + TB::chunk_off(row, chunk));
     u16x8 w = *p;
@@ -192,6 +192,7 @@ __device__ __forceinline__ void clear_odd(char* b_base, int pos0, __attribute__(
     }
     *p = w;
   }
+  if (NW == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (other waves have nothing to do with the tile)
 }
 
 }  // namespace wir

@@ -101,11 +101,11 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
         lse = rec.alloc(torch.empty(heads, tokens, dtype=torch.float32, device=device))
     if tokens == 0:
         return _results(given, (out, lse))
-    waves, two = _forward_form(heads // shared, tokens, batch, d)
-    blocks = tokens // (256 if waves == 8 and not two else 128) + batch + 1
+    kind, rows, waves, two = _forward_form(heads, shared, tokens, batch, d)
+    blocks = tokens // rows + batch + 1
     args = _Args(*[None] * 6, *(s for x in (q, k, v, out) for s in x.stride()[:2]), *lse.stride(), batch, tokens, heads,
                  heads // shared, blocks, flags | (4 if two else 0))
-    launch(rec, device, "attn_packed.hsaco", f"wir_attn_packed_d{d}" + ("_w8" if waves == 8 else "") + ("_causal" if causal else ""),
+    launch(rec, device, "attn_packed_split.hsaco" if kind == "_split" else "attn_packed.hsaco", f"wir_attn_packed_d{d}{kind}" + ("_causal" if causal else ""),
            (blocks * (heads // 2 if two else heads), 1, 1), (64 * waves, 1, 1), args,
            {"q": q, "k": k, "v": v, "out": out, "lse": lse, "offsets": offsets})
     if rec:
@@ -113,18 +113,42 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
     return _results(given, (out, lse))
 
 
-def _forward_form(group: int, tokens: int, batch: int, d: int) -> Tuple[int, bool]:
-    """(waves of a workgroup, whether it takes two heads) of the forward.  Eight
-    waves are two groups of four with the same tiles: two heads that share keys
-    and values, or 256 rows of one head.  They pay at D = 128 in long sequences;
+# A launch of the split kernels (32 rows a workgroup, whose waves divide the other side) against one of 128 rows: us of
+# 64 keys (queries) that a workgroup of 128 rows walks, of the start of one of 32, and its part of that walk.  By launches of
+# 5 x 90 to 2 x 4096 tokens, 8/8 and 16/4 heads, causal; us, 128 rows / 32: forward D = 64, 8 heads, 1 x 512 10.9 / 6.8, 2 x
+# 1024 17.2 / 14.3, 8 x 256 7.8 / 10.7; dQ D = 128 1 x 512 20.9 / 12.5, 1 x 4096 117 / 112, 32 x 64 11.5 / 22; dK/dV D = 64, 16/4
+# heads, 1 x 512 59.5 / 17.8, 8 x 512 59.7 / 32.1, 64 x 64 14.8 / 21.1, D = 128 2 x 1024 108 / 63, 8 x 1024 115 / 152.
+_SPLIT_US = {("forward", 64): (0.82, 2.7, 0.20), ("forward", 128): (1.2, 3.8, 0.31), ("dq", 64): (1.18, 4.3, 0.20),
+             ("dq", 128): (1.75, 6.0, 0.20), ("dkdv", 64): (1.7, 4.4, 0.17), ("dkdv", 128): (1.66, 6.0, 0.50)}
+
+
+def _splits(part: str, heads: int, walks: int, tokens: int, batch: int, d: int) -> bool:
+    """Whether a launch over ``heads`` heads, whose workgroups walk a sequence ``walks``
+    times, goes to the split kernels.  The lengths are on the GPU: their average decides."""
+    tile, start, share = _SPLIT_US[part, d]
+    walk = tile * walks * tokens / (64 * max(batch, 1))
+    rounds = (tokens / 32 + batch) * heads / 256   # of one workgroup a CU
+    rounds = 1 if rounds <= 1 else rounds + 0.5
+    return 3 + rounds * (start + share * walk) < 5.5 + walk
+
+
+def _forward_form(heads: int, shared: int, tokens: int, batch: int, d: int) -> Tuple[str, int, int, bool]:
+    """(kind of the kernel, query rows and waves of a workgroup, whether it takes two heads) of the forward.
+
+    Eight waves are two groups of four with the same tiles: two heads that share
+    keys and values, or 256 rows of one head.  They pay at D = 128 in long sequences;
     the lengths are on the GPU, so their average decides.  us, four / eight waves,
     batches of 32768 tokens in sequences of 128, 256, 512, 1024, 2048, 4096:
     32/8 heads, not causal 290 / 327, 240 / 257, 359 / 334, 558 / 532, 976 / 949, 1840
     / 1750; causal 284 / 338, 208 / 225, 260 / 263, 368 / 371, 589 / 587, 1024 / 992;
     16/16 heads, not causal 170 / 157, 139 / 213, 192 / 200, 283 / 285, 506 / 494, 932 / 893."""
+    if _splits("forward", heads, 1, tokens, batch, d):
+        return "_split", 32, 4, False
     average = tokens / max(batch, 1)
-    two = group % 2 == 0
-    return (8, two) if d == 128 and average >= (512 if two else 2048) else (4, False)
+    two = heads // shared % 2 == 0
+    if d == 128 and average >= (512 if two else 2048) and tokens * heads >= 1 << 17:   # (two such workgroups a CU)
+        return "_w8", 128 if two else 256, 8, two
+    return "", 128, 4, False
 
 
 def _results(given, done):
@@ -186,14 +210,17 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
         workspace = rec.alloc(torch.empty(floats, dtype=torch.float32, device=device))
     if tokens == 0:
         return _results(given, tuple(grads))
-    blocks = tokens // ROWS + batch + 1
-    args = _GradArgs(*[None] * 11, *(s for x in (q, k, v, o, do, lse, *grads) for s in x.stride()[:2]), batch, tokens, heads,
-                     heads // shared, blocks, flags)
     names = {"q": q, "k": k, "v": v, "o": o, "d_o": do, "lse": lse, "offsets": offsets, "dq": grads[0], "dk": grads[1],
              "dv": grads[2], "stats": workspace}
-    for kernel, programs in (("dq", heads), ("dkdv", shared)):
-        launch(rec, device, "attn_packed_bwd.hsaco", f"wir_attn_packed_{kernel}_d{d}" + ("_causal" if causal else ""),
-               (blocks * programs, 1, 1), (512 if kernel == "dkdv" and d == 128 else 256, 1, 1), args, names)
+    strides = [s for x in (q, k, v, o, do, lse, *grads) for s in x.stride()[:2]]
+    for part, programs in (("dq", heads), ("dkdv", shared)):
+        split = _splits(part, programs, heads // programs, tokens, batch, d)
+        blocks = tokens // (32 if split else ROWS) + batch + 1
+        threads = 512 if part == "dkdv" and (d == 64) == split else 256
+        args = _GradArgs(*[None] * 11, *strides, batch, tokens, heads, heads // shared, blocks, flags)
+        launch(rec, device, "attn_packed_split.hsaco" if split else "attn_packed_bwd.hsaco",
+               f"wir_attn_packed_{part}_d{d}" + ("_split" if split else "") + ("_causal" if causal else ""),
+               (blocks * programs, 1, 1), (threads, 1, 1), args, names)
     if rec:
         _backward_plans.add(causal, rec, *grads)
     return _results(given, tuple(grads))
