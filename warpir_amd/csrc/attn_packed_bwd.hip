@@ -15,110 +15,194 @@ using wir::i64;
 
 constexpr int WAVES = wir::PACKED_WAVES, ROWS = wir::PACKED_ROWS;
 
-// dQ of one block of 128 query rows, 32 a wave.
-template <int D, int KT, bool CAUSAL>
-__device__ __forceinline__ bool dq_block(const wir::packed_bwd_args& a, const wir::Rows& r, int head, char* smem, bool careful) {
+// dQ of one block of 128 query rows, 32 a wave.  In the time of a tile of 32
+// keys t a wave takes the product of dS(t - 1) with K(t - 1), the scores of t,
+// q . k and dO . v in turn, and their exponentials; the operands of both are
+// one stream of LDS reads that runs AHEAD products before their use.
+template <int D, bool CAUSAL>
+struct Dq {
+  static constexpr int KT = 32, AHEAD = 5, KS = D / 16, CB = D / 32;
+  static constexpr int SCORES = 2 * KS, PRODUCTS = KT / 16 * CB;   // products of a wave for a tile
   typedef wir::STile<KT, D, wir::BOTH> TK;
   typedef wir::STile<KT, D, wir::ROWREAD> TV;
-  constexpr float c = wir::PackedScale<D>::c;
-  const int wave = wir::wave_id(), lane = wir::lane_id();
-  const int row0 = r.row0 + wave * 32, kv = head / a.group;
+  typedef __attribute__((address_space(3))) wir::bf16x8 lds_bf16x8;
+  typedef __attribute__((address_space(3))) wir::i16x4 lds_i16x4;
+  typedef __attribute__((address_space(3))) wir::Odd<D> lds_odd;
+  // LDS: three tiles of K, two of V, notes of what is odd
+  static constexpr int VALUES = 3 * TK::BYTES, ODD = VALUES + 2 * TV::BYTES, BYTES = ODD + sizeof(wir::Odd<D>);
+  static_assert(WAVES * 32 * D * 2 <= ODD, "the output goes through the tiles' LDS");
+
+  const wir::packed_bwd_args& a;
+  const wir::Rows& r;
+  char* smem;
+  int wave, lane, row0, tiles;
   wir::HeadTiles<TK> K;
   wir::HeadTiles<TV> V;
-  K.init(a.k + kv * a.kh + r.start * a.kt, a.kt, r.len);
-  V.init(a.v + kv * a.vh + r.start * a.vt, a.vt, r.len);
-  const int keys = CAUSAL ? min(r.len, r.row0 + ROWS) : r.len, tiles = (keys + KT - 1) / KT;
-  auto load = [&](int t) {
-    char* at = smem + t % 2 * TK::BYTES;
-    K.load(at, t, wave);
-    V.load(at + 2 * TK::BYTES, t, wave);
-  };
-  auto* odd = (__attribute__((address_space(3))) wir::Odd<D>*)wir::lds(smem + 4 * TK::BYTES);
-  if (careful) wir::no_odd<false, WAVES>(odd);
-  wir::RowFrags<32, 1, D / 16> q, d_o, o;
-  wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
-  wir::packed_rows(d_o, a.d_o + head * a.gh + r.start * a.gt, a.gt, row0, r.len);
-  wir::packed_rows(o, a.o + head * a.oh + r.start * a.ot, a.ot, row0, r.len);
-  const int row = row0 + lane % 32;
-  float lse = a.lse[head * a.lh + (r.start + min(row, r.len - 1)) * a.lt];
-  wir::RVec<32, 32> dots;
-  wir::row_dot(dots, d_o, o);
-  if (lane < 32 && row < r.len) {
-    float* to = a.stats + (i64)head * a.tokens + r.start + row;
-    to[0] = -lse * wir::PackedScale<D>::root;
-    to[(i64)a.heads * a.tokens] = -dots.v[0];
-  }
-  lse *= 1.4426950408889634f;
+  unsigned k_at, v_at, tr_at;      // the lane's places in a tile, as operands of the scores and of the product
+  wir::RowFrags<32, 1, KS> q, d_o;
   wir::RTile<32, 32, D> acc;
-  wir::fill(acc, 0.f);
-  load(0);
-  for (int t = 0; t < tiles; ++t) {
-    char *kt = smem + t % 2 * TK::BYTES, *vt = kt + 2 * TK::BYTES;
+  wir::RTile<32, 32, KT> s, dp;
+  wir::BTile<32, 32, KT> ds;
+  wir::f32x16 dots;                // -D_p of the lane's row, what dO . v begins with
+  float lse;                       // in log2 units
+
+  __device__ __forceinline__ Dq(const wir::packed_bwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
+
+  __device__ __forceinline__ void product(const wir::bf16x8& b, int i) {
+    const int g = 2 * (i / CB), cb = i % CB;
+    acc.f[cb][0] = wir::MF<32>::mma(b, wir::cat(ds.f[0][0][g], ds.f[0][0][g + 1]), acc.f[cb][0]);
+  }
+
+  // The product of tile t - 1 (PRODUCT), whose keys are in slot `before`, and the scores of tile t (SCORE), in `slot`.
+  template <bool PRODUCT, bool SCORE>
+  __device__ __forceinline__ void stream(int t, int slot, int before) {
+    constexpr int N0 = PRODUCT ? PRODUCTS : 0, N = N0 + (SCORE ? SCORES : 0);
+    const unsigned from = tr_at + before * TK::BYTES, keys = k_at + slot * TK::BYTES, values = v_at + t % 2 * TV::BYTES;
+    wir::bf16x8 ring[AHEAD + 1];
+    auto read = [&](auto at) {
+      constexpr int n = decltype(at)::value, i = n - N0;
+      if constexpr (n < N0) {
+        const unsigned tile = from ^ (n % CB * 64);
+        constexpr int rows = n / CB * 16 * D * 2;   // (two groups of eight rows)
+        const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + rows));
+        const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((tile ^ 32) + rows + 8 * D * 2));
+        ring[n % (AHEAD + 1)] = wir::cat(__builtin_bit_cast(wir::bf16x4, lo), __builtin_bit_cast(wir::bf16x4, hi));
+      } else {
+        ring[n % (AHEAD + 1)] = *(lds_bf16x8*)((i % 2 ? values : keys) ^ (i / 2 * 32));
+      }
+    };
+    __builtin_amdgcn_s_setprio(1);
+    wir::static_for<0, (AHEAD < N ? AHEAD : N)>(read);
+    wir::static_for<0, N>([&](auto at) {
+      constexpr int n = decltype(at)::value, i = n - N0;
+      if constexpr (n + AHEAD < N) read(wir::ic<n + AHEAD>{});
+      __builtin_amdgcn_sched_barrier(0);
+      const wir::bf16x8& b = ring[n % (AHEAD + 1)];
+      if constexpr (n < N0) product(b, n);
+      else if constexpr (i % 2 == 0) s.f[0][0] = wir::MF<32>::mma(b, q.f[0][i / 2], i < 2 ? wir::f32x16{} : s.f[0][0]);
+      else dp.f[0][0] = wir::MF<32>::mma(b, d_o.f[0][i / 2], i < 2 ? dots : dp.f[0][0]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  __device__ __forceinline__ void finish_scores(int t) {
+    constexpr float c = wir::PackedScale<D>::c;
     const int col0 = t * KT;
-    wir::wait_vm_barrier<0>();
-    if (t + 1 < tiles) load(t + 1);
-    if (CAUSAL && !careful && col0 > row0 + 31) continue;   // no row of the wave sees the tile
-    wir::RTile<32, 32, KT> s, dp;
-    wir::BTile<32, 32, KT> ds;
-    wir::mma_ABt_frags<32, 32, KT, TK, D / 16>(s, q, kt, 0);
-    const bool edge = CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len;
-    if (edge) {
-      wir::seldom();
-      wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
-    }
-    wir::mma_ABt_frags<32, 32, KT, TV, D / 16>(dp, d_o, vt, 0);
 #pragma unroll
-    for (int cb = 0; cb < KT / 32; ++cb)
+    for (int i = 0; i < 16; ++i) {
+      s.f[0][0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s.f[0][0][i], c, -lse));
+      dp.f[0][0][i] *= s.f[0][0][i];
+    }
+    if (CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len) {   // (a value that a row does not see may be NaN)
+      wir::seldom();
+      const int row = row0 + lane % 32;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s.f[cb][0][i], c, -lse));
-        dp.f[cb][0][i] = p * (dp.f[cb][0][i] - dots.v[0]);
-        s.f[cb][0][i] = p;
+        const int col = col0 + wir::ccol<32>(i, lane / 32);
+        dp.f[0][0][i] = (CAUSAL ? col <= row : col < r.len) ? dp.f[0][0][i] : 0.f;
       }
-    if (edge) {   // (a value that a row does not see may be NaN)
-      wir::seldom();
-#pragma unroll
-      for (int cb = 0; cb < KT / 32; ++cb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dp.f[cb][0][i] = s.f[cb][0][i] == 0.f ? 0.f : dp.f[cb][0][i];
     }
     wir::to_bf16(ds, dp);
-    if (careful) {
-      wir::barrier();
-      wir::clear_odd<false, WAVES, TK>(kt, col0, odd);
-      wir::barrier();
-    }
-    wir::mma_rAB<32, 32, KT, D, TK>(acc, ds, kt, 0);
   }
-  if (!careful) {
-    if (wir::any_wave(wir::has_nan(acc, row < r.len), smem + 4 * TK::BYTES)) return true;
-  } else {
-    wir::wait_vm_barrier<0>();
-  }
-#pragma unroll
-  for (int cb = 0; cb < D / 32; ++cb)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc.f[cb][0][i] *= wir::PackedScale<D>::s;
-  if (careful) {
-#pragma unroll
-    for (int cb = 0; cb < D / 32; ++cb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
-        const int first = min(odd->at[0][d], min(odd->at[1][d], odd->at[2][d]));
-        acc.f[cb][0][i] = (CAUSAL ? row : r.len - 1) >= first ? __builtin_nanf("") : acc.f[cb][0][i];
-      }
-  }
-  wir::store_tile_staged<true>(wir::packed_head(a.dq, a.dqh, a.dqt, head, r.start, r.len, D), acc, 0, 0, row0, 0,
-                               smem + wave * 32 * D * 2);
-  return false;
-}
 
-template <int D, int KT, bool CAUSAL>
+  __device__ __forceinline__ bool run(int head, bool careful) {
+    wave = wir::wave_id(), lane = wir::lane_id();
+    row0 = r.row0 + wave * 32;
+    const int kv = head / a.group, keys = CAUSAL ? min(r.len, r.row0 + ROWS) : r.len;
+    tiles = (keys + KT - 1) / KT;
+    const int mine = row0 >= r.len ? 0 : CAUSAL ? min(tiles, (row0 + 31) / KT + 1) : tiles;   // tiles that the wave's rows see
+    K.init(a.k + kv * a.kh + r.start * a.kt, a.kt, r.len);
+    V.init(a.v + kv * a.vh + r.start * a.vt, a.vt, r.len);
+    const int part = lane % 16;   // of the transposed reads
+    k_at = wir::lds_addr(smem) + TK::chunk_off(lane % 32, lane / 32);
+    v_at = wir::lds_addr(smem) + VALUES + TV::chunk_off(lane % 32, lane / 32);
+    tr_at = wir::lds_addr(smem) + TK::elem_off(lane / 32 * 4 + part / 4, lane % 32 / 16 * 16 + 4 * (part % 4));
+    auto* odd = (lds_odd*)wir::lds(smem + ODD);
+    if (careful) wir::no_odd<false, WAVES>(odd);
+    K.load(smem, 0, wave);
+    V.load(smem + VALUES, 0, wave);
+    wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
+    wir::packed_rows(d_o, a.d_o + head * a.gh + r.start * a.gt, a.gt, row0, r.len);
+    const int row = row0 + lane % 32;
+    lse = a.lse[head * a.lh + (r.start + min(row, r.len - 1)) * a.lt];
+    {
+      wir::RowFrags<32, 1, KS> o;
+      wir::packed_rows(o, a.o + head * a.oh + r.start * a.ot, a.ot, row0, r.len);
+      wir::RVec<32, 32> sum;
+      wir::row_dot(sum, d_o, o);
+      dots = wir::f32x16{} - sum.v[0];
+    }
+    if (lane < 32 && row < r.len) {
+      float* to = a.stats + (i64)head * a.tokens + r.start + row;
+      to[0] = -lse * wir::PackedScale<D>::root;
+      to[(i64)a.heads * a.tokens] = dots[0];
+    }
+    lse *= 1.4426950408889634f;
+    wir::fill(acc, 0.f);
+    int t = 0, slot = 0, before = 2;   // of tile t, of t - 1
+    auto settle = [&]() {   // tile t has come, t + 1 is asked for
+      wir::wait_vm_barrier<0>();
+      const int next = slot == 2 ? 0 : slot + 1;
+      if (t + 1 < tiles) {
+        K.load(smem + next * TK::BYTES, t + 1, wave);
+        V.load(smem + VALUES + (t + 1) % 2 * TV::BYTES, t + 1, wave);
+      }
+      if (careful && t > 0) {
+        wir::clear_odd<false, WAVES, TK>(smem + before * TK::BYTES, (t - 1) * KT, odd);
+        wir::barrier();
+      }
+    };
+    auto advance = [&]() {
+      ++t;
+      before = slot;
+      slot = slot == 2 ? 0 : slot + 1;
+    };
+    if (mine > 0) {
+      settle();
+      stream<false, true>(t, slot, before);
+      finish_scores(t);
+      advance();
+      while (t < mine) {
+        settle();
+        stream<true, true>(t, slot, before);
+        finish_scores(t);
+        advance();
+      }
+      settle();
+      stream<true, false>(t, slot, before);
+      advance();
+    }
+    while (t <= tiles) {
+      settle();
+      advance();
+    }
+    if (!careful) {
+      if (wir::any_wave(wir::has_nan(acc, row < r.len), smem + ODD)) return true;
+    } else {
+      wir::wait_vm_barrier<0>();
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) acc.f[cb][0] *= wir::PackedScale<D>::s;
+    if (careful) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
+          const int first = min(odd->at[0][d], min(odd->at[1][d], odd->at[2][d]));
+          acc.f[cb][0][i] = (CAUSAL ? row : r.len - 1) >= first ? __builtin_nanf("") : acc.f[cb][0][i];
+        }
+    }
+    wir::store_tile_staged<true>(wir::packed_head(a.dq, a.dqh, a.dqt, head, r.start, r.len, D), acc, 0, 0, row0, 0,
+                                 smem + wave * 32 * D * 2);
+    return false;
+  }
+};
+
+template <int D, bool CAUSAL>
 __device__ __forceinline__ void dq_kernel(const wir::packed_bwd_args& a) {
-  constexpr int STAGE = WAVES * 32 * D * 2, TILES = 4 * KT * D * 2;
-  static_assert(STAGE <= TILES, "the output goes through the tiles' LDS");
-  __shared__ __attribute__((aligned(1024))) char smem[TILES + sizeof(wir::Odd<D>)];
+  __shared__ __attribute__((aligned(1024))) char smem[Dq<D, CAUSAL>::BYTES];
   int x, head;
   wir::packed_program(a.blocks, a.heads, x, head);
   if (CAUSAL) x = a.blocks - 1 - x;   // a sequence's longest block first
@@ -128,8 +212,9 @@ __device__ __forceinline__ void dq_kernel(const wir::packed_bwd_args& a) {
     if (a.flags & 1) wir::packed_zero_rest(a.dq, a.dqh, a.dqt, r, head, D, ROWS);
     return;
   }
+  Dq<D, CAUSAL> p(a, r, smem);
   bool careful = false;
-  while (dq_block<D, KT, CAUSAL>(a, r, head, smem, careful)) careful = true;
+  while (p.run(head, careful)) careful = true;
 }
 
 // dK and dV of one block of 128 keys, 32 a wave, over the tiles of QT queries of the group's heads one after another.
@@ -522,10 +607,10 @@ __device__ __forceinline__ void dkdv_kernel8(const wir::packed_bwd_args& a) {
                                             amdgpu_waves_per_eu(WAVES_A_SIMD, WAVES_A_SIMD)))           \
   NAME(const wir::packed_bwd_args args) { CALL(args); }
 
-PACKED_KERNEL(wir_attn_packed_dq_d64, (dq_kernel<64, 32, false>), 3)
-PACKED_KERNEL(wir_attn_packed_dq_d64_causal, (dq_kernel<64, 32, true>), 3)
-PACKED_KERNEL(wir_attn_packed_dq_d128, (dq_kernel<128, 32, false>), 2)
-PACKED_KERNEL(wir_attn_packed_dq_d128_causal, (dq_kernel<128, 32, true>), 2)
+PACKED_KERNEL(wir_attn_packed_dq_d64, (dq_kernel<64, false>), 3)
+PACKED_KERNEL(wir_attn_packed_dq_d64_causal, (dq_kernel<64, true>), 3)
+PACKED_KERNEL(wir_attn_packed_dq_d128, (dq_kernel<128, false>), 2)
+PACKED_KERNEL(wir_attn_packed_dq_d128_causal, (dq_kernel<128, true>), 2)
 PACKED_KERNEL(wir_attn_packed_dkdv_d64, (dkdv_kernel<64, 32, false>), 2)
 PACKED_KERNEL(wir_attn_packed_dkdv_d64_causal, (dkdv_kernel<64, 32, true>), 2)
 PACKED_KERNEL8(wir_attn_packed_dkdv_d128, (dkdv_kernel8<128, false>))
