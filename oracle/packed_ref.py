@@ -81,6 +81,9 @@ def rope_axes_ref(x, angle, interleaved=False, back=False):
     return out, bound
 
 
+RECIPROCAL = float(torch.tensor(1.0) / torch.tensor(127.0))   # rounded to fp32
+
+
 def quantize_ref(x):
     """(codes, scale): one value at a time, ties to even."""
     codes, scales = torch.zeros(x.shape, dtype=torch.int8), torch.zeros(x.shape[0])
@@ -88,7 +91,7 @@ def quantize_ref(x):
         if not bool(row.isfinite().all()):
             scales[m] = math.nan
             continue
-        scales[m] = max(float((row.abs().max() / 127).float()), 2.0 ** -126)
+        scales[m] = max(float((row.abs().max() * RECIPROCAL).float()), 2.0 ** -126)
         s = float(scales[m])
         for k, value in enumerate(row.tolist()):
             # s and the value are dyadic: the quotient's distance from whole numbers is exact in integers

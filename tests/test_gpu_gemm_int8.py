@@ -36,6 +36,17 @@ def test_quantize(gpu, rows, width):
     assert bool((given[:, :16] == 9).all()) and bool((given[:, width + 16:] == 9).all())
 
 
+def test_quantize_as_torch_divides(gpu):
+    """Scales, and so codes, of a program that had them from torch on the GPU: bit for bit."""
+    x = seeded_normal((4096, 256), 3).cuda()
+    x[:, 0] = torch.arange(0x3f80, 0x3f80 + 4096, dtype=torch.int16, device="cuda").view(torch.bfloat16)   # every mantissa
+    x[:, 1:] = x[:, 1:].clamp(-1, 1)
+    codes, scale = api.quantize_int8(x)
+    want = x.float().abs().amax(1) / 127
+    assert torch.equal(scale, want)
+    assert torch.equal(codes, (x.double() / want.double()[:, None]).round().to(torch.int8))
+
+
 def test_quantize_borders(gpu):
     """Quotients on and next to the borders between codes, magnitudes from the smallest to the largest, what is no number."""
     tie = torch.arange(-127, 128).float()

@@ -1,8 +1,9 @@
 // gemm_int8.hip -- tokens in 8-bit integers with a scale each, and the product
 // of two matrices of such rows (warpir_amd.api.quantize_int8, gemm_int8).
 //
-//   scale_m = max(max_k |x_mk| / 127, 2^-126),  code_mk = the integer nearest to
-//   x_mk / scale_m, ties to even;
+//   scale_m = max(max_k |x_mk| * r, 2^-126) with r = 1 / 127 rounded to fp32 (torch
+// divides a GPU tensor by a number like this, so amax(1) / 127 there has the same
+// bits),  code_mk = the integer nearest to x_mk / scale_m, ties to even;
 //   out_mn = bf16((float)(sum_k a_mk b_nk) * a_scale_m * b_scale_n), the sum
 // exact in 32-bit integers.
 #include "wir_cdna4.h"
@@ -88,7 +89,7 @@ __device__ __forceinline__ void quantize(const quantize_args& a) {
     for (int w = 0; w < W; ++w) top = larger(top, tops[w]);
   }
   const bool finite = top < 0x7f80u;
-  const float scale = fmaxf(__uint_as_float(top << 16) / 127.0f, 0x1p-126f);
+  const float scale = fmaxf(__uint_as_float(top << 16) * (1.0f / 127.0f), 0x1p-126f);
   const float inv = finite ? 1.0f / scale : 0.f;
   i8x16* codes = (i8x16*)(a.codes + row * a.cs);
 #pragma unroll

@@ -32,9 +32,9 @@ def _pitch(t) -> int:
 def quantize_int8(x, codes=None, scale=None) -> Tuple[object, object]:
     """The rows of ``x`` ``[M, K]`` (bf16, K a multiple of 16, 16-byte aligned rows) in
     8-bit integers: ``(codes, scale)``, int8 ``[M, K]`` and fp32 ``[M]``.  A row's scale is
-    its largest magnitude over 127 (2^-126 at least), its codes the integers
-    nearest to ``x / scale``, ties to even: -127 to 127.  The scale of a row with an
-    infinity or NaN is NaN, and its codes are 0.  Made for ``gemm_int8``: of tokens,
+    its largest magnitude times 1 / 127, each rounded to fp32 (as torch's ``amax(1) / 127``
+    on a GPU; 2^-126 at least), its codes the integers nearest to ``x / scale``, ties to
+    even: -127 to 127.  The scale of a row with an infinity or NaN is NaN, and its codes are 0.  Made for ``gemm_int8``: of tokens,
     and of a weight's channels where they are rows."""
     import torch
 
