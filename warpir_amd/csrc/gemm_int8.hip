@@ -17,6 +17,7 @@ typedef long long i64;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 typedef signed char i8x16 __attribute__((ext_vector_type(16)));
 
@@ -134,17 +135,18 @@ struct Codes {
     }
   }
 
-  // The bytes from k on; whole: the row holds 128 more (else those past its end read as zeros).
+  // The wave's j-th load of the bytes from k on; whole: the rows hold 128 more (else those past their end read as zeros).
+  __device__ __forceinline__ void load(char* tile, int k, int width, int wave, int j) const {
+    const unsigned to = wir::lds_addr(tile + (wave + j * NW) * 1024);
+    if (k + 128 <= width)
+      wir::dma16_s(base + k, off[j], to);
+    else
+      wir::dma16_v(k + chunk[j] < width ? (const void*)(base + k + off[j]) : (const void*)wir::zero_page, to);
+  }
+
   __device__ __forceinline__ void load(char* tile, int k, int width, int wave) const {
-    const bool whole = k + 128 <= width;
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const unsigned to = wir::lds_addr(tile + (wave + j * NW) * 1024);
-      if (whole)
-        wir::dma16_s(base + k, off[j], to);
-      else
-        wir::dma16_v(k + chunk[j] < width ? (const void*)(base + k + off[j]) : (const void*)wir::zero_page, to);
-    }
+    for (int j = 0; j < EACH; ++j) load(tile, k, width, wave, j);
   }
 };
 
@@ -205,47 +207,50 @@ __device__ __forceinline__ void store_rows(const gemm_args& g, const wir::RTile<
     store_narrow<1>(g, t, row0, col0, stage);
 }
 
-// Output tiles of BM x BN, a wave's part WM x WN, over a ring of S tiles of 128
-// bytes of each row.
+// Output tiles of BM x BN over a ring of S tiles of 128 bytes of each row.  A
+// wave takes WM x WN of it, and of each row's bytes 1 / KW: KW waves have one
+// part of the output, whose sums they share out and add at the end.
 //
 // WHOLE: a wave's operands of the next tile are read while this one's products
 // run, from registers.  Without (parts whose operands do not fit twice): a
 // quarter of a tile ahead, and the last quarter's products run behind the
 // barrier that the next tile needs, under the reads of its first operands.
-template <int BM, int BN, int WM, int WN, int S, bool WHOLE>
+template <int BM, int BN, int WM, int WN, int KW, int S, bool WHOLE>
 __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
-  constexpr int NW = BM / WM * (BN / WN), RB = WM / 32, CB = WN / 32;
+  constexpr int PARTS = BM / WM * (BN / WN), NW = PARTS * KW, RB = WM / 32, CB = WN / 32, KS = 4 / KW;
+  constexpr int OC = KW > 1 ? CB / 2 : CB, OR = KW > 2 ? RB / 2 : RB, GIVEN = CB * RB - OC * OR;   // blocks that a wave finishes, and gives
+  static_assert(OC * OR * KW == CB * RB && (WHOLE || KW == 1), "the waves of a part finish it between them");
   typedef Codes<BM, NW> CA;
   typedef Codes<BN, NW> CBt;
   constexpr int SLOT = CA::T::BYTES + CBt::T::BYTES, EACH = CA::EACH + CBt::EACH;
-  constexpr int STAGE = (WM * WN > 32 * (WN + 4) ? WM * WN : 32 * (WN + 4)) * 2;   // bytes of a wave's output on its way
-  static_assert(NW * STAGE <= S * SLOT, "the output goes through the tiles' LDS");
+  constexpr int STAGE = (OR > 1 ? OR * 32 * OC * 32 : 32 * (OC * 32 + 4)) * 2;   // bytes of a wave's output on its way
+  static_assert(NW * STAGE <= S * SLOT && NW * GIVEN * 4096 <= S * SLOT, "the output goes through the tiles' LDS");
   __shared__ __attribute__((aligned(1024))) char smem[S * SLOT];
   const int nx = (g.n + BN - 1) / BN, ny = (g.m + BM - 1) / BM;
   int x, y;
   wir::grouped_tile<8>(wir::remap_xcd(blockIdx.x, nx * ny), nx, ny, x, y);
   const int wave = wir::wave_id(), lane = wir::lane_id();
-  const int row0 = wave / (BN / WN) * WM, col0 = wave % (BN / WN) * WN;
+  const int part = wave % PARTS, kw = wave / PARTS, row0 = part / (BN / WN) * WM, col0 = part % (BN / WN) * WN;
   CA a;
   CBt b;
   a.init(g.a, g.as, y * BM, g.m, wave);
   b.init(g.b, g.bs, x * BN, g.n, wave);
   const int steps = (g.k + 127) / 128;
-  auto load = [&](int t, int slot) {
+  auto load = [&](int t, int slot, int j) {
     char* at = smem + slot * SLOT;
-    a.load(at, t * 128, g.k, wave);
-    b.load(at + CA::T::BYTES, t * 128, g.k, wave);
+    if (j < CA::EACH) a.load(at, t * 128, g.k, wave, j);
+    else b.load(at + CA::T::BYTES, t * 128, g.k, wave, j - CA::EACH);
   };
   i32x16 acc[CB][RB];
 #pragma unroll
   for (int c = 0; c < CB; ++c)
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[c][r] = i32x16{};
-  constexpr int SETS = WHOLE ? 8 : 2;
+  constexpr int SETS = WHOLE ? 2 * KS : 2;
   bf16x8 fa[SETS][RB], fb[SETS][CB];
   // (the swizzle repeats every 16 rows: a step along the row is an exclusive or, blocks of 32 rows are offsets)
-  const unsigned a_at = wir::lds_addr(smem) + CA::T::chunk_off(row0 + lane % 32, lane / 32);
-  const unsigned b_at = wir::lds_addr(smem) + CA::T::BYTES + CBt::T::chunk_off(col0 + lane % 32, lane / 32);
+  const unsigned a_at = wir::lds_addr(smem) + CA::T::chunk_off(row0 + lane % 32, kw * KS * 2 + lane / 32);
+  const unsigned b_at = wir::lds_addr(smem) + CA::T::BYTES + CBt::T::chunk_off(col0 + lane % 32, kw * KS * 2 + lane / 32);
   typedef __attribute__((address_space(3))) bf16x8 lds_bf16x8;
   auto read = [&](int slot, int ks, int set) {
     const unsigned at = (a_at ^ ks * 32) + slot * SLOT, bt = (b_at ^ ks * 32) + slot * SLOT;
@@ -254,46 +259,62 @@ __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
 #pragma unroll
     for (int c = 0; c < CB; ++c) fb[set][c] = *(lds_bf16x8*)(bt + c * 32 * 128);
   };
-  auto products = [&](int set) {
+  // The products of a quarter of a tile; `between` them, the n-th of its calls behind the n-th.
+  auto products = [&](int set, auto between) {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int c = 0; c < CB; ++c)
 #pragma unroll
-      for (int r = 0; r < RB; ++r) acc[c][r] = mma(fb[set][c], fa[set][r], acc[c][r]);
+      for (int r = 0; r < RB; ++r) {
+        acc[c][r] = mma(fb[set][c], fa[set][r], acc[c][r]);
+        between(c * RB + r);
+      }
     __builtin_amdgcn_s_setprio(0);
   };
-  // Tile t + 1 has come, t + 2 .. t + S - 1 may be on their way; nobody reads tile t's slot any more: t + S goes there.
-  auto settle = [&](int t, int slot) {
+  // Tile t + 1 has come, t + 2 .. t + S - 1 may be on their way; nobody reads tile t's slot any more.
+  auto settle = [&](int t) {
     if (t + S <= steps) wir::wait_vm_barrier<(S - 2) * EACH>();
     else wir::wait_vm_barrier<0>();
-    if (t + S < steps) load(t + S, slot);
+  };
+  // Tile t + S goes to t's slot, in the shade of `all` products (a wave's loads queue: in a row before its products, they
+  // hold those back): those behind the n-th of them.
+  auto load_behind = [&](int t, int slot, int n, int all) {
+    if (t + S >= steps) return;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j)
+      if (j * all / EACH == n) load(t + S, slot, j);
+    __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll
   for (int t = 0; t < S; ++t)
-    if (t < steps) load(t, t);
+    if (t < steps)
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) load(t, t, j);
   if (steps >= S) wir::wait_vm_barrier<(S - 1) * EACH>();
   else wir::wait_vm_barrier<0>();
   int slot = 0;
   if (WHOLE) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) read(0, ks, ks);
+    for (int ks = 0; ks < KS; ++ks) read(0, ks, ks);
     auto step = [&](int t, int set) {
       const int next = slot == S - 1 ? 0 : slot + 1;
-      settle(t, slot);
+      settle(t);
       if (t + 1 < steps) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) read(next, ks, (4 - set) + ks);
+        for (int ks = 0; ks < KS; ++ks) read(next, ks, (KS - set) + ks);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) products(set + ks);
+      for (int ks = 0; ks < KS; ++ks)
+        products(set + ks, [&](int n) { load_behind(t, slot, ks * CB * RB + n, KS * CB * RB); });
       __builtin_amdgcn_sched_barrier(0);
       slot = next;
     };
     int t = 0;
     for (; t + 2 <= steps; t += 2) {
       step(t, 0);
-      step(t + 1, 4);
+      step(t + 1, KS);
     }
     if (t < steps) step(t, 0);
   } else {
@@ -304,34 +325,75 @@ __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
       for (int ks = 0; ks < 3; ++ks) {
         read(slot, ks + 1, (ks + 1) % 2);
         __builtin_amdgcn_sched_barrier(0);
-        products(ks % 2);
+        products(ks % 2, [](int) {});
         __builtin_amdgcn_sched_barrier(0);
       }
-      settle(t, slot);
+      settle(t);
       if (t + 1 < steps) read(next, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
-      products(1);
+      products(1, [&](int n) { load_behind(t, slot, n, CB * RB); });
       __builtin_amdgcn_sched_barrier(0);
       slot = next;
     }
   }
   if (WHOLE) wir::barrier();   // (the last tile's reads: the LDS takes the output)
-  // a lane holds row lane % 32 of each block of rows, 16 columns of each block of columns
-  const int lh = lane / 32;
-  wir::RTile<32, WM, WN> out;
+  const int c0 = KW > 1 ? kw % 2 * OC : 0, r0 = KW > 2 ? kw / 2 * OR : 0;   // of the wave's own blocks
+  if constexpr (KW > 1) {
+    // block `at` of the wave's in a row of those that wave `by` gives: not its own ones, in order
+    auto given = [&](int by, int c, int r) {
+      const int bc = by % 2, br = KW > 2 ? by / 2 : 0, at = c * RB + r;
+      const int before = KW > 2 ? at > bc * RB + br : c > bc ? RB : 0;   // its own ones before it
+      return (lds_i32x4*)wir::lds(smem + ((part * KW + by) * GIVEN + at - before) * 4096) + lane;
+    };
 #pragma unroll
-  for (int c = 0; c < CB; ++c)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 sb = scales_at(g.b_scale, x * BN + col0 + c * 32 + wir::ccol<32>(4 * q, lh), g.n);
+    for (int c = 0; c < CB; ++c)
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        const float sa = g.a_scale[min(y * BM + row0 + r * 32 + lane % 32, g.m - 1)];
+        if (c / OC == kw % 2 && (KW == 2 || r / OR == kw / 2)) continue;
+        auto* to = given(kw, c, r);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) to[q * 64] = i32x4{acc[c][r][4 * q], acc[c][r][4 * q + 1], acc[c][r][4 * q + 2], acc[c][r][4 * q + 3]};
+      }
+    wir::barrier();
+#pragma unroll
+    for (int c = 0; c < OC; ++c)
+#pragma unroll
+      for (int r = 0; r < OR; ++r) {
+        // (a wave's own blocks by selection: registers have no run-time index)
+        i32x16 sum = acc[c][r];
+#pragma unroll
+        for (int w = 1; w < KW; ++w)
+          if (kw == w) sum = acc[(w % 2) * OC + c][(KW > 2 ? w / 2 * OR : 0) + r];
+#pragma unroll
+        for (int w = 1; w < KW; ++w) {
+          const auto* from = given((kw + w) % KW, c0 + c, r0 + r);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const i32x4 x = from[q * 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[4 * q + i] += x[i];
+          }
+        }
+        acc[c][r] = sum;
+      }
+    wir::barrier();
+  }
+  // a lane holds row lane % 32 of each block of rows, 16 columns of each block of columns
+  const int lh = lane / 32, orow = y * BM + row0 + r0 * 32, ocol = x * BN + col0 + c0 * 32;
+  wir::RTile<32, 32 * OR, 32 * OC> out;
+#pragma unroll
+  for (int c = 0; c < OC; ++c)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 sb = scales_at(g.b_scale, ocol + c * 32 + wir::ccol<32>(4 * q, lh), g.n);
+#pragma unroll
+      for (int r = 0; r < OR; ++r) {
+        const float sa = g.a_scale[min(orow + r * 32 + lane % 32, g.m - 1)];
 #pragma unroll
         for (int i = 0; i < 4; ++i) out.f[c][r][4 * q + i] = (float)acc[c][r][4 * q + i] * sa * sb[i];
       }
     }
-  store_rows(g, out, y * BM + row0, x * BN + col0, smem + wave * STAGE);
+  store_rows(g, out, orow, ocol, smem + wave * STAGE);
 }
 
 // Few tokens, M <= 16 MT: a workgroup takes CH channels, its W waves every W-th
@@ -342,7 +404,6 @@ __device__ __forceinline__ void gemm_few(const gemm_args& g) {
   constexpr int CT = (CH + 15) / 16;
   typedef Codes<CH, 1> CB;
   typedef Codes<16 * MT, 1> CA;
-  typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
   typedef __attribute__((address_space(3))) int lds_int;
   constexpr int SLOT = CB::T::BYTES + CA::T::BYTES, EACH = CB::EACH + CA::EACH, SUMS = CT * MT * 1024;
   static_assert(CT * 16 * 128 <= SLOT && SUMS <= S * SLOT, "operands of channels past CH are read, and dropped");
@@ -428,12 +489,12 @@ QUANTIZE_KERNEL(wir_quantize_int8_w4_n4, 4, 4)
                                             amdgpu_waves_per_eu(WAVES_A_SIMD, WAVES_A_SIMD)))           \
   NAME(const gemm_args args) { gemm_tiled<__VA_ARGS__>(args); }
 
-GEMM_KERNEL(wir_gemm_int8_256, 512, 2, 256, 256, 128, 64, 2, false)
-GEMM_KERNEL(wir_gemm_int8_256x128, 512, 2, 256, 128, 64, 64, 3, true)
-GEMM_KERNEL(wir_gemm_int8_128_w4, 256, 2, 128, 128, 64, 64, 2, false)
-GEMM_KERNEL(wir_gemm_int8_128, 512, 2, 128, 128, 64, 32, 3, true)
-GEMM_KERNEL(wir_gemm_int8_128x64, 256, 2, 128, 64, 64, 32, 3, true)
-GEMM_KERNEL(wir_gemm_int8_64, 256, 2, 64, 64, 32, 32, 4, true)
+GEMM_KERNEL(wir_gemm_int8_256, 512, 2, 256, 256, 128, 64, 1, 2, false)
+GEMM_KERNEL(wir_gemm_int8_256x128, 512, 2, 256, 128, 64, 64, 1, 3, true)
+GEMM_KERNEL(wir_gemm_int8_128_w4, 256, 2, 128, 128, 64, 64, 1, 2, false)
+GEMM_KERNEL(wir_gemm_int8_128, 512, 2, 128, 128, 64, 64, 2, 3, true)
+GEMM_KERNEL(wir_gemm_int8_128x64, 256, 2, 128, 64, 64, 64, 2, 3, true)
+GEMM_KERNEL(wir_gemm_int8_64, 256, 2, 64, 64, 64, 64, 4, 4, true)
 
 #define FEW_KERNEL(NAME, MT, CH, W, S) \
   extern "C" __global__ void __launch_bounds__(64 * W) NAME(const gemm_args args) { gemm_few<MT, CH, W, S>(args); }
