@@ -117,6 +117,54 @@ GEMM = [(t, *int8._TILES[t][:3]) for t in int8._TILES] + [
     for r, c in ((16, 16), (16, 24), (16, 32), (16, 64), (32, 16), (32, 24), (32, 32), (64, 16), (64, 32))]
 
 
+@pytest.mark.parametrize("parts", [1, 2, 3, 7, 16])
+def test_gemm_divided(gpu, monkeypatch, parts):
+    """Sums over parts of K, of one step of 128 and more, the last part shorter."""
+    monkeypatch.setattr(int8, "_gemm_form", lambda m, n, k: ("64_split", 64, 64, 256))
+    monkeypatch.setattr(int8, "_gemm_plans", DevicePlans("gemm_int8"))
+    for m, n, k in ((1, 1, 16), (65, 3, 2000), (64, 64, 128 * 16), (130, 197, 6160), (100, 520, 128 * 33 + 16)):
+        steps = -(-k // 128)
+        each = -(-steps // min(parts, steps))
+        monkeypatch.setattr(int8, "_gemm_splits", lambda m, n, k: (-(-steps // each), each))
+        announce(f"gemm int8 {m} x {n} x {k} in {-(-steps // each)} parts")
+        operands = product._operands(m, n, k, m + n)
+        for _ in range(3):   # the call and its plan
+            product._check(api.gemm_int8(*operands), *operands)
+        wide = torch.full((m, n + 6), 5.0, dtype=torch.bfloat16, device="cuda")
+        assert torch.equal(api.gemm_int8(*operands, out=wide[:, 3:n + 3]), api.gemm_int8(*operands))
+        assert bool((wide[:, :3] == 5.0).all()) and bool((wide[:, n + 3:] == 5.0).all())
+
+
+def test_gemm_divided_extremes(gpu):
+    """The largest sums over parts of K, as the rules choose them."""
+    k = 131056
+    assert int8._gemm_form(66, 2, k)[0] == "64_split"
+    a = torch.full((66, k), -128, dtype=torch.int8, device="cuda")
+    b = torch.stack((torch.full((k,), -128, dtype=torch.int8), torch.full((k,), 127, dtype=torch.int8))).cuda()
+    sa, sb = torch.full((66,), 2.0, device="cuda"), torch.tensor([1.0, 0.5], device="cuda")
+    product._check(api.gemm_int8(a, b, sa, sb), a, b, sa, sb)
+
+
+def test_gemm_divided_graphs(gpu):
+    """Two graphs with a workspace each, replayed in turn with eager calls between them."""
+    m, n, k = 150, 300, 4096
+    assert int8._gemm_form(m, n, k)[0] == "64_split"
+    held = [product._operands(m, n, k, seed) for seed in (1, 2)]
+    want = [api.gemm_int8(*x) for x in held]
+    graphs = []
+    for x in held:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = api.gemm_int8(*x)
+        graphs.append((graph, out))
+    for i in range(6):
+        graph, out = graphs[i % 2]
+        graph.replay()
+        got = api.gemm_int8(*held[1 - i % 2])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i % 2]) and torch.equal(got, want[1 - i % 2])
+
+
 @pytest.mark.parametrize("form", GEMM, ids=lambda f: f[0])
 def test_gemm(gpu, monkeypatch, form):
     rows = form[1]

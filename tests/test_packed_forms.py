@@ -12,10 +12,14 @@ def test_product_tiles():
     named = {int8._gemm_form(m, n, k) for m in SIZES for n in (1, 64, 1000, 4096, 5000, 6144, 8192, 16384, 40000)
              for k in (16, 512, 4096, 14336)}
     assert {f[0] for f in named if f[0] in int8._TILES} == set(int8._TILES)
+    assert ("64_split", 64, 64, 256) in named
     assert all(f[1:] == int8._TILES[f[0]][:3] for f in named if f[0] in int8._TILES)
-    few = {f[0] for f in named if f[0] not in int8._TILES}
+    few = {f[0] for f in named if f[0] not in int8._TILES} - {"64_split"}
     assert few == {f"few{r}_c{c}" for r, c in ((16, 16), (16, 24), (16, 32), (16, 64), (32, 16), (32, 24), (32, 32), (64, 16),
                                                (64, 32))}
+    for m, n, k in ((100, 1024, 4096), (150, 300, 16384), (64, 64, 16384), (70, 16, 131056)):
+        steps, (splits, each) = -(-k // 128), int8._gemm_splits(m, n, k)
+        assert int8._gemm_form(m, n, k)[0] == "64_split" and splits > 1 and (splits - 1) * each < steps <= splits * each
     for m in range(1, 65):
         kernel, rows, columns, threads = int8._gemm_form(m, 4096, 4096)
         assert rows >= m and columns % 8 == 0 and threads in (256, 512)

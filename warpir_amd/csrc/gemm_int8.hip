@@ -112,8 +112,10 @@ struct gemm_args {
   const float* a_scale;   // [M]
   const float* b_scale;   // [N]
   bf16* out;              // [M, N]
+  int* partial;           // [splits][tile][32 x 32 block][1024]: sums over a part of K
   i64 as, bs, os;         // row strides
   int m, n, k;
+  int splits, each;       // parts of K, steps of 128 of one
 };
 
 // ROWS rows of a matrix of codes, 128 of each row's bytes a step, as a tile of 16-byte chunks in LDS.
@@ -207,6 +209,27 @@ __device__ __forceinline__ void store_rows(const gemm_args& g, const wir::RTile<
     store_narrow<1>(g, t, row0, col0, stage);
 }
 
+// Blocks of 32 x 32 sums from (row0, col0) on, the first OC x OR of acc, scaled and rounded, by way of `stage` in LDS.
+template <int OC, int OR, int CB, int RB>
+__device__ __forceinline__ void finish(const gemm_args& g, const i32x16 (&acc)[CB][RB], int row0, int col0, char* stage) {
+  // a lane holds row lane % 32 of each block of rows, 16 columns of each block of columns
+  const int lane = wir::lane_id();
+  wir::RTile<32, 32 * OR, 32 * OC> out;
+#pragma unroll
+  for (int c = 0; c < OC; ++c)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 sb = scales_at(g.b_scale, col0 + c * 32 + wir::ccol<32>(4 * q, lane / 32), g.n);
+#pragma unroll
+      for (int r = 0; r < OR; ++r) {
+        const float sa = g.a_scale[min(row0 + r * 32 + lane % 32, g.m - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out.f[c][r][4 * q + i] = (float)acc[c][r][4 * q + i] * sa * sb[i];
+      }
+    }
+  store_rows(g, out, row0, col0, stage);
+}
+
 // Output tiles of BM x BN over a ring of S tiles of 128 bytes of each row.  A
 // wave takes WM x WN of it, and of each row's bytes 1 / KW: KW waves have one
 // part of the output, whose sums they share out and add at the end.
@@ -215,7 +238,10 @@ __device__ __forceinline__ void store_rows(const gemm_args& g, const wir::RTile<
 // run, from registers.  Without (parts whose operands do not fit twice): a
 // quarter of a tile ahead, and the last quarter's products run behind the
 // barrier that the next tile needs, under the reads of its first operands.
-template <int BM, int BN, int WM, int WN, int KW, int S, bool WHOLE>
+//
+// SPLIT: of few tiles, a workgroup each for a part of K, whose sums
+// gemm_join adds (integers: in any order the same).
+template <int BM, int BN, int WM, int WN, int KW, int S, bool WHOLE, bool SPLIT = false>
 __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
   constexpr int PARTS = BM / WM * (BN / WN), NW = PARTS * KW, RB = WM / 32, CB = WN / 32, KS = 4 / KW;
   constexpr int OC = KW > 1 ? CB / 2 : CB, OR = KW > 2 ? RB / 2 : RB, GIVEN = CB * RB - OC * OR;   // blocks that a wave finishes, and gives
@@ -228,18 +254,20 @@ __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
   __shared__ __attribute__((aligned(1024))) char smem[S * SLOT];
   const int nx = (g.n + BN - 1) / BN, ny = (g.m + BM - 1) / BM;
   int x, y;
-  wir::grouped_tile<8>(wir::remap_xcd(blockIdx.x, nx * ny), nx, ny, x, y);
+  const int id = wir::remap_xcd(blockIdx.x, nx * ny * (SPLIT ? g.splits : 1)), split = SPLIT ? id / (nx * ny) : 0;
+  wir::grouped_tile<8>(id - split * nx * ny, nx, ny, x, y);
+  const int k0 = SPLIT ? split * g.each * 128 : 0, width = SPLIT ? min(g.k - k0, g.each * 128) : g.k;
   const int wave = wir::wave_id(), lane = wir::lane_id();
   const int part = wave % PARTS, kw = wave / PARTS, row0 = part / (BN / WN) * WM, col0 = part % (BN / WN) * WN;
   CA a;
   CBt b;
-  a.init(g.a, g.as, y * BM, g.m, wave);
-  b.init(g.b, g.bs, x * BN, g.n, wave);
-  const int steps = (g.k + 127) / 128;
+  a.init(g.a + k0, g.as, y * BM, g.m, wave);
+  b.init(g.b + k0, g.bs, x * BN, g.n, wave);
+  const int steps = (width + 127) / 128;
   auto load = [&](int t, int slot, int j) {
     char* at = smem + slot * SLOT;
-    if (j < CA::EACH) a.load(at, t * 128, g.k, wave, j);
-    else b.load(at + CA::T::BYTES, t * 128, g.k, wave, j - CA::EACH);
+    if (j < CA::EACH) a.load(at, t * 128, width, wave, j);
+    else b.load(at + CA::T::BYTES, t * 128, width, wave, j - CA::EACH);
   };
   i32x16 acc[CB][RB];
 #pragma unroll
@@ -378,22 +406,32 @@ __device__ __forceinline__ void gemm_tiled(const gemm_args& g) {
       }
     wir::barrier();
   }
-  // a lane holds row lane % 32 of each block of rows, 16 columns of each block of columns
-  const int lh = lane / 32, orow = y * BM + row0 + r0 * 32, ocol = x * BN + col0 + c0 * 32;
-  wir::RTile<32, 32 * OR, 32 * OC> out;
+  if constexpr (SPLIT) {
+    static_assert(OC * OR == 1, "");
+    auto* to = (i32x4*)(g.partial + ((i64)(split * ny * nx + y * nx + x) * NW + wave) * 1024) + lane;
 #pragma unroll
-  for (int c = 0; c < OC; ++c)
+    for (int q = 0; q < 4; ++q) to[q * 64] = i32x4{acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]};
+    return;
+  }
+  finish<OC, OR>(g, acc, y * BM + row0 + r0 * 32, x * BN + col0 + c0 * 32, smem + wave * STAGE);
+}
+
+// The sums of a 64 x 64 tile over the parts of K, a wave's block as gemm_tiled<64, 64, 64, 64, 4, ..> left it.
+__device__ __forceinline__ void gemm_join(const gemm_args& g) {
+  __shared__ __attribute__((aligned(1024))) char smem[4 * 32 * 36 * 2];
+  const int nx = (g.n + 63) / 64, ny = (g.m + 63) / 64, wave = wir::wave_id(), lane = wir::lane_id();
+  const auto* from = (const i32x4*)(g.partial + ((i64)blockIdx.x * 4 + wave) * 1024) + lane;
+  i32x16 acc[1][1] = {};
+  for (int split = 0; split < g.splits; ++split) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const f32x4 sb = scales_at(g.b_scale, ocol + c * 32 + wir::ccol<32>(4 * q, lh), g.n);
+      const i32x4 x = from[q * 64];
 #pragma unroll
-      for (int r = 0; r < OR; ++r) {
-        const float sa = g.a_scale[min(orow + r * 32 + lane % 32, g.m - 1)];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out.f[c][r][4 * q + i] = (float)acc[c][r][4 * q + i] * sa * sb[i];
-      }
+      for (int i = 0; i < 4; ++i) acc[0][0][4 * q + i] += x[i];
     }
-  store_rows(g, out, orow, ocol, smem + wave * STAGE);
+    from += (i64)nx * ny * 1024;
+  }
+  finish<1, 1>(g, acc, (int)blockIdx.x / nx * 64 + wave / 2 * 32, (int)blockIdx.x % nx * 64 + wave % 2 * 32, smem + wave * 32 * 36 * 2);
 }
 
 // Few tokens, M <= 16 MT: a workgroup takes CH channels, its W waves every W-th
@@ -495,6 +533,9 @@ GEMM_KERNEL(wir_gemm_int8_128_w4, 256, 2, 128, 128, 64, 64, 1, 2, false)
 GEMM_KERNEL(wir_gemm_int8_128, 512, 2, 128, 128, 64, 64, 2, 3, true)
 GEMM_KERNEL(wir_gemm_int8_128x64, 256, 2, 128, 64, 64, 64, 2, 3, true)
 GEMM_KERNEL(wir_gemm_int8_64, 256, 2, 64, 64, 64, 64, 4, 4, true)
+GEMM_KERNEL(wir_gemm_int8_64_split, 256, 2, 64, 64, 64, 64, 4, 4, true, true)
+
+extern "C" __global__ void __launch_bounds__(256) wir_gemm_int8_join(const gemm_args args) { gemm_join(args); }
 
 #define FEW_KERNEL(NAME, MT, CH, W, S) \
   extern "C" __global__ void __launch_bounds__(64 * W) NAME(const gemm_args args) { gemm_few<MT, CH, W, S>(args); }

@@ -20,8 +20,8 @@ class _QuantizeArgs(ctypes.Structure):
 
 
 class _Args(ctypes.Structure):
-    _fields_ = [*((n, ctypes.c_void_p) for n in ("a", "b", "a_scale", "b_scale", "out")),
-                *((n, ctypes.c_longlong) for n in ("as_", "bs", "os")), *((n, ctypes.c_int) for n in "mnk")]
+    _fields_ = [*((n, ctypes.c_void_p) for n in ("a", "b", "a_scale", "b_scale", "out", "partial")),
+                *((n, ctypes.c_longlong) for n in ("as_", "bs", "os")), *((n, ctypes.c_int) for n in ("m", "n", "k", "splits", "each"))]
 
 
 def _pitch(t) -> int:
@@ -114,11 +114,16 @@ def gemm_int8(a, b, a_scale, b_scale, out=None):
     if k == 0:
         return out.zero_()
     variant, bm, bn, threads = _gemm_form(m, n, k)
-    programs = -(-m // bm) * -(-n // bn)
-    need(fn, programs * threads < 1 << 32, "2^32 threads or more in one call")
-    launch(rec, device, "gemm_int8.hsaco", f"wir_gemm_int8_{variant}", (programs, 1, 1), (threads, 1, 1),
-           _Args(*[None] * 5, _pitch(a), _pitch(b), _pitch(out), m, n, k),
-           {"a": a, "b": b, "a_scale": a_scale, "b_scale": b_scale, "out": out})
+    tiles = -(-m // bm) * -(-n // bn)
+    need(fn, tiles * threads < 1 << 32, "2^32 threads or more in one call")
+    tensors = {"a": a, "b": b, "a_scale": a_scale, "b_scale": b_scale, "out": out}
+    splits, each = _gemm_splits(m, n, k) if variant == "64_split" else (1, 0)
+    args = _Args(*[None] * 6, _pitch(a), _pitch(b), _pitch(out), m, n, k, splits, each)
+    if variant == "64_split":
+        tensors["partial"] = rec.alloc(torch.empty(splits * tiles * bm * bn, dtype=torch.int32, device=device))
+    launch(rec, device, "gemm_int8.hsaco", f"wir_gemm_int8_{variant}", (splits * tiles, 1, 1), (threads, 1, 1), args, tensors)
+    if variant == "64_split":
+        launch(rec, device, "gemm_int8.hsaco", "wir_gemm_int8_join", (tiles, 1, 1), (threads, 1, 1), args, tensors)
     if rec:
         _gemm_plans.add(0, rec, out)
     return out
@@ -129,27 +134,42 @@ def gemm_int8(a, b, a_scale, b_scale, out=None):
 # rounds of them and a rest r (of 1), has
 #   step = light + busy * r                                  R = 0, or one whole round
 #        = full * R, plus the same line from light to full for the rest.
-# Least-squares fits (rms 5-9% in log time) to 43 products from 65 x 640 x 1680 to 8192 x 7816 x 7648; the tile with the
-# smallest estimate was within 1.3% (geometric mean; 17% at worst) of the fastest.
+# Least-squares fits (rms 4-8% in log time) to 33 products from 65 x 640 x 1680 to 8192 x 8192 x 8192; the tile with the
+# smallest estimate was within 0.7% (geometric mean; 14% at worst) of the fastest.
 _TILES = {
-    "256": (256, 256, 512, 1, (8.55, 1.448, 0.194, 2.027, 0.416)),
-    "256x128": (256, 128, 512, 1, (5.67, 0.937, 0.0, 1.133, 0.551)),
-    "128_w4": (128, 128, 256, 2, (4.97, 0.692, 0.399, 1.196, 0.443)),
-    "128": (128, 128, 512, 1, (3.82, 0.613, 0.0, 0.677, 0.684)),
-    "128x64": (128, 64, 256, 2, (3.89, 0.488, 0.260, 0.810, 0.511)),
-    "64": (64, 64, 256, 2, (3.65, 0.324, 0.203, 0.526, 0.696)),
+    "256": (256, 256, 512, 1, (7.14, 1.242, 0.302, 1.785, 0.339)),
+    "256x128": (256, 128, 512, 1, (4.42, 0.833, 0.137, 1.092, 0.333)),
+    "128_w4": (128, 128, 256, 2, (2.69, 0.816, 0.342, 1.234, 0.127)),
+    "128": (128, 128, 512, 1, (4.35, 0.519, 0.0, 0.631, 0.620)),
+    "128x64": (128, 64, 256, 2, (3.62, 0.447, 0.135, 0.717, 0.421)),
+    "64": (64, 64, 256, 2, (3.52, 0.311, 0.094, 0.446, 0.920)),
 }
 
 
-def _estimate(tile: str, m: int, n: int, k: int) -> float:
+def _estimate(tile: str, m: int, n: int, k: int, splits: int = 1) -> float:
     bm, bn, _, held, (fixed, light, busy, full, per_mn) = _TILES[tile]
-    rounds, rest = divmod(-(-m // bm) * -(-n // bn), 256 * held)
+    programs = -(-m // bm) * -(-n // bn) * splits
+    rounds, rest = divmod(programs, 256 * held)
     rest /= 256 * held
     if rounds == 0 or (rounds == 1 and rest == 0):
         step = light + busy * (rounds + rest)
     else:
         step = full * rounds + (light + (full - light) * rest if rest else 0.0)
-    return fixed + -(-k // 128) * step + per_mn * 1e-6 * m * n
+    us = fixed + -(--(-k // 128) // splits) * step
+    return us + per_mn * 1e-6 * m * n if splits == 1 else us + 1.78 + 0.323 * splits + 0.00816 * programs
+
+
+@functools.lru_cache(maxsize=1024)
+def _gemm_splits(m: int, n: int, k: int) -> Tuple[int, int]:
+    """(parts, steps of 128 of one) of a product whose K is divided: at most what a round of workgroups holds.
+
+    us by parts: 150 x 300 x 16384 1 45.0, 2 26.6, 4 17.2, 8 13.8, 16 14.9; 100 x 1024 x 4096 14.1, 11.6, 10.3, 11.2,
+    15.4; 512 x 512 x 8192 23.9, 17.2, 14.1, 17.1, 24.3; 512 x 512 x 2048 8.9, 9.7, 10.1, 14.6; 200 x 4096 x 4096 14.4, 17.1."""
+    steps, tiles = -(-k // 128), -(-m // 64) * -(-n // 64)
+    splits = min((s for s in (1, 2, 3, 4, 6, 8, 12, 16) if s <= steps and (s == 1 or s * tiles <= 512)),
+                 key=lambda s: _estimate("64", m, n, k, s))
+    each = -(-steps // splits)
+    return -(-steps // each), each
 
 
 @functools.lru_cache(maxsize=1024)
@@ -162,13 +182,23 @@ def _gemm_form(m: int, n: int, k: int) -> Tuple[str, int, int, int]:
     workgroup, 16 tokens: N = 4096, K = 4096 6.2 / 6.6 / 6.7 / 8.8, 6144 x 4096 8.8 / 7.4 /
     7.8 / 9.3, 8192 x 8192 16.1 / 18.3 / 13.6 / 16.9, 32768 x 4096 36.8 / 35.0 / 33.3 / 29.5 (64 x 64
     tiles 14.8, 15.1, 27.2, 31.9); 64 tokens, 16 / 32 channels: 4096 x 4096 8.4 / 10.0, 8192 x 8192
-    25.3 / 19.1 (tiles 15.4, 27.2)."""
+    25.3 / 19.1 (tiles 15.4, 27.2).
+
+    Few tiles of 64 x 64 with a long K are divided along it, and a second kernel
+    joins the sums (`_gemm_splits`); with up to 4096 channels for 33 to 64 tokens too (us,
+    undivided / divided: 64 x 1024, K = 4096 7.2 / 9.8, 8192 about 11.5 / 12, 16384 20.8 / 14.1)."""
+    splits = _gemm_splits(m, n, k)[0]
+    divided = _estimate("64", m, n, k, splits) if splits > 1 else float("inf")
+    if 32 < m <= 64 and n <= 4096 and divided < 2.9 + 0.14 * -(-k // 128):
+        return "64_split", 64, 64, 256
     if m <= 64:
         rows = 16 if m <= 16 else 32 if m <= 32 else 64
         columns = 16 if n <= 4096 else 24 if n <= 6144 and rows < 64 else 64 if n >= 16384 and rows == 16 else 32
         waves = 4 if rows == 64 or (rows, columns) == (32, 32) else 8
         return f"few{rows}_c{columns}", rows, columns, 64 * waves
     tile = min(_TILES, key=lambda t: _estimate(t, m, n, k))
+    if divided < _estimate(tile, m, n, k):
+        return "64_split", 64, 64, 256
     return (tile, *_TILES[tile][:3])
 
 
