@@ -29,11 +29,11 @@ using wir::i64;
 //
 // Measured: 8 x 4096 tokens, 32/8 heads of 128: 1.80 ms (1220 TFLOP/s), causal
 // 1.00 ms (1100; with four waves 1.84 and 1.02); 16 heads of 64: 0.57 ms (970), 64
-// x 512 tokens 97 us (700).  At D = 128, causal, matrix instructions run in 64% of
-// the cycles.  An operand from LDS serves the 32 rows of one wave: 1 KB in the 32
-// cycles of a product, so that four SIMDs at full rate would take all of LDS's 128
-// bytes a cycle and leave the tiles' writes none.  Of 950 us (16 heads of 128, 8 x
-// 4096) the exponentials are 63 and the tiles' loads 105, both 177.  At D = 64 the
+// x 512 tokens 97 us (700).  At D = 128 LDS bounds it: an operand of 1 KB serves
+// the 32 rows of one wave, a product of 32 cycles, and takes LDS 8 cycles as it
+// lies and 16 transposed, so that four SIMDs' products of both kinds, 64 cycles,
+// ask for 96 of its cycles: matrix instructions run in 64% of them, causal.  Of 950
+// us (16 heads of 128, 8 x 4096) the exponentials are 63, the tiles' loads 105, both 177.  At D = 64 the
 // exponentials weigh twice as much (matrix instructions 38% of the cycles in 48
 // sequences of up to 1024 tokens), and short sequences pay 5 us a round of
 // workgroups for the first tile's way from memory and the last store.  Not faster:

@@ -23,9 +23,9 @@ constexpr int WAVES = wir::PACKED_WAVES, ROWS = wir::PACKED_ROWS;
 //
 // Measured: 8 x 4096 tokens, 16 heads of 128: 1.37 ms (its three products 1200
 // TFLOP/s), causal 0.78; 64 x 512 tokens, 16 heads of 64: 0.14 ms (720).  At D =
-// 128 matrix instructions run in 69% of the cycles; LDS has to read 1 KB for each,
-// as in the forward.  Tiles of 32 keys, because three of K and two of V of 64 would
-// leave room for one workgroup a CU.
+// 128 LDS bounds it, as the forward: four SIMDs' three products, 96 cycles, ask for
+// 128 of its cycles, and matrix instructions run in 69% of them.  Tiles of 32 keys,
+// because three of K and two of V of 64 would leave room for one workgroup a CU.
 template <int D, bool CAUSAL>
 struct Dq {
   static constexpr int KT = 32, AHEAD = 5, KS = D / 16, CB = D / 32;
@@ -355,9 +355,12 @@ __device__ __forceinline__ bool dkdv_block(const wir::packed_bwd_args& a, const 
 //
 // For D = 128: 8 x 4096 tokens, 16 heads: 2.1 ms (four products, 1050 TFLOP/s),
 // causal 1.27; 4 x 4096, 32/8 heads, causal 1.05 (all of it in a wave, one wave a
-// SIMD, 1.56).  Matrix instructions run in 55% of the cycles.  LDS reads 1 KB for
-// each of them and a quarter of that for what the waves hand on, which with the
-// tiles' writes caps them at 74%.
+// SIMD, 1.56).  LDS bounds it: of a tile's operands the waves take 16 KB each as
+// they lie, 16 KB transposed (at half the rate) and 4 KB that they hand on, which
+// with the tile's writes are 3584 cycles for 2048 of products; matrix instructions
+// run in 55% of the cycles, and without the tiles' loads it is 5% faster.  Tiles
+// from the last one down, so that workgroups share them in L2, take a 28th of the
+// bytes from memory and as long (D = 64: 10% longer).
 template <int D, bool CAUSAL>
 struct Paired {
   static constexpr int NW = 8, QT = 64, AHEAD = 5, KS = D / 16, CB = D / 32;
