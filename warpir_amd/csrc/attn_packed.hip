@@ -128,10 +128,7 @@ struct Forward {
   __device__ __forceinline__ void softmax(int t) {
     constexpr float c = wir::PackedScale<D>::c;
     const int col0 = t * TILE;
-    if (CAUSAL ? col0 + TILE - 1 > row0 : col0 + TILE > r.len) {
-      wir::seldom();
-      wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
-    }
+    if (CAUSAL ? col0 + TILE - 1 > row0 : col0 + TILE > r.len) wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
     float sum = exponentials();   // (not a number before the first tile, whose m is -inf)
     if (__builtin_amdgcn_ballot_w64(!(sum <= LIMIT)) != 0) {
       wir::seldom();

@@ -21,14 +21,14 @@ constexpr int WAVES = wir::PACKED_WAVES, ROWS = wir::PACKED_ROWS;
 // one stream of LDS reads that runs AHEAD products before their use.  dS is
 // rounded to bf16 as the product's operand; P, dO . v and the sums are fp32.
 //
-// Measured: 8 x 4096 tokens, 16 heads of 128: 1.37 ms (its three products 1200
-// TFLOP/s), causal 0.78; 64 x 512 tokens, 16 heads of 64: 0.14 ms (720).  At D =
+// Measured: 8 x 4096 tokens, 16 heads of 128: 1.31 ms (its three products 1260
+// TFLOP/s), causal 0.72; 64 x 512 tokens, 16 heads of 64: 0.14 ms (740).  At D =
 // 128 LDS bounds it, as the forward: four SIMDs' three products, 96 cycles, ask for
 // 128 of its cycles, and matrix instructions run in 69% of them.  Tiles of 32 keys,
 // because three of K and two of V of 64 would leave room for one workgroup a CU.
 template <int D, bool CAUSAL>
 struct Dq {
-  static constexpr int KT = 32, AHEAD = 5, KS = D / 16, CB = D / 32;
+  static constexpr int KT = 32, AHEAD = D == 64 ? 3 : 5, KS = D / 16, CB = D / 32;
   static constexpr int SCORES = 2 * KS, PRODUCTS = KT / 16 * CB;   // products of a wave for a tile
   typedef wir::STile<KT, D, wir::BOTH> TK;
   typedef wir::STile<KT, D, wir::ROWREAD> TV;
@@ -102,11 +102,10 @@ struct Dq {
       dp.f[0][0][i] *= s.f[0][0][i];
     }
     if (CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len) {   // (a value that a row does not see may be NaN)
-      wir::seldom();
-      const int row = row0 + lane % 32;
+      const int row = row0 + lane % 32, half = wir::seldom(lane / 32);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int col = col0 + wir::ccol<32>(i, lane / 32);
+        const int col = col0 + wir::ccol<32>(i, half);
         dp.f[0][0][i] = (CAUSAL ? col <= row : col < r.len) ? dp.f[0][0][i] : 0.f;
       }
     }
@@ -226,124 +225,219 @@ __device__ __forceinline__ void dq_kernel(const wir::packed_bwd_args& a) {
 
 // dK and dV of one block of 128 keys, 32 a wave, over the tiles of QT queries of
 // the group's heads one after another (so the sums over a group are in one wave's
-// registers, in an order that the lengths fix).  P and dS are rounded to bf16 as
-// the products' operands.
+// registers, in an order that the lengths fix).  In the time of a tile t a wave
+// takes the products of P and dS of t - 1 with dO and Q, the scores of t, q . k
+// and v . dO in turn, and their exponentials; the operands of both are one
+// stream of LDS reads that runs AHEAD products before their use.  P and dS are
+// rounded to bf16 as the products' operands.
 //
-// For D = 64, where both sums fit with two waves a SIMD.  64 x 512 tokens, 16 heads:
-// 0.21 ms (650 TFLOP/s); 8 x 4096, 32 heads, causal 1.26-1.39 (as pairs of waves,
-// below, 1.70).
+// For D = 64, where both sums fit with two waves a SIMD.  8 x 4096 tokens, 32 heads:
+// 1.94 ms (four products, 1130 TFLOP/s), causal 1.21; 64 x 512, 16 heads 0.17 (815).
+// (Tiles of 32 queries 2.2, 1.39 and 0.18 ms; pairs of waves as below 1.70, causal.)
 template <int D, int QT, bool CAUSAL>
-__device__ __forceinline__ bool dkdv_block(const wir::packed_bwd_args& a, const wir::Rows& r, int kv, char* smem, bool careful) {
+struct Dkdv {
+  static constexpr int AHEAD = 4, KS = D / 16, CB = D / 32, QB = QT / 32;
+  static constexpr int SCORES = 2 * KS * QB, PRODUCTS = 2 * CB * (QT / 16);   // products of a wave for a tile
   typedef wir::STile<QT, D, wir::BOTH> T;
-  constexpr float c = wir::PackedScale<D>::c;
-  static_assert(WAVES * 32 * D * 2 <= 4 * T::BYTES, "the outputs go through the tiles' LDS");
-  constexpr int VEC = 4 * T::BYTES, ODD = VEC + 4 * QT * 4;
-  const int wave = wir::wave_id(), lane = wir::lane_id();
-  const int row0 = r.row0 + wave * 32;
-  const int first = CAUSAL ? r.row0 / QT : 0, tiles = (r.len + QT - 1) / QT;
-  wir::HeadTiles<T> Q, G;
-  Q.init(a.q + r.start * a.qt, a.qt, r.len);
-  G.init(a.d_o + r.start * a.gt, a.gt, r.len);
-  auto load = [&](int head, int t, int slot) {
-    char* at = smem + slot * T::BYTES;
-    Q.base = (const char*)(a.q + head * a.qh + r.start * a.qt);
-    G.base = (const char*)(a.d_o + head * a.gh + r.start * a.gt);
-    Q.load(at, t, wave);
-    G.load(at + 2 * T::BYTES, t, wave);
-    if (wave < 2 && lane < QT) {   // a wave each for the LSEs and the D_p
-      const float* from = a.stats + ((i64)(wave * a.heads + head) * a.tokens + r.start);
-      wir::dma4_v(from + min(t * QT + lane, r.len - 1), wir::lds_addr(smem + VEC + (2 * wave + slot) * QT * 4));
-    }
+  typedef __attribute__((address_space(3))) wir::bf16x8 lds_bf16x8;
+  typedef __attribute__((address_space(3))) wir::i16x4 lds_i16x4;
+  typedef __attribute__((address_space(3))) wir::f32x4 lds_f32x4;
+  typedef __attribute__((address_space(3))) wir::Odd<D> lds_odd;
+  // LDS: three slots of a Q and a dO tile, the tiles' statistics, notes of what is odd
+  static constexpr int SLOT = 2 * T::BYTES, VEC = 3 * SLOT, ODD = VEC + 3 * 2 * QT * 4, BYTES = ODD + 2 * sizeof(wir::Odd<D>);
+  static_assert(WAVES * 32 * D * 2 <= VEC, "the outputs go through the tiles' LDS");
+
+  struct At {
+    int head, t;
   };
-  auto* odd = (__attribute__((address_space(3))) wir::Odd<D>*)wir::lds(smem + ODD);
-  if (careful) wir::no_odd<true, WAVES>(odd), wir::no_odd<true, WAVES>(odd + 1);
-  wir::RowFrags<32, 1, D / 16> k, v;
-  wir::packed_rows(k, a.k + kv * a.kh + r.start * a.kt, a.kt, row0, r.len);
-  wir::packed_rows(v, a.v + kv * a.vh + r.start * a.vt, a.vt, row0, r.len);
+
+  const wir::packed_bwd_args& a;
+  const wir::Rows& r;
+  char* smem;
+  int wave, lane, row0, first, tiles;
+  wir::HeadTiles<T> Q, G;
+  unsigned row_at, tr_at;          // the lane's places in a tile, as operands of the scores and of the products
+  wir::RowFrags<32, 1, KS> k, v;
   wir::RTile<32, 32, D> dk, dv;
-  wir::fill(dk, 0.f);
-  wir::fill(dv, 0.f);
-  int head = kv * a.group, t = first, slot = 0;
-  const int last = head + a.group;
-  load(head, t, 0);
-  while (head < last) {
-    int head1 = head, t1 = t + 1;   // the next tile
-    if (t1 == tiles) ++head1, t1 = first;
-    char *qt = smem + slot * T::BYTES, *dot = qt + 2 * T::BYTES;
-    const int col0 = t * QT;
-    wir::wait_vm_barrier<0>();
-    if (head1 < last) load(head1, t1, slot ^ 1);
-    if (!CAUSAL || careful || col0 + QT - 1 >= row0) {   // (else no row of the wave is seen from the tile)
-      wir::RTile<32, 32, QT> s, dp;
-      wir::BTile<32, 32, QT> pb, ds;
-      wir::CVec<32, QT> lse, dots;
-      wir::load_cvec_lds(lse, smem + VEC + slot * QT * 4, 0);
-      wir::load_cvec_lds(dots, smem + VEC + (2 + slot) * QT * 4, 0);
-      wir::mma_ABt_frags<32, 32, QT, T, D / 16>(s, k, qt, 0);
-      wir::mma_ABt_frags<32, 32, QT, T, D / 16>(dp, v, dot, 0);
-#pragma unroll
-      for (int cb = 0; cb < QT / 32; ++cb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f((s.f[cb][0][i] + lse.v[cb][i]) * c);
-          dp.f[cb][0][i] = p * (dp.f[cb][0][i] + dots.v[cb][i]);
-          s.f[cb][0][i] = p;
-        }
-      // (a query that does not see the row may hold NaN; past the end the last one stands again)
-      if ((CAUSAL && col0 < row0 + 31) || col0 + QT > r.len) {
-        wir::seldom();
-#pragma unroll
-        for (int cb = 0; cb < QT / 32; ++cb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int col = col0 + cb * 32 + wir::ccol<32>(i, lane / 32);
-            const bool seen = (!CAUSAL || row0 + lane % 32 <= col) && col < r.len;
-            s.f[cb][0][i] = seen ? s.f[cb][0][i] : 0.f;
-            dp.f[cb][0][i] = seen ? dp.f[cb][0][i] : 0.f;
-          }
-      }
-      wir::to_bf16(pb, s);
-      wir::to_bf16(ds, dp);
-      if (careful) {
-        wir::barrier();
-        wir::clear_odd<true, WAVES, T>(qt, col0, odd);
-        wir::clear_odd<true, WAVES, T>(dot, col0, odd + 1);
-        wir::barrier();
-      }
-      wir::mma_rAB<32, 32, QT, D, T>(dv, pb, dot, 0);
-      wir::mma_rAB<32, 32, QT, D, T>(dk, ds, qt, 0);
+  wir::RTile<32, 32, QT> s, dp;
+  wir::BTile<32, 32, QT> pb, ds;
+
+  __device__ __forceinline__ Dkdv(const wir::packed_bwd_args& args, const wir::Rows& rows, char* lds) : a(args), r(rows), smem(lds) {}
+
+  __device__ __forceinline__ At after(At i) const { return i.t + 1 < tiles ? At{i.head, i.t + 1} : At{i.head + 1, first}; }
+
+  __device__ __forceinline__ void load(At i, int slot) {
+    char* at = smem + slot * SLOT;
+    Q.base = (const char*)(a.q + i.head * a.qh + r.start * a.qt);
+    G.base = (const char*)(a.d_o + i.head * a.gh + r.start * a.gt);
+    Q.load(at, i.t, wave);
+    G.load(at + T::BYTES, i.t, wave);
+    if (wave < 2 && lane < QT) {   // a wave each for the two statistics
+      const float* from = a.stats + ((i64)(wave * a.heads + i.head) * a.tokens + r.start);
+      wir::dma4_v(from + min(i.t * QT + lane, r.len - 1), wir::lds_addr(smem + VEC + (2 * slot + wave) * QT * 4));
     }
-    head = head1, t = t1, slot ^= 1;
   }
-  if (!careful) {
-    const bool in = row0 + lane % 32 < r.len, nan = wir::has_nan(dk, in) || wir::has_nan(dv, in);
-    if (wir::any_wave(nan, smem + ODD)) return true;
-  } else {
-    wir::wait_vm_barrier<0>();
+
+  // The scores' sums begin with the statistics: p = exp2(c (q . k - LSE sqrt(D))), dP - D_p = dO . v - D_p.
+  __device__ __forceinline__ void begin_scores(int slot) {
+    const auto* vec = (lds_f32x4*)wir::lds(smem + VEC + 2 * slot * QT * 4 + lane / 32 * 16);
+#pragma unroll
+    for (int cb = 0; cb < QB; ++cb)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const wir::f32x4 x0 = vec[8 * cb + 2 * g], x1 = vec[QT / 4 + 8 * cb + 2 * g];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s.f[cb][0][4 * g + j] = x0[j], dp.f[cb][0][4 * g + j] = x1[j];
+      }
   }
+
+  // The products of the tile in `before` (PRODUCT) and the scores of that in `slot` (SCORE).
+  template <bool PRODUCT, bool SCORE>
+  __device__ __forceinline__ void stream(int slot, int before) {
+    constexpr int N0 = PRODUCT ? PRODUCTS : 0, N = N0 + (SCORE ? SCORES : 0);
+    const unsigned from = tr_at + before * SLOT, rows = row_at + slot * SLOT;
+    wir::bf16x8 ring[AHEAD + 1];
+    auto read = [&](auto at) {
+      constexpr int n = decltype(at)::value, i = n - N0;
+      if constexpr (n < N0) {   // dO for dV and Q for dK in turn
+        constexpr int cb = n / 2 % CB, down = n / 2 / CB * 16 * D * 2;   // (two groups of eight rows)
+        const unsigned tile = (from + (n % 2 ? 0 : T::BYTES)) ^ (cb * 64);
+        const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + down));
+        const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)((tile ^ 32) + down + 8 * D * 2));
+        ring[n % (AHEAD + 1)] = wir::cat(__builtin_bit_cast(wir::bf16x4, lo), __builtin_bit_cast(wir::bf16x4, hi));
+      } else {                  // Q and dO in turn
+        ring[n % (AHEAD + 1)] = *(lds_bf16x8*)((rows ^ (i / 2 % KS * 32)) + i % 2 * T::BYTES + i / 2 / KS * 32 * D * 2);
+      }
+    };
+    if (SCORE) begin_scores(slot);
+    __builtin_amdgcn_s_setprio(1);
+    wir::static_for<0, AHEAD>(read);
+    wir::static_for<0, N>([&](auto at) {
+      constexpr int n = decltype(at)::value, i = n - N0;
+      if constexpr (n + AHEAD < N) read(wir::ic<n + AHEAD>{});
+      __builtin_amdgcn_sched_barrier(0);
+      const wir::bf16x8& b = ring[n % (AHEAD + 1)];
+      if constexpr (n < N0) {
+        constexpr int cb = n / 2 % CB, g = 2 * (n / 2 / CB);
+        auto& acc = n % 2 ? dk : dv;
+        const auto& x = n % 2 ? ds : pb;
+        acc.f[cb][0] = wir::MF<32>::mma(b, wir::cat(x.f[g / 4][0][g % 4], x.f[g / 4][0][g % 4 + 1]), acc.f[cb][0]);
+      } else if constexpr (i % 2 == 0) {
+        s.f[i / 2 / KS][0] = wir::MF<32>::mma(b, k.f[0][i / 2 % KS], s.f[i / 2 / KS][0]);
+      } else {
+        dp.f[i / 2 / KS][0] = wir::MF<32>::mma(b, v.f[0][i / 2 % KS], dp.f[i / 2 / KS][0]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  __device__ __forceinline__ void finish_scores(int t) {
+    constexpr float c = wir::PackedScale<D>::c;
+    const int col0 = t * QT;
 #pragma unroll
-  for (int cb = 0; cb < D / 32; ++cb)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dk.f[cb][0][i] *= wir::PackedScale<D>::s;
-  if (careful) {
-    const int row = CAUSAL ? row0 + lane % 32 : 0;   // the first query that sees it
-#pragma unroll
-    for (int cb = 0; cb < D / 32; ++cb)
+    for (int cb = 0; cb < QB; ++cb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
-        const int end_k = max(odd->at[0][d], max(odd->at[1][d], odd->at[2][d]));
-        const int end_v = max(odd[1].at[0][d], max(odd[1].at[1][d], odd[1].at[2][d]));
-        dk.f[cb][0][i] = row <= end_k ? __builtin_nanf("") : dk.f[cb][0][i];
-        dv.f[cb][0][i] = row <= end_v ? __builtin_nanf("") : dv.f[cb][0][i];
+        s.f[cb][0][i] = __builtin_amdgcn_exp2f(s.f[cb][0][i] * c);
+        dp.f[cb][0][i] *= s.f[cb][0][i];
       }
+    // (a query that does not see the row may hold NaN; past the end the last one stands again)
+    if ((CAUSAL && col0 < row0 + 31) || col0 + QT > r.len) {
+      const int half = wir::seldom(lane / 32);
+#pragma unroll
+      for (int cb = 0; cb < QB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int col = col0 + cb * 32 + wir::ccol<32>(i, half);
+          const bool seen = (!CAUSAL || row0 + lane % 32 <= col) && col < r.len;
+          s.f[cb][0][i] = seen ? s.f[cb][0][i] : 0.f;
+          dp.f[cb][0][i] = seen ? dp.f[cb][0][i] : 0.f;
+        }
+    }
+    wir::to_bf16(pb, s);
+    wir::to_bf16(ds, dp);
   }
-  char* stage = smem + wave * 32 * D * 2;
-  wir::store_tile_staged<true>(wir::packed_head(a.dk, a.dkh, a.dkt, kv, r.start, r.len, D), dk, 0, 0, row0, 0, stage);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the wave's own part of the LDS: its reads are done)
-  wir::store_tile_staged<true>(wir::packed_head(a.dv, a.dvh, a.dvt, kv, r.start, r.len, D), dv, 0, 0, row0, 0, stage);
-  return false;
-}
+
+  __device__ __forceinline__ bool run(int kv, bool careful) {
+    wave = wir::wave_id(), lane = wir::lane_id();
+    row0 = r.row0 + wave * 32;
+    first = CAUSAL ? r.row0 / QT : 0, tiles = (r.len + QT - 1) / QT;
+    Q.init(a.q + r.start * a.qt, a.qt, r.len);
+    G.init(a.d_o + r.start * a.gt, a.gt, r.len);
+    const int part = lane % 16;   // of the transposed reads
+    row_at = wir::lds_addr(smem) + T::chunk_off(lane % 32, lane / 32);
+    tr_at = wir::lds_addr(smem) + T::elem_off(lane / 32 * 4 + part / 4, lane % 32 / 16 * 16 + 4 * (part % 4));
+    auto* odd = (lds_odd*)wir::lds(smem + ODD);
+    if (careful) wir::no_odd<true, WAVES>(odd), wir::no_odd<true, WAVES>(odd + 1);
+    At now{kv * a.group, first};
+    const int end = now.head + a.group;
+    const int mine = row0 >= r.len ? tiles : CAUSAL ? row0 / QT : first;   // the first tile with queries that see the wave's rows
+    load(now, 0);
+    wir::packed_rows(k, a.k + kv * a.kh + r.start * a.kt, a.kt, row0, r.len);
+    wir::packed_rows(v, a.v + kv * a.vh + r.start * a.vt, a.vt, row0, r.len);
+    wir::fill(dk, 0.f);
+    wir::fill(dv, 0.f);
+    int slot = 0, before = 2;   // of the tile, of the one before
+    auto settle = [&]() {       // the tile has come, the next one is asked for
+      const At next = after(now);
+      wir::wait_vm_barrier<0>();
+      if (next.head < end) load(next, slot == 2 ? 0 : slot + 1);
+    };
+    auto step = [&]() {
+      const int t = now.t;
+      now = after(now), before = slot, slot = slot == 2 ? 0 : slot + 1;
+      settle();
+      if (careful) {
+        wir::clear_odd<true, WAVES, T>(smem + before * SLOT, t * QT, odd);
+        wir::clear_odd<true, WAVES, T>(smem + before * SLOT + T::BYTES, t * QT, odd + 1);
+        wir::barrier();
+      }
+    };
+    settle();
+    while (now.head < end) {
+      const int head = now.head;
+      while (now.head == head && now.t < mine) step();
+      if (now.head != head) continue;
+      stream<false, true>(slot, before);
+      finish_scores(now.t);
+      for (step(); now.head == head; step()) {
+        stream<true, true>(slot, before);
+        finish_scores(now.t);
+      }
+      stream<true, false>(slot, before);
+    }
+    const int row = row0 + lane % 32;
+    if (!careful) {
+      const bool in = row < r.len, nan = wir::has_nan(dk, in) || wir::has_nan(dv, in);
+      if (wir::any_wave(nan, smem + ODD)) return true;
+    } else {
+      wir::wait_vm_barrier<0>();
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk.f[cb][0][i] *= wir::PackedScale<D>::s;
+    if (careful) {
+      const int from = CAUSAL ? row : 0;   // the first query that sees it
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
+          const int end_k = max(odd->at[0][d], max(odd->at[1][d], odd->at[2][d]));
+          const int end_v = max(odd[1].at[0][d], max(odd[1].at[1][d], odd[1].at[2][d]));
+          dk.f[cb][0][i] = from <= end_k ? __builtin_nanf("") : dk.f[cb][0][i];
+          dv.f[cb][0][i] = from <= end_v ? __builtin_nanf("") : dv.f[cb][0][i];
+        }
+    }
+    char* stage = smem + wave * 32 * D * 2;
+    wir::store_tile_staged<true>(wir::packed_head(a.dk, a.dkh, a.dkt, kv, r.start, r.len, D), dk, 0, 0, row0, 0, stage);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the wave's own part of the LDS: its reads are done)
+    wir::store_tile_staged<true>(wir::packed_head(a.dv, a.dvh, a.dvt, kv, r.start, r.len, D), dv, 0, 0, row0, 0, stage);
+    return false;
+  }
+};
 
 // The same with eight waves, of which two share 32 keys: one takes the scores of
 // a tile's first 32 queries and dV, the other those of its last 32 and dK.  A
@@ -353,8 +447,8 @@ __device__ __forceinline__ bool dkdv_block(const wir::packed_bwd_args& a, const 
 // tile t and the scores of tile t + 1, in opposite orders.  The operands of both
 // are one stream of LDS reads that runs AHEAD products before their use.
 //
-// For D = 128: 8 x 4096 tokens, 16 heads: 2.1 ms (four products, 1050 TFLOP/s),
-// causal 1.27; 4 x 4096, 32/8 heads, causal 1.05 (all of it in a wave, one wave a
+// For D = 128: 8 x 4096 tokens, 16 heads: 2.03 ms (four products, 1080 TFLOP/s),
+// causal 1.21; 4 x 4096, 32/8 heads, causal 1.05 (all of it in a wave, one wave a
 // SIMD, 1.56).  LDS bounds it: of a tile's operands the waves take 16 KB each as
 // they lie, 16 KB transposed (at half the rate) and 4 KB that they hand on, which
 // with the tile's writes are 3584 cycles for 2048 of products; matrix instructions
@@ -459,10 +553,10 @@ struct Paired {
     }
     // (a query that does not see the row may hold NaN; past the end the last one stands again)
     if ((CAUSAL && col0 < row0 + 31) || col0 + 32 > r.len) {
-      wir::seldom();
+      const int half = wir::seldom(lane / 32);
 #pragma unroll
       for (int n = 0; n < 16; ++n) {
-        const int col = col0 + wir::ccol<32>(n, lane / 32);
+        const int col = col0 + wir::ccol<32>(n, half);
         const bool seen = (!CAUSAL || row0 + lane % 32 <= col) && col < r.len;
         s.f[0][0][n] = seen ? s.f[0][0][n] : 0.f;
         dp.f[0][0][n] = seen ? dp.f[0][0][n] : 0.f;
@@ -588,7 +682,7 @@ struct Paired {
 
 template <int D, int QT, bool CAUSAL>
 __device__ __forceinline__ void dkdv_kernel(const wir::packed_bwd_args& a) {
-  __shared__ __attribute__((aligned(1024))) char smem[4 * QT * D * 2 + 16 * QT + 2 * sizeof(wir::Odd<D>)];
+  __shared__ __attribute__((aligned(1024))) char smem[Dkdv<D, QT, CAUSAL>::BYTES];
   int x, kv;
   wir::packed_program(a.blocks, a.heads / a.group, x, kv);   // a sequence's longest block is its first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
@@ -598,8 +692,9 @@ __device__ __forceinline__ void dkdv_kernel(const wir::packed_bwd_args& a) {
     if (a.flags & 4) wir::packed_zero_rest(a.dv, a.dvh, a.dvt, r, kv, D, ROWS);
     return;
   }
+  Dkdv<D, QT, CAUSAL> p(a, r, smem);
   bool careful = false;
-  while (dkdv_block<D, QT, CAUSAL>(a, r, kv, smem, careful)) careful = true;
+  while (p.run(kv, careful)) careful = true;
 }
 
 template <int D, bool CAUSAL>
@@ -634,7 +729,7 @@ PACKED_KERNEL(wir_attn_packed_dq_d64, (dq_kernel<64, false>), 3)
 PACKED_KERNEL(wir_attn_packed_dq_d64_causal, (dq_kernel<64, true>), 3)
 PACKED_KERNEL(wir_attn_packed_dq_d128, (dq_kernel<128, false>), 2)
 PACKED_KERNEL(wir_attn_packed_dq_d128_causal, (dq_kernel<128, true>), 2)
-PACKED_KERNEL(wir_attn_packed_dkdv_d64, (dkdv_kernel<64, 32, false>), 2)
-PACKED_KERNEL(wir_attn_packed_dkdv_d64_causal, (dkdv_kernel<64, 32, true>), 2)
+PACKED_KERNEL(wir_attn_packed_dkdv_d64, (dkdv_kernel<64, 64, false>), 2)
+PACKED_KERNEL(wir_attn_packed_dkdv_d64_causal, (dkdv_kernel<64, 64, true>), 2)
 PACKED_KERNEL8(wir_attn_packed_dkdv_d128, (dkdv_kernel8<128, false>))
 PACKED_KERNEL8(wir_attn_packed_dkdv_d128_causal, (dkdv_kernel8<128, true>))

@@ -144,10 +144,7 @@ struct ForwardSplit {
       wait_tile<EACH>(more);
       wir::RTile<32, 32, KT> s;
       wir::mma_ABt_frags<32, 32, KT, TK, D / 16>(s, q, kt, 0);
-      if (CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len) {
-        wir::seldom();
-        wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
-      }
+      if (CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len) wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
       float top = s.f[0][0][0];
 #pragma unroll
       for (int cb = 0; cb < KT / 32; ++cb)
@@ -276,10 +273,7 @@ struct DqSplit {
       wir::BTile<32, 32, KT> ds;
       wir::mma_ABt_frags<32, 32, KT, TK, D / 16>(s, q, kt, 0);
       const bool edge = CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len;
-      if (edge) {
-        wir::seldom();
-        wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
-      }
+      if (edge) wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
       wir::mma_ABt_frags<32, 32, KT, TV, D / 16>(dp, d_o, vt, 0);
 #pragma unroll
       for (int cb = 0; cb < KT / 32; ++cb)

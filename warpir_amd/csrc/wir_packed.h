@@ -111,11 +111,16 @@ __device__ __forceinline__ void packed_rows(RowFrags<32, 1, KS>& fr, const bf16*
 
 // In a branch that few tiles take: keeps the compiler from computing it for all of them and selecting.
 __device__ __forceinline__ void seldom() { asm volatile(""); }
+// The same, and what follows from x is computed in that branch, not kept in registers from before a loop.
+__device__ __forceinline__ int seldom(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // Keep (row, col) for col <= row (CAUSAL), or for col < cols; elsewhere -inf.
 template <bool CAUSAL, int MS, int R, int C>
 __device__ __forceinline__ void packed_mask(RTile<MS, R, C>& t, int row0, int col0, int cols) {
-  const int lane = lane_id(), lr = lane % MS, lh = lane / MS;
+  const int lane = lane_id(), lr = lane % MS, lh = seldom(lane / MS);
 #pragma unroll
   for (int cb = 0; cb < t.CB; ++cb)
 #pragma unroll
