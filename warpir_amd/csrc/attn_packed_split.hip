@@ -9,9 +9,9 @@
 // waves' order, in fp32.  Operands are rounded as there.
 //
 // Measured, this / 128 rows a workgroup: forward of 5 sequences of up to 150
-// tokens, 16/4 heads of 128, causal 11.1 / 8.8 us, of 1 x 512, 8 heads of 64 6.8 /
-// 10.9; dQ of 1 x 512, 8 heads of 128 12.5 / 20.9; dK/dV of 1 x 512, 16/4 heads of
-// 64 17.8 / 59.5.  The rule is in packed.py.
+// tokens, 16/4 heads of 128, causal 11.1 / 8.8 us, of 1 x 512, 8 heads of 64 7.4 /
+// 11.2; dQ of 1 x 512, 8 heads of 128 13.0 / 19.0; dK/dV of 1 x 512, 16/4 heads of
+// 64 18.2 / 44.9.  The rule is in packed.py.
 #include "wir_packed_args.h"
 
 namespace {

@@ -115,11 +115,12 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
 
 # A launch of the split kernels (32 rows a workgroup, whose waves divide the other side) against one of 128 rows: us of
 # 64 keys (queries) that a workgroup of 128 rows walks, of the start of one of 32, and its part of that walk.  By launches of
-# 5 x 90 to 2 x 4096 tokens, 8/8 and 16/4 heads, causal; us, 128 rows / 32: forward D = 64, 8 heads, 1 x 512 10.9 / 6.8, 2 x
-# 1024 17.2 / 14.3, 8 x 256 7.8 / 10.7; dQ D = 128 1 x 512 20.9 / 12.5, 1 x 4096 117 / 112, 32 x 64 11.5 / 22; dK/dV D = 64, 16/4
-# heads, 1 x 512 59.5 / 17.8, 8 x 512 59.7 / 32.1, 64 x 64 14.8 / 21.1, D = 128 2 x 1024 108 / 63, 8 x 1024 115 / 152.
-_SPLIT_US = {("forward", 64): (0.82, 2.7, 0.20), ("forward", 128): (1.2, 3.8, 0.31), ("dq", 64): (1.18, 4.3, 0.20),
-             ("dq", 128): (1.75, 6.0, 0.20), ("dkdv", 64): (1.7, 4.4, 0.17), ("dkdv", 128): (1.66, 6.0, 0.50)}
+# 5 x 90 to 2 x 4096 tokens, 8/8 and 16/4 heads, causal; us, 128 rows / 32: forward D = 64, 8 heads, 1 x 512 11.2 / 7.4, 2 x
+# 1024 16.8 / 14.2, 8 x 256 8.5 / 10.5; dQ D = 128 1 x 512 19.0 / 13.0, 1 x 4096 106 / 113, 32 x 64 13.6 / 22.4; dK/dV D = 64, 16/4
+# heads, 1 x 512 44.9 / 18.2, 8 x 512 46.0 / 33.0, 64 x 64 14.9 / 21.0, D = 128 2 x 1024 108 / 63, 8 x 1024 117 / 155.  The
+# rule's choice is within 0.7% (geometric mean) of the faster one, dQ's at D = 64 and dK/dV's at 128 included.
+_SPLIT_US = {("forward", 64): (0.72, 2.67, 0.22), ("forward", 128): (1.23, 3.18, 0.27), ("dq", 64): (1.19, 3.55, 0.18),
+             ("dq", 128): (1.91, 4.64, 0.19), ("dkdv", 64): (1.29, 3.70, 0.17), ("dkdv", 128): (1.96, 4.26, 0.26)}
 
 
 def _splits(part: str, heads: int, walks: int, tokens: int, batch: int, d: int) -> bool:
