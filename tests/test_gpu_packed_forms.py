@@ -81,11 +81,30 @@ def test_given_results_and_graphs(gpu, take, form):
 
 
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("batch", [63, 64, 4200])
+@pytest.mark.parametrize("batch", [62, 63, 64, 65, 510, 511, 512, 4200])
 def test_many_sequences(gpu, take, form, batch):
     announce(form)
     take(form)
     attention.test_many_sequences(gpu, batch)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("batch", [3, 70, 600])
+def test_offsets_that_do_not_ascend(gpu, take, form, batch):
+    """They give wrong rows and no more: what lies beside the results stays."""
+    announce(f"{form}, {batch} wild offsets")
+    take(form)
+    gen = torch.Generator().manual_seed(batch)
+    t = 900
+    offsets = torch.randint(-100, t + 100, (batch + 1,), generator=gen, dtype=torch.int32).cuda()
+    q, k, v = attention._inputs(2, 1, 128, t, True)
+    big = torch.full((t, 4, 128), 5.0, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    lse = torch.full((4, t), 7.0, device="cuda")
+    o, l = api.attention_packed(q, k, v, offsets, out=big[1:3], lse=lse[1:3])
+    do = attention.seeded_normal((2, t, 128), 3).cuda()
+    grads = torch.full((t, 6, 128), 5.0, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    api.attention_packed_backward(q, k, v, o.nan_to_num(0.0), l.clamp(-50, 50), do, offsets, dq=grads[1:3], dk=grads[3:4], dv=grads[4:5])
+    assert bool((big[[0, 3]] == 5.0).all()) and bool((lse[[0, 3]] == 7.0).all()) and bool((grads[[0, 5]] == 5.0).all())
 
 
 @pytest.mark.parametrize("d", [64, 128])

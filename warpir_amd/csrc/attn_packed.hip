@@ -238,7 +238,7 @@ __device__ __forceinline__ void forward(const wir::packed_fwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[Forward<D, CAUSAL, NW>::BYTES];
   int x, head;
   const int two = NW == 8 && a.flags & 4, rows = NW == 4 || two ? 128 : 256;
-  wir::packed_program(a.blocks, two ? a.heads / 2 : a.heads, x, head);
+  wir::packed_program(a, two ? a.heads / 2 : a.heads, rows, x, head);
   if (two) head *= 2;
   if (CAUSAL) x = a.blocks - 1 - x;   // a sequence's longest block first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x, rows);

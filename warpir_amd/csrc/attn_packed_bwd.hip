@@ -210,7 +210,7 @@ template <int D, bool CAUSAL>
 __device__ __forceinline__ void dq_kernel(const wir::packed_bwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[Dq<D, CAUSAL>::BYTES];
   int x, head;
-  wir::packed_program(a.blocks, a.heads, x, head);
+  wir::packed_program(a, a.heads, ROWS, x, head);
   if (CAUSAL) x = a.blocks - 1 - x;   // a sequence's longest block first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
@@ -684,7 +684,7 @@ template <int D, int QT, bool CAUSAL>
 __device__ __forceinline__ void dkdv_kernel(const wir::packed_bwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[Dkdv<D, QT, CAUSAL>::BYTES];
   int x, kv;
-  wir::packed_program(a.blocks, a.heads / a.group, x, kv);   // a sequence's longest block is its first
+  wir::packed_program(a, a.heads / a.group, ROWS, x, kv);   // a sequence's longest block is its first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
   if (r.rest) {
@@ -701,7 +701,7 @@ template <int D, bool CAUSAL>
 __device__ __forceinline__ void dkdv_kernel8(const wir::packed_bwd_args& a) {
   __shared__ __attribute__((aligned(1024))) char smem[Paired<D, CAUSAL>::BYTES];
   int x, kv;
-  wir::packed_program(a.blocks, a.heads / a.group, x, kv);   // a sequence's longest block is its first
+  wir::packed_program(a, a.heads / a.group, ROWS, x, kv);   // a sequence's longest block is its first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)
   if (r.rest) {

@@ -413,7 +413,7 @@ template <class Split, int W, bool LONGEST_LAST, class Args, class Rest>
 __device__ __forceinline__ void program(const Args& a, int heads, Rest rest) {
   __shared__ __attribute__((aligned(1024))) char smem[Split::BYTES];
   int x, head;
-  wir::packed_program(a.blocks, heads, x, head);
+  wir::packed_program(a, heads, ROWS, x, head);
   if (LONGEST_LAST) x = a.blocks - 1 - x;   // a sequence's longest block first
   const wir::Rows r = wir::packed_block(a.offsets, a.batch, a.tokens, x, ROWS);
   if (r.row0 < 0 || r.row0 >= r.len) return;   // (a number that no block has)

@@ -56,10 +56,18 @@ __device__ __forceinline__ Rows packed_block(const int* offsets, int batch, int 
 
 // Program -> (block, head).  The programs of one XCD are of few heads, so that
 // a head's keys and values stay in its L2.
-__device__ __forceinline__ void packed_program(int blocks, int heads, int& x, int& head) {
-  const int id = remap_xcd(blockIdx.x, blocks * heads);
-  head = id / blocks;
-  x = id - head * blocks;
+//
+// Where sequences are about as long as a block, every second number is no
+// block's, and programs go to the XCD's 32 CUs in turn: half of the CUs would get only
+// those.  There the even ones of 64 blocks come first (256 x 128 tokens, 32/8 heads
+// of 128, causal: forward 285 -> 199 us, backward 856 -> 542; other lengths would be 2 to 7% slower).
+template <class Args>
+__device__ __forceinline__ void packed_program(const Args& a, int heads, int rows, int& x, int& head) {
+  const int id = remap_xcd(blockIdx.x, a.blocks * heads);
+  head = id / a.blocks;
+  x = id - head * a.blocks;
+  const i64 tokens = a.tokens, one = (i64)rows * a.batch;   // (of one block a sequence)
+  if (4 * tokens > 3 * one && 2 * tokens < 3 * one && (x | 63) < a.blocks) x = (x & ~63) | (x & 31) << 1 | (x >> 5 & 1);
 }
 
 // One head of one sequence as a tensor of its own: rows past its end read as zeros and are not stored.
