@@ -70,7 +70,8 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
     ``causal`` only those up to their own.  Tokens behind ``offsets[-1]`` belong to no
     sequence: a given ``out`` or ``lse`` keeps what it has there, an allocated one
     holds 0 and -inf.  In a captured graph the offsets may change between
-    replays.  What a row does not see does not reach it, be it infinite or NaN.
+    replays.  What a row does not see does not reach it, be it infinite or NaN.  A key
+    whose score is -inf weighs nothing; a row with no other has O NaN and LSE -inf.
 
     An allocated ``O`` lies token by token, so that ``O.transpose(0, 1).reshape(T, H * D)``
     is the next product's operand as it is.  ``out`` may be ``q`` itself."""
