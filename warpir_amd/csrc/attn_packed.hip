@@ -218,12 +218,8 @@ struct Forward {
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
-          const bool nan = row >= odd->at[0][d], up = row >= odd->at[1][d], down = row >= odd->at[2][d];
-          const float x = o.f[cb][0][i];
-          o.f[cb][0][i] = nan || (up && down) ? __builtin_nanf("") : up ? x + __builtin_inff() : down ? x - __builtin_inff() : x;
-        }
+        for (int i = 0; i < 16; ++i)
+          o.f[cb][0][i] = wir::with_odd<false>(odd, cb * 32 + wir::ccol<32>(i, lane / 32), row, o.f[cb][0][i]);
     }
     const auto O = wir::packed_head(a.out, a.oh, a.ot, head, r.start, r.len, D);
     wir::store_tile_staged<true>(O, o, 0, 0, row0, 0, smem + wave * 32 * D * 2);

@@ -419,16 +419,16 @@ struct Dkdv {
 #pragma unroll
       for (int i = 0; i < 16; ++i) dk.f[cb][0][i] *= wir::PackedScale<D>::s;
     if (careful) {
-      const int from = CAUSAL ? row : 0;   // the first query that sees it
+      // (the scores of an infinite query are no numbers, and dS with them; an infinite dO makes a sum of dV infinite)
+      const int from = CAUSAL ? row : 0;   // the first query that sees the row
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int d = cb * 32 + wir::ccol<32>(i, lane / 32);
           const int end_k = max(odd->at[0][d], max(odd->at[1][d], odd->at[2][d]));
-          const int end_v = max(odd[1].at[0][d], max(odd[1].at[1][d], odd[1].at[2][d]));
           dk.f[cb][0][i] = from <= end_k ? __builtin_nanf("") : dk.f[cb][0][i];
-          dv.f[cb][0][i] = from <= end_v ? __builtin_nanf("") : dv.f[cb][0][i];
+          dv.f[cb][0][i] = wir::with_odd<true>(odd + 1, d, from, dv.f[cb][0][i]);
         }
     }
     char* stage = smem + wave * 32 * D * 2;
@@ -663,14 +663,15 @@ struct Paired {
 #pragma unroll
       for (int n = 0; n < 16; ++n) acc.f[cb][0][n] *= role ? wir::PackedScale<D>::s : 1.f;
     if (careful) {
+      const int from = CAUSAL ? row : 0;   // as in Dkdv
       const auto* mine = odd + (role ? 0 : 1);
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
           const int d = cb * 32 + wir::ccol<32>(n, lane / 32);
-          const int until = max(mine->at[0][d], max(mine->at[1][d], mine->at[2][d]));
-          acc.f[cb][0][n] = (CAUSAL ? row : 0) <= until ? __builtin_nanf("") : acc.f[cb][0][n];
+          const float x = acc.f[cb][0][n], y = wir::with_odd<true>(mine, d, from, x);
+          acc.f[cb][0][n] = role && y != x ? __builtin_nanf("") : y;
         }
     }
     const auto out = role ? wir::packed_head(a.dk, a.dkh, a.dkt, kv, r.start, r.len, D)

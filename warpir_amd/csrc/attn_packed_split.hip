@@ -210,8 +210,7 @@ struct ForwardSplit {
     all.store(a.out + head * a.oh + (r.start + row0) * a.ot, a.ot, rows, [&](int row, int d, float x) {
       if (!careful) return x;
       const int last = CAUSAL ? row0 + row : r.len - 1;   // the last position that the row sees
-      const bool nan = last >= odd->at[0][d], up = last >= odd->at[1][d], down = last >= odd->at[2][d];
-      return nan || (up && down) ? __builtin_nanf("") : up ? x + __builtin_inff() : down ? x - __builtin_inff() : x;
+      return wir::with_odd<false, D>(odd, d, last, x);
     });
     return false;
   }
@@ -396,15 +395,15 @@ struct DkdvSplit {
       const bool nan = keys.nan(rows) || values.nan(rows);
       if (wir::any_wave(nan, smem + ODD)) return true;
     }
-    auto finish = [&](const lds_odd* notes) {
-      return [=](int at, int d, float x) {
-        if (!careful) return x;
-        const int until = max(notes->at[0][d], max(notes->at[1][d], notes->at[2][d]));
-        return (CAUSAL ? row0 + at : 0) <= until ? __builtin_nanf("") : x;
-      };
-    };
-    keys.store(a.dk + kv * a.dkh + (r.start + row0) * a.dkt, a.dkt, rows, finish(odd));
-    values.store(a.dv + kv * a.dvh + (r.start + row0) * a.dvt, a.dvt, rows, finish(odd + 1));
+    // (the scores of an infinite query are no numbers, and dS with them; an infinite dO makes a sum of dV infinite)
+    keys.store(a.dk + kv * a.dkh + (r.start + row0) * a.dkt, a.dkt, rows, [=](int at, int d, float x) {
+      if (!careful) return x;
+      const int until = max(odd->at[0][d], max(odd->at[1][d], odd->at[2][d]));
+      return (CAUSAL ? row0 + at : 0) <= until ? __builtin_nanf("") : x;
+    });
+    values.store(a.dv + kv * a.dvh + (r.start + row0) * a.dvt, a.dvt, rows, [=](int at, int d, float x) {
+      return careful ? wir::with_odd<true, D>(odd + 1, d, CAUSAL ? row0 + at : 0, x) : x;
+    });
     return false;
   }
 };

@@ -208,4 +208,12 @@ __device__ __forceinline__ void clear_odd(char* b_base, int pos0, __attribute__(
   if (NW == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (other waves have nothing to do with the tile)
 }
 
+// x, a sum over column d without its odd values, with those that `row` sees: positions up to it (LAST: from it on).
+template <bool LAST, int D>
+__device__ __forceinline__ float with_odd(const __attribute__((address_space(3))) Odd<D>* odd, int d, int row, float x) {
+  auto sees = [&](int i) { return LAST ? row <= odd->at[i][d] : row >= odd->at[i][d]; };
+  const bool nan = sees(0), up = sees(1), down = sees(2);
+  return nan || (up && down) ? __builtin_nanf("") : up ? x + __builtin_inff() : down ? x - __builtin_inff() : x;
+}
+
 }  // namespace wir
