@@ -79,3 +79,21 @@ def test_infinite_output_gradients_of_both_signs(gpu, take, d, form, causal):   
         expected[0, 100:300, 3] = expected[1, 100:300, 7] = math.nan
         expected[1, 100:300, 9] = math.inf
     assert _same(dv, expected)
+
+
+@pytest.mark.parametrize("d,form", [(64, f) for f in FORMS[:2]] + [(128, f) for f in FORMS])
+def test_infinite_value_of_a_key_without_weight(gpu, take, d, form):   # noqa: F811
+    """Row 1 of two tokens: P of key 0 is too small for 32 bits, its value infinite.  dS = P (inf - inf) is no number
+    all the same, and dQ with it."""
+    announce(f"packed attention backward D{d} {form}, an infinite value of a key without weight")
+    take(form)
+    q, k, v = (x.clone() for x in attention._inputs(2, 1, d, 2, False))
+    q[:, 1, 0], k[:, 0, 0], k[:, 1, 0] = 100.0, -100.0, 1.0
+    v[:, 0, 3] = math.inf
+    do = seeded_normal((2, 2, d), 7).cuda()
+    offsets = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    o, lse = api.attention_packed(q, k, v, offsets)
+    assert bool((o[:, 1, 3] == math.inf).all())
+    for causal in (True, False):
+        dq = api.attention_packed_backward(q, k, v, o, lse, do, offsets, causal=causal)[0]
+        assert bool(dq[:, 1].isnan().all())

@@ -271,17 +271,23 @@ struct DqSplit {
       wir::RTile<32, 32, KT> s, dp;
       wir::BTile<32, 32, KT> ds;
       wir::mma_ABt_frags<32, 32, KT, TK, D / 16>(s, q, kt, 0);
-      const bool edge = CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len;
-      if (edge) wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
       wir::mma_ABt_frags<32, 32, KT, TV, D / 16>(dp, d_o, vt, 0);
 #pragma unroll
       for (int cb = 0; cb < KT / 32; ++cb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s.f[cb][0][i], c, -lse));
-          const float x = p * (dp.f[cb][0][i] - dots.v[0]);
-          ds.f[cb][0][i / 4][i % 4] = (bf16)(edge && p == 0.f ? 0.f : x);   // (a value that a row does not see may be NaN)
-        }
+        for (int i = 0; i < 16; ++i)
+          dp.f[cb][0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s.f[cb][0][i], c, -lse)) * (dp.f[cb][0][i] - dots.v[0]);
+      if (CAUSAL ? col0 + KT - 1 > row0 : col0 + KT > r.len) {   // (a value that a row does not see may be NaN)
+        const int half = wir::seldom(lane / 32);
+#pragma unroll
+        for (int cb = 0; cb < KT / 32; ++cb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int col = col0 + cb * 32 + wir::ccol<32>(i, half);
+            dp.f[cb][0][i] = (CAUSAL ? col <= row : col < r.len) ? dp.f[cb][0][i] : 0.f;
+          }
+      }
+      wir::to_bf16(ds, dp);
       if (careful) wir::clear_odd<false, 1, TK>(kt, col0, odd);
       wir::mma_rAB<32, 32, KT, D, TK>(acc, ds, kt, 0);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the slot is read: it may be loaded again)
