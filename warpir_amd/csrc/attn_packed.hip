@@ -110,15 +110,15 @@ struct Forward {
     __builtin_amdgcn_s_setprio(0);
   }
 
-  // p and the lane's sum of it, over 2^base.
-  __device__ __forceinline__ float exponentials(float base) {
+  // p and the lane's sum of it, with m as it is.
+  __device__ __forceinline__ float exponentials() {
     constexpr float c = wir::PackedScale<D>::c;
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s.f[cb][0][i], c, -base));
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s.f[cb][0][i], c, -m));
         sum[i % 2] += x;
         p.f[cb][0][i / 4][i % 4] = (bf16)x;   // (the product's operand; the sum has the value itself)
       }
@@ -129,7 +129,7 @@ struct Forward {
     constexpr float c = wir::PackedScale<D>::c;
     const int col0 = t * TILE;
     if (CAUSAL ? col0 + TILE - 1 > row0 : col0 + TILE > r.len) wir::packed_mask<CAUSAL>(s, row0, col0, r.len);
-    float sum = exponentials(m);   // (not a number below LIMIT as long as m is -inf)
+    float sum = exponentials();   // (infinite where the first scores are met that are not -inf)
     if (__builtin_amdgcn_ballot_w64(!(sum <= LIMIT)) != 0) {
       wir::seldom();
       float top = s.f[0][0][0];
@@ -141,13 +141,12 @@ struct Forward {
       const float asked = wir::lane_group_reduce<32>(sum <= LIMIT ? 0.f : 1.f, wir::OpMax());
       top = fmaxf(wir::lane_group_reduce<32>(top, wir::OpMax()) * c, m);
       top = asked != 0.f ? top : m;
-      const float base = top == -__builtin_inff() ? 0.f : top;   // (a row whose scores are all -inf so far)
-      const float corr = __builtin_amdgcn_exp2f(m - base);
+      const float corr = __builtin_amdgcn_exp2f(m - top);
       m = top;
       l *= corr;
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) o.f[cb][0] *= corr;
-      sum = exponentials(base);
+      sum = exponentials();
     }
     l += sum;
   }
@@ -202,7 +201,8 @@ struct Forward {
     if (careful) wir::no_odd<false, NW>(odd);
     K.load(smem, 0, wave);
     wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
-    m = -__builtin_inff(), l = 0.f;
+    // below every score but -inf, from which it differs by a number: a row whose scores are all -inf so far has sums of 0
+    m = -3.4028234663852886e38f, l = 0.f;
     wir::fill(o, 0.f);
     if (NW == 4 || second == 0) walk<0>(careful, odd);
     else walk<1>(careful, odd);
