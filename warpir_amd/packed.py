@@ -59,6 +59,11 @@ def _by_token(heads, tokens, d, device, rec):
     return rec.alloc(torch.empty(tokens, heads, d, dtype=torch.bfloat16, device=device).transpose(0, 1))
 
 
+# what a given result and another tensor of the call must not share; past the first ones, pairs that may be one tensor
+_FORWARD_PAIRS = ("out", "lse", "out", "k", "out", "v", "out", "offsets", "lse", "q", "lse", "k", "lse", "v", "lse", "offsets",
+                  "out", "q")
+
+
 def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) -> Tuple[object, object]:
     """Attention over packed sequences: ``q`` ``[H, T, D]``, ``k`` and ``v`` ``[H_kv, T, D]``
     (bf16, D = 64 or 128, H a multiple of H_kv; any 16-byte aligned rows, so
@@ -74,12 +79,13 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
     whose score is -inf weighs nothing; a row with no other has O NaN and LSE -inf.
 
     An allocated ``O`` lies token by token, so that ``O.transpose(0, 1).reshape(T, H * D)``
-    is the next product's operand as it is.  ``out`` may be ``q`` itself."""
+    is the next product's operand as it is.  ``out`` may be ``q`` itself; other memory
+    that ``out`` or ``lse`` shares with a tensor of the call is refused."""
     import torch
 
     fn, done, given = "attention_packed", None, None
     if out is not None or lse is not None:
-        apart(fn, ("out", "lse", "out", "k", "out", "v", "out", "q"), 3, out, lse, out, k, out, v, out, q)
+        apart(fn, _FORWARD_PAIRS, 8, out, lse, out, k, out, v, out, offsets, lse, q, lse, k, lse, v, lse, offsets, out, q)
         given = out, lse
         out = own(out, q)
     planned = type(causal) is bool
@@ -158,10 +164,12 @@ def _results(given, done):
     return done if given is None else tuple(x if g is None else g for g, x in zip(given, done))
 
 
-# what a given gradient and another tensor of the call must not share; past the first ones, pairs that may be one tensor
-_BACKWARD_PAIRS = ("dq", "dk", "dq", "dv", "dk", "dv", "dq", "q", "dq", "k", "dq", "v", "dq", "o", "dq", "do",
-                   "dk", "q", "dk", "v", "dk", "o", "dk", "do", "dv", "q", "dv", "k", "dv", "o", "dv", "do",
-                   "dk", "k", "dv", "v")
+# the same of a given gradient or workspace
+_BACKWARD_PAIRS = ("dq", "dk", "dq", "dv", "dk", "dv", "dq", "q", "dq", "k", "dq", "v", "dq", "o", "dq", "do", "dq", "lse", "dq", "offsets",
+                   "dk", "q", "dk", "v", "dk", "o", "dk", "do", "dk", "lse", "dk", "offsets",
+                   "dv", "q", "dv", "k", "dv", "o", "dv", "do", "dv", "lse", "dv", "offsets",
+                   "workspace", "q", "workspace", "k", "workspace", "v", "workspace", "o", "workspace", "do", "workspace", "lse",
+                   "workspace", "offsets", "workspace", "dq", "workspace", "dk", "workspace", "dv", "dk", "k", "dv", "v")
 
 
 def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True, dq=None, dk=None, dv=None,
@@ -173,15 +181,18 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
 
     Tokens behind ``offsets[-1]`` get no gradient: given tensors keep what they
     have there, allocated ones (which lie token by token) hold 0.  ``dk`` may be
-    ``k`` itself and ``dv`` ``v``; other shared memory is refused.  ``workspace`` holds two
-    numbers for each query head and token (fp32, at least ``2 * H * T`` elements,
-    allocated if omitted); one call at a time may use it."""
+    ``k`` itself and ``dv`` ``v``; other memory that they or ``workspace`` share with a
+    tensor of the call is refused.  ``workspace`` holds two numbers for each query head
+    and token (fp32, at least ``2 * H * T`` elements, allocated if omitted); one call at
+    a time may use it."""
     import torch
 
     fn, done, given = "attention_packed_backward", None, None
-    if dq is not None or dk is not None or dv is not None:
-        apart(fn, _BACKWARD_PAIRS, 16, dq, dk, dq, dv, dk, dv, dq, q, dq, k, dq, v, dq, o, dq, do,
-              dk, q, dk, v, dk, o, dk, do, dv, q, dv, k, dv, o, dv, do, dk, k, dv, v)
+    if dq is not None or dk is not None or dv is not None or workspace is not None:
+        ws = workspace
+        apart(fn, _BACKWARD_PAIRS, 32, dq, dk, dq, dv, dk, dv, dq, q, dq, k, dq, v, dq, o, dq, do, dq, lse, dq, offsets,
+              dk, q, dk, v, dk, o, dk, do, dk, lse, dk, offsets, dv, q, dv, k, dv, o, dv, do, dv, lse, dv, offsets,
+              ws, q, ws, k, ws, v, ws, o, ws, do, ws, lse, ws, offsets, ws, dq, ws, dk, ws, dv, dk, k, dv, v)
         given = dq, dk, dv
         dk, dv = own(dk, k), own(dv, v)
     tensors = (q, k, v, o, lse, do, offsets, dq, dk, dv)
