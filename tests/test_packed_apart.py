@@ -11,7 +11,7 @@ from warpir_amd.runtime import PKG_DIR
 
 pytestmark = pytest.mark.skipif(not os.path.exists(os.path.join(PKG_DIR, "_wir_plans.so")), reason="not built")
 
-f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
+f32, i32, i8, bf16 = torch.float32, torch.int32, torch.int8, torch.bfloat16
 H, HK, T, D = 4, 2, 30, 64
 
 
@@ -83,3 +83,13 @@ def test_gradients_that_pass():
     _passes(api.attention_packed_backward, **a, workspace=ws)
     _passes(api.attention_packed_backward, **a, workspace=ws, dq=torch.zeros_like(a["q"]), dk=a["k"], dv=a["v"])
     _refused(api.attention_packed_backward, "dk and dv", **a, dk=a["k"], dv=a["k"].view(a["k"].shape))
+
+
+def test_quantize():
+    x = torch.zeros(64, 64, dtype=bf16)
+    _refused(api.quantize_int8, "scale and x", x=x, scale=_as(x, f32, 64))
+    _refused(api.quantize_int8, "scale and x", x=x, codes=torch.zeros(64, 64, dtype=i8), scale=_as(x, f32, 64))
+    _refused(api.quantize_int8, "codes and x", x=x, codes=_as(x, i8, 64, 64))
+    codes = torch.zeros(64, 64, dtype=i8)
+    _refused(api.quantize_int8, "codes and scale", x=x, codes=codes, scale=_as(codes, f32, 64))
+    _passes(api.quantize_int8, x=x, codes=codes, scale=torch.zeros(64))

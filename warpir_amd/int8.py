@@ -34,13 +34,14 @@ def quantize_int8(x, codes=None, scale=None) -> Tuple[object, object]:
     8-bit integers: ``(codes, scale)``, int8 ``[M, K]`` and fp32 ``[M]``.  A row's scale is
     its largest magnitude times 1 / 127, each rounded to fp32 (as torch's ``amax(1) / 127``
     on a GPU; 2^-126 at least), its codes the integers nearest to ``x / scale``, ties to
-    even: -127 to 127.  The scale of a row with an infinity or NaN is NaN, and its codes are 0.  Made for ``gemm_int8``: of tokens,
-    and of a weight's channels where they are rows."""
+    even: -127 to 127.  The scale of a row with an infinity or NaN is NaN, and its
+    codes are 0.  Made for ``gemm_int8``: of tokens, and of a weight's channels where
+    they are rows.  ``codes`` and ``scale`` share no memory with one another or with ``x``."""
     import torch
 
     fn, done = "quantize_int8", None
-    if codes is not None:
-        apart(fn, ("codes", "scale", "codes", "x"), 2, codes, scale, codes, x)
+    if codes is not None or scale is not None:
+        apart(fn, ("codes", "scale", "codes", "x", "scale", "x"), 3, codes, scale, codes, x, scale, x)
     done = _quantize_plans.run(0, x, codes, scale)
     if done is not None and done is not False:
         return done
