@@ -93,3 +93,20 @@ def test_quantize():
     codes = torch.zeros(64, 64, dtype=i8)
     _refused(api.quantize_int8, "codes and scale", x=x, codes=codes, scale=_as(codes, f32, 64))
     _passes(api.quantize_int8, x=x, codes=codes, scale=torch.zeros(64))
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("name", ["cos", "sin", "positions"])
+def test_rotation(name, side, back):
+    call = api.rope_axes_backward if back else api.rope_axes
+    outs = ("dq", "dk") if back else ("q_out", "k_out")
+    ins = ("dq_out", "dk_out") if back else ("q", "k")
+    room = torch.zeros(2 * 4 * 8 * 64, dtype=bf16)
+    a = {ins[0]: torch.zeros(2, 4, 8, 64, dtype=bf16), ins[1]: torch.zeros(2, 2, 8, 64, dtype=bf16), "cos": torch.zeros(16, 24),
+         "sin": torch.zeros(16, 24), "positions": torch.zeros(3, 8, dtype=i32), "sections": (8, 8, 8)}
+    given = {outs[side]: _as(room, bf16, 2, 2 if side else 4, 8, 64)}
+    _passes(call, **a, **given)
+    _passes(call, **a, **{outs[side]: a[ins[side]]})
+    a[name] = _as(room, i32, 3, 8) if name == "positions" else _as(room, f32, 16, 24)
+    _refused(call, f"{outs[side]} and {name}", **a, **given)

@@ -271,6 +271,12 @@ def _sections(fn: str, sections, interleaved, back: bool):
     return flags, pairs, ends, any(n % 4 for n in ends)
 
 
+# what a given output and another tensor of the call must not share, with the pairs that may be one tensor last
+_AXES_PAIRS = tuple((q_out, k_out, q_out, k, k_out, q, q_out, "cos", q_out, "sin", q_out, "positions", k_out, "cos", k_out, "sin",
+                     k_out, "positions", q_out, q, k_out, k)
+                    for q, k, q_out, k_out in (("q", "k", "q_out", "k_out"), ("dq_out", "dk_out", "dq", "dk")))
+
+
 def _rotate_axes(fn, plans, back, names, q, k, cos, sin, positions, sections, interleaved, q_out, k_out):
     import torch
 
@@ -281,8 +287,8 @@ def _rotate_axes(fn, plans, back, names, q, k, cos, sin, positions, sections, in
     given = None
     if q_out is not None or k_out is not None:
         need(fn, q_out is not k_out, f"{names[2]} and {names[3]} are one tensor")
-        apart(fn, (names[2], names[3], names[2], names[1], names[3], names[0], names[2], names[0], names[3], names[1]), 3,
-              q_out, k_out, q_out, k, k_out, q, q_out, q, k_out, k)
+        apart(fn, _AXES_PAIRS[back], 9, q_out, k_out, q_out, k, k_out, q, q_out, cos, q_out, sin, q_out, positions, k_out, cos,
+              k_out, sin, k_out, positions, q_out, q, k_out, k)
         given = q_out, k_out
         q_out, k_out = own(q_out, q), own(k_out, k)
     done = plans.run(key, q, k, cos, sin, positions, q_out, k_out)
@@ -341,7 +347,7 @@ def rope_axes(q, k, cos, sin, positions, sections, interleaved: bool = False, q_
 
     Packed sequences are one with B = 1 and the positions of each of them.
     ``q_out`` may be ``q`` itself and ``k_out`` ``k``; memory that an output shares
-    otherwise with the other, ``q`` or ``k`` is refused."""
+    otherwise with a tensor of the call is refused."""
     return _rotate_axes("rope_axes", _axes_plans, False, ("q", "k", "q_out", "k_out"), q, k, cos, sin, positions,
                         sections, interleaved, q_out, k_out)
 
