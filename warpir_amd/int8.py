@@ -112,8 +112,8 @@ def gemm_int8(a, b, a_scale, b_scale, out=None):
         out = rec.alloc(torch.empty(m, n, dtype=torch.bfloat16, device=device))
     if m == 0 or n == 0:
         return out
-    if k == 0:
-        return out.zero_()
+    if k == 0:   # (0 times a scale, which may be infinite or NaN)
+        return out.copy_(a_scale[:, None] * 0.0 * b_scale)
     variant, bm, bn, threads = _gemm_form(m, n, k)
     tiles = -(-m // bm) * -(-n // bn)
     need(fn, tiles * threads < 1 << 32, "2^32 threads or more in one call")
