@@ -94,3 +94,45 @@ def test_no_key_has_a_score(gpu, take, d, form, causal):   # noqa: F811
     assert bool(o[:, 70:370].isnan().all()) and bool((lse[:, 70:370] == -math.inf).all())
     for at in (slice(0, 70), slice(370, 400)):
         assert torch.equal(o[:, at], want[0][:, at]) and torch.equal(lse[:, at], want[1][:, at])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("d,form", [(64, f) for f in FORMS[:2]] + [(128, f) for f in FORMS])
+def test_rows_that_see_an_infinite_key(gpu, take, d, form, value, causal):   # noqa: F811
+    """Column 0 of one key is infinite: rows of the other sign there have a score of -inf and go on without it, rows of
+    its sign have +inf and no results; the gradients are numbers where no such row has a part."""
+    announce(f"packed attention D{d} {form} causal={causal}, a key has {value}")
+    take(form)
+    h, hk, ends, at = 4, 2, [0, 100, 400, 430], 177
+    q, k, v = (x.clone() for x in attention._inputs(h, hk, d, ends[-1], False))
+    k[:, at, 0] = value
+    do = seeded_normal(q.shape, 9).cuda()
+    offsets = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    o, lse = api.attention_packed(q, k, v, offsets, causal=causal)
+    grads = api.attention_packed_backward(q, k, v, o, lse, do, offsets, causal=causal)
+
+    tokens = torch.arange(ends[-1])
+    sees = (tokens >= (at if causal else 100)) & (tokens < 400)
+    cq, ck, cv = (x.cpu().double() for x in (q, k, v))
+    bad = sees & (cq[:, :, 0] * value > 0)                  # [H, T]
+    assert bool(o[bad].isnan().all()) and not bool(lse[bad].isfinite().any())
+    # to the others the key is as far away as one can be; its scores with rows of its sign are not compared
+    ck[:, at, 0] = 0
+    _, _, _, scores = packed_attention_ref(cq, ck, cv, ends, False)
+    ck[:, at, 0] = math.copysign(1e30, value)
+    ref, ref_lse, weight, _ = packed_attention_ref(cq, ck, cv, ends, causal)
+    e = 2 * (d + 8) * U * scores + 2 ** -20
+    off, tol = (o.cpu().double() - ref).abs(), 2 ** -8 * ref.abs() + (2 ** -8 + 2 * e[..., None] + 4 * 300 * U) * weight
+    assert bool((off <= tol)[~bad].all()), off[~bad].max()
+    off = (lse.cpu().double() - ref_lse).abs()
+    assert bool((off <= e + 2 * 300 * U + 4 * U * ref_lse.abs())[~bad].all()), off[~bad].max()
+
+    dq, dk, dv = (g.cpu() for g in grads)
+    assert bool(dq[bad].isnan().all()) and bool(dq[~bad][:, 1:].isfinite().all())
+    assert torch.equal(dq[~bad][:, 0].isnan(), sees.expand(h, -1)[~bad])    # 0 times the infinity
+    for j in range(hk):
+        rows = bad[2 * j:2 * j + 2].any(0)
+        hit = (tokens >= 100) & (tokens < 400) & ((tokens <= int(tokens[rows].max())) if causal else bool(rows.any()))
+        assert bool(dk[j, hit].isnan().all()) and bool(dv[j, hit].isnan().all())
+        assert bool(dk[j, ~hit].isfinite().all()) and bool(dv[j, ~hit].isfinite().all())
