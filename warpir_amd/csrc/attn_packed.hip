@@ -203,6 +203,7 @@ struct Forward {
     wir::packed_rows(q, a.q + head * a.qh + r.start * a.qt, a.qt, row0, r.len);
     // below every score but -inf, from which it differs by a number: a row whose scores are all -inf so far has sums of 0
     m = -3.4028234663852886e38f, l = 0.f;
+    asm volatile("" : "+v"(m));   // (as a known number it and its negative would hold registers throughout: 1.5% more cycles)
     wir::fill(o, 0.f);
     if (NW == 4 || second == 0) walk<0>(careful, odd);
     else walk<1>(careful, odd);
