@@ -32,7 +32,7 @@ using wir::i64;
 // x 512 tokens 97 us (700).  At D = 128 LDS bounds it: an operand of 1 KB serves
 // the 32 rows of one wave, a product of 32 cycles, and takes LDS 8 cycles as it
 // lies and 16 transposed, so that four SIMDs' products of both kinds, 64 cycles,
-// ask for 96 of its cycles: matrix instructions run in 64% of them, causal.  Of 950
+// ask for 96 of its cycles: matrix instructions run in 65% of them, causal.  Of 950
 // us (16 heads of 128, 8 x 4096) the exponentials are 63, the tiles' loads 105, both 177.  At D = 64 the
 // exponentials weigh twice as much (matrix instructions 38% of the cycles in 48
 // sequences of up to 1024 tokens), and short sequences pay 5 us a round of

@@ -236,7 +236,7 @@ __device__ __forceinline__ void finish(const gemm_args& g, const i32x16 (&acc)[C
 // wave takes WM x WN of it, and of each row's bytes 1 / KW: KW waves have one
 // part of the output, whose sums they share out and add at the end.
 //
-// Measured: 8192 x 8192 x 8192 in 463 us (2375 TOP/s, the library's product 512),
+// Measured: 8192 x 8192 x 8192 in 451 to 464 us by the card (2370-2440 TOP/s, the library's product 512),
 // where the clock is what the power leaves; 777 x 4100 x 4096 in 22.3 us.  Small tiles
 // are bound by LDS, which takes 32 KB a step and reads 64 to 96: of 22 us without
 // the loads 16, without the products 17, without the reads 19.  Two waves of 64 x

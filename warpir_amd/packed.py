@@ -77,6 +77,8 @@ def attention_packed(q, k, v, offsets, causal: bool = True, out=None, lse=None) 
     holds 0 and -inf.  In a captured graph the offsets may change between
     replays.  What a row does not see does not reach it, be it infinite or NaN.  A key
     whose score is -inf weighs nothing; a row with no other has O NaN and LSE -inf.
+    Sums over the keys are divided by their weight at the end: values of v up to 2^96
+    in magnitude cannot overflow on the way.
 
     An allocated ``O`` lies token by token, so that ``O.transpose(0, 1).reshape(T, H * D)``
     is the next product's operand as it is.  ``out`` may be ``q`` itself; other memory
@@ -177,7 +179,8 @@ def attention_packed_backward(q, k, v, o, lse, do, offsets, causal: bool = True,
     """Gradients ``(dq, dk, dv)`` (bf16) of ``attention_packed`` from its inputs, its
     outputs ``o`` and ``lse`` and the gradient ``do`` of ``o`` (bf16 ``[H, T, D]``, any
     row-aligned layout); ``causal`` as in the forward.  The sums over a
-    key/value head's query heads are in 32 bits, in an order that the lengths fix.
+    key/value head's query heads are in 32 bits, in an order that the shapes and the
+    lengths fix (T with the tokens behind the last sequence).
 
     Tokens behind ``offsets[-1]`` get no gradient: given tensors keep what they
     have there, allocated ones (which lie token by token) hold 0.  ``dk`` may be
